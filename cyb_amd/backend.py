@@ -38,6 +38,7 @@ _CALLS_PATH = os.path.join(_HERE, "lib", "_torch_calls.so")
 
 F32, F16, BF16 = 0, 1, 2
 EPILOGUES = {"none": 0, "add": 1, "swiglu": 2}      # enum cybq_epilogue
+SCORES = {"softmax": 0, "sigmoid": 1}               # enum cybq_score
 _DTYPE_CODES = {"torch.float32": F32, "torch.float16": F16, "torch.bfloat16": BF16,
                 "float32": F32, "float16": F16}
 _ITEMSIZE = {F32: 4, F16: 2, BF16: 2}
@@ -94,6 +95,9 @@ def load_library() -> ctypes.CDLL:
     lib.cybq_set_prefill_mode.argtypes = [vp, ci]
     lib.cybq_set_decode_mode.argtypes = [vp, ci]
     lib.cybq_matmul_many.argtypes = [vp, i64, vp, vp, vp, ci, i64, ci, vp]
+    lib.cybq_route.argtypes = [vp, vp, ci, i64, i64, i64, ci, vp, i64, i64, ci, ci, ctypes.c_float, vp, vp, vp]
+    lib.cybq_matmul_experts.argtypes = [vp, vp, i64, vp, ci, i64, i64, vp, vp, ci, ci, vp]
+    lib.cybq_matmul_experts_sum.argtypes = [vp, vp, i64, vp, ci, i64, i64, vp, vp, vp, vp, ci, vp]
     lib.cybq_dequant.argtypes = [vp, vp, vp, vp]
     lib.cybq_quantize.argtypes = [vp, ci, vp, i64, i64, vp, vp, vp]
     # diagnostics (cyb_amd/csrc/cybq_debug.h), not part of the operator interface
@@ -430,6 +434,58 @@ class Backend:
         self._check(self._lib.cybq_matmul_norm(self._ctx, w.handle, _ptr(x), _dtype_code(x, None), M, _ptr(gamma),
                                                _dtype_code(gamma, None), ctypes.c_float(eps), _ptr(y),
                                                _dtype_code(y, None), EPILOGUES[epilogue], _ptr(residual), stream))
+
+    # ---- mixture of experts
+    def _check_pairs(self, ids, weights=None):
+        """(T, top_k) of a [T, top_k] int32 tensor of expert ids, with fp32 weights of the same shape."""
+        if ids.dim() != 2 or str(ids.dtype) != "torch.int32":
+            raise CybqError(-2, "bad shape", "ids must be an int32 tensor [tokens, top_k]")
+        if weights is not None and (tuple(weights.shape) != tuple(ids.shape) or str(weights.dtype) != "torch.float32"):
+            raise CybqError(-2, "bad shape", "weights must be a float32 tensor of the shape of ids")
+        self._check_tensor(ids, "ids", ids.numel())
+        self._check_tensor(weights, "weights", ids.numel())
+        return ids.shape
+
+    def route(self, logits, ids, weights, score: str = "softmax", bias=None, groups: int = 1, top_groups: Optional[int] = None,
+              group_best: int = 1, renormalise: bool = True, scale: float = 1.0, stream: int = 0) -> None:
+        """cybq_route: logits [T, E] -> the experts ids [T, top_k] (int32) of every token and their weights (float32)."""
+        if score not in SCORES:
+            raise CybqError(-1, "invalid argument", f"unknown score {score!r}")
+        T, k = self._check_pairs(ids, weights)
+        if logits.dim() != 2 or logits.shape[0] != T:
+            raise CybqError(-2, "bad shape", f"logits must be [{T}, experts]")
+        E = logits.shape[1]
+        self._check_tensor(logits, "logits", T * E)
+        self._check_tensor(bias, "bias", E)
+        if bias is not None and str(bias.dtype) != "torch.float32":
+            raise CybqError(-1, "invalid argument", "bias must be float32")
+        self._check(self._lib.cybq_route(self._ctx, _ptr(logits), _dtype_code(logits, None), T, E, k, SCORES[score], _ptr(bias), groups,
+                                         groups if top_groups is None else top_groups, group_best, 1 if renormalise else 0,
+                                         ctypes.c_float(scale), _ptr(ids), _ptr(weights), stream))
+
+    def matmul_experts(self, w: QWeight, experts: int, x, ids, y, epilogue: str = "none", stream: int = 0) -> None:
+        """cybq_matmul_experts: y[t * top_k + j] = epilogue(x[t] W_e^T), e = ids[t, j]; w is a stack of `experts` weights
+        (epilogue "swiglu": fuse_pairs of the gate stack and the up stack).  Rows of y whose id is no expert stay."""
+        if epilogue not in EPILOGUES:
+            raise CybqError(-1, "invalid argument", f"unknown epilogue {epilogue!r}")
+        T, k = self._check_pairs(ids)
+        n = w.N // max(experts, 1) // (2 if epilogue == "swiglu" else 1)
+        self._check_tensor(x, "x", T * w.K)
+        self._check_tensor(y, "y", T * k * n)
+        self._check(self._lib.cybq_matmul_experts(self._ctx, w.handle, experts, _ptr(x), _dtype_code(x, None), T, k, _ptr(ids), _ptr(y),
+                                                  _dtype_code(y, None), EPILOGUES[epilogue], stream))
+
+    def matmul_experts_sum(self, w: QWeight, experts: int, x, ids, weights, y, residual=None, stream: int = 0) -> None:
+        """cybq_matmul_experts_sum: y[t] = residual[t] + sum_j weights[t, j] * (x[t * top_k + j] W_e^T), e = ids[t, j]."""
+        T, k = self._check_pairs(ids, weights)
+        n = w.N // max(experts, 1)
+        self._check_tensor(x, "x", T * k * w.K)
+        self._check_tensor(y, "y", T * n)
+        self._check_tensor(residual, "residual", T * n)
+        if residual is not None and residual.dtype != y.dtype:
+            raise CybqError(-1, "invalid argument", "residual must have y's dtype")
+        self._check(self._lib.cybq_matmul_experts_sum(self._ctx, w.handle, experts, _ptr(x), _dtype_code(x, None), T, k, _ptr(ids),
+                                                      _ptr(weights), _ptr(residual), _ptr(y), _dtype_code(y, None), stream))
 
     def fuse_pairs(self, gate: QWeight, up: QWeight, name: Optional[str] = None) -> QWeight:
         """One weight holding gate and up projections interleaved by 16-row strip (device to device)."""

@@ -3,6 +3,7 @@
 // this boundary.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <atomic>
 #include <cstdio>
 #include <cstring>
@@ -640,6 +641,105 @@ int cybq_weight_fuse_pairs(cybq_ctx* ctx, const cybq_weight* gate, const cybq_we
     w->wide_scales = wide_gate || wide_up;
     *out = w;
     return CYBQ_OK;
+}
+
+int cybq_route(cybq_ctx* ctx, const void* logits, cybq_dtype ldt, int64_t T, int64_t E, int64_t top_k, cybq_score score, const float* bias,
+               int64_t groups, int64_t top_groups, int group_best, int renormalise, float scale, int32_t* ids, float* weights, void* stream)
+{
+    if (!ctx) return CYBQ_ERR_INVALID;
+    if (T && (!logits || !ids || !weights)) return fail(ctx, CYBQ_ERR_INVALID, "logits / ids / weights is NULL");
+    if (!dtype_ok(ldt)) return fail(ctx, CYBQ_ERR_INVALID, "unknown dtype");
+    if (score != CYBQ_SCORE_SOFTMAX && score != CYBQ_SCORE_SIGMOID) return fail(ctx, CYBQ_ERR_INVALID, "unknown score");
+    if (T < 0 || T > (1 << 24)) return fail(ctx, CYBQ_ERR_SHAPE, "T must be in 0..2^24");
+    if (E < 1 || E > CYBQ_MAX_EXPERTS) return fail(ctx, CYBQ_ERR_SHAPE, "E must be in 1..CYBQ_MAX_EXPERTS");
+    if (groups < 1 || groups > 64 || E % groups) return fail(ctx, CYBQ_ERR_SHAPE, "groups must be in 1..64 and divide E");
+    if (top_groups < 1 || top_groups > groups) return fail(ctx, CYBQ_ERR_SHAPE, "top_groups must be in 1..groups");
+    if (group_best != 1 && group_best != 2) return fail(ctx, CYBQ_ERR_INVALID, "group_best must be 1 or 2");
+    if (top_k < 1 || top_k > CYBQ_MAX_TOP_K || top_k > top_groups * (E / groups))
+        return fail(ctx, CYBQ_ERR_SHAPE, "top_k must be in 1..CYBQ_MAX_TOP_K and no more than the experts of top_groups groups");
+    if (reinterpret_cast<uintptr_t>(logits) % dtype_size(ldt) || reinterpret_cast<uintptr_t>(ids) % 4 || reinterpret_cast<uintptr_t>(weights) % 4 ||
+        reinterpret_cast<uintptr_t>(bias) % 4)
+        return fail(ctx, CYBQ_ERR_ALIGN, "logits / bias / ids / weights is not aligned to its element size");
+    if (T == 0) return CYBQ_OK;
+    DeviceGuard guard(ctx->device);
+    if (guard.err != hipSuccess) return fail_hip(ctx, guard.err, "hipSetDevice");
+    const hipError_t e = cybq::launch_route(logits, ldt, T, (int)E, (int)top_k, score, bias, (int)groups, (int)top_groups, group_best, renormalise != 0,
+                                            scale, ids, weights, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return fail_hip(ctx, e, "route launch");
+    return CYBQ_OK;
+}
+
+namespace {
+// sum: x has a row for every pair and y is [T, n], the weighted sum over a token's pairs
+int matmul_experts(cybq_ctx* ctx, const cybq_weight* w, int64_t E, const void* x, cybq_dtype xdt, int64_t T, int64_t top_k, const int32_t* ids,
+                   const float* weights, const void* residual, void* y, cybq_dtype ydt, bool pair, bool sum, void* stream)
+{
+    if (!ctx) return CYBQ_ERR_INVALID;
+    if (!w || (T && (!x || !y || !ids || (sum && !weights)))) return fail(ctx, CYBQ_ERR_INVALID, "w / x / ids / weights / y is NULL");
+    if (!dtype_ok(xdt) || !dtype_ok(ydt)) return fail(ctx, CYBQ_ERR_INVALID, "unknown dtype");
+    if (T < 0 || T > (1 << 24)) return fail(ctx, CYBQ_ERR_SHAPE, "T must be in 0..2^24");
+    if (E < 1 || E > CYBQ_MAX_EXPERTS) return fail(ctx, CYBQ_ERR_SHAPE, "E must be in 1..CYBQ_MAX_EXPERTS");
+    if (top_k < 1 || top_k > CYBQ_MAX_TOP_K) return fail(ctx, CYBQ_ERR_SHAPE, "top_k must be in 1..CYBQ_MAX_TOP_K");
+    if (w->device != ctx->device) return fail(ctx, CYBQ_ERR_INVALID, "weight lives on another device");
+    if (pair && !w->paired) return fail(ctx, CYBQ_ERR_INVALID, "CYBQ_EPI_SWIGLU needs a weight made by cybq_weight_fuse_pairs");
+    const int step = pair ? 32 : 16;
+    if (w->N % E || w->N / E % step)
+        return fail(ctx, CYBQ_ERR_SHAPE, "the weight must have E times a multiple of 16 rows (of gate and of up, for CYBQ_EPI_SWIGLU)");
+    if (!aligned16(x)) return fail(ctx, CYBQ_ERR_ALIGN, "x must be 16-byte aligned");
+    if (reinterpret_cast<uintptr_t>(y) % dtype_size(ydt) || reinterpret_cast<uintptr_t>(residual) % dtype_size(ydt))
+        return fail(ctx, CYBQ_ERR_ALIGN, "y / residual is not aligned to its element size");
+    if (reinterpret_cast<uintptr_t>(ids) % 4 || reinterpret_cast<uintptr_t>(weights) % 4)
+        return fail(ctx, CYBQ_ERR_ALIGN, "ids / weights is not aligned to its element size");
+    if (T == 0) return CYBQ_OK;
+    // tokens per round: their pairs' lists and (sum) sums in the scratch, their rows within the 32-bit offsets of the kernels
+    const int64_t n_out = w->N / E / (pair ? 2 : 1);
+    const size_t scratch = ctx->workspace_bytes - cybq::kDecodeScratchBytes;
+    const size_t row_bytes = (size_t)w->K * dtype_size(xdt) * (sum ? top_k : 1);
+    const size_t z_bytes = sum ? (size_t)top_k * n_out * sizeof(float) : 0;
+    int64_t round = std::min<int64_t>({T, 65535, ((int64_t)1 << 20) / top_k, (int64_t)(((size_t)1 << 32) / row_bytes) - 1});
+    if (z_bytes) round = std::min<int64_t>(round, (int64_t)((scratch - ((size_t)16 << 20)) / z_bytes));
+    if (round < 1) return fail(ctx, CYBQ_ERR_UNSUPPORTED, "one token's rows do not fit the scratch");
+    const size_t lists_bytes = cybq::experts_lists_bytes(round * top_k, (int)E);
+    DeviceGuard guard(ctx->device);
+    if (guard.err != hipSuccess) return fail_hip(ctx, guard.err, "hipSetDevice");
+    mark_use(w, stream);
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    const cybq::WeightView v = view_of(w);
+    char* const lists = static_cast<char*>(ctx->workspace);
+    float* const z = reinterpret_cast<float*>(lists + lists_bytes);
+    hipError_t e = hipSuccess;
+    for (int64_t t0 = 0; t0 < T && e == hipSuccess; t0 += round) {
+        const int64_t tokens = std::min(round, T - t0), pairs = tokens * top_k;
+        const int32_t* const my_ids = ids + t0 * top_k;
+        const char* const my_x = static_cast<const char*>(x) + (size_t)t0 * row_bytes;
+        const size_t row_out = (size_t)n_out * dtype_size(ydt);
+        char* const my_y = static_cast<char*>(y) + (size_t)t0 * (sum ? 1 : top_k) * row_out;
+        if (!sum) {
+            e = cybq::launch_experts(v, (int)E, pair, my_x, xdt, pairs, (int)top_k, my_ids, my_y, ydt, ctx->num_cus, lists, st);
+            continue;
+        }
+        e = cybq::launch_experts(v, (int)E, false, my_x, xdt, pairs, 1, my_ids, z, CYBQ_F32, ctx->num_cus, lists, st);
+        if (e == hipSuccess)
+            e = cybq::launch_experts_sum(z, my_ids, weights + t0 * top_k, residual ? static_cast<const char*>(residual) + (size_t)t0 * row_out : nullptr,
+                                         tokens, (int)top_k, (int)E, (int)n_out, my_y, ydt, st);
+    }
+    if (e != hipSuccess) return fail_hip(ctx, e, "experts launch");
+    return CYBQ_OK;
+}
+}  // namespace
+
+int cybq_matmul_experts(cybq_ctx* ctx, const cybq_weight* w, int64_t E, const void* x, cybq_dtype xdt, int64_t T, int64_t top_k, const int32_t* ids,
+                        void* y, cybq_dtype ydt, cybq_epilogue epilogue, void* stream)
+{
+    if (!ctx) return CYBQ_ERR_INVALID;
+    if (epilogue != CYBQ_EPI_NONE && epilogue != CYBQ_EPI_SWIGLU) return fail(ctx, CYBQ_ERR_INVALID, "cybq_matmul_experts takes CYBQ_EPI_NONE or CYBQ_EPI_SWIGLU");
+    return matmul_experts(ctx, w, E, x, xdt, T, top_k, ids, nullptr, nullptr, y, ydt, epilogue == CYBQ_EPI_SWIGLU, false, stream);
+}
+
+int cybq_matmul_experts_sum(cybq_ctx* ctx, const cybq_weight* w, int64_t E, const void* x, cybq_dtype xdt, int64_t T, int64_t top_k, const int32_t* ids,
+                            const float* weights, const void* residual, void* y, cybq_dtype ydt, void* stream)
+{
+    return matmul_experts(ctx, w, E, x, xdt, T, top_k, ids, weights, residual, y, ydt, false, true, stream);
 }
 
 int cybq_set_prefill_mode(cybq_ctx* ctx, cybq_prefill_mode mode)

@@ -95,6 +95,18 @@ bool gemm_rows_takes(const WeightView& w, int M, int num_cus, const Epilogue& ep
 hipError_t launch_quantize(int bits, const float* src, int N, int K, void* q_out, void* s_out,
                            hipStream_t st);
 
+// mixture of experts: the router (route.hip); score: 0 softmax, 1 sigmoid
+hipError_t launch_route(const void* logits, int ldt, int64_t T, int E, int top_k, int score, const float* bias, int groups, int top_groups,
+                        int group_best, bool renormalise, float scale, int32_t* ids, float* weights, hipStream_t st);
+// products of P pairs' rows with the weights of their experts (experts.hip): pair p is row p / xdiv of x and expert ids[p] of the E
+// stacked in w, out-of-range ids are left out.  lists: experts_lists_bytes of scratch
+size_t experts_lists_bytes(int64_t P, int E);
+hipError_t launch_experts(const WeightView& w, int E, bool pair, const void* x, int xdt, int64_t P, int xdiv, const int32_t* ids, void* y, int ydt,
+                          int num_cus, void* lists, hipStream_t st);
+// y[t] = residual[t] + sum_j weights[t, j] * z[t * top_k + j]
+hipError_t launch_experts_sum(const float* z, const int32_t* ids, const float* weights, const void* residual, int64_t T, int top_k, int E, int N, void* y,
+                              int ydt, hipStream_t st);
+
 // Kernels that need more dynamic LDS than the default 64 KB say so when the library is loaded:
 // naming LdsRequest<&kernel, bytes>::registered anywhere in a launcher puts the pair on a list
 // (a static initialiser, run before any call).  cybq_init walks the list for its device, so

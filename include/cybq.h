@@ -277,6 +277,54 @@ int cybq_matmul_many_norm(cybq_ctx* ctx, int64_t count, const cybq_weight* const
                           void* const* y, const int* epilogue, const void* const* residual,
                           cybq_dtype xdt, int64_t M, cybq_dtype ydt, void* stream);
 
+/* ---- mixture of experts --------------------------------------------------
+ *
+ * The FFN of a mixture-of-experts layer: a router chooses top_k of E experts per token, the token's row goes through
+ * those experts' gate / up and down projections, and the results are added with the router's weights.  The reference
+ * names no such model; formulas, entry points and limits are this library's choice.
+ *
+ * A stack of E experts is ONE weight of E * n rows (expert e is rows [e * n, (e + 1) * n)), uploaded like any other
+ * tensor; n must be a multiple of 16.  Gate and up of all experts: cybq_weight_fuse_pairs of the two stacks.
+ * ids[t * top_k + j] is the expert of pair (t, j), token t's j-th.  An id outside 0 .. E - 1 is no expert (the rows of a
+ * padded batch, experts that live elsewhere): nothing is read for it.  An expert may be named twice, by one token too.
+ * Limits: E <= CYBQ_MAX_EXPERTS, top_k <= CYBQ_MAX_TOP_K.  ids and weights are device memory; calls neither look at
+ * them on the host nor allocate, so they can be captured.  Like all calls they share the context's scratch: calls on
+ * one context (replays of its graphs too) must not overlap in time. */
+#define CYBQ_MAX_EXPERTS 1024
+#define CYBQ_MAX_TOP_K 64
+
+typedef enum cybq_score { CYBQ_SCORE_SOFTMAX = 0, CYBQ_SCORE_SIGMOID = 1 } cybq_score;
+
+/* The router, from its logits [T,E] (any dtype; T >= 0):
+ *     s = softmax_e(logits) or 1 / (1 + exp(-logits));   c = s + bias   (bias: [E], or NULL: c in the order of the logits)
+ *     E experts in `groups` runs of E / groups; a group's score is the sum of its group_best (1 or 2) largest c (s where
+ *     bias is NULL), the experts of the top_groups best groups stand for choice
+ *     ids[t, 0 .. top_k) = the largest c among them in falling order, of equal ones the lowest index first
+ *     weights[t, j] = s[ids[t, j]], divided by their sum over j if `renormalise`, times `scale`
+ * All in fp64, weights rounded once.  A logit of -inf or NaN scores 0 and is chosen after all others; logits of +inf
+ * share a softmax among them; a row without any score above 0 has weights of 0 (never NaN).  A bias of NaN counts as
+ * -inf.  top_k <= top_groups * (E / groups). */
+int cybq_route(cybq_ctx* ctx, const void* logits, cybq_dtype ldt, int64_t T, int64_t E, int64_t top_k, cybq_score score,
+               const float* bias, int64_t groups, int64_t top_groups, int group_best, int renormalise, float scale,
+               int32_t* ids, float* weights, void* stream);
+
+/* The rows of T tokens through their experts:  y[t * top_k + j, :] = epilogue(x[t, :] W_e^T), e = ids[t * top_k + j].
+ *   x [T,K] of xdt, 16-byte aligned; y [T * top_k, n] of ydt ([.., n / 2] with CYBQ_EPI_SWIGLU, w from
+ *   cybq_weight_fuse_pairs), must not overlap x.  CYBQ_EPI_ADD is not taken.  Rows of y without an expert stay as
+ *   they were.  T >= 0.  Operands are exact whatever the context's modes (integers q, the groups' scales in fp32 on
+ *   their sums, fp32 rows in three bf16 parts); |x| of bf16 and fp32 rows up to 4e34, as in the decode kernels: the row
+ *   of a larger element, Inf or NaN gives Inf or NaN, other rows are not touched by it. */
+int cybq_matmul_experts(cybq_ctx* ctx, const cybq_weight* w, int64_t E, const void* x, cybq_dtype xdt, int64_t T,
+                        int64_t top_k, const int32_t* ids, void* y, cybq_dtype ydt, cybq_epilogue epilogue, void* stream);
+
+/* The way back:  y[t, :] = residual[t, :] + sum_j weights[t * top_k + j] * (x[t * top_k + j, :] W_e^T), e = ids[t * top_k + j].
+ *   x [T * top_k, K]; weights fp32; residual [T, n] of ydt or NULL (zeros), may alias y; y [T, n], every row is
+ *   written.  Added in fp32 in the order of j, rounded once.  CYBQ_ERR_UNSUPPORTED where one token's top_k * n sums
+ *   do not fit the scratch. */
+int cybq_matmul_experts_sum(cybq_ctx* ctx, const cybq_weight* w, int64_t E, const void* x, cybq_dtype xdt, int64_t T,
+                            int64_t top_k, const int32_t* ids, const float* weights, const void* residual, void* y,
+                            cybq_dtype ydt, void* stream);
+
 /* Replaces: nothing the runtime calls per token; it is the verification hook
  * ("dequantised weights match bit-exactly"): out[N,K] f32 = f32(scale) * q. */
 int cybq_dequant(cybq_ctx* ctx, const cybq_weight* w, float* out, void* stream);

@@ -18,6 +18,8 @@ pub struct cybq_weight {
 }
 
 pub const CYBQ_GROUP: c_int = 32;
+pub const CYBQ_MAX_EXPERTS: c_int = 1024;
+pub const CYBQ_MAX_TOP_K: c_int = 64;
 
 // enum cybq_status
 pub const CYBQ_OK: c_int = 0;
@@ -49,6 +51,9 @@ pub const CYBQ_DECODE_EXACT: c_int = 1;
 pub const CYBQ_EPI_NONE: c_int = 0;
 pub const CYBQ_EPI_ADD: c_int = 1;
 pub const CYBQ_EPI_SWIGLU: c_int = 2;
+// enum cybq_score
+pub const CYBQ_SCORE_SOFTMAX: c_int = 0;
+pub const CYBQ_SCORE_SIGMOID: c_int = 1;
 
 extern "C" {
     pub fn cybq_init(device: c_int, out: *mut *mut cybq_ctx) -> c_int;
@@ -92,6 +97,19 @@ extern "C" {
                                  x: *const *const c_void, gamma: *const *const c_void, gdt: c_int, eps: c_float,
                                  y: *const *mut c_void, epilogue: *const c_int, residual: *const *const c_void,
                                  xdt: c_int, M: i64, ydt: c_int, stream: *mut c_void) -> c_int;
+    pub fn cybq_route(ctx: *mut cybq_ctx, logits: *const c_void, ldt: c_int, T: i64, E: i64,
+                      top_k: i64, score: c_int, bias: *const c_float, groups: i64,
+                      top_groups: i64, group_best: c_int, renormalise: c_int, scale: c_float,
+                      ids: *mut i32, weights: *mut c_float, stream: *mut c_void) -> c_int;
+    pub fn cybq_matmul_experts(ctx: *mut cybq_ctx, w: *const cybq_weight, E: i64,
+                               x: *const c_void, xdt: c_int, T: i64, top_k: i64,
+                               ids: *const i32, y: *mut c_void, ydt: c_int, epilogue: c_int,
+                               stream: *mut c_void) -> c_int;
+    pub fn cybq_matmul_experts_sum(ctx: *mut cybq_ctx, w: *const cybq_weight, E: i64,
+                                   x: *const c_void, xdt: c_int, T: i64, top_k: i64,
+                                   ids: *const i32, weights: *const c_float,
+                                   residual: *const c_void, y: *mut c_void, ydt: c_int,
+                                   stream: *mut c_void) -> c_int;
     pub fn cybq_dequant(ctx: *mut cybq_ctx, w: *const cybq_weight, out: *mut c_float, stream: *mut c_void) -> c_int;
     pub fn cybq_quantize(ctx: *mut cybq_ctx, quant: c_int, src: *const c_float, N: i64, K: i64, q_out: *mut c_void,
                          scales_out: *mut c_void, stream: *mut c_void) -> c_int;
