@@ -104,6 +104,7 @@ def load_library() -> ctypes.CDLL:
     lib.cybq_debug_set_gemm_tuning.argtypes = [ci]
     lib.cybq_debug_prefill_plan.argtypes = [vp, vp, ci, i64, ci, ci, ctypes.POINTER(ci)]
     lib.cybq_debug_set_gemv_tuning.argtypes = [ci, ci, ci]
+    lib.cybq_debug_set_experts_tuning.argtypes = [ci, ci, ci]
     lib.cybq_debug_read_weight.argtypes = [vp, i64, vp, ci, vp, vp, vp]
     lib.cybq_debug_read_pattern.argtypes = [vp, i64, vp, ci, vp]
     lib.cybq_debug_mfma_loop.argtypes = [vp, ci, ci, vp, vp]
@@ -451,6 +452,12 @@ class Backend:
         """cybq_route: logits [T, E] -> the experts ids [T, top_k] (int32) of every token and their weights (float32)."""
         if score not in SCORES:
             raise CybqError(-1, "invalid argument", f"unknown score {score!r}")
+        calls = _calls or _load_calls()
+        if calls:
+            rc = calls.route(self._addr, self.device, logits, ids, weights, SCORES[score], bias, groups, top_groups, group_best, renormalise,
+                             scale, stream)
+            if rc <= 0:
+                return self._check(rc)
         T, k = self._check_pairs(ids, weights)
         if logits.dim() != 2 or logits.shape[0] != T:
             raise CybqError(-2, "bad shape", f"logits must be [{T}, experts]")
@@ -468,6 +475,11 @@ class Backend:
         (epilogue "swiglu": fuse_pairs of the gate stack and the up stack).  Rows of y whose id is no expert stay."""
         if epilogue not in EPILOGUES:
             raise CybqError(-1, "invalid argument", f"unknown epilogue {epilogue!r}")
+        calls = _calls or _load_calls()
+        if calls:
+            rc = calls.experts(self._addr, self.device, w._addr, experts, x, ids, y, EPILOGUES[epilogue], stream)
+            if rc <= 0:
+                return self._check(rc)
         T, k = self._check_pairs(ids)
         n = w.N // max(experts, 1) // (2 if epilogue == "swiglu" else 1)
         self._check_tensor(x, "x", T * w.K)
@@ -477,6 +489,11 @@ class Backend:
 
     def matmul_experts_sum(self, w: QWeight, experts: int, x, ids, weights, y, residual=None, stream: int = 0) -> None:
         """cybq_matmul_experts_sum: y[t] = residual[t] + sum_j weights[t, j] * (x[t * top_k + j] W_e^T), e = ids[t, j]."""
+        calls = _calls or _load_calls()
+        if calls:
+            rc = calls.experts_sum(self._addr, self.device, w._addr, experts, x, ids, weights, y, residual, stream)
+            if rc <= 0:
+                return self._check(rc)
         T, k = self._check_pairs(ids, weights)
         n = w.N // max(experts, 1)
         self._check_tensor(x, "x", T * k * w.K)
@@ -590,6 +607,10 @@ class Backend:
         plan = (ctypes.c_int * 4)()
         self._check(self._lib.cybq_debug_prefill_plan(self._ctx, w.handle, xdt, M, 1 if norm else 0, EPILOGUES[epilogue], plan))
         return {"kernel": {1: "rows", 2: "tiles", 3: "roles", 4: "cols"}.get(plan[0]), "nf": plan[1], "splits": plan[2], "stage_rows": plan[3]}
+
+    def set_experts_tuning(self, cols: int = 0, many: int = 0, token: int = 0) -> None:
+        """Diagnostics: which kernels matmul_experts and matmul_experts_sum take (cybq_debug.h); 0 = automatic."""
+        self._check(self._lib.cybq_debug_set_experts_tuning(cols, many, token))
 
     def set_gemv_tuning(self, waves: int = 0, rows_kernel: int = 0, unroll: int = 0) -> None:
         """Diagnostics: waves per workgroup; decode kernel choice (0 auto, 1 always the

@@ -691,23 +691,44 @@ int matmul_experts(cybq_ctx* ctx, const cybq_weight* w, int64_t E, const void* x
     if (reinterpret_cast<uintptr_t>(ids) % 4 || reinterpret_cast<uintptr_t>(weights) % 4)
         return fail(ctx, CYBQ_ERR_ALIGN, "ids / weights is not aligned to its element size");
     if (T == 0) return CYBQ_OK;
-    // tokens per round: their pairs' lists and (sum) sums in the scratch, their rows within the 32-bit offsets of the kernels
-    const int64_t n_out = w->N / E / (pair ? 2 : 1);
-    const size_t scratch = ctx->workspace_bytes - cybq::kDecodeScratchBytes;
-    const size_t row_bytes = (size_t)w->K * dtype_size(xdt) * (sum ? top_k : 1);
-    const size_t z_bytes = sum ? (size_t)top_k * n_out * sizeof(float) : 0;
-    int64_t round = std::min<int64_t>({T, 65535, ((int64_t)1 << 20) / top_k, (int64_t)(((size_t)1 << 32) / row_bytes) - 1});
-    if (z_bytes) round = std::min<int64_t>(round, (int64_t)((scratch - ((size_t)16 << 20)) / z_bytes));
-    if (round < 1) return fail(ctx, CYBQ_ERR_UNSUPPORTED, "one token's rows do not fit the scratch");
-    const size_t lists_bytes = cybq::experts_lists_bytes(round * top_k, (int)E);
     DeviceGuard guard(ctx->device);
     if (guard.err != hipSuccess) return fail_hip(ctx, guard.err, "hipSetDevice");
-    mark_use(w, stream);
     hipStream_t st = static_cast<hipStream_t>(stream);
     const cybq::WeightView v = view_of(w);
-    char* const lists = static_cast<char*>(ctx->workspace);
-    float* const z = reinterpret_cast<float*>(lists + lists_bytes);
     hipError_t e = hipSuccess;
+    // operands rounded to f16 (2e-4 relative L2) only where y is rounded to bf16 (1.6e-3) anyway
+    bool fast = ydt == CYBQ_BF16 && !ctx->prefill_exact && cybq::experts_many(v, (int)E, xdt, T * top_k);
+    if (fast) {
+        bool wide = false;
+        e = weight_is_wide(w, &wide);
+        if (e != hipSuccess) return fail_hip(ctx, e, "scale scan");
+        fast = !wide;
+    }
+    mark_use(w, stream);
+    // tokens per round: their pairs' lists, staged rows and (sum) sums in the scratch, their rows within the 32-bit offsets of the kernels
+    const int64_t n_out = w->N / E / (pair ? 2 : 1), x_rows = sum ? top_k : 1;
+    const size_t scratch = ctx->workspace_bytes - cybq::kDecodeScratchBytes - ((size_t)16 << 20);
+    const size_t row_bytes = (size_t)w->K * dtype_size(xdt) * x_rows;
+    const bool staged = fast && xdt == CYBQ_BF16;
+    const size_t token_bytes = (staged ? row_bytes + x_rows * 4 : 0) + (sum ? (size_t)top_k * n_out * sizeof(float) : 0);
+    int64_t round = std::min<int64_t>({T, 65535, ((int64_t)1 << 20) / top_k, (int64_t)(((size_t)1 << 32) / row_bytes) - 1});
+    if (token_bytes) round = std::min<int64_t>(round, (int64_t)(scratch / token_bytes));
+    // the way back without sums in memory: few tokens, or a token whose sums do not fit
+    if (sum && (cybq::experts_sum_by_token(v, (int)E, T, (int)top_k) || (round < 1 && cybq::experts_token_serves(v)))) {
+        for (int64_t t0 = 0, tokens; t0 < T && e == hipSuccess; t0 += tokens) {
+            tokens = std::min<int64_t>(T - t0, 65535);
+            const size_t at = (size_t)t0 * n_out * dtype_size(ydt);
+            e = cybq::launch_experts_token(v, (int)E, static_cast<const char*>(x) + (size_t)t0 * row_bytes, xdt, tokens, (int)top_k, ids + t0 * top_k,
+                                           weights + t0 * top_k, residual ? static_cast<const char*>(residual) + at : nullptr,
+                                           static_cast<char*>(y) + at, ydt, st);
+        }
+        if (e != hipSuccess) return fail_hip(ctx, e, "experts launch");
+        return CYBQ_OK;
+    }
+    if (round < 1) return fail(ctx, CYBQ_ERR_UNSUPPORTED, "one token's rows do not fit the scratch");
+    char* const lists = static_cast<char*>(ctx->workspace);
+    char* const stage = lists + cybq::experts_lists_bytes(round * top_k, (int)E);
+    float* const z = reinterpret_cast<float*>(stage + (staged ? cybq::experts_stage_bytes(round * x_rows, (int)w->K) : 0));
     for (int64_t t0 = 0; t0 < T && e == hipSuccess; t0 += round) {
         const int64_t tokens = std::min(round, T - t0), pairs = tokens * top_k;
         const int32_t* const my_ids = ids + t0 * top_k;
@@ -715,10 +736,10 @@ int matmul_experts(cybq_ctx* ctx, const cybq_weight* w, int64_t E, const void* x
         const size_t row_out = (size_t)n_out * dtype_size(ydt);
         char* const my_y = static_cast<char*>(y) + (size_t)t0 * (sum ? 1 : top_k) * row_out;
         if (!sum) {
-            e = cybq::launch_experts(v, (int)E, pair, my_x, xdt, pairs, (int)top_k, my_ids, my_y, ydt, ctx->num_cus, lists, st);
+            e = cybq::launch_experts(v, (int)E, pair, my_x, xdt, pairs, (int)top_k, (int)top_k, my_ids, my_y, ydt, ctx->num_cus, fast, lists, stage, st);
             continue;
         }
-        e = cybq::launch_experts(v, (int)E, false, my_x, xdt, pairs, 1, my_ids, z, CYBQ_F32, ctx->num_cus, lists, st);
+        e = cybq::launch_experts(v, (int)E, false, my_x, xdt, pairs, (int)top_k, 1, my_ids, z, CYBQ_F32, ctx->num_cus, fast, lists, stage, st);
         if (e == hipSuccess)
             e = cybq::launch_experts_sum(z, my_ids, weights + t0 * top_k, residual ? static_cast<const char*>(residual) + (size_t)t0 * row_out : nullptr,
                                          tokens, (int)top_k, (int)E, (int)n_out, my_y, ydt, st);
@@ -852,6 +873,13 @@ int cybq_debug_prefill_plan(cybq_ctx* ctx, const cybq_weight* w, cybq_dtype xdt,
     plan[1] = r.nf;
     plan[2] = r.splits;
     plan[3] = r.stage_rows;
+    return CYBQ_OK;
+}
+
+int cybq_debug_set_experts_tuning(int cols, int many, int token)
+{
+    if ((cols != 0 && cols != 1 && cols != 2 && cols != 4 && cols != 8) || many < 0 || token < 0 || token > 2) return CYBQ_ERR_INVALID;
+    cybq::set_experts_tuning(cols, many, token);
     return CYBQ_OK;
 }
 

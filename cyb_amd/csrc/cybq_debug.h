@@ -70,6 +70,11 @@ int cybq_debug_mfma_loop(cybq_ctx* ctx, int waves_per_simd, int iters, float* si
  * Bytes into the CUs = CUs * bytes * iters. */
 int cybq_debug_cache_read(cybq_ctx* ctx, const void* buf, int64_t bytes, int waves, int in_flight, int iters, void* stream);
 
+/* Which kernels the products of a mixture of experts take.  cols: waves side by side with few rows to an expert (1, 2, 4, 8).
+ * many: pairs per expert that is met from which the kernel for many rows takes the call.  token: 1 the way back always token by token,
+ * 2 never.  0 = automatic. */
+int cybq_debug_set_experts_tuning(int cols, int many, int token);
+
 #ifdef __cplusplus
 }
 #endif

@@ -99,10 +99,21 @@ hipError_t launch_quantize(int bits, const float* src, int N, int K, void* q_out
 hipError_t launch_route(const void* logits, int ldt, int64_t T, int E, int top_k, int score, const float* bias, int groups, int top_groups,
                         int group_best, bool renormalise, float scale, int32_t* ids, float* weights, hipStream_t st);
 // products of P pairs' rows with the weights of their experts (experts.hip): pair p is row p / xdiv of x and expert ids[p] of the E
-// stacked in w, out-of-range ids are left out.  lists: experts_lists_bytes of scratch
+// stacked in w, out-of-range ids are left out.  fast: where there are many rows to an expert, operands round_f16(scale * q) (w's scales are
+// not wide).  lists: experts_lists_bytes of scratch; stage: experts_stage_bytes for the rows of x, where experts_many, fast and bf16 rows
+bool experts_many(const WeightView& w, int E, int xdt, int64_t P);
 size_t experts_lists_bytes(int64_t P, int E);
-hipError_t launch_experts(const WeightView& w, int E, bool pair, const void* x, int xdt, int64_t P, int xdiv, const int32_t* ids, void* y, int ydt,
-                          int num_cus, void* lists, hipStream_t st);
+size_t experts_stage_bytes(int64_t rows, int K);
+hipError_t launch_experts(const WeightView& w, int E, bool pair, const void* x, int xdt, int64_t P, int top_k, int xdiv, const int32_t* ids, void* y, int ydt,
+                          int num_cus, bool fast, void* lists, void* stage, hipStream_t st);
+// few tokens: y[t] = residual[t] + sum_j weights[t, j] * (x[t * top_k + j] W_ids[t, j]^T) in one launch, without scratch
+bool experts_token_serves(const WeightView& w);                  // whether it can (K up to 524288; up to 65535 tokens)
+bool experts_sum_by_token(const WeightView& w, int E, int64_t T, int top_k);       // whether it is the quicker way
+hipError_t launch_experts_token(const WeightView& w, int E, const void* x, int xdt, int64_t T, int top_k, const int32_t* ids, const float* weights,
+                                const void* residual, void* y, int ydt, hipStream_t st);
+// test/bench hook: waves side by side with few rows to an expert (1, 2, 4, 8), pairs per expert from which there are many, the way back
+// token by token (1) or with sums in memory (2); 0 = automatic
+void set_experts_tuning(int cols, int many, int token);
 // y[t] = residual[t] + sum_j weights[t, j] * z[t * top_k + j]
 hipError_t launch_experts_sum(const float* z, const int32_t* ids, const float* weights, const void* residual, int64_t T, int top_k, int E, int N, void* y,
                               int ydt, hipStream_t st);

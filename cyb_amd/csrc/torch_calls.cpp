@@ -1,4 +1,5 @@
-// torch_calls.cpp - the Python binding's call path for torch tensors: Backend.matmul / matmul_ex / matmul_norm / matmul_static.
+// torch_calls.cpp - the Python binding's call path for torch tensors: Backend.matmul / matmul_ex / matmul_norm / matmul_static,
+// route / matmul_experts / matmul_experts_sum.
 //
 // A small linear is bound by the host: the launch itself takes 2.9 us of host time, the kernel behind it less.  Looking
 // the tensors over in Python (shape, device, contiguity, type, address: a dozen attribute calls) and going through
@@ -165,7 +166,112 @@ PyObject* matmul_fused(PyObject* const* a, Py_ssize_t n)
     return answer(rc);
 }
 
+// a contiguous [T, k] tensor of one type on the device -> its address
+void* matrix(PyObject* o, int device, at::ScalarType type, int64_t* rows, int64_t* cols)
+{
+    if (!THPVariable_CheckExact(o)) return nullptr;
+    const at::Tensor& t = THPVariable_Unpack(o);
+    if (!t.is_cuda() || t.get_device() != device || t.dim() != 2 || t.scalar_type() != type || !t.is_contiguous() || t.numel() == 0) return nullptr;
+    *rows = t.size(0);
+    *cols = t.size(1);
+    return t.data_ptr();
+}
+
+// route(ctx, device, logits, ids, weights, score, bias or None, groups, top_groups or None, group_best, renormalise, scale, stream)
+PyObject* route(PyObject* const* a, Py_ssize_t n)
+{
+    int64_t ctx, device, score, groups, top_groups, best, stream, T, k, T2, k2;
+    if (n != 13 || !as_int(a[0], &ctx) || !ctx || !as_int(a[1], &device) || !as_int(a[5], &score) || !as_int(a[7], &groups) || !as_int(a[9], &best) ||
+        !as_int(a[12], &stream) || !PyBool_Check(a[10]) || !PyFloat_CheckExact(a[11]))
+        return answer(kSlow);
+    top_groups = groups;
+    if (a[8] != Py_None && !as_int(a[8], &top_groups)) return answer(kSlow);
+    void* ids = matrix(a[3], (int)device, at::kInt, &T, &k);
+    if (!ids) return answer(kSlow);
+    void* weights = matrix(a[4], (int)device, at::kFloat, &T2, &k2);
+    if (!weights || T2 != T || k2 != k || !THPVariable_CheckExact(a[2])) return answer(kSlow);
+    const at::Tensor& z = THPVariable_Unpack(a[2]);
+    if (z.dim() != 2 || z.size(0) != T) return answer(kSlow);
+    const int64_t E = z.size(1);
+    int ldt = 0, bdt = CYBQ_F32;
+    void* logits = address(a[2], (int)device, T * E, &ldt);
+    void* bias = nullptr;
+    if (!logits || (a[6] != Py_None && !(bias = address(a[6], (int)device, E, &bdt))) || bdt != CYBQ_F32) return answer(kSlow);
+    int rc;
+    {
+        Unlocked u;
+        rc = cybq_route(reinterpret_cast<cybq_ctx*>(static_cast<uintptr_t>(ctx)), logits, (cybq_dtype)ldt, T, E, k, (cybq_score)score,
+                        static_cast<const float*>(bias), groups, top_groups, (int)best, a[10] == Py_True, (float)PyFloat_AS_DOUBLE(a[11]),
+                        static_cast<int32_t*>(ids), static_cast<float*>(weights), reinterpret_cast<void*>(static_cast<uintptr_t>(stream)));
+    }
+    return answer(rc);
+}
+
+// what matmul_experts and matmul_experts_sum share: ctx, device, weight address, experts, ids, stream
+struct Pairs {
+    cybq_ctx* ctx;
+    const cybq_weight* w;
+    int64_t device, E, T, k, N = 0, K = 0;
+    int32_t* ids;
+    void* stream;
+};
+
+bool pairs_of(PyObject* const* a, PyObject* ids, PyObject* stream, Pairs* r)
+{
+    int64_t ctx, w, st;
+    if (!as_int(a[0], &ctx) || !as_int(a[1], &r->device) || !as_int(a[2], &w) || !as_int(a[3], &r->E) || !as_int(stream, &st) || !ctx || !w || r->E < 1) return false;
+    r->ctx = reinterpret_cast<cybq_ctx*>(static_cast<uintptr_t>(ctx));
+    r->w = reinterpret_cast<const cybq_weight*>(static_cast<uintptr_t>(w));
+    r->stream = reinterpret_cast<void*>(static_cast<uintptr_t>(st));
+    r->ids = static_cast<int32_t*>(matrix(ids, (int)r->device, at::kInt, &r->T, &r->k));
+    return r->ids && cybq_weight_info(r->w, nullptr, &r->N, &r->K, nullptr) == CYBQ_OK;
+}
+
+// experts(ctx, device, w, experts, x, ids, y, epilogue, stream)
+PyObject* experts(PyObject* const* a, Py_ssize_t n)
+{
+    Pairs r;
+    int64_t epi;
+    if (n != 9 || !pairs_of(a, a[5], a[8], &r) || !as_int(a[7], &epi)) return answer(kSlow);
+    int xdt = 0, ydt = 0;
+    void* x = address(a[4], (int)r.device, r.T * r.K, &xdt);
+    void* y = address(a[6], (int)r.device, r.T * r.k * (r.N / r.E / (epi == CYBQ_EPI_SWIGLU ? 2 : 1)), &ydt);
+    if (!x || !y) return answer(kSlow);
+    int rc;
+    {
+        Unlocked u;
+        rc = cybq_matmul_experts(r.ctx, r.w, r.E, x, (cybq_dtype)xdt, r.T, r.k, r.ids, y, (cybq_dtype)ydt, (cybq_epilogue)epi, r.stream);
+    }
+    return answer(rc);
+}
+
+// experts_sum(ctx, device, w, experts, x, ids, weights, y, residual or None, stream)
+PyObject* experts_sum(PyObject* const* a, Py_ssize_t n)
+{
+    Pairs r;
+    int64_t T, k;
+    if (n != 10 || !pairs_of(a, a[5], a[9], &r)) return answer(kSlow);
+    void* weights = matrix(a[6], (int)r.device, at::kFloat, &T, &k);
+    if (!weights || T != r.T || k != r.k) return answer(kSlow);
+    int xdt = 0, ydt = 0, rdt = 0;
+    void* x = address(a[4], (int)r.device, r.T * r.k * r.K, &xdt);
+    void* y = address(a[7], (int)r.device, r.T * (r.N / r.E), &ydt);
+    void* residual = nullptr;
+    if (!x || !y) return answer(kSlow);
+    if (a[8] != Py_None && (!(residual = address(a[8], (int)r.device, r.T * (r.N / r.E), &rdt)) || rdt != ydt)) return answer(kSlow);
+    int rc;
+    {
+        Unlocked u;
+        rc = cybq_matmul_experts_sum(r.ctx, r.w, r.E, x, (cybq_dtype)xdt, r.T, r.k, r.ids, static_cast<const float*>(weights), residual, y,
+                                     (cybq_dtype)ydt, r.stream);
+    }
+    return answer(rc);
+}
+
 PyMethodDef kMethods[] = {
+    {"route", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(entry<route>)), METH_FASTCALL, nullptr},
+    {"experts", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(entry<experts>)), METH_FASTCALL, nullptr},
+    {"experts_sum", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(entry<experts_sum>)), METH_FASTCALL, nullptr},
     {"matmul", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(entry<matmul>)), METH_FASTCALL, nullptr},
     {"matmul_static", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(entry<matmul_static>)), METH_FASTCALL, nullptr},
     {"matmul_fused", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(entry<matmul_fused>)), METH_FASTCALL, nullptr},

@@ -319,8 +319,8 @@ int cybq_matmul_experts(cybq_ctx* ctx, const cybq_weight* w, int64_t E, const vo
 
 /* The way back:  y[t, :] = residual[t, :] + sum_j weights[t * top_k + j] * (x[t * top_k + j, :] W_e^T), e = ids[t * top_k + j].
  *   x [T * top_k, K]; weights fp32; residual [T, n] of ydt or NULL (zeros), may alias y; y [T, n], every row is
- *   written.  Added in fp32 in the order of j, rounded once.  CYBQ_ERR_UNSUPPORTED where one token's top_k * n sums
- *   do not fit the scratch. */
+ *   written.  Added in fp32 in a fixed order, rounded once.  CYBQ_ERR_UNSUPPORTED for K over 524288 where one token's
+ *   top_k * n sums do not fit the scratch. */
 int cybq_matmul_experts_sum(cybq_ctx* ctx, const cybq_weight* w, int64_t E, const void* x, cybq_dtype xdt, int64_t T,
                             int64_t top_k, const int32_t* ids, const float* weights, const void* residual, void* y,
                             cybq_dtype ydt, void* stream);
