@@ -697,7 +697,7 @@ int matmul_experts(cybq_ctx* ctx, const cybq_weight* w, int64_t E, const void* x
     const cybq::WeightView v = view_of(w);
     hipError_t e = hipSuccess;
     // operands rounded to f16 (2e-4 relative L2) only where y is rounded to bf16 (1.6e-3) anyway
-    bool fast = ydt == CYBQ_BF16 && !ctx->prefill_exact && cybq::experts_many(v, (int)E, xdt, T * top_k);
+    bool fast = ydt == CYBQ_BF16 && !ctx->prefill_exact && cybq::experts_many(v, (int)E, xdt, T * top_k, true);
     if (fast) {
         bool wide = false;
         e = weight_is_wide(w, &wide);

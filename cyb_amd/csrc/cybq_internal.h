@@ -101,7 +101,7 @@ hipError_t launch_route(const void* logits, int ldt, int64_t T, int E, int top_k
 // products of P pairs' rows with the weights of their experts (experts.hip): pair p is row p / xdiv of x and expert ids[p] of the E
 // stacked in w, out-of-range ids are left out.  fast: where there are many rows to an expert, operands round_f16(scale * q) (w's scales are
 // not wide).  lists: experts_lists_bytes of scratch; stage: experts_stage_bytes for the rows of x, where experts_many, fast and bf16 rows
-bool experts_many(const WeightView& w, int E, int xdt, int64_t P);
+bool experts_many(const WeightView& w, int E, int xdt, int64_t P, bool fast);
 size_t experts_lists_bytes(int64_t P, int E);
 size_t experts_stage_bytes(int64_t rows, int K);
 hipError_t launch_experts(const WeightView& w, int E, bool pair, const void* x, int xdt, int64_t P, int top_k, int xdiv, const int32_t* ids, void* y, int ydt,

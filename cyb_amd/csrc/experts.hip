@@ -1088,9 +1088,9 @@ void set_experts_tuning(int cols, int many, int token) { g_tuning = {cols, many,
 
 size_t experts_lists_bytes(int64_t P, int E) { return ((size_t)(lists_order_at(P, E) + P) * 4 + 255) / 256 * 256; }
 
-bool experts_many(const WeightView& w, int E, int xdt, int64_t P)
+bool experts_many(const WeightView& w, int E, int xdt, int64_t P, bool fast)
 {
-    const int thr = g_tuning.many ? g_tuning.many : 16;
+    const int thr = g_tuning.many ? g_tuning.many : w.bits == 8 ? 20 : fast ? 24 : 40;
     return xdt != kF32 && P >= thr * std::min<int64_t>(P, E);
 }
 
@@ -1101,7 +1101,7 @@ hipError_t launch_experts(const WeightView& w, int E, bool pair, const void* x, 
 {
     const int strips = w.NT / E, n_out = strips * 16 / (pair ? 2 : 1);
     const int64_t met = std::min<int64_t>(P, E);
-    const bool many = experts_many(w, E, xdt, P);
+    const bool many = experts_many(w, E, xdt, P, fast);
     int32_t* const L = static_cast<int32_t*>(lists);
     const bool listed = many || P > kMaxDirect;
     const int op = fast ? 2 : xdt == kF16 ? 0 : 1;
