@@ -668,26 +668,26 @@ __device__ __forceinline__ void many_tile(const ExpertsArgs& g, int e, const int
     const uint8_t* const wsrc = g.w + ((int64_t)e * g.strips + strip) * g.KT * kTileBytes<BITS>;
     const uint32_t wstep = (uint32_t)(second - strip) * (uint32_t)(g.KT * kTileBytes<BITS>);
     const uint32_t q_off = (uint32_t)lane * 16u, sc_off = (lane >= 8 ? wstep : 0u) + (uint32_t)(kTileQBytes<BITS> + (lane & 7) * 16);
-    // (workgroups that share rows start at different K tiles: they would ask the same channels of the L2 for the same lines at the same moment)
     const int whole = G / 4;
-    const int turn = 0;
-    auto copy = [&](int step, int buf) {
-        const int kt = step < whole ? (step + turn < whole ? step + turn : step + turn - whole) : min(step, g.KT - 1);
-        const uint32_t at = (uint32_t)(buf * S::STEP);
-        const uint32_t from = (uint32_t)min(kt * 4 + (wave & 1) * 2 + (piece >> 2), G - 1) * 64u + (uint32_t)(piece & 3) * 16u;   // (past the end of a row: its last group)
-#pragma unroll
-        for (int c = 0; c < S::XC; c++) copy_to_lds(at + xblk[c] * 1024, g.x, xoff[c] + from);
-        const uint8_t* const src = wsrc + (int64_t)kt * kTileBytes<BITS>;
-        const uint32_t wat = at + S::XTILE + wave * S::WTILE;
-#pragma unroll
-        for (int q = 0; q < BITS / 4; q++) {
-            copy_to_lds(wat + q * 1024, src + q * 1024, q_off);
-            copy_to_lds(wat + S::WQ + q * 1024, src + wstep + q * 1024, q_off);
+    // piece c of step `step`: the words, which come from further away, the scales, the rows' blocks
+    constexpr int PIECES = S::XC + S::WC;
+    auto copy_piece = [&](auto c_, int step, int buf) {
+        constexpr int c = decltype(c_)::value;
+        const int kt = min(step, g.KT - 1);
+        const uint32_t at = (uint32_t)(buf * S::STEP), wat = at + S::XTILE + wave * S::WTILE;
+        if constexpr (c + 1 < S::WC) {
+            constexpr int q = c / 2, second_strip = c % 2;
+            copy_to_lds(wat + second_strip * S::WQ + q * 1024, wsrc + (int64_t)kt * kTileBytes<BITS> + (second_strip ? wstep : 0u) + q * 1024, q_off);
+        } else if constexpr (c < S::WC) {
+            copy_lanes_to_lds(wat + 2 * S::WQ, wsrc + (int64_t)kt * kTileBytes<BITS>, sc_off, 0xffffull);
+        } else {
+            constexpr int block = c - S::WC;
+            const uint32_t from = (uint32_t)min(kt * 4 + (wave & 1) * 2 + (piece >> 2), G - 1) * 64u + (uint32_t)(piece & 3) * 16u;   // (past the end of a row: its last group)
+            copy_to_lds(at + xblk[block] * 1024, g.x, xoff[block] + from);
         }
-        copy_lanes_to_lds(wat + 2 * S::WQ, src, sc_off, 0xffffull);
     };
 #pragma unroll
-    for (int d = 0; d < D - 1; d++) copy(d, d);
+    for (int d = 0; d < D - 1; d++) static_for<0, PIECES>([&](auto c_) { copy_piece(c_, d, d); });
 
     float4_t acc[RB][CS];
 #pragma unroll
@@ -750,14 +750,14 @@ __device__ __forceinline__ void many_tile(const ExpertsArgs& g, int e, const int
         b.u[k] = v;
     };
     Words w[2];
-    Frag16 b[2][CS], a[3];
+    Frag16 b[2][CS], a[4];
     float4_t d[3], bias[2];                                      // exact operands: products on their way to the sums
     int buf = 0;
     auto read_a = [&](Frag16& f, const uint8_t* at, int i, int j) { f.u = *reinterpret_cast<const u32x4_t*>(at + i * 4096 + (j ? raw ^ 64u : raw)); };
     constexpr int MMAS = RB * CS;
-    // Group J of a step's two: the products of the operands b[J] with all rows, in an order that is kept: between the MFMAs the rows' operands two
+    // Group J of a step's two: the products of the operands b[J] with all rows, in an order that is kept: between the MFMAs the rows' operands three
     // row blocks ahead, the words of the next group's operands (`next`: of this step's or the next one's words), a row block at a time.
-    auto group = [&](auto j_, const uint8_t* at, const uint8_t* at_next, const Words& now, const Words& next) {
+    auto group = [&](auto j_, const uint8_t* at, const uint8_t* at_next, const Words& now, const Words& next, int copy_step, int free) {
         constexpr int J = decltype(j_)::value;
         auto scaled = [&](auto m_) {
             constexpr int m = decltype(m_)::value, i = m / CS, s = m % CS;
@@ -768,17 +768,17 @@ __device__ __forceinline__ void many_tile(const ExpertsArgs& g, int e, const int
         static_for<0, MMAS>([&](auto m_) {
             constexpr int m = decltype(m_)::value, i = m / CS, s = m % CS;
             if constexpr (s == 0) {
-                if constexpr (i + 2 < RB) read_a(a[(i + 2) % 3], at, i + 2, J);
+                if constexpr (i + 3 < RB) read_a(a[(i + 3) % 4], at, i + 3, J);
             }
             if constexpr (OP == 2) {
-                acc[i][s] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i % 3].h, b[J][s].h, acc[i][s], 0, 0, 0);
+                acc[i][s] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i % 4].h, b[J][s].h, acc[i][s], 0, 0, 0);
             } else if constexpr (OP == 0) {
-                d[m % 3] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i % 3].h, b[J][s].h, (float4_t){0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+                d[m % 3] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i % 4].h, b[J][s].h, (float4_t){0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
             } else {
                 if constexpr (s == 0 && i == 0) bias[0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[0].b, off.b, (float4_t){0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
-                d[m % 3] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i % 3].b, b[J][s].b, bias[i & 1], 0, 0, 0);
+                d[m % 3] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i % 4].b, b[J][s].b, bias[i & 1], 0, 0, 0);
                 if constexpr (s == 2 && i + 1 < RB)
-                    bias[(i + 1) & 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[(i + 1) % 3].b, off.b, (float4_t){0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+                    bias[(i + 1) & 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[(i + 1) % 4].b, off.b, (float4_t){0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
             }
             if constexpr (OP != 2 && m >= 2) scaled(std::integral_constant<int, (m >= 2 ? m - 2 : 0)>{});
             // the next group's words: from LDS since the first row block, so behind it where there are more
@@ -788,15 +788,19 @@ __device__ __forceinline__ void many_tile(const ExpertsArgs& g, int e, const int
 #pragma unroll
                 for (int k = lo; k < hi; k++) operand_word(b[1 - J][k >> 2], next, k >> 2, 1 - J, k & 3);
             }
+            // the copies spread out: all at once behind the barrier they held up the MFMAs behind them until the address unit had taken
+            // them in (1024 rows on 8 experts of 4096 -> 14336: 560 us)
+            if constexpr (J == 1) static_for<m * PIECES / MMAS, (m + 1) * PIECES / MMAS>([&](auto c_) { copy_piece(c_, copy_step, free); });
             if constexpr (s == CS - 1) __builtin_amdgcn_sched_barrier(0);
         });
         if constexpr (OP != 2) {
             scaled(std::integral_constant<int, (MMAS >= 2 ? MMAS - 2 : 0)>{});
             scaled(std::integral_constant<int, MMAS - 1>{});
         }
-        // the first two row blocks of what follows
+        // the first three row blocks of what follows
         read_a(a[0], at_next, 0, 1 - J);
         if constexpr (RB > 1) read_a(a[1], at_next, 1, 1 - J);
+        if constexpr (RB > 2) read_a(a[2], at_next, 2, 1 - J);
     };
     // One barrier per step, in its middle.  Ahead of it the first group's products, whose operands are there; behind it the next step's copies
     // are in LDS and the last step's place is free.
@@ -804,6 +808,7 @@ __device__ __forceinline__ void many_tile(const ExpertsArgs& g, int e, const int
     read_words(w[0], smem);
     read_a(a[0], smem, 0, 0);
     if constexpr (RB > 1) read_a(a[1], smem, 1, 0);
+    if constexpr (RB > 2) read_a(a[2], smem, 2, 0);
 #pragma unroll
     for (int s = 0; s < CS; s++)
 #pragma unroll
@@ -813,11 +818,11 @@ __device__ __forceinline__ void many_tile(const ExpertsArgs& g, int e, const int
         const int free = buf == 0 ? D - 1 : buf - 1;
         buf = buf + 1 == D ? 0 : buf + 1;
         const uint8_t* const at_next = smem + buf * S::STEP;
-        if (first) group(std::integral_constant<int, 0>{}, at, at, now, now);
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((D - 3) * (S::XC + S::WC)) : "memory");
+        if (first) group(std::integral_constant<int, 0>{}, at, at, now, now, 0, 0);
+        // (no wait for reads of LDS: those on their way are of this step's place, the last step's went into MFMAs ahead of here)
+        asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((D - 3) * (S::XC + S::WC)) : "memory");
         read_words(next, at_next);
-        copy(step + D - 1, free);
-        if (second) group(std::integral_constant<int, 1>{}, at, at_next, now, next);
+        if (second) group(std::integral_constant<int, 1>{}, at, at_next, now, next, step + D - 1, free);
     };
     // (whole K tiles by themselves: a body that may end early costs a move of every sum per step)
     int step = 0;
