@@ -258,8 +258,8 @@ __device__ __forceinline__ void split_f32(const u32x4_t& lo, const u32x4_t& hi, 
 }
 
 // Strips strip0 + 2 col, + 1 of expert e against the pairs list[0 .. n), n <= 8 * XB.
-template <int BITS, int XM, bool PAIR, int XB, int COLS, int BUDGET, class List>
-__device__ __forceinline__ void expert_tile(const ExpertsArgs& g, int e, List list, int n, int strip0, uint8_t* smem)
+template <int BITS, int XM, bool PAIR, int XB, int COLS, int BUDGET>
+__device__ __forceinline__ void expert_tile(const ExpertsArgs& g, int e, const int32_t* list, int n, int strip0, uint8_t* smem)
 {
     using S = Shape<BITS, XM, XB, COLS, BUDGET>;
     constexpr int D = S::D, RB = S::RB, KH = S::KH, OPM = XM == XF16 ? XF16 : XBF16;
@@ -935,15 +935,16 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(4, 4))) voi
 {
     // (the copies count LDS addresses from zero: these kernels have no static LDS)
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
-    uint16_t* const rows = reinterpret_cast<uint16_t*>(smem + few_ring<BITS, XM, COLS>());
+    int32_t* const rows = reinterpret_cast<int32_t*>(smem + few_ring<BITS, XM, COLS>());          // the pairs of the expert, kMaxDirect at a time
     const int lane = threadIdx.x & 63, slot = blockIdx.y, strip0 = blockIdx.x * (2 * COLS);
     const int e = __builtin_amdgcn_readfirstlane(g.by_pair ? g.ids[slot] : slot);
     if ((unsigned)e >= (unsigned)g.E) return;
-    auto all = [&](auto list, int n) {
+    auto all = [&](int n) {
+        const int32_t* const list = rows;
         for (int r0 = 0; r0 < n;) {
             if (r0) __syncthreads();
             if (n - r0 == 1) {
-                expert_row<BITS, XM, PAIR, COLS>(g, e, __builtin_amdgcn_readfirstlane((int)list[r0]), strip0, smem);
+                expert_row<BITS, XM, PAIR, COLS>(g, e, __builtin_amdgcn_readfirstlane(list[r0]), strip0, smem);
                 r0 += 1;
                 continue;
             }
@@ -958,27 +959,33 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(4, 4))) voi
         }
     };
     if (g.lists) {
-        const int a = __builtin_amdgcn_readfirstlane(g.lists[e]);
-        all(g.lists + lists_order_at(g.P, g.E) + a, __builtin_amdgcn_readfirstlane(g.lists[e + 1]) - a);
+        const int a = __builtin_amdgcn_readfirstlane(g.lists[e]), n = __builtin_amdgcn_readfirstlane(g.lists[e + 1]) - a;
+        const int32_t* const order = g.lists + lists_order_at(g.P, g.E) + a;
+        for (int r = 0; r < n; r += kMaxDirect) {
+            if (r) __syncthreads();
+            if (r + (int)threadIdx.x < n) rows[threadIdx.x] = order[r + threadIdx.x];
+            __syncthreads();
+            all(min(n - r, kMaxDirect));
+        }
         return;
     }
     // the expert's pairs among the ids; every wave looks for itself
     int n = 0, first = -1;
     if (g.single) {
         n = 1;
-        if (threadIdx.x == 0) rows[0] = (uint16_t)slot;
+        if (threadIdx.x == 0) rows[0] = slot;
     } else {
         for (int p0 = 0; p0 < (int)g.P; p0 += 64) {
             const bool mine = p0 + lane < (int)g.P && g.ids[p0 + lane] == e;
             const uint64_t who = __ballot(mine);
-            if (mine && threadIdx.x < 64) rows[n + __popcll(who & ((1ull << lane) - 1))] = (uint16_t)(p0 + lane);
+            if (mine && threadIdx.x < 64) rows[n + __popcll(who & ((1ull << lane) - 1))] = p0 + lane;
             if (who && first < 0) first = p0 + __builtin_ctzll(who);
             n += __popcll(who);
         }
         if (n == 0 || (g.by_pair && first != slot)) return;
     }
     __syncthreads();
-    all(static_cast<const uint16_t*>(rows), n);
+    all(n);
 }
 
 // ---- few tokens, the way back: a token's experts one after the other as one long K, their weights on the groups' scales --------------
@@ -1059,7 +1066,7 @@ __global__ __launch_bounds__(256) void experts_sum_kernel(const float* __restric
 template <int BITS, int XM, bool PAIR, int COLS>
 void launch_few(ExpertsArgs g, int slots, hipStream_t st)
 {
-    constexpr int lds = few_ring<BITS, XM, COLS>() + kMaxDirect * 2;
+    constexpr int lds = few_ring<BITS, XM, COLS>() + kMaxDirect * 4;
     (void)LdsRequest<&experts_few_kernel<BITS, XM, PAIR, COLS>, lds>::registered;
     g.groups = (g.strips + 2 * COLS - 1) / (2 * COLS);
     experts_few_kernel<BITS, XM, PAIR, COLS><<<dim3(g.groups, slots), dim3(512), lds, st>>>(g);
