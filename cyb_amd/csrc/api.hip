@@ -683,6 +683,7 @@ int matmul_experts(cybq_ctx* ctx, const cybq_weight* w, int64_t E, const void* x
     if (w->device != ctx->device) return fail(ctx, CYBQ_ERR_INVALID, "weight lives on another device");
     if (pair && !w->paired) return fail(ctx, CYBQ_ERR_INVALID, "CYBQ_EPI_SWIGLU needs a weight made by cybq_weight_fuse_pairs");
     const int step = pair ? 32 : 16;
+    if (w->K > (1 << 24)) return fail(ctx, CYBQ_ERR_SHAPE, "K must be at most 2^24");
     if (w->N % E || w->N / E % step)
         return fail(ctx, CYBQ_ERR_SHAPE, "the weight must have E times a multiple of 16 rows (of gate and of up, for CYBQ_EPI_SWIGLU)");
     if (!aligned16(x)) return fail(ctx, CYBQ_ERR_ALIGN, "x must be 16-byte aligned");

@@ -7,7 +7,7 @@ piece, then `Answer { tokens, tok_per_s, tok_in_s, tok_out_s, .. }`
 (/root/reference/shell/src/worlds/soma_bridge.rs:252-277); the UI keeps running
 means of `tok_in_s` / `tok_out_s` (/root/reference/shell/src/worlds/models/mod.rs:44-52)
 and compares them with `SPEED_ANCHORS` (same file, :116).  This module walks the
-same two phases over the quantised linears only:
+same two phases over the quantised linears only (and, with --experts, over the router and the experts of every layer):
 
   prefill  the prompt in chunks of `chunk` tokens, every chunk one pass of
            `cybq_matmul_many` over the stack with bf16 activations (M = chunk),
@@ -35,9 +35,9 @@ class Answer:
     tok_out_s: float       # generated tokens / decode time
 
 
-def ask(backend: Backend, st: stk.LinearStack, prompt_tokens: int, new_tokens: int, chunk: int = 512,
+def ask(backend: Backend, st, prompt_tokens: int, new_tokens: int, chunk: int = 512,
         batch: int = 1, shapes: Optional[Dict[str, tuple]] = None, stream: int = 0) -> Iterator[dict]:
-    """Yields {"Prefill": {"done", "total"}} per chunk, {"Delta": i} per decode step and finally
+    """Walks a LinearStack or an ExpertStack.  Yields {"Prefill": {"done", "total"}} per chunk, {"Delta": i} per decode step and finally
     {"Answer": Answer}.  Device work is timed with events on the launch stream."""
     import torch
     if prompt_tokens < 0 or new_tokens < 0 or chunk < 1 or batch < 1 or batch > 16:
@@ -45,21 +45,20 @@ def ask(backend: Backend, st: stk.LinearStack, prompt_tokens: int, new_tokens: i
     t_wall = time.time()
     yield {"Prefill": {"done": 0, "total": prompt_tokens}}
     ms_in = 0.0
-    plans = {}
+    steps = {}
 
-    def plan_for(M: int, xdtype):
-        if M not in plans:
-            edges = stk.edges_for(st, M, shapes=shapes, xdtype=xdtype)
-            plans[M] = (stk.plan(st, edges), edges)
-        return plans[M][0]
+    def step_for(M: int, xdtype):
+        if M not in steps:
+            steps[M] = stk.stepper(st, M, shapes=shapes, xdtype=xdtype)
+        return steps[M]
 
     done = 0
     while done < prompt_tokens:
         M = min(chunk, prompt_tokens - done)
-        pl = plan_for(M, torch.bfloat16 if M > 16 else torch.float16)
+        step = step_for(M, torch.bfloat16 if M > 16 else torch.float16)
         a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
         a.record()
-        backend.matmul_many(pl, M, stream)
+        step(stream)
         b.record()
         b.synchronize()
         ms_in += a.elapsed_time(b)
@@ -68,13 +67,13 @@ def ask(backend: Backend, st: stk.LinearStack, prompt_tokens: int, new_tokens: i
 
     ms_out = 0.0
     if new_tokens:
-        pl = plan_for(batch, torch.float16)
-        backend.matmul_many(pl, batch, stream)                 # first touch of this plan's buffers, untimed
+        step = step_for(batch, torch.float16)
+        step(stream)                                           # first touch of this plan's buffers, untimed
         torch.cuda.synchronize()
         a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
         a.record()
         for i in range(new_tokens):
-            backend.matmul_many(pl, batch, stream)
+            step(stream)
         b.record()
         b.synchronize()
         ms_out = a.elapsed_time(b)
@@ -97,13 +96,18 @@ def main(argv=None) -> int:
     ap.add_argument("--layers", type=int, default=32)
     ap.add_argument("--separate", action="store_true", help="q/k/v and gate/up as separate launches (224 per step)")
     ap.add_argument("--epilogues", action="store_true", help="SwiGLU and residual adds fused into the linears")
+    ap.add_argument("--experts", type=int, default=0, help="FFNs of this many experts (hidden 2048, width 768) instead of the Llama-3-8B shapes")
+    ap.add_argument("--top-k", type=int, default=8, help="experts per token")
     args = ap.parse_args(argv)
     import torch
     torch.cuda.init()          # torch brings its own HIP runtime: let it find the device before libcybq does
     be = Backend(0)
     shapes = None if args.separate else stk.fused_shapes()
-    st = stk.build(be, layers=args.layers, shapes=shapes, order=list(shapes) if shapes else None,
-                   epilogues=args.epilogues and shapes is not None)
+    if args.experts:
+        st = stk.build_experts(be, layers=args.layers, experts=args.experts, top_k=args.top_k)
+    else:
+        st = stk.build(be, layers=args.layers, shapes=shapes, order=list(shapes) if shapes else None,
+                       epilogues=args.epilogues and shapes is not None)
     for ev in ask(be, st, args.prompt, args.new, args.chunk, args.batch, shapes=shapes):
         if "Prefill" in ev:
             p = ev["Prefill"]

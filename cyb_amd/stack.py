@@ -18,7 +18,7 @@ from dataclasses import dataclass, field
 from typing import Dict, List
 
 from . import formats, synth
-from .backend import Backend, QMatMul, QWeight
+from .backend import Backend, CybqError, QMatMul, QWeight
 
 LINEAR_ORDER = ["q_proj", "k_proj", "v_proj", "o_proj", "gate_proj", "up_proj", "down_proj"]
 _PREFIX = {"q_proj": "self_attn", "k_proj": "self_attn", "v_proj": "self_attn", "o_proj": "self_attn",
@@ -148,3 +148,109 @@ def plan(stack: LinearStack, edges):
         return stack.backend.plan_many(stack.weights, xs, ys, gammas=gammas, eps=stack.eps)
     res = [edges[f"res.{n.N}"] if e == "add" else None for n, e in zip(stack.nodes, stack.epilogues)]
     return stack.backend.plan_many(stack.weights, xs, ys, stack.epilogues, res, gammas=gammas, eps=stack.eps)
+
+
+def stepper(stack, M: int, shapes: Dict[str, tuple] = None, xdtype=None):
+    """One step of M rows as a call: step(stream).  The plan and its buffers live as long as the call does."""
+    if isinstance(stack, ExpertStack):
+        return stack.stepper(M, xdtype)
+    edges = edges_for(stack, M, shapes=shapes, xdtype=xdtype)
+    p = plan(stack, edges)
+
+    def step(stream: int = 0) -> None:
+        stack.backend.matmul_many(p, M, stream)
+    step.edges = edges
+    return step
+
+
+@dataclass
+class ExpertStack:
+    """The decode-step stack of a model whose FFNs are mixtures of experts: per layer q/k/v and o as in LinearStack, a router
+    (a Q8 linear, then Backend.route) and the experts' gate / up and down (matmul_experts, matmul_experts_sum), the
+    residual added on the way back."""
+    backend: Backend
+    layers: int
+    bits: int
+    experts: int
+    top_k: int
+    hidden: int
+    width: int
+    qkv: List[QWeight] = field(default_factory=list)
+    o: List[QWeight] = field(default_factory=list)
+    router: List[QWeight] = field(default_factory=list)
+    gate_up: List[QWeight] = field(default_factory=list)      # fuse_pairs of [experts * width, hidden] twice
+    down: List[QWeight] = field(default_factory=list)         # [experts * hidden, width]
+
+    @property
+    def weights(self) -> List[QWeight]:
+        return self.qkv + self.o + self.router + self.gate_up + self.down
+
+    @property
+    def weight_bytes(self) -> int:
+        return sum(w.algorithmic_bytes for w in self.weights)
+
+    @property
+    def nodes(self) -> List[str]:
+        """The calls of one step."""
+        return ["qkv", "o", "router", "route", "gate_up", "down"] * self.layers
+
+    def stepper(self, M: int, xdtype=None, seed: int = 5):
+        import torch
+        xdtype = xdtype or torch.float16
+        be, dev = self.backend, f"cuda:{self.backend.device}"
+        b = {"x": torch.from_numpy(synth.activations(seed, M, self.hidden)).to(dev).to(xdtype),
+             "attn": torch.from_numpy(synth.activations(seed, M, self.hidden, stream=1)).to(dev).to(xdtype),
+             "mid": torch.empty((M, self.hidden), dtype=xdtype, device=dev),
+             "qkv": torch.empty((M, self.qkv[0].N), dtype=torch.float32, device=dev),
+             "logits": torch.empty((M, self.experts), dtype=torch.float32, device=dev),
+             "ids": torch.empty((M, self.top_k), dtype=torch.int32, device=dev),
+             "weights": torch.empty((M, self.top_k), dtype=torch.float32, device=dev),
+             "h": torch.empty((M * self.top_k, self.width), dtype=xdtype, device=dev),
+             "y": torch.empty((M, self.hidden), dtype=xdtype, device=dev)}
+
+        def step(stream: int = 0) -> None:
+            for i in range(self.layers):
+                be.matmul(self.qkv[i], b["x"], b["qkv"], stream=stream)
+                be.matmul_ex(self.o[i], b["attn"], b["mid"], "add", b["x"], stream=stream)
+                be.matmul(self.router[i], b["mid"], b["logits"], stream=stream)
+                be.route(b["logits"], b["ids"], b["weights"], stream=stream)
+                be.matmul_experts(self.gate_up[i], self.experts, b["mid"], b["ids"], b["h"], "swiglu", stream=stream)
+                be.matmul_experts_sum(self.down[i], self.experts, b["h"], b["ids"], b["weights"], b["y"], b["mid"], stream=stream)
+        step.edges = b
+        return step
+
+
+def build_experts(backend: Backend, layers: int = 4, bits: int = formats.Q4, experts: int = 128, top_k: int = 8, hidden: int = 2048,
+                  width: int = 768, qkv: int = None, seed: int = 5) -> ExpertStack:
+    """Random-init stack of expert layers with N(0, 0.02) weights quantised on the device, a stack of experts at a time."""
+    import torch
+    if width % 32 or hidden % 32 or not 1 <= top_k <= experts:
+        raise CybqError(-2, "bad shape", "hidden and width must be multiples of 32, top_k in 1 .. experts")
+    st = ExpertStack(backend, layers, bits, experts, top_k, hidden, width)
+    dev = f"cuda:{backend.device}"
+    gen = torch.Generator(device=dev)
+    gen.manual_seed((synth.BASE_SEED ^ seed) & 0x7FFFFFFF)
+
+    def tensor(quant: int, N: int, K: int, name: str = None) -> QWeight:
+        q = torch.empty(N * K * quant // 8, dtype=torch.uint8, device=dev)
+        s = torch.empty(N * (K // 32), dtype=torch.int16, device=dev)
+        rows = max(16, (1 << 26) // K // 16 * 16)                     # a quarter of a gigabyte of fp32 at a time
+        for r in range(0, N, rows):
+            n = min(rows, N - r)
+            w = torch.empty((n, K), dtype=torch.float32, device=dev).normal_(0.0, 0.02, generator=gen)
+            backend.quantize(quant, w, n, K, q[r * K * quant // 8:], s[r * (K // 32):])
+            torch.cuda.synchronize()
+        out = backend.weight_from_device(quant, N, K, q, s, name=name)
+        torch.cuda.synchronize()                                      # q and s are released
+        return out
+
+    for i in range(layers):
+        st.qkv.append(tensor(bits, qkv or hidden * 5 // 4, hidden, tensor_name(i, "qkv_proj")))
+        st.o.append(tensor(bits, hidden, hidden, tensor_name(i, "o_proj")))
+        st.router.append(tensor(formats.Q8, experts, hidden, f"model.layers.{i}.mlp.gate.weight"))
+        gate, up = tensor(bits, experts * width, hidden), tensor(bits, experts * width, hidden)
+        st.gate_up.append(backend.fuse_pairs(gate, up, name=f"model.layers.{i}.mlp.experts.gate_up_proj.weight"))
+        gate.free()
+        up.free()
+        st.down.append(tensor(bits, experts * hidden, width, f"model.layers.{i}.mlp.experts.down_proj.weight"))
+    return st

@@ -311,15 +311,19 @@ int cybq_route(cybq_ctx* ctx, const void* logits, cybq_dtype ldt, int64_t T, int
 /* The rows of T tokens through their experts:  y[t * top_k + j, :] = epilogue(x[t, :] W_e^T), e = ids[t * top_k + j].
  *   x [T,K] of xdt, 16-byte aligned; y [T * top_k, n] of ydt ([.., n / 2] with CYBQ_EPI_SWIGLU, w from
  *   cybq_weight_fuse_pairs), must not overlap x.  CYBQ_EPI_ADD is not taken.  Rows of y without an expert stay as
- *   they were.  T >= 0.  Operands are exact whatever the context's modes (integers q, the groups' scales in fp32 on
- *   their sums, fp32 rows in three bf16 parts); |x| of bf16 and fp32 rows up to 4e34, as in the decode kernels: the row
- *   of a larger element, Inf or NaN gives Inf or NaN, other rows are not touched by it. */
+ *   they were.  T >= 0, K <= 2^24.
+ * Operands are exact whatever the decode mode: the integers q, the groups' scales in fp32 on their sums, fp32 rows in
+ * three bf16 parts (below 1e-6 relative L2 on fp32 y; |x| of bf16 and fp32 rows up to 4e34, as in the decode kernels).
+ * With CYBQ_PREFILL_FAST, 16-bit rows, a y of bf16 and 24 (Q8: 20) pairs and more per expert they are round_f16(scale * q)
+ * instead, bf16 rows f16 behind a power of two (2e-4 next to the 1.6e-3 of y's own rounding; not for weights with wide
+ * scales).  Which it is goes by the whole call, so the last bits of a row may change with the batch.  A row with an
+ * element that is Inf, NaN or beyond the range above gives Inf or NaN; other rows are not touched by it. */
 int cybq_matmul_experts(cybq_ctx* ctx, const cybq_weight* w, int64_t E, const void* x, cybq_dtype xdt, int64_t T,
                         int64_t top_k, const int32_t* ids, void* y, cybq_dtype ydt, cybq_epilogue epilogue, void* stream);
 
 /* The way back:  y[t, :] = residual[t, :] + sum_j weights[t * top_k + j] * (x[t * top_k + j, :] W_e^T), e = ids[t * top_k + j].
  *   x [T * top_k, K]; weights fp32; residual [T, n] of ydt or NULL (zeros), may alias y; y [T, n], every row is
- *   written.  Added in fp32 in a fixed order, rounded once.  CYBQ_ERR_UNSUPPORTED for K over 524288 where one token's
+ *   written.  Added in fp32 in a fixed order, rounded once; operands as above.  CYBQ_ERR_UNSUPPORTED for K over 524288 where one token's
  *   top_k * n sums do not fit the scratch. */
 int cybq_matmul_experts_sum(cybq_ctx* ctx, const cybq_weight* w, int64_t E, const void* x, cybq_dtype xdt, int64_t T,
                             int64_t top_k, const int32_t* ids, const float* weights, const void* residual, void* y,

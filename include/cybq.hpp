@@ -143,6 +143,24 @@ public:
     {
         return wrap(cybq_matmul_norm(ctx_, w.get(), x, xdt, M, gamma, gdt, eps, y, ydt, epilogue, residual, stream));
     }
+    // mixture of experts: the router, then the rows through their experts and back
+    Status route(const void* logits, cybq_dtype ldt, int64_t T, int64_t E, int64_t top_k, cybq_score score, const float* bias,
+                 int64_t groups, int64_t top_groups, int group_best, bool renormalise, float scale, int32_t* ids, float* weights,
+                 void* stream = nullptr)
+    {
+        return wrap(cybq_route(ctx_, logits, ldt, T, E, top_k, score, bias, groups, top_groups, group_best, renormalise ? 1 : 0, scale,
+                               ids, weights, stream));
+    }
+    Status matmul_experts(const Weight& w, int64_t E, const void* x, cybq_dtype xdt, int64_t T, int64_t top_k, const int32_t* ids,
+                          void* y, cybq_dtype ydt, cybq_epilogue epilogue = CYBQ_EPI_NONE, void* stream = nullptr)
+    {
+        return wrap(cybq_matmul_experts(ctx_, w.get(), E, x, xdt, T, top_k, ids, y, ydt, epilogue, stream));
+    }
+    Status matmul_experts_sum(const Weight& w, int64_t E, const void* x, cybq_dtype xdt, int64_t T, int64_t top_k, const int32_t* ids,
+                              const float* weights, const void* residual, void* y, cybq_dtype ydt, void* stream = nullptr)
+    {
+        return wrap(cybq_matmul_experts_sum(ctx_, w.get(), E, x, xdt, T, top_k, ids, weights, residual, y, ydt, stream));
+    }
     Status dequant(const Weight& w, float* out, void* stream = nullptr)
     {
         return wrap(cybq_dequant(ctx_, w.get(), out, stream));

@@ -325,14 +325,16 @@ def test_rows_that_are_not_finite_stay_among_themselves(backend):
             x = _rows((T, K), dt, 4)
             ids = _ids(T, k, E, 5)
             x[1, 7], x[3, K - 1] = float("inf"), float("nan")
-            y = torch.empty((T * k, n), device="cuda")
-            backend.matmul_experts(w, E, x, ids, y)
-            torch.cuda.synchronize()
             bad = torch.zeros(T, dtype=torch.bool, device="cuda")
             bad[[1, 3]] = True
             rows = bad.repeat_interleave(k)
-            assert not torch.isfinite(y[rows]).any()
-            _close(y[~rows], _products(torch.where(bad[:, None], 0, x), k, wd, ids)[~rows], TIGHT, (T, dt))
+            ref = _products(torch.where(bad[:, None], 0, x), k, wd, ids)
+            for ydt in ("f32", "bf16"):                               # (many rows and bf16: rounded operands)
+                y = torch.empty((T * k, n), device="cuda", dtype=TDT[ydt])
+                backend.matmul_experts(w, E, x, ids, y)
+                torch.cuda.synchronize()
+                assert not torch.isfinite(y[rows]).any()
+                _close(y[~rows], ref[~rows], TIGHT + HALF_STEP[ydt], (T, dt, ydt))
     w.free()
 
 
@@ -367,6 +369,140 @@ def test_fp32_rows_keep_their_bits(backend):
     torch.cuda.synchronize()
     _close(y, _products(x, 1, wd, ids), 2e-6)
     w.free()
+
+
+@pytest.fixture
+def tuned(backend):
+    yield backend.set_experts_tuning
+    backend.set_experts_tuning()
+
+
+@gpu
+@pytest.mark.parametrize("cols", [1, 2, 4, 8])
+@pytest.mark.parametrize("T", [1, 2, 9, 40, 150])
+def test_few_rows_whatever_the_waves_do(backend, tuned, cols, T):
+    """One row and up to 8, 16, 32, 64 at a time and the rest, K shorter than the waves that share it out, strips that no workgroup divides."""
+    tuned(cols, 1 << 20, 2)
+    for bits in (4, 8):
+        for xdt in ("f16", "bf16", "f32"):
+            for n, K in ((144, 1312), (16, 96), (208, 32)):
+                _check_up(backend, bits, 3, n, K, T, 2, xdt, "f32", "padded", seed=T)
+            _check_up(backend, bits, 3, 112, 864, T, 1, xdt, xdt, "few", swiglu=True, seed=T)
+            _check_down(backend, bits, 3, 144, 1312, T, 2, xdt, "f32", seed=T)
+
+
+@gpu
+@pytest.mark.parametrize("T", [1, 5, 33])
+def test_the_way_back_token_by_token(backend, tuned, T):
+    tuned(0, 0, 1)
+    for bits in (4, 8):
+        for xdt in ("f16", "bf16", "f32"):
+            for E, n, K, k, how in ((3, 16, 32, 1, "spread"), (9, 144, 1312, 3, "padded"), (5, 48, 4128, 7, "few"), (4, 32, 160, 64, "padded")):
+                _check_down(backend, bits, E, n, K, T, k, xdt, "f32" if K > 100 else xdt, how, seed=K)
+
+
+@gpu
+@pytest.mark.parametrize("mode", ["fast", "exact"])
+@pytest.mark.parametrize("T", [1, 17, 40, 70, 100, 113, 128, 300])
+def test_many_rows_whatever_the_mode(backend, tuned, mode, T):
+    """All row blocks of a tile; K of whole tiles, of 1, 2 and 3 groups behind them or alone.  With a y of bf16 FAST mode rounds the operands."""
+    tuned(0, 1, 2)
+    backend.set_prefill_mode(mode)
+    try:
+        for bits in (4, 8):
+            for xdt in ("f16", "bf16"):
+                for n, K in ((272, 512), (48, 416), (528, 576), (16, 96), (32, 32), (64, 1184)):
+                    for ydt in ("f32", "bf16"):
+                        _check_up(backend, bits, 2, n, K, T, 1, xdt, ydt, "padded", seed=T)
+                _check_up(backend, bits, 2, 160, 672, T, 2, xdt, "bf16", swiglu=True, seed=T)
+                _check_down(backend, bits, 2, 272, 416, T, 2, xdt, "bf16", "padded", seed=T)
+    finally:
+        backend.set_prefill_mode("fast")
+
+
+@gpu
+def test_rounded_operands_where_y_is_rounded_more(backend):
+    """FAST mode: a weight of round_f16(scale * q) is off by 2^-11 / sqrt(3) at most on average, 3e-4 on y, next to at most
+    2^-8 / sqrt(3) of y's own rounding (both independent from element to element): 2.28e-3 together."""
+    E, n, K, T, k = 4, 256, 1024, 200, 2
+    w, wd = _stack(backend, 4, E, n, K, 1)
+    ids = _ids(T, k, E, 2)
+    for xdt in ("bf16", "f16"):
+        x = _rows((T, K), xdt, 3)
+        ref = _products(x, k, wd, ids)
+        y, exact = (torch.empty((T * k, n), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+        backend.matmul_experts(w, E, x, ids, y)
+        try:
+            backend.set_prefill_mode("exact")
+            backend.matmul_experts(w, E, x, ids, exact)
+        finally:
+            backend.set_prefill_mode("fast")
+        torch.cuda.synchronize()
+        for got, most in ((y, 2.28e-3), (exact, 2.0 ** -8 / 3 ** 0.5)):
+            err = ((got.double() - ref).norm() / ref.norm()).item()
+            assert err < most, (xdt, err)
+        assert not torch.equal(y, exact)
+    w.free()
+
+
+@gpu
+def test_rounded_operands_of_rows_of_any_size_and_wide_scales(backend):
+    """bf16 rows of 1e-30 and 1e30 become f16 behind a power of two; a weight whose scale * q leaves f16 keeps exact operands."""
+    E, n, K, T = 3, 32, 256, 150
+    for scale in (0.01, 3.0e4):
+        w, wd = _stack(backend, 4, E, n, K, 6, scale)
+        size = torch.tensor([1e-30, 1e30 if scale < 1 else 1e25, 1.0, 1e-38], device="cuda").repeat(T)[:T, None]
+        x = (_rows((T, K), "f32", 8) * size).bfloat16()
+        x[5] = 0
+        ids = _ids(T, 1, E, 9)
+        y = torch.empty((T, n), dtype=torch.bfloat16, device="cuda")
+        backend.matmul_experts(w, E, x, ids, y)
+        torch.cuda.synchronize()
+        ref = _products(x, 1, wd, ids)
+        keep = ref.abs().amax(dim=1) > 1e-36                          # (below, y itself has no bits left)
+        assert (y[5] == 0).all()
+        _close(y[keep], ref[keep], HALF_STEP["bf16"] + 3e-4, scale)
+        w.free()
+
+
+@gpu
+def test_lists_of_many_experts_and_pairs(backend, tuned):
+    """1024 experts, 40000 pairs, a third of them with none: against the same products expert by expert."""
+    _check_up(backend, 4, 1024, 16, 32, 5000, 8, "f16", "f32", "padded", seed=3)
+    tuned(0, 1, 2)
+    _check_up(backend, 8, 1024, 16, 64, 5000, 8, "bf16", "f32", "padded", seed=4)
+    _check_up(backend, 4, 1, 16, 64, 66000, 1, "f16", "f16", "one", seed=5)
+
+
+@gpu
+@pytest.mark.parametrize("T", [3, 60, 600])
+def test_the_same_bits_every_time(backend, T):
+    run, _, bufs, _, _ = _layer(backend, T, 16, 4, 256, 160, "bf16", 90)
+    run(backend)
+    torch.cuda.synchronize()
+    first = {n: b.clone() for n, b in bufs.items()}
+    for _ in range(3):
+        run(backend)
+        torch.cuda.synchronize()
+        assert all(torch.equal(first[n], b) for n, b in bufs.items())
+
+
+@gpu
+def test_two_contexts_on_two_streams(backend):
+    """Each context has scratch of its own: calls of two of them may overlap."""
+    other = Backend(0)
+    try:
+        sides = [torch.cuda.Stream(), torch.cuda.Stream()]
+        runs = [_layer(be, 400, 8, 4, 512, 256, "bf16", 100 + i) for i, be in enumerate((backend, other))]
+        torch.cuda.synchronize()
+        for _ in range(5):
+            for (run, *_), be, s in zip(runs, (backend, other), sides):
+                run(be, s.cuda_stream)
+        torch.cuda.synchronize()
+        for _, want, bufs, _, _ in runs:
+            _close(bufs["y"], want()[1], 4 * TIGHT + 2 * HALF_STEP["bf16"])
+    finally:
+        other.close()
 
 
 def _layer(backend, T, E, k, hidden, width, dt, seed=0):
@@ -410,18 +546,18 @@ def test_a_layer(backend, T, dt):
 
 
 @gpu
-@pytest.mark.parametrize("T", [1, 12, 300])
-def test_a_captured_layer_follows_its_inputs(T):
+@pytest.mark.parametrize("T,dt", [(1, "f16"), (12, "f16"), (300, "f16"), (300, "bf16")])
+def test_a_captured_layer_follows_its_inputs(T, dt):
     """One recording, replayed with other rows and other logits, eager calls of the context between the replays."""
     be = Backend(0)
     try:
-        run, want, bufs, x, logits = _layer(be, T, 16, 4, 256, 160, "f16", 30)
+        run, want, bufs, x, logits = _layer(be, T, 16, 4, 256, 160, dt, 30)
         side = torch.cuda.Stream()
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph, stream=side):                    # the first launches of this context
             run(be, torch.cuda.current_stream().cuda_stream)
         for i in range(4):
-            x.copy_(_rows(tuple(x.shape), "f16", 50 + i))
+            x.copy_(_rows(tuple(x.shape), dt, 50 + i))
             logits.copy_(_rows(tuple(logits.shape), "f32", 60 + i))
             for b in bufs.values():
                 b.fill_(-3)
@@ -430,7 +566,7 @@ def test_a_captured_layer_follows_its_inputs(T):
             got = {n: b.clone() for n, b in bufs.items()}
             ids, ref = want()
             assert torch.equal(got["ids"], ids)
-            _close(got["y"], ref, 4 * TIGHT + 2 * HALF_STEP["f16"], i)
+            _close(got["y"], ref, 4 * TIGHT + 2 * HALF_STEP[dt], i)
             run(be)
             torch.cuda.synchronize()
             assert all(torch.equal(got[n], b) for n, b in bufs.items())      # the same bits as eager calls
@@ -450,6 +586,55 @@ def test_another_stream(backend):
             _close(bufs["y"], want()[1], 4 * TIGHT + 2 * HALF_STEP["bf16"], T)
 
 
+# ---- the stack and the driver ----------------------------------------------------------------------------------------
+
+@gpu
+@pytest.mark.parametrize("M,dt", [(1, "f16"), (5, "f16"), (260, "bf16")])
+def test_a_step_of_the_expert_stack(backend, M, dt):
+    """The last layer's calls recomputed in float64 from its dequantised weights and the rows it was given."""
+    from cyb_amd import stack
+    E, k, hidden, width = 12, 3, 256, 96
+    st = stack.build_experts(backend, layers=2, experts=E, top_k=k, hidden=hidden, width=width, seed=3)
+    assert len(st.weights) == 10 and len(st.nodes) == 12
+    step = stack.stepper(st, M, xdtype=TDT[dt])
+    step()
+    torch.cuda.synchronize()
+    b = step.edges
+
+    def values(w):
+        out = torch.empty((w.N, w.K), device="cuda")
+        backend.dequant(w, out)
+        torch.cuda.synchronize()
+        return out.double()
+
+    logits = b["mid"].double() @ values(st.router[-1]).T.contiguous()
+    assert ((b["logits"].double() - logits).norm() / logits.norm()).item() < 5e-4
+    rid, rw = _route_ref(b["logits"].double().cpu().numpy(), k)
+    assert np.array_equal(b["ids"].cpu().numpy(), rid)
+    strips = values(st.gate_up[-1]).reshape(E, width // 16, 2, 16, hidden)
+    g = _products(b["mid"], k, strips[:, :, 0].reshape(E, width, hidden), b["ids"])
+    u = _products(b["mid"], k, strips[:, :, 1].reshape(E, width, hidden), b["ids"])
+    _close(b["h"], g * torch.sigmoid(g) * u, 3 * TIGHT + HALF_STEP[dt])
+    z = _products(b["h"], 1, values(st.down[-1]).reshape(E, hidden, width), b["ids"]) * torch.from_numpy(rw).cuda().reshape(-1, 1)
+    _close(b["y"], b["mid"].double() + z.reshape(M, k, hidden).sum(dim=1), 4 * TIGHT + HALF_STEP[dt])
+    with pytest.raises(CybqError):
+        stack.build_experts(backend, layers=1, experts=2, top_k=3, hidden=256, width=96)
+    for w in st.weights:
+        w.free()
+
+
+@gpu
+def test_the_driver_walks_experts(backend):
+    from cyb_amd import driver, stack
+    st = stack.build_experts(backend, layers=2, experts=8, top_k=2, hidden=256, width=64)
+    evs = list(driver.ask(backend, st, prompt_tokens=150, new_tokens=4, chunk=64))
+    assert [e["Prefill"]["done"] for e in evs if "Prefill" in e] == [0, 64, 128, 150]
+    assert sum("Delta" in e for e in evs) == 4 and evs[-1]["Answer"].tokens == 4
+    assert evs[-1]["Answer"].tok_in_s > 0 and evs[-1]["Answer"].tok_out_s > 0
+    for w in st.weights:
+        w.free()
+
+
 # ---- refusals ----------------------------------------------------------------------------------------------------
 
 def _status(call):
@@ -467,6 +652,11 @@ def test_refusals(backend):
     g = torch.zeros((2, 2), device="cuda")
     y = torch.zeros((4, 48), device="cuda")
     z = torch.zeros((2, 8), device="cuda")
+    assert _status(lambda: be.matmul_experts(w, 4, x, ids.t(), y)) == -2               # not contiguous
+    assert _status(lambda: be.matmul_experts(w, 4, x[:1], ids, y)) == -2 and _status(lambda: be.matmul_experts(w, 4, x, ids, y[:3])) == -2
+    assert _status(lambda: be.matmul_experts_sum(w, 4, torch.zeros((4, 64), device="cuda"), ids, g, y[:2], y[:2].half())) == -1
+    assert _status(lambda: be.route(z, ids, g, bias=torch.zeros(8, device="cuda", dtype=torch.float16))) == -1
+    assert _status(lambda: be.set_experts_tuning(3)) == -1
     assert _status(lambda: be.matmul_experts(w, 5, x, ids, y)) == -2                   # 192 rows
     assert _status(lambda: be.matmul_experts(w, 8, x, ids, y)) == -2                   # 24 rows each are no multiple of 16
     assert _status(lambda: be.matmul_experts(w, 0, x, ids, y)) == -2
