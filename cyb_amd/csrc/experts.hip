@@ -5,8 +5,20 @@
 //
 //   out[p, :] = x[p / xdiv, :] W_ids[p]^T         xdiv = top_k: the tokens' rows; 1: a row of its own for every pair
 //
-// Operands are exact in every kernel: the integers q (bf16 rows: biased, and a second product that takes the bias off), each
-// group's sums times its scale in fp32.  No row statistics, no staging, and scales that leave f16's range when multiplied with q do no harm.
+// The kernels, by the number of rows that an expert has:
+//   few   experts_few_kernel    one pass over each met expert's weights, HBM-bound; pieces of 1, 8, 16, 32 or 64 rows
+//   many  experts_many_kernel   tiles of 64 or 128 rows, bound by what a CU's vector, matrix and memory pipes do between two barriers
+//   back  experts_token_kernel  a few tokens, all their experts as one long K, no sums in memory; else few / many into fp32 sums [P, n] in the
+//                               scratch and experts_sum_kernel
+// Operands are exact - the integers q (bf16 and fp32 rows: biased, and a second product that takes the bias off), each group's sums times its
+// scale in fp32, so scales that leave f16's range when multiplied with q do no harm - but for many rows and a y of bf16 in FAST mode, where they
+// are round_f16(scale * q): 2e-4 relative L2 next to the 1.6e-3 of y's own rounding, and no FMAs behind the MFMAs.
+//
+// us per call, weights from HBM (bytes of the met experts' weights, rows and outputs; products without the bias'):
+//   up, 8 of 128 experts of 2048 -> 2 x 768, Q4, one f16 token 5.3 (14 MB); back 6.4 (7 MB)         the launch, three trips to memory, the stream
+//   up, 2 of 8 of 4096 -> 2 x 14336, 16 bf16 tokens 98 (524 MB: 5.3 TB/s); back, 32 f16 tokens 46 - 57 (267 MB: 4.7 - 5.8 TB/s)           HBM
+//   up, 4 of 60 of 2592 -> 2 x 1040, Q8, 37 f16 tokens 55 - 69 (306 MB at most)                                                       HBM
+//   up, 8 of 128, 2048 bf16 tokens 158 - 170 (103 GFLOP: 0.63 PFLOP/s); back 156 - 164; 2 of 8 wide ones, 1024 tokens 508 - 529 (481 GFLOP: 0.93)
 #include <algorithm>
 #include <type_traits>
 
@@ -198,6 +210,8 @@ __global__ __launch_bounds__(1024) void experts_prepare_kernel(const int32_t* __
 // up strip) against up to 16 * RB of the expert's rows.  A step is KH K tiles: the rows of each are gathered into LDS once, whole 128-byte
 // lines per eight lanes, pieces permuted so that the reads meet no bank conflicts; a wave's own weight tiles pass through LDS as well, only to
 // be on their way without registers (global_load_lds).  D steps have a place in LDS, copies are counted by hand: they retire in order.
+// (Weights and rows straight into registers, as operands: rows cost 64 separate accesses per load; 16 tokens on the wide experts 208 us
+// against 101, 37 on 60 Q8 experts 124 against 46.)
 struct ExpertsArgs {
     const uint8_t* w;
     const void* x;
@@ -638,7 +652,12 @@ __device__ __forceinline__ void expert_row(const ExpertsArgs& g, int e, int p, i
 //
 // The lists' row tiles.  Workgroup = a tile of up to 16 * RB rows x 16 strips: four waves side by side with four strips each, times two that
 // share out every K tile, two groups of 32 each.  A weight operand is made once and meets all rows; rows are read from LDS by four waves, not
-// eight (with two strips to a wave and whole K tiles the reads alone took 3100 cycles of a step's 2048 of MFMAs).
+// eight.  Between two MFMAs stand two vector instructions that make the next group's operands, so a wave's MFMAs are hardly ever held up by them;
+// clumps of them ahead of the MFMAs, and all copies at once behind the barrier, cost 7 %.  2 of 8 experts of 4096 -> 2 x 14336, 1024 bf16 tokens: 860 us
+// with exact operands and two workgroups of 64 rows to a CU, 685 with rounded ones, 596 with one of 128 rows, 529 now; without its
+// copies 411, without its MFMAs 412, so it is neither alone but what of both does not overlap: eight waves that meet at a barrier per K tile.
+// Tried: workgroups that stay and look the next item up behind the products (529 -> 550: tiles differ in length); K tiles started at
+// different places by the workgroups that share rows (566 -> 692); row tiles outermost (566 -> 590).
 //   OP 0 / 1  exact operands, f16 / bf16 rows: a strip and group starts from zero (bf16: from the product that takes the bias off, one
 //             for four strips), its sums are scaled on their way into the fp32 accumulators, four FMAs per MFMA
 //   OP 2      f16 rows (bf16 ones behind a power of two per row), operands round_f16(scale * q), one MFMA and no FMAs
@@ -1132,6 +1151,9 @@ void set_experts_tuning(int cols, int many, int token) { g_tuning = {cols, many,
 
 size_t experts_lists_bytes(int64_t P, int E) { return ((size_t)(lists_order_at(P, E) + P) * 4 + 255) / 256 * 256; }
 
+// Where the tiles of many rows beat one pass of few.  us, few / many at 16, 24, 32, 48 rows to an expert: Q4, rounded operands, up 8 of 128 of 2048 -> 2 x 768
+// 64 / 65, 85 / 77, 105 / 86, 134 / 98, 2 of 8 of 4096 -> 2 x 14336 124 / 138, 143 / 146, 176 / 164, 258 / 194; exact operands 59 / 73, 76 / 88, 92 / 98, 127 / 118 and
+// 116 / 150, 136 / 150, 162 / 185, 234 / 213; Q8, exact, 109 / 103, 126 / 118, 153 / 119, 196 / 132 and 204 / 227, 217 / 225, 264 / 237, 372 / 245.
 bool experts_many(const WeightView& w, int E, int xdt, int64_t P, bool fast)
 {
     const int thr = g_tuning.many ? g_tuning.many : w.bits == 8 ? 20 : fast ? 24 : 40;
@@ -1181,7 +1203,11 @@ hipError_t launch_experts(const WeightView& w, int E, bool pair, const void* x, 
         return hipGetLastError();
     }
     const int slots = g.by_pair ? (int)P : E;
-    // waves side by side, or behind each other along K where that leaves CUs without work
+    // Waves side by side, or behind each other along K where that leaves CUs without work: of strips of met experts per CU there go 16 to a
+    // workgroup of eight waves side by side, 8, 4, 2.  us per call with 8 / 4 / 2 / 1 side by side, up, Q4, f16 rows: 8 of 128 experts of 2048 -> 2 x 768 at
+    // 1 / 4 / 16 tokens 12.6 / 7.9 / 5.5 / 5.4, 16.2 / 13.9 / 13.9 / 15.3, 31.8 / 30.5 / 32.5 / 39.6; back, 2 of 8 of 14336 -> 4096 at 16 tokens (2048 strips) 84.5 / 48.6 /
+    // 45.0 / 44.0.  Eight only on a short K (few steps to a workgroup): 8 of 256 of 1024 -> 2 x 512 at 16 tokens 15.0 / 16.4 / 19.4, Q8 20.9 / 24.0 / 29.2,
+    // but Q8 6 of 64 of 2048 -> 2 x 1408 62.5 / 56.5 / 61.5.
     const int64_t work = met * strips;
     const int cols = g_tuning.cols ? g_tuning.cols : work >= (w.bits == 8 ? 12 : 32) * num_cus && w.KT <= 12 ? 8 : work > 8 * num_cus || w.KT < 4 ? 4 : work >= 4 * num_cus || w.KT < 8 ? 2 : 1;
     auto go = [&](auto b_, auto x_, auto pair_) {
@@ -1202,6 +1228,9 @@ hipError_t launch_experts(const WeightView& w, int E, bool pair, const void* x, 
     return hipGetLastError();
 }
 
+// Token by token: no second launch and no sums in memory, but an expert's weights come once per token.  us, token by token / with sums in memory, 1, 2, 4, 8
+// tokens: 8 of 128 of 768 -> 2048 6.7 / 9.3, 6.7 / 9.6, 9.4 / 11.6, 16.5 / 16.4; 8 of 256 of 512 -> 1024 5.3 / 7.9, 5.3 / 8.8, 5.5 / 9.2, 7.7 / 10.5; 2 of 8 of 14336 -> 4096
+// 19.3 / 17.1, 29 / 27, 52 / 39, 97 / 43: up to 36864 tiles of weights, and no more pairs than experts.
 bool experts_sum_by_token(const WeightView& w, int E, int64_t T, int top_k)
 {
     if (!experts_token_serves(w)) return false;
