@@ -686,6 +686,7 @@ int matmul_experts(cybq_ctx* ctx, const cybq_weight* w, int64_t E, const void* x
     if (w->K > (1 << 24)) return fail(ctx, CYBQ_ERR_SHAPE, "K must be at most 2^24");
     if (w->N % E || w->N / E % step)
         return fail(ctx, CYBQ_ERR_SHAPE, "the weight must have E times a multiple of 16 rows (of gate and of up, for CYBQ_EPI_SWIGLU)");
+    if (w->N / E > cybq::kMaxExpertRows) return fail(ctx, CYBQ_ERR_SHAPE, "an expert must have at most 2^26 rows");
     if (!aligned16(x)) return fail(ctx, CYBQ_ERR_ALIGN, "x must be 16-byte aligned");
     if (reinterpret_cast<uintptr_t>(y) % dtype_size(ydt) || reinterpret_cast<uintptr_t>(residual) % dtype_size(ydt))
         return fail(ctx, CYBQ_ERR_ALIGN, "y / residual is not aligned to its element size");
@@ -714,6 +715,7 @@ int matmul_experts(cybq_ctx* ctx, const cybq_weight* w, int64_t E, const void* x
     const size_t token_bytes = (staged ? row_bytes + x_rows * 4 : 0) + (sum ? (size_t)top_k * n_out * sizeof(float) : 0);
     int64_t round = std::min<int64_t>({T, 65535, ((int64_t)1 << 20) / top_k, (int64_t)(((size_t)1 << 32) / row_bytes) - 1});
     if (token_bytes) round = std::min<int64_t>(round, (int64_t)(scratch / token_bytes));
+    round = std::min(round, cybq::experts_pairs_max(v, (int)E) / top_k);
     // the way back without sums in memory: few tokens, or a token whose sums do not fit
     if (sum && (cybq::experts_sum_by_token(v, (int)E, T, (int)top_k) || (round < 1 && cybq::experts_token_serves(v)))) {
         for (int64_t t0 = 0, tokens; t0 < T && e == hipSuccess; t0 += tokens) {

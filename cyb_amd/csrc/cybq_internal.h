@@ -104,6 +104,8 @@ hipError_t launch_route(const void* logits, int ldt, int64_t T, int E, int top_k
 bool experts_many(const WeightView& w, int E, int xdt, int64_t P, bool fast);
 size_t experts_lists_bytes(int64_t P, int E);
 size_t experts_stage_bytes(int64_t rows, int K);
+int64_t experts_pairs_max(const WeightView& w, int E);
+constexpr int64_t kMaxExpertRows = (int64_t)1 << 26;             // of one expert: what a grid of one token or row tile may cover
 hipError_t launch_experts(const WeightView& w, int E, bool pair, const void* x, int xdt, int64_t P, int top_k, int xdiv, const int32_t* ids, void* y, int ydt,
                           int num_cus, bool fast, void* lists, void* stage, hipStream_t st);
 // few tokens: y[t] = residual[t] + sum_j weights[t, j] * (x[t * top_k + j] W_ids[t, j]^T) in one launch, without scratch

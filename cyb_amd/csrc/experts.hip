@@ -1160,6 +1160,9 @@ bool experts_many(const WeightView& w, int E, int xdt, int64_t P, bool fast)
     return xdt != kF32 && P >= thr * std::min<int64_t>(P, E);
 }
 
+// pairs of a launch (1024 at least, but for E < 17 960): a grid has fewer than 2^32 threads (at most E + P / 64 row tiles by strips / 16 workgroups of 512)
+int64_t experts_pairs_max(const WeightView& w, int E) { return (((int64_t)1 << 23) / ((w.NT / E + 15) / 16) - E - 1) * kRowTile; }
+
 size_t experts_stage_bytes(int64_t rows, int K) { return (size_t)rows * K * 2 + ((size_t)rows * 4 + 255) / 256 * 256; }
 
 hipError_t launch_experts(const WeightView& w, int E, bool pair, const void* x, int xdt, int64_t P, int top_k, int xdiv, const int32_t* ids, void* y, int ydt,

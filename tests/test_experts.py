@@ -317,6 +317,41 @@ def test_a_token_whose_sums_do_not_fit_the_scratch(backend):
 
 
 @gpu
+def test_row_tiles_beyond_one_grid(backend):
+    """2^20 pairs on wide experts: more row tiles by strips than a grid has threads for; nearly all pairs have no expert."""
+    E, n, K, T, k = 2, 1 << 16, 32, 65535, 16
+    if torch.cuda.mem_get_info()[0] < 160 << 30:
+        pytest.skip("y alone is 137 GB")
+    gate, gd = _stack(backend, 4, E, n, K, 1)
+    up, ud = _stack(backend, 4, E, n, K, 2)
+    w = backend.fuse_pairs(gate, up)
+    x = _rows((T, K), "bf16", 3)
+    ids = torch.full((T, k), -1, dtype=torch.int32, device="cuda")
+    at = torch.tensor([0, 1, 40000, T - 1], device="cuda")
+    ids[at, torch.tensor([0, 15, 7, 15], device="cuda")] = torch.tensor([1, 0, 1, 0], dtype=torch.int32, device="cuda")
+    pairs = (ids.reshape(-1) >= 0).nonzero().reshape(-1)
+    y = torch.empty((T * k, n), dtype=torch.bfloat16, device="cuda")
+    y[pairs[-1] - 1] = 7.0
+    backend.matmul_experts(w, E, x, ids, y, "swiglu")
+    torch.cuda.synchronize()
+    some, e = x[at].contiguous(), ids.reshape(-1)[pairs].reshape(-1, 1).contiguous()
+    ref = _products(some, 1, gd, e)
+    ref = ref * torch.sigmoid(ref) * _products(some, 1, ud, e)
+    _close(y[pairs], ref, 3 * TIGHT + HALF_STEP["bf16"])
+    assert (y[pairs[-1] - 1] == 7.0).all()
+    del y
+    torch.cuda.empty_cache()
+    w.free()
+    q = torch.zeros(((1 << 26) + 16) * 16, dtype=torch.uint8, device="cuda")
+    s = torch.zeros((1 << 26) + 16, dtype=torch.int16, device="cuda")
+    w = backend.weight_from_device(4, (1 << 26) + 16, K, q, s)
+    with pytest.raises(Exception, match="2\\^26 rows"):
+        backend.matmul_experts(w, 1, x[:1], ids[:1, :1].contiguous(), torch.empty((1, (1 << 26) + 16), dtype=torch.float16, device="cuda"))
+    torch.cuda.synchronize()
+    w.free()
+
+
+@gpu
 def test_rows_that_are_not_finite_stay_among_themselves(backend):
     E, n, K, k = 4, 64, 352, 2
     w, wd = _stack(backend, 4, E, n, K, 3)
