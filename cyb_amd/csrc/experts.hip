@@ -40,51 +40,55 @@ __host__ __device__ inline int64_t lists_tiles_max(int64_t P, int E) { return P 
 __host__ __device__ inline int64_t lists_tiles_at(int E) { return (E + 2 + 3) / 4 * 4; }
 __host__ __device__ inline int64_t lists_order_at(int64_t P, int E) { return lists_tiles_at(E) + 4 * lists_tiles_max(P, E); }
 
-__device__ __forceinline__ int block_exclusive_scan(int v, int* wave_sums, int* total)
+// sums of v over the threads ahead of this one, of all threads in `total`; two sums at a time.  wave_sums: [16]
+__device__ __forceinline__ int2 block_exclusive_scan(int2 v, int2* wave_sums, int2* total)
 {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-    int s = v;
+    int2 s = v;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
-        const int o = __shfl_up(s, d);
-        if (lane >= d) s += o;
+        const int2 o = make_int2(__shfl_up(s.x, d), __shfl_up(s.y, d));
+        if (lane >= d) s = make_int2(s.x + o.x, s.y + o.y);
     }
     if (lane == 63) wave_sums[wave] = s;
     __syncthreads();
-    int before = 0, all = 0;
+    int2 before = {0, 0}, all = {0, 0};
     for (int i = 0; i < waves; i++) {
-        const int w = wave_sums[i];
-        if (i < wave) before += w;
-        all += w;
+        const int2 w = wave_sums[i];
+        if (i < wave) before = make_int2(before.x + w.x, before.y + w.y);
+        all = make_int2(all.x + w.x, all.y + w.y);
     }
-    __syncthreads();
     *total = all;
-    return before + s - v;
+    return make_int2(before.x + s.x - v.x, before.y + s.y - v.y);
 }
 
 // Every workgroup counts all pairs (per expert: all of them, and those ahead of its own share), scans the counts, and places its share:
 // a histogram per wave, whose lanes with the same expert find each other by one ballot per bit of the id, so the order does not hang on
-// atomics.  (One workgroup alone placed 16384 pairs in 12 us.)  `block` of `blocks`, 1024 threads.
+// atomics.  (Launch and all, 16384 pairs 8.6 us, 2048 6.6; one workgroup alone placed 16384 in 12, the ids asked for pass by pass and two scans 9.6.)  `block` of `blocks`, 1024 threads.
 __device__ __forceinline__ void make_lists(const int32_t* __restrict__ ids, int P, int E, int bits, int row_tile, int block, int blocks, int32_t* __restrict__ out,
                                            int* lds)
 {
-    int *const total = lds, *const before = lds + E, *const hist = lds + 2 * E, *const wave_sums = lds + 18 * E;      // hist: [16][E]
+    int *const total = lds, *const before = lds + E, *const hist = lds + 2 * E;      // hist: [16][E]
+    int2* const wave_sums = reinterpret_cast<int2*>(lds + 18 * E);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    for (int i = tid; i < 18 * E; i += 1024) lds[i] = 0;
-    __syncthreads();
     const int share = (P + blocks * 1024 - 1) / (blocks * 1024) * 64;         // pairs per wave, whole rounds of 64
     const int first = min(block * 16 * share, P), lo = min(first + wave * share, P), hi = min(lo + share, P);
     int* const my = hist + wave * E;
-    int32_t id[16];
-    auto request = [&](int p0, int end, int step) {              // sixteen ids at a time: one trip to memory, not sixteen
+    int32_t id[16], own[16];
+    auto request = [&](int32_t (&id)[16], int p0, int end, int step) {        // sixteen ids at a time: one trip to memory, not sixteen
 #pragma unroll
         for (int i = 0; i < 16; i++) {
             const int p = p0 + i * step;
             id[i] = p < end ? ids[p] : -1;
         }
     };
+    // the first of both passes on their way while LDS is cleared
+    request(id, tid, P, 1024);
+    request(own, lo + lane, hi, 64);
+    for (int i = tid; i < 18 * E; i += 1024) lds[i] = 0;
+    __syncthreads();
     for (int p0 = tid; p0 < P; p0 += 16384) {
-        request(p0, P, 1024);
+        if (p0 >= 16384) request(id, p0, P, 1024);
 #pragma unroll
         for (int i = 0; i < 16; i++)
             if ((unsigned)id[i] < (unsigned)E) {
@@ -93,17 +97,17 @@ __device__ __forceinline__ void make_lists(const int32_t* __restrict__ ids, int 
             }
     }
     for (int p0 = lo; p0 < hi; p0 += 1024) {
-        request(p0 + lane, hi, 64);
+        if (p0 > lo) request(own, p0 + lane, hi, 64);
 #pragma unroll
         for (int i = 0; i < 16; i++)
-            if ((unsigned)id[i] < (unsigned)E) atomicAdd(&my[id[i]], 1);
+            if ((unsigned)own[i] < (unsigned)E) atomicAdd(&my[own[i]], 1);
     }
     __syncthreads();
     const int count = tid < E ? total[tid] : 0;
-    int pairs, tiles_total;
-    const int start = block_exclusive_scan(count, wave_sums, &pairs);
     const int n_tiles = (count + row_tile - 1) / row_tile;
-    const int tile0 = block_exclusive_scan(n_tiles, wave_sums, &tiles_total);
+    int2 all;
+    const int2 ahead = block_exclusive_scan(make_int2(count, n_tiles), wave_sums, &all);
+    const int start = ahead.x, tile0 = ahead.y;
     if (tid < E) {
         int at = start + before[tid], h[16];
 #pragma unroll
@@ -122,17 +126,17 @@ __device__ __forceinline__ void make_lists(const int32_t* __restrict__ ids, int 
         }
     }
     if (block == 0 && tid == 0) {
-        out[E] = pairs;
-        out[E + 1] = tiles_total;
+        out[E] = all.x;
+        out[E + 1] = all.y;
     }
     __syncthreads();
     int32_t* const order = out + lists_order_at(P, E);
     for (int p0 = lo; p0 < hi; p0 += 1024) {
-        if (share > 1024) request(p0 + lane, hi, 64);            // (else they are still there)
+        if (share > 1024) request(own, p0 + lane, hi, 64);       // (else they are still there)
         for (int i = 0; i < 16 && p0 + i * 64 < hi; i++) {
-            const int e = id[0];
+            const int e = own[0];
 #pragma unroll
-            for (int k = 0; k < 15; k++) id[k] = id[k + 1];
+            for (int k = 0; k < 15; k++) own[k] = own[k + 1];
             const bool there = (unsigned)e < (unsigned)E;
             uint64_t same = __ballot(there);
             for (int b = 0; b < bits; b++) {
@@ -199,7 +203,7 @@ __global__ __launch_bounds__(1024) void experts_prepare_kernel(const int32_t* __
                                                                int32_t* __restrict__ lists, const uint16_t* __restrict__ x, int xdiv, int K,
                                                                uint16_t* __restrict__ staged, float* __restrict__ unscale)
 {
-    extern __shared__ int lists_lds[];                           // 18 * E, then 16 wave sums
+    extern __shared__ int lists_lds[];                           // 18 * E, then 16 pairs of wave sums
     if ((int)blockIdx.x < list_blocks) make_lists(ids, P, E, bits, row_tile, blockIdx.x, list_blocks, lists, lists_lds);
     else stage_row(x, xdiv == 1 ? ids : nullptr, E, P / xdiv, K, (int64_t)((int)blockIdx.x - list_blocks) * 16 + (threadIdx.x >> 6), staged, unscale);
 }
@@ -1181,9 +1185,9 @@ hipError_t launch_experts(const WeightView& w, int E, bool pair, const void* x, 
     if (listed) {
         int bits = 0;
         while ((1 << bits) < E) bits++;
-        (void)LdsRequest<&experts_prepare_kernel, (18 * 1024 + 16) * 4>::registered;
+        (void)LdsRequest<&experts_prepare_kernel, (18 * 1024 + 32) * 4>::registered;
         const int list_blocks = (int)std::min<int64_t>((P + 2047) / 2048, 32);
-        experts_prepare_kernel<<<dim3((unsigned)(list_blocks + (staged ? (rows + 15) / 16 : 0))), 1024, (18 * E + 16) * 4, st>>>(
+        experts_prepare_kernel<<<dim3((unsigned)(list_blocks + (staged ? (rows + 15) / 16 : 0))), 1024, (18 * E + 32) * 4, st>>>(
             ids, (int)P, E, bits, many_rows(w.bits, op), list_blocks, L, static_cast<const uint16_t*>(x), xdiv, w.K, half, unscale);
     }
     ExpertsArgs g = {w.base, x, ids, listed ? L : nullptr, P, xdiv, w.K, w.KT, strips, E, 0, !listed && P <= top_k, !listed && (P <= top_k || P <= E), y, ydt, n_out, nullptr};
