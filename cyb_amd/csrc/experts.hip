@@ -64,7 +64,8 @@ __device__ __forceinline__ int2 block_exclusive_scan(int2 v, int2* wave_sums, in
 
 // Every workgroup counts all pairs (per expert: all of them, and those ahead of its own share), scans the counts, and places its share:
 // a histogram per wave, whose lanes with the same expert find each other by one ballot per bit of the id, so the order does not hang on
-// atomics.  (Launch and all, 16384 pairs 8.6 us, 2048 6.6; one workgroup alone placed 16384 in 12, the ids asked for pass by pass and two scans 9.6.)  `block` of `blocks`, 1024 threads.
+// atomics.  `block` of `blocks`, 1024 threads.  Launch and all, 16384 pairs 8.6 us, 2048 6.6 (with the ids asked for pass by pass and two
+// scans 9.6 and 7.1; one workgroup alone placed 16384 in 12).
 __device__ __forceinline__ void make_lists(const int32_t* __restrict__ ids, int P, int E, int bits, int row_tile, int block, int blocks, int32_t* __restrict__ out,
                                            int* lds)
 {
