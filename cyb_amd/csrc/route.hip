@@ -24,11 +24,14 @@ namespace {
 
 constexpr double kNone = -__builtin_inf();
 
-__device__ __forceinline__ float logit_at(const void* z, int dt, int64_t i)
+// The logits' type is the kernel's: with branches on it between the loads the compiler once (a variant of the rounds, E > 512, a bias) left the
+// index of the bias undefined where the logits were bf16.
+template <int LDT>
+__device__ __forceinline__ float logit_at(const void* z, int64_t i)
 {
-    if (dt == kF32) return static_cast<const float*>(z)[i];
-    if (dt == kF16) return (float)static_cast<const _Float16*>(z)[i];
-    return __builtin_bit_cast(float, (uint32_t) static_cast<const uint16_t*>(z)[i] << 16);
+    if constexpr (LDT == kF32) return static_cast<const float*>(z)[i];
+    else if constexpr (LDT == kF16) return (float)static_cast<const _Float16*>(z)[i];
+    else return __builtin_bit_cast(float, (uint32_t) static_cast<const uint16_t*>(z)[i] << 16);
 }
 
 // v of the lane that step STEP pairs this one with: 0 .. 3 within 16 lanes (mirrors pair lanes whose groups agree in themselves by then),
@@ -106,8 +109,8 @@ template <bool BIAS> struct ChoiceType { typedef float type; };
 template <> struct ChoiceType<true> { typedef double type; };
 
 // PER: experts per lane
-template <int PER, bool BIAS>
-__global__ __launch_bounds__(256) void route_kernel(const void* __restrict__ logits, int ldt, int T, int E, int top_k, int score,
+template <int PER, bool BIAS, int LDT>
+__global__ __launch_bounds__(256) void route_kernel(const void* __restrict__ logits, int T, int E, int top_k, int score,
                                                     const float* __restrict__ bias, int groups, int top_groups, int group_best, int renormalise,
                                                     float scale, int32_t* __restrict__ ids, float* __restrict__ weights)
 {
@@ -126,7 +129,7 @@ __global__ __launch_bounds__(256) void route_kernel(const void* __restrict__ log
     for (int i = 0; i < PER; i++) {
         const int e = i * 64 + lane;
         stands[i] = e < E;
-        z[i] = stands[i] ? logit_at(logits, ldt, (int64_t)t * E + e) : none;
+        z[i] = stands[i] ? logit_at<LDT>(logits, (int64_t)t * E + e) : none;
         if (BIAS) b[i] = stands[i] ? bias[e] : 0.f;
     }
     float top = none;
@@ -248,17 +251,21 @@ hipError_t launch_route(const void* logits, int ldt, int64_t T, int E, int top_k
     const dim3 grid((unsigned)((T + waves - 1) / waves)), block(waves * 64);
     const int per = (E + 63) / 64;
     auto go = [&](auto kernel) {
-        kernel<<<grid, block, groups > 1 ? (size_t)waves * E * 8 : 0, st>>>(logits, ldt, (int)T, E, top_k, score, bias, groups, top_groups, group_best, renormalise ? 1 : 0, scale, ids, weights);
+        kernel<<<grid, block, groups > 1 ? (size_t)waves * E * 8 : 0, st>>>(logits, (int)T, E, top_k, score, bias, groups, top_groups, group_best, renormalise ? 1 : 0, scale, ids, weights);
     };
-    auto with = [&](auto bias_) {
+    auto with = [&](auto bias_, auto ldt_) {
         constexpr bool B = decltype(bias_)::value;
-        if (per <= 1) go(route_kernel<1, B>);
-        else if (per <= 2) go(route_kernel<2, B>);
-        else if (per <= 4) go(route_kernel<4, B>);
-        else if (per <= 8) go(route_kernel<8, B>);
-        else go(route_kernel<16, B>);
+        constexpr int L = decltype(ldt_)::value;
+        if (per <= 1) go(route_kernel<1, B, L>);
+        else if (per <= 2) go(route_kernel<2, B, L>);
+        else if (per <= 4) go(route_kernel<4, B, L>);
+        else if (per <= 8) go(route_kernel<8, B, L>);
+        else go(route_kernel<16, B, L>);
     };
-    bias ? with(std::true_type{}) : with(std::false_type{});
+    auto with_bias = [&](auto ldt_) { bias ? with(std::true_type{}, ldt_) : with(std::false_type{}, ldt_); };
+    if (ldt == kF32) with_bias(std::integral_constant<int, kF32>{});
+    else if (ldt == kF16) with_bias(std::integral_constant<int, kF16>{});
+    else with_bias(std::integral_constant<int, kBF16>{});
     return hipGetLastError();
 }
 
