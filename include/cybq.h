@@ -313,7 +313,10 @@ int cybq_route(cybq_ctx* ctx, const void* logits, cybq_dtype ldt, int64_t T, int
  *   cybq_weight_fuse_pairs), must not overlap x.  CYBQ_EPI_ADD is not taken.  Rows of y without an expert stay as
  *   they were.  T >= 0, K <= 2^24.
  * Operands are exact whatever the decode mode: the integers q, the groups' scales in fp32 on their sums, fp32 rows in
- * three bf16 parts (below 1e-6 relative L2 on fp32 y; |x| of bf16 and fp32 rows up to 4e34, as in the decode kernels).
+ * three bf16 parts (|x| of bf16 and fp32 rows up to 4e34, as in the decode kernels).  The G = K / 32 groups of a row are
+ * added one after another in fp32, so the error grows with K.  Relative L2 of an fp32 y, rows and weights of both signs:
+ * below 2^-24 (4 + sqrt(G)) for 16-bit rows (7e-7 at K = 2048, 1.5e-6 at 14336, 8e-6 at 524288), below
+ * 2^-24 (8 + 2 sqrt(G)) for fp32 rows (1.4e-6, 3e-6, 1.6e-5).
  * With CYBQ_PREFILL_FAST, 16-bit rows, a y of bf16 and 24 (Q8: 20) pairs and more per expert they are round_f16(scale * q)
  * instead, bf16 rows f16 behind a power of two (2e-4 next to the 1.6e-3 of y's own rounding; not for weights with wide
  * scales).  Which it is goes by the whole call, so the last bits of a row may change with the batch.  A row with an
