@@ -319,8 +319,10 @@ int cybq_route(cybq_ctx* ctx, const void* logits, cybq_dtype ldt, int64_t T, int
  * 2^-24 (8 + 2 sqrt(G)) for fp32 rows (1.4e-6, 3e-6, 1.6e-5).
  * With CYBQ_PREFILL_FAST, 16-bit rows, a y of bf16 and 24 (Q8: 20) pairs and more per expert they are round_f16(scale * q)
  * instead, bf16 rows f16 behind a power of two (2e-4 next to the 1.6e-3 of y's own rounding; not for weights with wide
- * scales).  Which it is goes by the whole call, so the last bits of a row may change with the batch.  A row with an
- * element that is Inf, NaN or beyond the range above gives Inf or NaN; other rows are not touched by it. */
+ * scales).  The pairs per expert are T * top_k, absent ones too, over min(E, T * top_k) - of the call, and where it is worked
+ * on in rounds (sums or rows that do not fit the scratch, 2^20 pairs) of a round -, so the last bits of a row may change with
+ * the batch.  A row with an element that is Inf, NaN or beyond the range above gives Inf or NaN; other rows are not touched
+ * by it. */
 int cybq_matmul_experts(cybq_ctx* ctx, const cybq_weight* w, int64_t E, const void* x, cybq_dtype xdt, int64_t T,
                         int64_t top_k, const int32_t* ids, void* y, cybq_dtype ydt, cybq_epilogue epilogue, void* stream);
 

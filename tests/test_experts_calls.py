@@ -1,0 +1,68 @@
+"""Calls of the mixture-of-experts operators that meet the limits of a context's scratch, of a capture and of their arguments."""
+import pytest
+
+torch = pytest.importorskip("torch")
+gpu = pytest.mark.gpu
+
+
+def planes(bits, N, K, seed):
+    """A quantised tensor on the device (q, scales) and its float64 values."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    q = torch.randint(0, 256, (N * K * bits // 8,), dtype=torch.uint8, device="cuda", generator=g)
+    s = (0.01 * (0.5 + torch.rand((N, K // 32), device="cuda", generator=g))).half()
+    v = torch.stack([q & 15, q >> 4], dim=1).reshape(N, K).double() if bits == 4 else q.view(torch.int8).reshape(N, K).double()
+    v = torch.where(v >= 8, v - 16, v) if bits == 4 else v
+    return q, s.view(torch.int16), v * s.double().repeat_interleave(32, dim=1)
+
+
+def normal(shape, seed, dtype=torch.bfloat16):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.empty(shape, device="cuda").normal_(generator=g).to(dtype)
+
+
+def products(x, xdiv, wd, ids):
+    """float64 [P, n], zeros for pairs without an expert."""
+    flat = ids.reshape(-1).long()
+    out = torch.zeros((flat.numel(), wd.shape[1]), dtype=torch.float64, device="cuda")
+    for e in range(wd.shape[0]):
+        p = torch.nonzero(flat == e).reshape(-1)
+        if p.numel():
+            out[p] = x.double()[p // xdiv] @ wd[e].T.contiguous()
+    return out
+
+
+@gpu
+def test_rounds_that_the_scratch_sets(backend):
+    """4096 tokens x 8 x 2048 outputs: 268 MB of sums, more than the scratch has; with them the lists, the staged rows and their factors.  The last round
+    has fewer pairs than the kernel for many rows takes for 200 experts.  The decode kernels' tickets behind it all are zero at rest, and stay so."""
+    E, n, K, T, k = 200, 2048, 160, 4096, 8
+    q, s, wd = planes(4, E * n, K, 1)
+    w = backend.weight_from_device(4, E * n, K, q, s)
+    dq, ds, _ = planes(4, 4096, 4096, 2)
+    dense = backend.weight_from_device(4, 4096, 4096, dq, ds)
+    one = normal((1, 4096), 3, torch.float16)
+    before, after = (torch.empty((1, 4096), device="cuda") for _ in range(2))
+    backend.matmul(dense, one, before)
+    ids = torch.randint(0, E, (T, k), device="cuda", generator=torch.Generator(device="cuda").manual_seed(4)).int()
+    ids[T - 300:][torch.rand((300, k), device="cuda") < 0.3] = -1
+    ids[T - 7:] = E
+    x, residual = normal((T * k, K), 5), normal((T, n), 6)
+    g = torch.rand((T, k), device="cuda")
+    y = torch.full((T + 1, n), float("nan"), dtype=torch.bfloat16, device="cuda")
+    backend.matmul_experts_sum(w, E, x, ids, g, y[:T], residual)
+    backend.matmul(dense, one, after)
+    torch.cuda.synchronize()
+    assert torch.isnan(y[T]).all() and torch.equal(y[T - 7:T], residual[T - 7:]) and torch.equal(before, after)
+    z = products(x, 1, wd.reshape(E, n, K), ids) * g.double().reshape(-1, 1)
+    z = z.reshape(T, k, n)
+    ref = residual.double() + z.sum(dim=1)
+    # weights rounded to f16 (2^-11 at most), y to bf16 (2^-8): of the products' and of y's size
+    size = z.square().sum(dim=(1, 2)).sqrt() * 2.0 ** -11 + ref.norm(dim=1) * 2.0 ** -8
+    assert ((y[:T].double() - ref).norm(dim=1) <= size).all()
+    # the same tokens in calls that fit one round: the same bits, where the kernel is the same (the first round's)
+    some = torch.empty((1500, n), dtype=torch.bfloat16, device="cuda")
+    backend.matmul_experts_sum(w, E, x[:1500 * k], ids[:1500], g[:1500], some, residual[:1500])
+    torch.cuda.synchronize()
+    assert torch.equal(some, y[:1500])
+    for h in (w, dense):
+        h.free()
