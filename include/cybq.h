@@ -288,7 +288,9 @@ int cybq_matmul_many_norm(cybq_ctx* ctx, int64_t count, const cybq_weight* const
  * ids[t * top_k + j] is the expert of pair (t, j), token t's j-th.  An id outside 0 .. E - 1 is no expert (the rows of a
  * padded batch, experts that live elsewhere): nothing is read for it.  An expert may be named twice, by one token too.
  * Limits: E <= CYBQ_MAX_EXPERTS, top_k <= CYBQ_MAX_TOP_K, 2^26 rows per expert.  ids and weights are device memory; calls neither look at
- * them on the host nor allocate, so they can be captured.  Like all calls they share the context's scratch: calls on
+ * them on the host nor allocate, so they can be captured.  (The first call
+ * with CYBQ_PREFILL_FAST, many rows and a y of bf16 on a weight from cybq_weight_from_device waits once on the host, captured
+ * or not, for the scan of its scales.)  Like all calls they share the context's scratch: calls on
  * one context (replays of its graphs too) must not overlap in time. */
 #define CYBQ_MAX_EXPERTS 1024
 #define CYBQ_MAX_TOP_K 64

@@ -1,6 +1,8 @@
 """Calls of the mixture-of-experts operators that meet the limits of a context's scratch, of a capture and of their arguments."""
 import pytest
 
+from cyb_amd.backend import Backend
+
 torch = pytest.importorskip("torch")
 gpu = pytest.mark.gpu
 
@@ -66,3 +68,44 @@ def test_rounds_that_the_scratch_sets(backend):
     assert torch.equal(some, y[:1500])
     for h in (w, dense):
         h.free()
+
+
+@gpu
+@pytest.mark.parametrize("down", [False, True])
+def test_the_first_call_on_a_weight_may_sit_in_a_capture(down):
+    """Rounded operands hang on the scan of the weight's scales, which a stack made from device memory has not been asked for before its first call."""
+    be = Backend(0)
+    try:
+        E, n, K, T, k = 4, 64, 256, 150, 2
+        q, s, wd = planes(4, E * n, K, 7)
+        w = be.weight_from_device(4, E * n, K, q, s)
+        torch.cuda.synchronize()
+        ids = torch.randint(0, E, (T, k), device="cuda").int()
+        x, g = normal((T * k if down else T, K), 8), torch.rand((T, k), device="cuda")
+        y = torch.zeros((T if down else T * k, n), dtype=torch.bfloat16, device="cuda")
+
+        def call(stream=0):
+            if down:
+                be.matmul_experts_sum(w, E, x, ids, g, y, stream=stream)
+            else:
+                be.matmul_experts(w, E, x, ids, y, stream=stream)
+
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+            call(torch.cuda.current_stream().cuda_stream)
+        for i in range(3):
+            x.copy_(normal(tuple(x.shape), 10 + i))
+            y.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            got = y.clone()
+            call()
+            torch.cuda.synchronize()
+            assert torch.equal(got, y)
+            ref = products(x, 1 if down else k, wd.reshape(E, n, K), ids)
+            if down:
+                ref = (ref * g.double().reshape(-1, 1)).reshape(T, k, n).sum(dim=1)
+            assert ((got.double() - ref).norm() / ref.norm()).item() < 2.0 ** -8 + 2.0 ** -11
+        w.free()
+    finally:
+        be.close()
