@@ -1047,7 +1047,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(4, 4))) voi
 // ---- few tokens, the way back: a token's experts one after the other as one long K, their weights on the groups' scales --------------
 //
 // y[t, n] = residual[t, n] + sum over the pairs and K: workgroup = a strip of 16 columns and a token, its eight waves share out the
-// top_k * KT tiles.  One launch and no sums in memory, but an expert's weights are read once per token.
+// KT tiles of every pair that has an expert (a token's absent pairs cost nothing).  One launch and no sums in memory, but an expert's weights are
+// read once per token.
 struct TokenArgs {
     const uint8_t* w;
     const void* x;
@@ -1070,19 +1071,27 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(4, 4))) voi
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int N = g.strips * 16, n = strip * 16 + (lane & 15), G = g.K / kGroup;
     const int64_t p0 = (int64_t)t * g.top_k, at = (int64_t)t * N + n;
-    const int id = lane < g.top_k ? g.ids[p0 + lane] : -1;       // lane j: pair j's
-    const float weight = lane < g.top_k ? g.weights[p0 + lane] : 0.f;
+    int id = lane < g.top_k ? g.ids[p0 + lane] : -1, pair = lane;       // lane j: pair j's
+    float weight = lane < g.top_k ? g.weights[p0 + lane] : 0.f;
     const float first = g.residual ? load_out(g.residual, g.ydt, at) : 0.f;
-    const int tiles = g.top_k * g.KT;
-    float acc[2];
-    stream_row<BITS, XM, false>((tiles + 15) / 16, [&](int step, int s) {
+    const uint64_t with = __ballot((unsigned)id < (unsigned)g.E);
+    const int pairs = __popcll(with);
+    if (pairs != g.top_k) {
+        // lane j: the j-th pair that has an expert, in their order; the rest behind them, and no tile is theirs
+        const uint64_t below = (1ull << lane) - 1;
+        const int to = 4 * ((with >> lane) & 1 ? __popcll(with & below) : pairs + __popcll(~with & below));
+        id = __builtin_amdgcn_ds_permute(to, id);
+        pair = __builtin_amdgcn_ds_permute(to, pair);
+        weight = __builtin_bit_cast(float, __builtin_amdgcn_ds_permute(to, __builtin_bit_cast(int, weight)));
+    }
+    const int tiles = pairs * g.KT;
+    float acc[2] = {0.f, 0.f};
+    if (tiles) stream_row<BITS, XM, false>((tiles + 15) / 16, [&](int step, int s) {
         const int u = (step * 8 + wave) * 2 + s, v = min(u, tiles - 1);
         const int j = g.KT == 1 ? v : (int)__umulhi((uint32_t)v, g.per_kt), kt = v - j * g.KT;
-        const int e = __builtin_amdgcn_readlane(id, j);
-        const bool there = u < tiles && (unsigned)e < (unsigned)g.E;
-        return RowTile{g.w + (((int64_t)(there ? e : 0) * g.strips + strip) * g.KT + kt) * kTileBytes<BITS>,
-                       static_cast<const char*>(g.x) + (p0 + j) * g.K * XS + (int64_t)kt * (kTileK * XS), there ? min(G - kt * 4, 4) : 0,
-                       __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, weight), j))};
+        return RowTile{g.w + (((int64_t)__builtin_amdgcn_readlane(id, j) * g.strips + strip) * g.KT + kt) * kTileBytes<BITS>,
+                       static_cast<const char*>(g.x) + (p0 + __builtin_amdgcn_readlane(pair, j)) * g.K * XS + (int64_t)kt * (kTileK * XS),
+                       u < tiles ? min(G - kt * 4, 4) : 0, __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, weight), j))};
     }, acc, smem);
     float* const red = reinterpret_cast<float*>(smem);
     __syncthreads();

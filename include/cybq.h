@@ -286,12 +286,13 @@ int cybq_matmul_many_norm(cybq_ctx* ctx, int64_t count, const cybq_weight* const
  * A stack of E experts is ONE weight of E * n rows (expert e is rows [e * n, (e + 1) * n)), uploaded like any other
  * tensor; n must be a multiple of 16.  Gate and up of all experts: cybq_weight_fuse_pairs of the two stacks.
  * ids[t * top_k + j] is the expert of pair (t, j), token t's j-th.  An id outside 0 .. E - 1 is no expert (the rows of a
- * padded batch, experts that live elsewhere): nothing is read for it.  An expert may be named twice, by one token too.
- * Limits: E <= CYBQ_MAX_EXPERTS, top_k <= CYBQ_MAX_TOP_K, 2^26 rows per expert.  ids and weights are device memory; calls neither look at
- * them on the host nor allocate, so they can be captured.  (The first call
- * with CYBQ_PREFILL_FAST, many rows and a y of bf16 on a weight from cybq_weight_from_device waits once on the host, captured
- * or not, for the scan of its scales.)  Like all calls they share the context's scratch: calls on
- * one context (replays of its graphs too) must not overlap in time. */
+ * padded batch, experts that live elsewhere): no weights are read for it, and nothing of its row or its weight enters a
+ * result.  An expert may be named twice, by one token too.
+ * Limits: E <= CYBQ_MAX_EXPERTS, top_k <= CYBQ_MAX_TOP_K, 2^26 rows per expert.  ids and weights are device memory; calls
+ * neither look at them on the host nor allocate, so they can be captured.  (The first call with CYBQ_PREFILL_FAST, many rows
+ * and a y of bf16 on a weight from cybq_weight_from_device waits once on the host, captured or not, for the scan of its
+ * scales.)  Like all calls they share the context's scratch: calls on one context (replays of its graphs too) must not
+ * overlap in time. */
 #define CYBQ_MAX_EXPERTS 1024
 #define CYBQ_MAX_TOP_K 64
 

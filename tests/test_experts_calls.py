@@ -109,3 +109,37 @@ def test_the_first_call_on_a_weight_may_sit_in_a_capture(down):
         w.free()
     finally:
         be.close()
+
+
+@pytest.fixture
+def tuned(backend):
+    yield backend.set_experts_tuning
+    backend.set_experts_tuning()
+
+
+@gpu
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("K", [32, 768, 1312, 4096])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_pairs_without_an_expert_take_no_part_token_by_token(backend, tuned, bits, K, dt):
+    """A token's absent pairs leave no trace: the same bits as a call of the pairs that are there alone, whatever stands in the others' rows and weights."""
+    E, n, k = 9, 48, 8
+    q, s, _ = planes(bits, E * n, K, 11)
+    w = backend.weight_from_device(bits, E * n, K, q, s)
+    tuned(0, 0, 1)
+    for there in ([], [0], [7], [1, 4], [0, 2, 5], [1, 3, 4, 6, 7], list(range(8))):
+        T, j = 3, torch.tensor(there, dtype=torch.long, device="cuda")
+        x = normal((T, k, K), 12, dt)
+        ids = torch.randint(0, E, (T, k), device="cuda", generator=torch.Generator(device="cuda").manual_seed(13)).int()
+        g, residual = torch.rand((T, k), device="cuda"), normal((T, n), 14, torch.float32)
+        want = residual.clone()
+        if there:
+            backend.matmul_experts_sum(w, E, x[:, j].reshape(-1, K).contiguous(), ids[:, j].contiguous(), g[:, j].contiguous(), want, residual)
+        absent = torch.tensor([i for i in range(k) if i not in there], dtype=torch.long, device="cuda")
+        ids[:, absent], g[:, absent], x[:, absent] = -1, float("nan"), float("inf")
+        ids[1, absent] = E
+        y = torch.full((T, n), float("nan"), device="cuda")
+        backend.matmul_experts_sum(w, E, x.reshape(-1, K), ids, g, y, residual)
+        torch.cuda.synchronize()
+        assert torch.equal(y, want), there
+    w.free()
