@@ -5,6 +5,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <cstdio>
 #include <cstring>
 #include <mutex>
@@ -655,6 +656,7 @@ int cybq_route(cybq_ctx* ctx, const void* logits, cybq_dtype ldt, int64_t T, int
     if (groups < 1 || groups > 64 || E % groups) return fail(ctx, CYBQ_ERR_SHAPE, "groups must be in 1..64 and divide E");
     if (top_groups < 1 || top_groups > groups) return fail(ctx, CYBQ_ERR_SHAPE, "top_groups must be in 1..groups");
     if (group_best != 1 && group_best != 2) return fail(ctx, CYBQ_ERR_INVALID, "group_best must be 1 or 2");
+    if (!std::isfinite(scale)) return fail(ctx, CYBQ_ERR_INVALID, "scale must be finite");
     if (top_k < 1 || top_k > CYBQ_MAX_TOP_K || top_k > top_groups * (E / groups))
         return fail(ctx, CYBQ_ERR_SHAPE, "top_k must be in 1..CYBQ_MAX_TOP_K and no more than the experts of top_groups groups");
     if (reinterpret_cast<uintptr_t>(logits) % dtype_size(ldt) || reinterpret_cast<uintptr_t>(ids) % 4 || reinterpret_cast<uintptr_t>(weights) % 4 ||

@@ -1,7 +1,7 @@
 """Calls of the mixture-of-experts operators that meet the limits of a context's scratch, of a capture and of their arguments."""
 import pytest
 
-from cyb_amd.backend import Backend
+from cyb_amd.backend import Backend, CybqError
 
 torch = pytest.importorskip("torch")
 gpu = pytest.mark.gpu
@@ -143,3 +143,19 @@ def test_pairs_without_an_expert_take_no_part_token_by_token(backend, tuned, bit
         torch.cuda.synchronize()
         assert torch.equal(y, want), there
     w.free()
+
+
+@gpu
+def test_the_router_s_scale_is_finite(backend):
+    """Times a score of 0 an infinite scale would be NaN, which weights never are; rows without any score are what it would show in."""
+    z = torch.full((3, 8), float("-inf"), device="cuda")
+    ids, w = torch.full((3, 2), -5, dtype=torch.int32, device="cuda"), torch.full((3, 2), -5.0, device="cuda")
+    for scale in (float("inf"), float("-inf"), float("nan"), 1e300):                  # (1e300 is infinite as a float)
+        with pytest.raises(CybqError) as e:
+            backend.route(z, ids, w, scale=scale)
+        assert e.value.status == -1
+        torch.cuda.synchronize()
+        assert (ids == -5).all() and (w == -5).all()
+    backend.route(z, ids, w, scale=3.4e38)
+    torch.cuda.synchronize()
+    assert (w == 0).all() and (ids.cpu() == torch.tensor([0, 1])).all()
