@@ -288,7 +288,7 @@ int cybq_matmul_many_norm(cybq_ctx* ctx, int64_t count, const cybq_weight* const
  * ids[t * top_k + j] is the expert of pair (t, j), token t's j-th.  An id outside 0 .. E - 1 is no expert (the rows of a
  * padded batch, experts that live elsewhere): no weights are read for it, and nothing of its row or its weight enters a
  * result.  An expert may be named twice, by one token too.
- * Limits: E <= CYBQ_MAX_EXPERTS, top_k <= CYBQ_MAX_TOP_K, 2^26 rows per expert.  ids and weights are device
+ * Limits: E <= CYBQ_MAX_EXPERTS, top_k <= CYBQ_MAX_TOP_K, T <= 2^24, 2^26 rows per expert.  ids and weights are device
  * memory; calls neither look at them on the host nor allocate, so they can be captured.  (The first call with
  * CYBQ_PREFILL_FAST, many rows and a y of bf16 on a weight from cybq_weight_from_device waits once on the host, captured or
  * not, for the scan of its scales.)  Like all calls they share the context's scratch: calls on one context (replays of its
@@ -304,9 +304,10 @@ typedef enum cybq_score { CYBQ_SCORE_SOFTMAX = 0, CYBQ_SCORE_SIGMOID = 1 } cybq_
  *     bias is NULL), the experts of the top_groups best groups stand for choice
  *     ids[t, 0 .. top_k) = the largest c among them in falling order, of equal ones the lowest index first
  *     weights[t, j] = s[ids[t, j]], divided by their sum over j if `renormalise`, times `scale`
- * All in fp64, weights rounded once.  A logit of -inf or NaN scores 0 and is chosen after all others; logits of +inf
- * share a softmax among them; a row without any score above 0 has weights of 0 (never NaN).  A bias of NaN counts as -inf.  scale is
- * finite.  top_k <= top_groups * (E / groups). */
+ * All in fp64, weights rounded once.  A logit of -inf or NaN scores 0: without a bias it is chosen after all others, with one
+ * it stands with c = bias like any score of 0 (an expert that must not be chosen gets a bias of -inf); logits of +inf share a
+ * softmax among them; a row without any score above 0 has weights of 0 (never NaN).  A bias of NaN counts as -inf.  scale is
+ * finite.  top_k <= top_groups * (E / groups).  ids and weights must not overlap the logits or the bias. */
 int cybq_route(cybq_ctx* ctx, const void* logits, cybq_dtype ldt, int64_t T, int64_t E, int64_t top_k, cybq_score score,
                const float* bias, int64_t groups, int64_t top_groups, int group_best, int renormalise, float scale,
                int32_t* ids, float* weights, void* stream);
@@ -331,7 +332,7 @@ int cybq_matmul_experts(cybq_ctx* ctx, const cybq_weight* w, int64_t E, const vo
 
 /* The way back:  y[t, :] = residual[t, :] + sum_j weights[t * top_k + j] * (x[t * top_k + j, :] W_e^T), e = ids[t * top_k + j].
  *   x [T * top_k, K]; weights fp32; residual [T, n] of ydt or NULL (zeros), may alias y; y [T, n], every row is
- *   written.  Added in fp32 in a fixed order, rounded once; operands as above.
+ *   written and must not overlap x.  Added in fp32 in a fixed order, rounded once; operands as above.
  *   CYBQ_ERR_UNSUPPORTED for K over 524288 where one token's top_k * n sums do not fit the scratch or its top_k rows of x
  *   are over 2 GiB. */
 int cybq_matmul_experts_sum(cybq_ctx* ctx, const cybq_weight* w, int64_t E, const void* x, cybq_dtype xdt, int64_t T,

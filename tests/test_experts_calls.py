@@ -159,3 +159,19 @@ def test_the_router_s_scale_is_finite(backend):
     backend.route(z, ids, w, scale=3.4e38)
     torch.cuda.synchronize()
     assert (w == 0).all() and (ids.cpu() == torch.tensor([0, 1])).all()
+
+
+@gpu
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_a_logit_without_a_score_and_a_bias(backend, score):
+    """-inf and NaN score 0: behind all others without a bias, c = bias with one; a bias of -inf keeps an expert out."""
+    inf, nan = float("inf"), float("nan")
+    z = torch.tensor([[-inf, 0.0, nan, 0.5, 0.25, -3.0]], device="cuda")
+    bias = torch.tensor([2.0, 0.0, 3.0, -inf, 0.0, 0.0], device="cuda")
+    ids, w = torch.empty((1, 6), dtype=torch.int32, device="cuda"), torch.empty((1, 6), device="cuda")
+    backend.route(z, ids, w, score=score)
+    torch.cuda.synchronize()
+    assert ids.tolist() == [[3, 4, 1, 5, 0, 2]] and w[0, 4:].tolist() == [0.0, 0.0] and (w[0, :4] > 0).all()
+    backend.route(z, ids, w, score=score, bias=bias)
+    torch.cuda.synchronize()
+    assert ids.tolist() == [[2, 0, 4, 1, 5, 3]] and w[0, :2].tolist() == [0.0, 0.0] and (w[0, 2:] > 0).all()
