@@ -14,11 +14,15 @@
 // scale in fp32, so scales that leave f16's range when multiplied with q do no harm - but for many rows and a y of bf16 in FAST mode, where they
 // are round_f16(scale * q): 2e-4 relative L2 next to the 1.6e-3 of y's own rounding, and no FMAs behind the MFMAs.
 //
-// us per call, weights from HBM (bytes of the met experts' weights, rows and outputs; products without the bias'):
-//   up, 8 of 128 experts of 2048 -> 2 x 768, Q4, one f16 token 5.3 (14 MB); back 6.4 (7 MB)         the launch, three trips to memory, the stream
-//   up, 2 of 8 of 4096 -> 2 x 14336, 16 bf16 tokens 98 (524 MB: 5.3 TB/s); back, 32 f16 tokens 46 - 57 (267 MB: 4.7 - 5.8 TB/s)           HBM
-//   up, 4 of 60 of 2592 -> 2 x 1040, Q8, 37 f16 tokens 55 - 69 (306 MB at most)                                                       HBM
-//   up, 8 of 128, 2048 bf16 tokens 158 - 170 (103 GFLOP: 0.63 PFLOP/s); back 156 - 164; 2 of 8 wide ones, 1024 tokens 508 - 529 (481 GFLOP: 0.93)
+// us per call, weights from HBM: 680 MB of others' and more are read in between (bytes: weights of the experts that the timed ids meet, rows and
+// outputs; products without the bias'):
+//   up, 8 of 128 experts of 2048 -> 2 x 768, Q4, one f16 token 7.2 (14 MB; 5.1 - 5.8 where the 256 MB cache has them); back 6.9 (7 MB; 6.4)
+//                                                                                     the launch, three trips to memory, the stream
+//   up, 2 of 8 of 4096 -> 2 x 14336, 16 bf16 tokens 97 (7.75 met: 513 MB, 5.3 TB/s); back, 32 f16 tokens 58 (267 MB, 4.6 TB/s; 46 - 57 with
+//                                                                                     a part of them cached)                      HBM
+//   up, 4 of 60 of 2592 -> 2 x 1040, Q8, 37 f16 tokens 69 (51 met: 293 MB, 4.2 TB/s; 55 - 69 partly cached)                        HBM
+//   up, 8 of 128, 2048 bf16 tokens 155 - 173 (103 GFLOP: 0.60 - 0.67 PFLOP/s); back 156 - 167; 2 of 8 wide ones, 1024 tokens 508 - 541 (481 GFLOP:
+//   0.89 - 0.95), each over runs on several machines
 #include <algorithm>
 #include <type_traits>
 
@@ -661,7 +665,7 @@ __device__ __forceinline__ void expert_row(const ExpertsArgs& g, int e, int p, i
 // clumps of them ahead of the MFMAs, and all copies at once behind the barrier, cost 7 %.  2 of 8 experts of 4096 -> 2 x 14336, 1024 bf16 tokens: 860 us
 // with exact operands and two workgroups of 64 rows to a CU, 685 with rounded ones, 596 with one of 128 rows, 529 now; without its
 // copies 411, without its MFMAs 412, so it is neither alone but what of both does not overlap: eight waves that meet at a barrier per K tile.
-// Tried: workgroups that stay and look the next item up behind the products (529 -> 550: tiles differ in length); K tiles started at
+// Tried on that case, where a workgroup's start and end hardly count (32 K tiles): workgroups that stay and look the next item up behind the products (529 -> 550: tiles differ in length); K tiles started at
 // different places by the workgroups that share rows (566 -> 692); row tiles outermost (566 -> 590).
 //   OP 0 / 1  exact operands, f16 / bf16 rows: a strip and group starts from zero (bf16: from the product that takes the bias off, one
 //             for four strips), its sums are scaled on their way into the fp32 accumulators, four FMAs per MFMA

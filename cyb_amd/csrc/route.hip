@@ -11,8 +11,8 @@
 //
 // What bounds it is the length of one wave's chain: a launch with no work is 2 us, a trip to memory 1 us.  Lanes meet through DPP and the
 // row swaps, a few cycles each; through ds_bpermute (two per fp64 step, 100 cycles and more) a maximum took 900 cycles.  us before that / with
-// it / now (fp32 keys of c, groups' scores through LDS): one token of 128 experts 5.5 / 3.7 / 3.7 (the host), 48 tokens of 160 experts in 8 groups
-// 9.7 / 7.6 / 5.7, 8192 tokens of 256 experts in 8 groups 36 / 23.5 / 17 - 19, where what is left are the fp64 exponentials and divisions of 2 M scores and
+// it / now (fp32 keys of c, groups' scores through LDS): one token of 128 experts 5.5 / 3.7 / 3.7 - 4.5 (the host), 48 tokens of 160 experts in 8 groups
+// 9.7 / 7.6 / 5.5, 8192 tokens of 256 experts in 8 groups 36 / 23.5 / 17 - 19, where what is left are the fp64 exponentials and divisions of 2 M scores and
 // eight rounds of some 200 cycles, eight waves to a SIMD.
 #include <type_traits>
 
