@@ -665,8 +665,9 @@ __device__ __forceinline__ void expert_row(const ExpertsArgs& g, int e, int p, i
 // clumps of them ahead of the MFMAs, and all copies at once behind the barrier, cost 7 %.  2 of 8 experts of 4096 -> 2 x 14336, 1024 bf16 tokens: 860 us
 // with exact operands and two workgroups of 64 rows to a CU, 685 with rounded ones, 596 with one of 128 rows, 529 now; without its
 // copies 411, without its MFMAs 412, so it is neither alone but what of both does not overlap: eight waves that meet at a barrier per K tile.
-// Tried on that case, where a workgroup's start and end hardly count (32 K tiles): workgroups that stay and look the next item up behind the products (529 -> 550: tiles differ in length); K tiles started at
-// different places by the workgroups that share rows (566 -> 692); row tiles outermost (566 -> 590).
+// Tried on that case, where a workgroup's start and end hardly count (32 K tiles): workgroups that stay and look the next item up behind the
+// products (529 -> 550: tiles differ in length); K tiles started at different places by the workgroups that share rows (566 -> 692); row
+// tiles outermost (566 -> 590).
 //   OP 0 / 1  exact operands, f16 / bf16 rows: a strip and group starts from zero (bf16: from the product that takes the bias off, one
 //             for four strips), its sums are scaled on their way into the fp32 accumulators, four FMAs per MFMA
 //   OP 2      f16 rows (bf16 ones behind a power of two per row), operands round_f16(scale * q), one MFMA and no FMAs
