@@ -8,8 +8,8 @@ node, `Backend.run` executes it.  All arithmetic happens in libcybq.so
 (hand-written HIP, C ABI in include/cybq.h); this package never computes the
 op on the host and raises if the library is missing.
 """
-from .backend import Backend, CybqError, QMatMul, QWeight, library_path
+from .backend import Backend, CacheBatch, CybqError, KVCache, QMatMul, QWeight, library_path
 from . import container, driver, formats, stack, synth
 
-__all__ = ["Backend", "CybqError", "QMatMul", "QWeight", "library_path", "formats", "synth", "container", "stack", "driver"]
+__all__ = ["Backend", "CacheBatch", "CybqError", "KVCache", "QMatMul", "QWeight", "library_path", "formats", "synth", "container", "stack", "driver"]
 __version__ = "0.1.0"

@@ -39,6 +39,8 @@ _CALLS_PATH = os.path.join(_HERE, "lib", "_torch_calls.so")
 F32, F16, BF16 = 0, 1, 2
 EPILOGUES = {"none": 0, "add": 1, "swiglu": 2}      # enum cybq_epilogue
 SCORES = {"softmax": 0, "sigmoid": 1}               # enum cybq_score
+CACHE_KINDS = {"f16": 1, "bf16": 2, "q4": 4, "q8": 8}     # enum cybq_cache_kind
+ROPE_STYLES = {"halves": 0, "pairs": 1}             # enum cybq_rope_style
 _DTYPE_CODES = {"torch.float32": F32, "torch.float16": F16, "torch.bfloat16": BF16,
                 "float32": F32, "float16": F16}
 _ITEMSIZE = {F32: 4, F16: 2, BF16: 2}
@@ -98,6 +100,12 @@ def load_library() -> ctypes.CDLL:
     lib.cybq_route.argtypes = [vp, vp, ci, i64, i64, i64, ci, vp, i64, i64, ci, ci, ctypes.c_float, vp, vp, vp]
     lib.cybq_matmul_experts.argtypes = [vp, vp, i64, vp, ci, i64, i64, vp, vp, ci, ci, vp]
     lib.cybq_matmul_experts_sum.argtypes = [vp, vp, i64, vp, ci, i64, i64, vp, vp, vp, vp, ci, vp]
+    lib.cybq_cache_create.argtypes = [vp, ci, i64, i64, i64, i64, i64, ctypes.POINTER(vp)]
+    lib.cybq_cache_free.argtypes = [vp, vp]
+    lib.cybq_cache_info.argtypes = [vp, ctypes.POINTER(ci)] + [ctypes.POINTER(i64)] * 7 + [ctypes.POINTER(vp)]
+    lib.cybq_cache_append.argtypes = [vp, vp, i64, vp, vp, i64, i64, vp, i64, vp, i64, ci, vp, i64, i64, ci, vp, ci, vp]
+    lib.cybq_cache_read.argtypes = [vp, vp, i64, vp, vp, vp, ci, vp]
+    lib.cybq_attention.argtypes = [vp, vp, i64, vp, vp, i64, ci, i64, ctypes.c_float, i64, vp, vp]
     lib.cybq_dequant.argtypes = [vp, vp, vp, vp]
     lib.cybq_quantize.argtypes = [vp, ci, vp, i64, i64, vp, vp, vp]
     # diagnostics (cyb_amd/csrc/cybq_debug.h), not part of the operator interface
@@ -247,6 +255,61 @@ class MatmulPlan:
                     raise CybqError(-1, "invalid argument", "all gammas of a plan share one type")
                 self.gamma = arr(*[_ptr(g) for g in gammas])
                 self.keep = self.keep + (list(gammas),)
+
+
+class KVCache:
+    """The paged keys and values of a model's layers (cybq_cache): `pages` pages of `page` tokens for each of `layers` layers."""
+
+    def __init__(self, backend: "Backend", handle: int):
+        self._backend = backend
+        self._h = ctypes.c_void_p(handle)
+        kind, memory = ctypes.c_int(), ctypes.c_void_p()
+        n = [ctypes.c_int64() for _ in range(7)]
+        backend._check(backend._lib.cybq_cache_info(self._h, kind, *n, memory))
+        self.kind = next(k for k, v in CACHE_KINDS.items() if v == kind.value)
+        self.layers, self.kv_heads, self.dim, self.page, self.pages, self.page_bytes, self.layer_bytes = (v.value for v in n)
+        self.memory = memory.value                      # page p of layer l: page_bytes at memory + l * layer_bytes + p * page_bytes
+
+    @property
+    def handle(self) -> ctypes.c_void_p:
+        if not self._h:
+            raise CybqError(-1, "invalid argument", "cache already freed")
+        return self._h
+
+    def free(self) -> None:
+        if self._h and self._backend._ctx:
+            self._backend._lib.cybq_cache_free(self._backend._ctx, self._h)
+        self._h = ctypes.c_void_p()
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
+class _BatchStruct(ctypes.Structure):
+    _fields_ = [("seqs", ctypes.c_int64), ("rows", ctypes.c_int64), ("max_new", ctypes.c_int64), ("table_pages", ctypes.c_int64),
+                ("starts", ctypes.c_void_p), ("lengths", ctypes.c_void_p), ("tables", ctypes.c_void_p)]
+
+
+class CacheBatch:
+    """The rows of a step (cybq_batch): sequence b has rows starts[b] .. starts[b + 1], the last ones of its lengths[b] tokens, which lie in
+    the pages tables[b].  int32 tensors on the device; their contents may change between calls, they themselves are kept."""
+
+    def __init__(self, backend: "Backend", starts, lengths, tables, rows: int, max_new: Optional[int] = None):
+        if lengths.dim() != 1 or starts.dim() != 1 or tables.dim() != 2 or starts.shape[0] != lengths.shape[0] + 1 or tables.shape[0] != lengths.shape[0]:
+            raise CybqError(-2, "bad shape", "starts must be [seqs + 1], lengths [seqs], tables [seqs, pages]")
+        for t, what in ((starts, "starts"), (lengths, "lengths"), (tables, "tables")):
+            if str(t.dtype) != "torch.int32":
+                raise CybqError(-1, "invalid argument", f"{what} must be int32")
+            backend._check_tensor(t, what, t.numel())
+        self.keep = (starts, lengths, tables)
+        self.rows = rows
+        self._device = backend.device
+        self._s = _BatchStruct(lengths.shape[0], rows, max(1, rows if max_new is None else max_new), tables.shape[1], _ptr(starts), _ptr(lengths),
+                               _ptr(tables))
+        self._addr = ctypes.addressof(self._s)
 
 
 class Backend:
@@ -503,6 +566,85 @@ class Backend:
             raise CybqError(-1, "invalid argument", "residual must have y's dtype")
         self._check(self._lib.cybq_matmul_experts_sum(self._ctx, w.handle, experts, _ptr(x), _dtype_code(x, None), T, k, _ptr(ids),
                                                       _ptr(weights), _ptr(residual), _ptr(y), _dtype_code(y, None), stream))
+
+    # ---- paged key-value cache and attention
+    def kv_cache(self, kind: str, layers: int, kv_heads: int, dim: int, page: int, pages: int) -> KVCache:
+        """cybq_cache_create: kind "f16", "bf16", "q8" or "q4"; pages of `page` tokens (a power of two from 32 on)."""
+        if kind not in CACHE_KINDS:
+            raise CybqError(-1, "invalid argument", f"unknown cache kind {kind!r}")
+        out = ctypes.c_void_p()
+        self._check(self._lib.cybq_cache_create(self._ctx, CACHE_KINDS[kind], layers, kv_heads, dim, page, pages, ctypes.byref(out)))
+        return KVCache(self, out.value)
+
+    def cache_batch(self, starts, lengths, tables, rows: int, max_new: Optional[int] = None) -> CacheBatch:
+        """The rows of a step: see CacheBatch.  max_new: at least every sequence's rows (None: `rows`)."""
+        return CacheBatch(self, starts, lengths, tables, rows, max_new)
+
+    def _check_heads(self, t, what: str, rows: int, heads: Optional[int], dim: int) -> tuple:
+        """(heads, elements between rows) of a tensor [rows, heads, dim] whose rows may lie apart."""
+        if t.dim() != 3 or t.shape[0] < rows or t.shape[2] != dim or (heads is not None and t.shape[1] != heads):
+            raise CybqError(-2, "bad shape", f"{what} must be [{rows}, {'heads' if heads is None else heads}, {dim}]")
+        if not t.is_cuda or (t.device.index or 0) != self.device:
+            raise CybqError(-1, "invalid argument", f"{what} must live on cuda:{self.device}")
+        if t.numel() and ((t.stride(2) != 1 and dim > 1) or (t.stride(1) != dim and t.shape[1] > 1)):
+            raise CybqError(-2, "bad shape", f"the heads of a row of {what} must be contiguous")
+        return t.shape[1], t.stride(0) if t.shape[0] > 1 else t.shape[1] * dim
+
+    def _check_batch(self, cache: KVCache, batch: CacheBatch) -> int:
+        if batch._device != self.device:
+            raise CybqError(-1, "invalid argument", f"the batch must live on cuda:{self.device}")
+        return batch.rows
+
+    def cache_append(self, cache: KVCache, layer: int, batch: CacheBatch, q, k, v, q_out=None, rope=None, style: str = "halves",
+                     stream: int = 0) -> None:
+        """cybq_cache_append: k, v [rows, kv_heads, dim] into the cache, q [rows, heads, dim] (or None) to q_out; q and k turned by rope
+        [positions, pairs, 2] (fp32 cos, sin; None: not turned).  q, k and v may be slices of one projection's rows."""
+        if style not in ROPE_STYLES:
+            raise CybqError(-1, "invalid argument", f"unknown rope style {style!r}")
+        rows = self._check_batch(cache, batch)
+        _, ks = self._check_heads(k, "k", rows, cache.kv_heads, cache.dim)
+        _, vs = self._check_heads(v, "v", rows, cache.kv_heads, cache.dim)
+        heads, qs, qdt = 0, 0, F16
+        if (q is None) != (q_out is None):
+            raise CybqError(-1, "invalid argument", "q and q_out go together")
+        if q is not None:
+            heads, qs = self._check_heads(q, "q", rows, None, cache.dim)
+            self._check_heads(q_out, "q_out", rows, heads, cache.dim)
+            self._check_tensor(q_out, "q_out", rows * heads * cache.dim)
+            qdt = _dtype_code(q_out, None)
+        if k.dtype != v.dtype or (q is not None and q.dtype != k.dtype):
+            raise CybqError(-1, "invalid argument", "q, k and v share one type")
+        dt = _dtype_code(k, None)
+        positions = dims = 0
+        if rope is not None:
+            if rope.dim() != 3 or rope.shape[2] != 2 or str(rope.dtype) != "torch.float32":
+                raise CybqError(-2, "bad shape", "rope must be a float32 tensor [positions, pairs, 2]")
+            self._check_tensor(rope, "rope", rope.numel())
+            positions, dims = rope.shape[0], rope.shape[1] * 2
+        self._check(self._lib.cybq_cache_append(self._ctx, cache.handle, layer, batch._addr, _ptr(q), qs, heads, _ptr(k), ks, _ptr(v), vs,
+                                                dt, _ptr(rope), positions, dims, ROPE_STYLES[style], _ptr(q_out), qdt, stream))
+
+    def cache_read(self, cache: KVCache, layer: int, batch: CacheBatch, k, v, stream: int = 0) -> None:
+        """cybq_cache_read: what the cache holds for the batch's rows, to k and v [rows, kv_heads, dim]."""
+        rows = self._check_batch(cache, batch)
+        for t, what in ((k, "k"), (v, "v")):
+            self._check_heads(t, what, rows, cache.kv_heads, cache.dim)
+            self._check_tensor(t, what, rows * cache.kv_heads * cache.dim)
+        if k.dtype != v.dtype:
+            raise CybqError(-1, "invalid argument", "k and v share one type")
+        self._check(self._lib.cybq_cache_read(self._ctx, cache.handle, layer, batch._addr, _ptr(k), _ptr(v), _dtype_code(k, None), stream))
+
+    def attention(self, cache: KVCache, layer: int, batch: CacheBatch, q, y, scale: Optional[float] = None, window: int = 0, stream: int = 0) -> None:
+        """cybq_attention: y[t] = softmax(scale * q[t] . k) v over the tokens of row t's sequence up to its own, at most `window` of them (0: all).
+        q, y [rows, heads, dim]; scale None: dim ** -0.5."""
+        rows = self._check_batch(cache, batch)
+        heads, qs = self._check_heads(q, "q", rows, None, cache.dim)
+        self._check_heads(y, "y", rows, heads, cache.dim)
+        self._check_tensor(y, "y", rows * heads * cache.dim)
+        if q.dtype != y.dtype:
+            raise CybqError(-1, "invalid argument", "q and y share one type")
+        self._check(self._lib.cybq_attention(self._ctx, cache.handle, layer, batch._addr, _ptr(q), qs, _dtype_code(q, None), heads,
+                                             ctypes.c_float(cache.dim ** -0.5 if scale is None else scale), window, _ptr(y), stream))
 
     def fuse_pairs(self, gate: QWeight, up: QWeight, name: Optional[str] = None) -> QWeight:
         """One weight holding gate and up projections interleaved by 16-row strip (device to device)."""

@@ -14,6 +14,7 @@
 #include <vector>
 
 #include "../../include/cybq.h"
+#include "cache_parts.h"
 #include "cybq_debug.h"
 #include "cybq_internal.h"
 #include "pool.h"
@@ -25,7 +26,7 @@ struct cybq_ctx {
     bool prefill_exact = false;
     bool decode_exact = false;
     void* workspace = nullptr;          // scratch for the prefill path, allocated once at init
-    size_t workspace_bytes = 0;
+    size_t workspace_bytes = 0;         // (the tickets of cybq_attention, kAttnTicketBytes, lie behind them)
     std::string last_error;
     cybq::Uploader uploader;            // host memory -> native tiles; idle until the first upload
 };
@@ -47,6 +48,14 @@ struct cybq_weight {
     cybq::ScanSlot scan;
     std::mutex scan_mutex;
     std::atomic<bool> scan_read{false};
+};
+
+struct cybq_cache {
+    int device = 0;
+    int kind = 0;
+    int64_t layers = 0, kv_heads = 0, dim = 0, page_tokens = 0, pages = 0;
+    int64_t page_bytes = 0, layer_bytes = 0;
+    uint8_t* data = nullptr;
 };
 
 namespace cybq {
@@ -265,13 +274,14 @@ int cybq_init(int device, cybq_ctx** out)
     // 256 MiB of scratch for the prefill path: the activations restaged in MFMA operand
     // order (larger M is walked in row chunks) and the partial sums of a K split
     ctx->workspace_bytes = (size_t)256 << 20;
-    if (hipMalloc(&ctx->workspace, ctx->workspace_bytes) != hipSuccess) {
+    if (hipMalloc(&ctx->workspace, ctx->workspace_bytes + cybq::kAttnTicketBytes) != hipSuccess) {
         (void)hipGetLastError();
         delete ctx;
         return CYBQ_ERR_NOMEM;
     }
-    // the decode kernels' tickets (start of the scratch's tail) are zero at rest
-    if (hipMemset(static_cast<char*>(ctx->workspace) + ctx->workspace_bytes - cybq::kDecodeScratchBytes, 0, (size_t)1 << 16) != hipSuccess) {
+    // the decode kernels' tickets (start of the scratch's tail) and those of cybq_attention (behind the scratch) are zero at rest
+    if (hipMemset(static_cast<char*>(ctx->workspace) + ctx->workspace_bytes - cybq::kDecodeScratchBytes, 0, (size_t)1 << 16) != hipSuccess ||
+        hipMemset(static_cast<char*>(ctx->workspace) + ctx->workspace_bytes, 0, cybq::kAttnTicketBytes) != hipSuccess) {
         (void)hipGetLastError();
         (void)hipFree(ctx->workspace);
         delete ctx;
@@ -822,6 +832,214 @@ int cybq_matmul_many_norm(cybq_ctx* ctx, int64_t count, const cybq_weight* const
                               residual ? residual[i] : nullptr, stream, ctx->workspace, ctx->workspace_bytes);
         if (rc) return rc;
     }
+    return CYBQ_OK;
+}
+
+/* ---- paged key-value cache and attention ---- */
+
+int cybq_cache_create(cybq_ctx* ctx, cybq_cache_kind kind, int64_t layers, int64_t kv_heads, int64_t head_dim, int64_t page_tokens, int64_t pages,
+                      cybq_cache** out)
+{
+    if (!ctx) return CYBQ_ERR_INVALID;
+    if (!out) return fail(ctx, CYBQ_ERR_INVALID, "out is NULL");
+    *out = nullptr;
+    if (kind != CYBQ_CACHE_F16 && kind != CYBQ_CACHE_BF16 && kind != CYBQ_CACHE_Q4 && kind != CYBQ_CACHE_Q8)
+        return fail(ctx, CYBQ_ERR_INVALID, "unknown cache kind");
+    if (layers < 1 || layers > (1 << 20) || kv_heads < 1 || kv_heads > 4096 || pages < 1 || pages > (1 << 30))
+        return fail(ctx, CYBQ_ERR_SHAPE, "layers must be in 1..2^20, kv_heads in 1..4096, pages in 1..2^30");
+    if (head_dim != 64 && head_dim != 96 && head_dim != 128 && head_dim != 256) return fail(ctx, CYBQ_ERR_SHAPE, "head_dim must be 64, 96, 128 or 256");
+    if (page_tokens < 32 || page_tokens > 1024 || (page_tokens & (page_tokens - 1)))
+        return fail(ctx, CYBQ_ERR_SHAPE, "page_tokens must be a power of two in 32..1024");
+    const int64_t page_bytes = kv_heads * (page_tokens / cybq::kBlockTokens) * cybq::cache_block_bytes(kind, (int)head_dim);      // < 2^38
+    if ((double)page_bytes * (double)pages * (double)layers > 1e13) return fail(ctx, CYBQ_ERR_SHAPE, "cache too large");
+    DeviceGuard guard(ctx->device);
+    if (guard.err != hipSuccess) return fail_hip(ctx, guard.err, "hipSetDevice");
+    cybq_cache* c = new (std::nothrow) cybq_cache();
+    if (!c) return fail(ctx, CYBQ_ERR_NOMEM, "host allocation failed");
+    c->device = ctx->device;
+    c->kind = kind;
+    c->layers = layers;
+    c->kv_heads = kv_heads;
+    c->dim = head_dim;
+    c->page_tokens = page_tokens;
+    c->pages = pages;
+    c->page_bytes = page_bytes;
+    c->layer_bytes = page_bytes * pages;
+    const size_t bytes = (size_t)c->layer_bytes * (size_t)layers;
+    void* data = nullptr;
+    hipError_t e = hipMalloc(&data, bytes);
+    if (e == hipErrorOutOfMemory) {            // the memory of freed weights first
+        (void)hipGetLastError();
+        e = cybq::pool_trim(ctx->device);
+        if (e == hipSuccess) e = hipMalloc(&data, bytes);
+    }
+    if (e == hipSuccess) {
+        c->data = static_cast<uint8_t*>(data);
+        e = hipMemset(data, 0, bytes);
+        if (e == hipSuccess) e = hipDeviceSynchronize();
+    }
+    if (e != hipSuccess) {
+        if (c->data) (void)hipFree(c->data);
+        delete c;
+        return fail_hip(ctx, e, "cache allocation");
+    }
+    *out = c;
+    return CYBQ_OK;
+}
+
+int cybq_cache_free(cybq_ctx* ctx, cybq_cache* cache)
+{
+    if (!ctx) return CYBQ_ERR_INVALID;
+    if (!cache) return CYBQ_OK;
+    DeviceGuard guard(cache->device);
+    if (guard.err != hipSuccess) return fail_hip(ctx, guard.err, "hipSetDevice");
+    const hipError_t e = hipFree(cache->data);
+    delete cache;
+    return e == hipSuccess ? CYBQ_OK : fail_hip(ctx, e, "hipFree(cache)");
+}
+
+int cybq_cache_info(const cybq_cache* cache, int* kind, int64_t* layers, int64_t* kv_heads, int64_t* head_dim, int64_t* page_tokens, int64_t* pages,
+                    int64_t* page_bytes, int64_t* layer_bytes, void** memory)
+{
+    if (!cache) return CYBQ_ERR_INVALID;
+    if (kind) *kind = cache->kind;
+    if (layers) *layers = cache->layers;
+    if (kv_heads) *kv_heads = cache->kv_heads;
+    if (head_dim) *head_dim = cache->dim;
+    if (page_tokens) *page_tokens = cache->page_tokens;
+    if (pages) *pages = cache->pages;
+    if (page_bytes) *page_bytes = cache->page_bytes;
+    if (layer_bytes) *layer_bytes = cache->layer_bytes;
+    if (memory) *memory = cache->data;
+    return CYBQ_OK;
+}
+
+namespace {
+// what the calls on a cache check alike; *idle: no rows or no sequences
+int check_batch(cybq_ctx* ctx, const cybq_cache* cache, int64_t layer, const cybq_batch* batch, cybq::CacheView* c, cybq::BatchView* t, bool* idle)
+{
+    *idle = true;
+    if (!ctx) return CYBQ_ERR_INVALID;
+    if (!cache || !batch) return fail(ctx, CYBQ_ERR_INVALID, "cache / batch is NULL");
+    if (cache->device != ctx->device) return fail(ctx, CYBQ_ERR_INVALID, "cache lives on another device");
+    if (layer < 0 || layer >= cache->layers) return fail(ctx, CYBQ_ERR_SHAPE, "the cache has no such layer");
+    const cybq_batch& b = *batch;
+    if (b.seqs < 0 || b.seqs > 65536 || b.rows < 0 || b.rows > (1 << 24)) return fail(ctx, CYBQ_ERR_SHAPE, "seqs must be in 0..65536, rows in 0..2^24");
+    if (b.seqs == 0 || b.rows == 0) return CYBQ_OK;
+    if (!b.starts || !b.lengths || !b.tables) return fail(ctx, CYBQ_ERR_INVALID, "starts / lengths / tables is NULL");
+    if (b.max_new < 1 || b.max_new > (1 << 24)) return fail(ctx, CYBQ_ERR_SHAPE, "max_new must be in 1..2^24");
+    if (b.table_pages < 1 || b.table_pages > ((int64_t)1 << 30) / cache->page_tokens)
+        return fail(ctx, CYBQ_ERR_SHAPE, "table_pages must be at least 1, and table_pages * page_tokens at most 2^30");
+    if (reinterpret_cast<uintptr_t>(b.starts) % 4 || reinterpret_cast<uintptr_t>(b.lengths) % 4 || reinterpret_cast<uintptr_t>(b.tables) % 4)
+        return fail(ctx, CYBQ_ERR_ALIGN, "starts / lengths / tables is not aligned to its element size");
+    *idle = false;
+    c->base = cache->data + layer * cache->layer_bytes;
+    c->page_bytes = cache->page_bytes;
+    c->pages = (int)cache->pages;
+    c->page_shift = 0;
+    while (((int64_t)cybq::kBlockTokens << c->page_shift) < cache->page_tokens) c->page_shift++;
+    c->kv_heads = (int)cache->kv_heads;
+    c->dim = (int)cache->dim;
+    c->kind = cache->kind;
+    t->starts = b.starts;
+    t->lengths = b.lengths;
+    t->tables = b.tables;
+    t->seqs = (int)b.seqs;
+    t->rows = (int)b.rows;
+    t->max_new = (int)b.max_new;
+    t->table_pages = (int)b.table_pages;
+    return CYBQ_OK;
+}
+
+// rows of `heads` heads, `stride` elements apart: 16-byte aligned, none over another
+int check_rows(cybq_ctx* ctx, const cybq_cache* cache, const void* x, int64_t stride, int64_t heads, int dt)
+{
+    if (stride < heads * cache->dim || stride > (int64_t)1 << 32) return fail(ctx, CYBQ_ERR_SHAPE, "a stride is less than a row, or more than 2^32");
+    if (!aligned16(x) || stride * (int64_t)dtype_size(dt) % 16) return fail(ctx, CYBQ_ERR_ALIGN, "q / k / v and their rows must be 16-byte aligned");
+    return CYBQ_OK;
+}
+
+int check_heads(cybq_ctx* ctx, const cybq_cache* cache, int64_t q_heads)
+{
+    if (q_heads < 1 || q_heads > 65536 || q_heads % cache->kv_heads) return fail(ctx, CYBQ_ERR_SHAPE, "q_heads must be a multiple of kv_heads, at most 65536");
+    return CYBQ_OK;
+}
+}  // namespace
+
+int cybq_cache_append(cybq_ctx* ctx, cybq_cache* cache, int64_t layer, const cybq_batch* batch, const void* q, int64_t q_stride, int64_t q_heads,
+                      const void* k, int64_t k_stride, const void* v, int64_t v_stride, cybq_dtype dt, const float* rope, int64_t rope_positions,
+                      int64_t rope_dims, cybq_rope_style style, void* q_out, cybq_dtype qdt, void* stream)
+{
+    cybq::CacheView c;
+    cybq::BatchView t;
+    bool idle;
+    int rc = check_batch(ctx, cache, layer, batch, &c, &t, &idle);
+    if (rc) return rc;
+    if (!dtype_ok(dt) || (qdt != CYBQ_F16 && qdt != CYBQ_BF16)) return fail(ctx, CYBQ_ERR_INVALID, "unknown dtype (qdt must be CYBQ_F16 or CYBQ_BF16)");
+    if (style != CYBQ_ROPE_HALVES && style != CYBQ_ROPE_PAIRS) return fail(ctx, CYBQ_ERR_INVALID, "unknown rope style");
+    if (idle) return CYBQ_OK;
+    if (!k || !v || !q != !q_out) return fail(ctx, CYBQ_ERR_INVALID, "k / v is NULL, or one of q and q_out");
+    if (q && (rc = check_heads(ctx, cache, q_heads))) return rc;
+    if (q && (rc = check_rows(ctx, cache, q, q_stride, q_heads, dt))) return rc;
+    if ((rc = check_rows(ctx, cache, k, k_stride, cache->kv_heads, dt)) || (rc = check_rows(ctx, cache, v, v_stride, cache->kv_heads, dt))) return rc;
+    if (!aligned16(q_out) || !aligned16(rope)) return fail(ctx, CYBQ_ERR_ALIGN, "q_out / rope must be 16-byte aligned");
+    if (rope) {
+        if (rope_dims < 16 || rope_dims > cache->dim || rope_dims % 16) return fail(ctx, CYBQ_ERR_SHAPE, "rope_dims must be a multiple of 16, at most head_dim");
+        if (rope_positions < batch->table_pages * cache->page_tokens) return fail(ctx, CYBQ_ERR_SHAPE, "rope has fewer positions than the table");
+    }
+    DeviceGuard guard(ctx->device);
+    if (guard.err != hipSuccess) return fail_hip(ctx, guard.err, "hipSetDevice");
+    const hipError_t e = cybq::launch_cache_append(c, t, q, q_stride, q ? (int)(q_heads / cache->kv_heads) : 0, k, k_stride, v, v_stride, dt, rope,
+                                                   rope ? (int)rope_dims : 0, style == CYBQ_ROPE_HALVES, q_out, qdt, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return fail_hip(ctx, e, "cache append launch");
+    return CYBQ_OK;
+}
+
+int cybq_cache_read(cybq_ctx* ctx, const cybq_cache* cache, int64_t layer, const cybq_batch* batch, void* k, void* v, cybq_dtype dt, void* stream)
+{
+    cybq::CacheView c;
+    cybq::BatchView t;
+    bool idle;
+    const int rc = check_batch(ctx, cache, layer, batch, &c, &t, &idle);
+    if (rc) return rc;
+    if (!dtype_ok(dt)) return fail(ctx, CYBQ_ERR_INVALID, "unknown dtype");
+    if (idle) return CYBQ_OK;
+    if (!k || !v) return fail(ctx, CYBQ_ERR_INVALID, "k / v is NULL");
+    if (!aligned16(k) || !aligned16(v)) return fail(ctx, CYBQ_ERR_ALIGN, "k / v must be 16-byte aligned");
+    DeviceGuard guard(ctx->device);
+    if (guard.err != hipSuccess) return fail_hip(ctx, guard.err, "hipSetDevice");
+    const hipError_t e = cybq::launch_cache_read(c, t, k, v, dt, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return fail_hip(ctx, e, "cache read launch");
+    return CYBQ_OK;
+}
+
+int cybq_attention(cybq_ctx* ctx, const cybq_cache* cache, int64_t layer, const cybq_batch* batch, const void* q, int64_t q_stride, cybq_dtype qdt,
+                   int64_t q_heads, float scale, int64_t window, void* y, void* stream)
+{
+    cybq::CacheView c;
+    cybq::BatchView t;
+    bool idle;
+    int rc = check_batch(ctx, cache, layer, batch, &c, &t, &idle);
+    if (rc) return rc;
+    if (qdt != CYBQ_F16 && qdt != CYBQ_BF16) return fail(ctx, CYBQ_ERR_INVALID, "qdt must be CYBQ_F16 or CYBQ_BF16");
+    if ((cache->kind == CYBQ_CACHE_F16 && qdt != CYBQ_F16) || (cache->kind == CYBQ_CACHE_BF16 && qdt != CYBQ_BF16))
+        return fail(ctx, CYBQ_ERR_UNSUPPORTED, "rows on a cache of 16 bits have the cache's type");
+    if (!(scale > 0.f) || !std::isfinite(scale)) return fail(ctx, CYBQ_ERR_INVALID, "scale must be positive and finite");
+    if (window < 0) return fail(ctx, CYBQ_ERR_SHAPE, "window must be at least 0");
+    if ((rc = check_heads(ctx, cache, q_heads))) return rc;
+    if (idle) return CYBQ_OK;
+    if (!q || !y) return fail(ctx, CYBQ_ERR_INVALID, "q / y is NULL");
+    if ((rc = check_rows(ctx, cache, q, q_stride, q_heads, qdt))) return rc;
+    if (reinterpret_cast<uintptr_t>(y) % 8) return fail(ctx, CYBQ_ERR_ALIGN, "y must be 8-byte aligned");
+    const int group = (int)(q_heads / cache->kv_heads);
+    if (cybq::attention_units_max(t, c.kv_heads, group) > cybq::attention_max_units())
+        return fail(ctx, CYBQ_ERR_UNSUPPORTED, "too many rows and heads for one call");
+    if (cybq::attention_scratch_bytes(c.dim) > ctx->workspace_bytes - cybq::kDecodeScratchBytes) return fail(ctx, CYBQ_ERR_UNSUPPORTED, "scratch too small");
+    DeviceGuard guard(ctx->device);
+    if (guard.err != hipSuccess) return fail_hip(ctx, guard.err, "hipSetDevice");
+    const hipError_t e = cybq::launch_attention(c, t, q, q_stride, qdt, group, scale, (int)std::min<int64_t>(window, (int64_t)1 << 30), y, ctx->workspace,
+                                                static_cast<char*>(ctx->workspace) + ctx->workspace_bytes, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return fail_hip(ctx, e, "attention launch");
     return CYBQ_OK;
 }
 

@@ -1,0 +1,533 @@
+// attention.hip - attention of new tokens over the paged cache (cache_parts.h).
+//
+//   s_j = scale q . k_j,  max(0, p - window + 1) <= j <= p,  in a page;     y = sum_j softmax(s)_j v_j;  nothing to see: y = 0
+//
+// One pass with a running maximum and sum per row, fp32.  Rows of one kv head - its `group` query heads of one new token after
+// another - stand side by side as columns of S^T = K Q^T, so a lane holds scores of one row only: maxima and sums meet other lanes
+// twice, and the scores are, as they lie, the operand of Y^T = V^T P^T.
+//
+// Operands.  16-bit caches: their own type, P of bf16 as two numbers (its 8 bits alone would be the result's error).  Q8, Q4: f16.  Keys are
+// the exact integers, their scales come in fp32 on each group's products; values are round_f16(scale q), 2^-12; P is f16 behind 2^14
+// (probabilities down to 2^-38 of the largest count, whatever their number); rows of bf16 become f16 behind a power of two.
+#include <algorithm>
+
+#include "cache_parts.h"
+#include "cybq_internal.h"
+
+namespace cybq {
+
+namespace {
+
+// Work is shared out on the device: lengths are known there only, and a captured call meets longer ones every time.  A unit is one tile
+// of rows of one sequence and kv head, and a part of the blocks that it sees; parts are as long as makes `target` units of all.
+struct AttnArgs {
+    CacheView c;
+    BatchView t;
+    const void* q;
+    void* y;
+    int64_t q_stride;
+    float* slabs;
+    unsigned* tickets;
+    int group, qdt, window, target, least;       // least: blocks of a part
+    float scale;                                 // times log2 e
+};
+
+constexpr int kMaxUnits = 1 << 24;               // of a call
+
+struct Unit {
+    Seq s;
+    int b, tile, head, split, splits, slab, ticket;
+};
+
+// first and last block that rows r0 .. r1 (positions p0 ..) see
+__device__ __forceinline__ void seen(const AttnArgs& a, int p_first, int p_last, int64_t capacity, int* lo, int* hi)
+{
+    const int64_t end = min((int64_t)p_last, capacity - 1);
+    const int first = a.window && p_first >= a.window ? p_first - a.window + 1 : 0;
+    *lo = first >> 5;
+    *hi = end < first ? *lo : (int)(end >> 5) + 1;
+}
+
+template <int ROWS>
+__device__ __forceinline__ bool find_unit(const AttnArgs& a, int u, Unit* out)
+{
+    const int lane = threadIdx.x & 63;
+    const int64_t capacity = (int64_t)a.t.table_pages << (a.c.page_shift + 5);
+    const int heads = a.c.kv_heads;
+    float work = 0.f;
+    for (int base = 0; base < a.t.seqs; base += 64) {
+        if (base + lane < a.t.seqs) {
+            const Seq s = seq_of(a.t, base + lane);
+            int lo, hi;
+            seen(a, s.len - s.n, s.len - 1, capacity, &lo, &hi);
+            work += (float)((s.n * a.group + ROWS - 1) / ROWS) * (float)(hi - lo);
+        }
+    }
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) work += __shfl_xor(work, m);
+    // (a little more, so that what is rounded never makes more parts than the slabs hold)
+    const int part = max(a.least, (int)fminf(work * (float)heads / (float)a.target * 1.0001f + 1.0f, 1.0e9f));
+    int64_t units = 0;
+    int slabs = 0, tickets = 0;
+    bool found = false;
+    for (int base = 0; base < a.t.seqs; base += 64) {
+        Seq s = {0, 0, 0};
+        int tiles = 0, splits = 0;
+        if (base + lane < a.t.seqs) {
+            s = seq_of(a.t, base + lane);
+            int lo, hi;
+            seen(a, s.len - s.n, s.len - 1, capacity, &lo, &hi);
+            tiles = (s.n * a.group + ROWS - 1) / ROWS;
+            splits = max(1, (hi - lo + part - 1) / part);
+        }
+        // (a batch whose starts make no sense may add up to anything: what cannot be right stays above every grid)
+        const int rows = min(tiles * heads, kMaxUnits + 1), mine = (int)min((int64_t)rows * splits, (int64_t)kMaxUnits + 1);
+        const int upto = wave_prefix(mine), slab_upto = wave_prefix(splits > 1 ? mine : 0), ticket_upto = wave_prefix(splits > 1 ? rows : 0);
+        const int total = __builtin_amdgcn_readlane(upto, 63);
+        if (!found && u < units + total) {
+            found = true;
+            const int l = __builtin_ctzll(__ballot((int)units + upto > u));
+            out->s.row0 = __builtin_amdgcn_readlane(s.row0, l);
+            out->s.n = __builtin_amdgcn_readlane(s.n, l);
+            out->s.len = __builtin_amdgcn_readlane(s.len, l);
+            out->b = base + l;
+            out->splits = __builtin_amdgcn_readlane(splits, l);
+            const int at = u - (int)units - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(mine, l));
+            out->split = at % out->splits;
+            const int rest = at / out->splits;
+            out->head = rest % heads;
+            out->tile = rest / heads;
+            out->slab = slabs + __builtin_amdgcn_readlane(slab_upto, l) - __builtin_amdgcn_readlane(mine, l) + at;
+            out->ticket = tickets + __builtin_amdgcn_readlane(ticket_upto, l) - __builtin_amdgcn_readlane(rows, l) + rest;
+        }
+        units += total;
+        slabs += __builtin_amdgcn_readlane(slab_upto, 63);
+        tickets += __builtin_amdgcn_readlane(ticket_upto, 63);
+    }
+    // more units than workgroups: the starts rise and fall.  Nobody begins what nobody could finish.
+    return found && units <= (int64_t)gridDim.x;
+}
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+template <int STEP>
+__device__ __forceinline__ float other_quarter(float v)
+{
+    const uint32_t u = __builtin_bit_cast(uint32_t, v);
+    const auto r = STEP == 16 ? __builtin_amdgcn_permlane16_swap(u, u, false, false) : __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return __builtin_bit_cast(float, (uint32_t)(threadIdx.x & STEP ? r[0] : r[1]));
+}
+
+template <int KIND>
+__device__ __forceinline__ float4_t mfma16(Frag16 a, Frag16 b, float4_t c)
+{
+    if constexpr (KIND == kCacheBF16) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.b, b.b, c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x32_f16(a.h, b.h, c, 0, 0, 0);
+}
+
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi)
+{
+    const half2_t v = {(_Float16)lo, (_Float16)hi};
+    return as_u32(v);
+}
+
+// a block's keys or values and their scales, as a lane has them from memory
+template <int KIND, int G>
+struct Half {
+    static constexpr int N = KIND == kCacheQ8 ? G : KIND == kCacheQ4 ? (G + 1) / 2 : 2 * G;
+    u32x4_t d[N];
+    u32x4_t s[cache_quantised(KIND) ? G : 1];
+    __device__ __forceinline__ void load(const uint8_t* p, int lane)
+    {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            if (KIND == kCacheQ4 && (G & 1) && i == N - 1) {
+                const u32x2_t v = *reinterpret_cast<const u32x2_t*>(p + i * 1024 + lane * 8);
+                d[i] = u32x4_t{v[0], v[1], 0u, 0u};
+            } else {
+                d[i] = *reinterpret_cast<const u32x4_t*>(p + i * 1024 + lane * 16);
+            }
+        }
+        if constexpr (cache_quantised(KIND)) {
+#pragma unroll
+            for (int g = 0; g < G; g++) s[g] = *reinterpret_cast<const u32x4_t*>(p + cache_data_bytes(KIND, 32 * G) + (g * 4 + (lane >> 4)) * 16);
+        }
+    }
+};
+
+// eight nibbles (bit 16 (s & 1) + 4 (s >> 1 & 1) + 8 (s >> 2)) -> exact f16 integers
+__device__ __forceinline__ void nibbles_f16(uint32_t w, uint32_t magic, uint32_t out[4])
+{
+    const half2_t sub = {(_Float16)-1032.0f, (_Float16)-1032.0f}, mul = {(_Float16)0.0625f, (_Float16)0.0625f}, add = {(_Float16)-72.0f, (_Float16)-72.0f};
+    const uint32_t h = w >> 8;
+    out[0] = as_u32(as_h2((w & 0x000F000Fu) | magic) + sub);
+    out[1] = as_u32(as_h2((w & 0x00F000F0u) | magic) * mul + add);
+    out[2] = as_u32(as_h2((h & 0x000F000Fu) | magic) + sub);
+    out[3] = as_u32(as_h2((h & 0x00F000F0u) | magic) * mul + add);
+}
+
+// keys of tile t16 and group g as operand: exact integers, or the values themselves
+template <int KIND, int G>
+__device__ __forceinline__ Frag16 key_operand(const Half<KIND, G>& k, int t16, int g, uint32_t magic)
+{
+    Frag16 f;
+    if constexpr (KIND == kCacheQ8) {
+        uint32_t o[4];
+        unpack_q8_f16(k.d[g][2 * t16], k.d[g][2 * t16 + 1], o);
+        f.u = u32x4_t{o[0], o[1], o[2], o[3]};
+    } else if constexpr (KIND == kCacheQ4) {
+        uint32_t o[4];
+        nibbles_f16(k.d[g >> 1][(g & 1) * 2 + t16], magic, o);
+        f.u = u32x4_t{o[0], o[1], o[2], o[3]};
+    } else {
+        f.u = k.d[t16 * G + g];
+    }
+    return f;
+}
+
+// values of dimensions 16 dt .. as operand, scales on them
+template <int KIND, int G>
+__device__ __forceinline__ Frag16 value_operand(const Half<KIND, G>& v, int dt, uint32_t magic)
+{
+    Frag16 f;
+    if constexpr (cache_quantised(KIND)) {
+        const int g = dt >> 1;
+        uint32_t o[4];
+        if constexpr (KIND == kCacheQ8) {
+            unpack_q8_f16(v.d[g][2 * (dt & 1)], v.d[g][2 * (dt & 1) + 1], o);
+        } else {
+            const half2_t sub = {(_Float16)-1032.0f, (_Float16)-1032.0f}, mul = {(_Float16)0.0625f, (_Float16)0.0625f},
+                          add = {(_Float16)-72.0f, (_Float16)-72.0f};
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const uint32_t w = v.d[g >> 1][(g & 1) * 2 + (i >> 1)] >> (8 * (i & 1));
+                o[i] = dt & 1 ? as_u32(as_h2((w & 0x00F000F0u) | magic) * mul + add) : as_u32(as_h2((w & 0x000F000Fu) | magic) + sub);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) f.u[i] = as_u32(as_h2(o[i]) * as_h2(v.s[g][i]));
+    } else {
+        f.u = v.d[dt];
+    }
+    return f;
+}
+
+__device__ __forceinline__ void store_row4(void* y, int dt, int64_t at, float4_t v)
+{
+    u32x2_t w;
+    if (dt == kF16) w = u32x2_t{pack_half2(v[0], v[1]), pack_half2(v[2], v[3])};
+    else w = u32x2_t{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+    *reinterpret_cast<u32x2_t*>(static_cast<uint16_t*>(y) + at) = w;
+}
+
+// Few rows: tiles of 16, eight waves that take a part's blocks in turn.  Keys of the next block are on their way while P is formed, values
+// while the next scores are.  Waves meet in LDS, the parts of a tile in slabs in memory: the part that is last adds them in order.
+constexpr int kWaves = 8, kRows = 16;
+
+template <int KIND, int G>
+__global__ __launch_bounds__(64 * kWaves) void attention_rows_kernel(AttnArgs a)
+{
+    constexpr int DIM = 32 * G, BLOCK = cache_block_bytes(KIND, DIM), HALF = cache_half_bytes(KIND, DIM), DT = 2 * G;
+    constexpr bool SPLIT_P = KIND == kCacheBF16;
+    constexpr float kShift = SPLIT_P ? 0.f : 14.f;
+    extern __shared__ float4_t lds[];                                 // [waves][DT][64], then [waves][16] maxima and sums
+    float* const stats = reinterpret_cast<float*>(lds + kWaves * DT * 64);
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q4 = lane >> 4, r = lane & 15;
+    const uint32_t magic = q4_magic_vgpr();
+    Unit u;
+    if (!find_unit<kRows>(a, blockIdx.x, &u)) return;
+    const int64_t capacity = (int64_t)a.t.table_pages << (a.c.page_shift + 5);
+    const int r0 = u.tile * kRows, rows = min(kRows, u.s.n * a.group - r0);
+    const int p0 = u.s.len - u.s.n, i_first = r0 / a.group, i_last = (r0 + rows - 1) / a.group;
+    int lo, hi;
+    seen(a, p0 + i_first, p0 + i_last, capacity, &lo, &hi);
+    const int each = (hi - lo) / u.splits, more = (hi - lo) % u.splits;
+    const int first = lo + u.split * each + min(u.split, more), last = first + each + (u.split < more ? 1 : 0);
+    // my row
+    const bool real = r < rows;
+    const int i = (r0 + (real ? r : 0)) / a.group, in_group = (r0 + (real ? r : 0)) - i * a.group;
+    const int p = p0 + i;
+    const int row_hi = real ? (int)min((int64_t)p, capacity - 1) : -1;
+    const int row_lo = a.window && p >= a.window ? p - a.window + 1 : 0;
+    const int all_hi = (int)min((int64_t)(p0 + i_first), capacity - 1);                       // every real row sees all of all_lo .. all_hi
+    const int all_lo = a.window && p0 + i_last >= a.window ? p0 + i_last - a.window + 1 : 0;
+    const int head = u.head * a.group + in_group;
+    Frag16 qf[G];
+    float c = a.scale;
+    {
+        const uint16_t* q = static_cast<const uint16_t*>(a.q) + (int64_t)(u.s.row0 + i) * a.q_stride + head * DIM + 8 * q4;
+#pragma unroll
+        for (int g = 0; g < G; g++) qf[g].u = real ? *reinterpret_cast<const u32x4_t*>(q + 32 * g) : u32x4_t{0u, 0u, 0u, 0u};
+        if (cache_quantised(KIND) && a.qdt == kBF16) {                // to f16: the row's largest at 2^14 .. 2^15
+            float x[8 * G], top = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8 * G; e++) {
+                const uint32_t w = qf[e >> 3].u[(e & 7) >> 1];
+                x[e] = __builtin_bit_cast(float, e & 1 ? w & 0xffff0000u : w << 16);
+                top = fmaxf(top, fabsf(x[e]));
+            }
+            top = fmaxf(top, other_quarter<16>(top));
+            top = fmaxf(top, other_quarter<32>(top));
+            const int e = (int)(__builtin_bit_cast(uint32_t, top) >> 23);
+            const int up = e == 0 || e == 255 ? 0 : max(-126, min(126, 141 - e));           // 2^up, and 2^-up, are normal numbers
+            const float f = __builtin_bit_cast(float, (uint32_t)(127 + up) << 23);
+            c *= __builtin_bit_cast(float, (uint32_t)(127 - up) << 23);
+#pragma unroll
+            for (int g = 0; g < G; g++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) qf[g].u[j] = pack_half2(x[8 * g + 2 * j] * f, x[8 * g + 2 * j + 1] * f);
+        }
+    }
+    const int32_t* const table = a.t.tables + (int64_t)u.b * a.t.table_pages;
+    const int in_page = (1 << a.c.page_shift) - 1;
+    auto block_of = [&](int blk) -> const uint8_t* {
+        if (blk >= last) return nullptr;
+        const int page = table[blk >> a.c.page_shift];
+        if ((unsigned)page >= (unsigned)a.c.pages) return nullptr;
+        return a.c.base + page * a.c.page_bytes + (int64_t)((u.head << a.c.page_shift) + (blk & in_page)) * BLOCK;
+    };
+    float4_t y[DT];
+#pragma unroll
+    for (int d = 0; d < DT; d++) y[d] = float4_t{0.f, 0.f, 0.f, 0.f};
+    const float none = -__builtin_inff();
+    float m = none, l = 0.f;                                          // m: of scores without their factor
+    Half<KIND, G> k, v;
+    int blk = first + wv;
+    auto next_there = [&](int from, const uint8_t** at) {             // the next of my blocks that has a page
+        for (*at = nullptr; from < last; from += kWaves)
+            if ((*at = block_of(from)) != nullptr) break;
+        return from;
+    };
+    const uint8_t* at;
+    blk = next_there(blk, &at);
+    if (at) {
+        k.load(at, lane);
+        v.load(at + HALF, lane);
+    }
+    while (at) {
+        float4_t s[2];
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            s[t] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int g = 0; g < G; g++) {
+                const Frag16 kf = key_operand<KIND, G>(k, t, g, magic);
+                if constexpr (cache_quantised(KIND)) {
+                    const float4_t part = mfma16<KIND>(kf, qf[g], float4_t{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const half2_t sc = as_h2(k.s[g][2 * t + (e >> 1)]);
+                        s[t][e] = __builtin_fmaf((float)sc[e & 1], part[e], s[t][e]);
+                    }
+                } else {
+                    s[t] = mfma16<KIND>(kf, qf[g], s[t]);
+                }
+            }
+        }
+        const int tok = blk * kBlockTokens + 4 * q4;
+        const uint8_t* next;
+        const int next_blk = next_there(blk + kWaves, &next);
+        if (next) k.load(next, lane);
+        if (blk * kBlockTokens < all_lo || blk * kBlockTokens + 31 > all_hi) {
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int j = tok + 16 * t + e;
+                    if (j < row_lo || j > row_hi) s[t][e] = none;
+                }
+        }
+        float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+        top = fmaxf(top, other_quarter<16>(top));
+        top = fmaxf(top, other_quarter<32>(top));
+        if (__ballot(top > m)) {
+            const float now = fmaxf(m, top);
+            const float f = m == none ? 0.f : exp2_fast((m - now) * c);
+            m = now;
+            l *= f;
+#pragma unroll
+            for (int d = 0; d < DT; d++) y[d] *= f;
+        }
+        const float off = kShift - (m == none ? 0.f : m * c);
+        Frag16 ph, pl;
+        float pr[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            pr[e] = exp2_fast(__builtin_fmaf(s[e >> 2][e & 3], c, off));
+            l += pr[e];
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            if constexpr (SPLIT_P) {
+                ph.u[j] = pack_bf16x2(pr[2 * j], pr[2 * j + 1]);
+                pl.u[j] = pack_bf16x2(pr[2 * j] - __builtin_bit_cast(float, ph.u[j] << 16), pr[2 * j + 1] - __builtin_bit_cast(float, ph.u[j] & 0xffff0000u));
+            } else {
+                ph.u[j] = pack_half2(pr[2 * j], pr[2 * j + 1]);
+            }
+        }
+#pragma unroll
+        for (int d = 0; d < DT; d++) {
+            const Frag16 vf = value_operand<KIND, G>(v, d, magic);
+            y[d] = mfma16<KIND>(vf, ph, y[d]);
+            if constexpr (SPLIT_P) y[d] = mfma16<KIND>(vf, pl, y[d]);
+        }
+        if (next) v.load(next + HALF, lane);
+        at = next;
+        blk = next_blk;
+    }
+    l += other_quarter<16>(l);
+    l += other_quarter<32>(l);
+    // waves meet
+    if (lane < 16) {
+        stats[wv * 16 + lane] = m * c;
+        stats[kWaves * 16 + wv * 16 + lane] = l;
+    }
+#pragma unroll
+    for (int d = 0; d < DT; d++) lds[(wv * DT + d) * 64 + lane] = y[d];
+    __syncthreads();
+    float top = none, sum = 0.f, f[kWaves];
+#pragma unroll
+    for (int w = 0; w < kWaves; w++) top = fmaxf(top, stats[w * 16 + r]);
+#pragma unroll
+    for (int w = 0; w < kWaves; w++) {
+        const float mw = stats[w * 16 + r];
+        f[w] = mw == none ? 0.f : exp2_fast(mw - top);
+        sum += f[w] * stats[kWaves * 16 + w * 16 + r];                // (a row of NaN has a sum of NaN and no maximum)
+    }
+    const int64_t row_at = ((int64_t)(u.s.row0 + i) * a.c.kv_heads * a.group + head) * DIM + 4 * q4;
+    constexpr int SLAB = DT * 64 * 4 + 32;                            // floats of a part: sums, maxima and sums of probabilities
+    float* const slab = a.slabs + (size_t)u.slab * SLAB;
+    for (int d = wv; d < DT; d += kWaves) {
+        float4_t o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < kWaves; w++) {
+            const float4_t part = lds[(w * DT + d) * 64 + lane];
+            if (f[w] != 0.f) o += part * f[w];
+        }
+        if (u.splits == 1) {
+            const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+            if (real) store_row4(a.y, a.qdt, row_at + 16 * d, o * inv);
+        } else if (real) {
+            const u32x2_t* w = reinterpret_cast<const u32x2_t*>(&o);
+            uint64_t* to = reinterpret_cast<uint64_t*>(slab + (d * 64 + lane) * 4);
+            __hip_atomic_store(to, __builtin_bit_cast(uint64_t, w[0]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+            __hip_atomic_store(to + 1, __builtin_bit_cast(uint64_t, w[1]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+        }
+    }
+    if (u.splits == 1) return;
+    if (threadIdx.x < 16) {
+        __hip_atomic_store(slab + DT * 64 * 4 + threadIdx.x, top, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+        __hip_atomic_store(slab + DT * 64 * 4 + 16 + threadIdx.x, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                  // my part of the slab has reached memory
+    __syncthreads();                                                  // (and everybody is done reading LDS)
+    unsigned* const flag = reinterpret_cast<unsigned*>(lds);
+    if (threadIdx.x == 0) {
+        const unsigned old = __hip_atomic_fetch_add(a.tickets + u.ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const bool end = old + 1u == (unsigned)u.splits;
+        if (end) __hip_atomic_store(a.tickets + u.ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        *flag = end ? 1u : 0u;
+    }
+    __syncthreads();
+    if (*flag == 0u) return;
+    __syncthreads();
+    // every part's maxima and sums of probabilities, then its sums
+    float* const all = reinterpret_cast<float*>(lds);
+    float* const of_tile = slab - (size_t)u.split * SLAB;
+    for (int e = threadIdx.x; e < u.splits * 32; e += 64 * kWaves)
+        all[e] = __hip_atomic_load(of_tile + (size_t)(e >> 5) * SLAB + DT * 64 * 4 + (e & 31), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+    __syncthreads();
+    top = none;
+    for (int e = 0; e < u.splits; e++) top = fmaxf(top, all[e * 32 + r]);
+    sum = 0.f;
+    for (int e = 0; e < u.splits; e++) sum += (all[e * 32 + r] == none ? 0.f : exp2_fast(all[e * 32 + r] - top)) * all[e * 32 + 16 + r];
+    if (!real) return;
+    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+    for (int d = wv; d < DT; d += kWaves) {
+        float4_t o = {0.f, 0.f, 0.f, 0.f};
+        constexpr int AHEAD = 8;
+        for (int e0 = 0; e0 < u.splits; e0 += AHEAD) {
+            uint64_t w[AHEAD][2];
+#pragma unroll
+            for (int e = 0; e < AHEAD; e++) {
+                const uint64_t* from = reinterpret_cast<const uint64_t*>(of_tile + (size_t)min(e0 + e, u.splits - 1) * SLAB + (d * 64 + lane) * 4);
+                w[e][0] = __hip_atomic_load(from, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+                w[e][1] = __hip_atomic_load(from + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+            }
+#pragma unroll
+            for (int e = 0; e < AHEAD; e++) {
+                if (e0 + e >= u.splits) break;
+                const float me = all[(e0 + e) * 32 + r];
+                const float fe = me == none ? 0.f : exp2_fast(me - top);
+                if (fe == 0.f) continue;
+                const float4_t part = {__builtin_bit_cast(float, (uint32_t)w[e][0]), __builtin_bit_cast(float, (uint32_t)(w[e][0] >> 32)),
+                                       __builtin_bit_cast(float, (uint32_t)w[e][1]), __builtin_bit_cast(float, (uint32_t)(w[e][1] >> 32))};
+                o += part * fe;
+            }
+        }
+        store_row4(a.y, a.qdt, row_at + 16 * d, o * inv);
+    }
+}
+
+template <int KIND, int G>
+hipError_t rows_as(const AttnArgs& a, unsigned grid, hipStream_t st)
+{
+    constexpr int bytes = kWaves * 2 * G * 64 * 16 + kWaves * 32 * 4;
+    (void)LdsRequest<&attention_rows_kernel<KIND, G>, bytes>::registered;
+    hipLaunchKernelGGL((attention_rows_kernel<KIND, G>), dim3(grid), dim3(64 * kWaves), bytes, st, a);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+// Parts of tiles that have more than one: at most 2 * target of them (a tile of b blocks has at most b / part + 1), of at most
+// `target` tiles.
+constexpr int kTarget = 256;
+
+int64_t attention_max_units() { return kMaxUnits; }
+
+size_t attention_scratch_bytes(int dim) { return (size_t)(2 * kTarget + 16) * ((size_t)dim / 16 * 64 * 4 + 32) * sizeof(float); }
+static_assert((2 * kTarget + 16) * sizeof(unsigned) <= kAttnTicketBytes, "a ticket per tile");
+static_assert(kTarget * 32 * 4 <= kWaves * 2 * 2 * 64 * 16 + kWaves * 32 * 4, "maxima and sums of a tile's parts fit LDS");
+
+int64_t attention_units_max(const BatchView& t, int kv_heads, int group)
+{
+    // tiles: (n * group + 15) / 16 of a sequence; parts: at most target more than tiles
+    return ((int64_t)t.rows * group / kRows + t.seqs) * kv_heads + 2 * kTarget;
+}
+
+hipError_t launch_attention(const CacheView& c, const BatchView& t, const void* q, int64_t q_stride, int qdt, int group, float scale, int window, void* y,
+                            void* scratch, void* tickets, hipStream_t st)
+{
+    AttnArgs a;
+    a.c = c;
+    a.t = t;
+    a.q = q;
+    a.y = y;
+    a.q_stride = q_stride;
+    a.slabs = static_cast<float*>(scratch);
+    a.tickets = static_cast<unsigned*>(tickets);
+    a.group = group;
+    a.qdt = qdt;
+    a.window = window;
+    a.target = kTarget;
+    a.least = kWaves;
+    a.scale = scale * 1.44269504088896340736f;
+    const unsigned grid = (unsigned)attention_units_max(t, c.kv_heads, group);
+#define CYBQ_ROWS(KIND)                              \
+    switch (c.dim) {                                 \
+        case 64: return rows_as<KIND, 2>(a, grid, st);  \
+        case 96: return rows_as<KIND, 3>(a, grid, st);  \
+        case 128: return rows_as<KIND, 4>(a, grid, st); \
+        default: return rows_as<KIND, 8>(a, grid, st);  \
+    }
+    switch (c.kind) {
+        case kCacheF16: CYBQ_ROWS(kCacheF16)
+        case kCacheBF16: CYBQ_ROWS(kCacheBF16)
+        case kCacheQ4: CYBQ_ROWS(kCacheQ4)
+        default: CYBQ_ROWS(kCacheQ8)
+    }
+#undef CYBQ_ROWS
+}
+
+}  // namespace cybq

@@ -120,6 +120,22 @@ void set_experts_tuning(int cols, int many, int token);
 hipError_t launch_experts_sum(const float* z, const int32_t* ids, const float* weights, const void* residual, int64_t T, int top_k, int E, int N, void* y,
                               int ydt, hipStream_t st);
 
+// paged key-value cache (cache.hip): the rows of a batch into their pages - turned by rope ([positions][rot / 2][2], nullptr: not), q to
+// q_out (nullptr: no q) -, and back out.  Rows' strides in elements; all rows 16-byte aligned, rot a multiple of 16.
+struct CacheView;
+struct BatchView;
+hipError_t launch_cache_append(const CacheView& c, const BatchView& t, const void* q, int64_t q_stride, int group, const void* k, int64_t k_stride,
+                               const void* v, int64_t v_stride, int dt, const float* rope, int rot, bool halves, void* q_out, int qdt, hipStream_t st);
+hipError_t launch_cache_read(const CacheView& c, const BatchView& t, void* k, void* v, int dt, hipStream_t st);
+// attention of the batch's rows over it (attention.hip); group: query heads per kv head.  scratch: attention_scratch_bytes; tickets:
+// kAttnTicketBytes that are zero at rest.  Calls that share them must not overlap.
+constexpr size_t kAttnTicketBytes = (size_t)1 << 16;
+size_t attention_scratch_bytes(int dim);
+int64_t attention_units_max(const BatchView& t, int kv_heads, int group);       // the call is for launch_attention up to ..
+int64_t attention_max_units();                                                  // .. this many
+hipError_t launch_attention(const CacheView& c, const BatchView& t, const void* q, int64_t q_stride, int qdt, int group, float scale, int window, void* y,
+                            void* scratch, void* tickets, hipStream_t st);
+
 // Kernels that need more dynamic LDS than the default 64 KB say so when the library is loaded:
 // naming LdsRequest<&kernel, bytes>::registered anywhere in a launcher puts the pair on a list
 // (a static initialiser, run before any call).  cybq_init walks the list for its device, so

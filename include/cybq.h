@@ -339,6 +339,80 @@ int cybq_matmul_experts_sum(cybq_ctx* ctx, const cybq_weight* w, int64_t E, cons
                             int64_t top_k, const int32_t* ids, const float* weights, const void* residual, void* y,
                             cybq_dtype ydt, void* stream);
 
+/* ---- paged key-value cache and attention ----------------------------------
+ *
+ * What stands between the QKV projection and the O projection of the decode loop ("QKV -> RoPE -> KV cache -> attention -> O
+ * proj", decide/pipeline.md:51).  The reference's own definitions of these ops are not visible in its tree; formulas, layout and limits
+ * are this library's choice.
+ *
+ * A cache holds the keys and values of `pages` pages of page_tokens tokens for every layer, allocated once.  Which page holds
+ * which tokens is the caller's affair: cybq_batch names, for every sequence of a call, its pages in order.  One table serves all layers.
+ * Kinds: 16 bits as they are, or the weights' own form: per 32 dimensions of a head d = f16(absmax / qmax), q = clamp(round(x / d)),
+ * ties away from zero, absmax / qmax and x / d rounded to fp32 first; qmax = 127 (Q8) or 7 (Q4).
+ * A cache holds finite numbers: NaN is stored as 0, what is beyond the kind's range at its end (F16 65504, BF16 its largest,
+ * Q8 and Q4 57344).  Pages are zeros until they are written. */
+typedef struct cybq_cache cybq_cache;
+
+typedef enum cybq_cache_kind { CYBQ_CACHE_F16 = 1, CYBQ_CACHE_BF16 = 2, CYBQ_CACHE_Q4 = 4, CYBQ_CACHE_Q8 = 8 } cybq_cache_kind;
+
+/* Which dimensions of a head turn together: i and i + rope_dims / 2, or 2 i and 2 i + 1 */
+typedef enum cybq_rope_style { CYBQ_ROPE_HALVES = 0, CYBQ_ROPE_PAIRS = 1 } cybq_rope_style;
+
+/* head_dim: 64, 96, 128 or 256; page_tokens: a power of two in 32 .. 1024.  The memory is the caller's from here on; it is
+ * cleared before the call returns.  A cache is for calls on its device, whichever context makes them. */
+int cybq_cache_create(cybq_ctx* ctx, cybq_cache_kind kind, int64_t layers, int64_t kv_heads, int64_t head_dim, int64_t page_tokens,
+                      int64_t pages, cybq_cache** out);
+/* Waits for the device. */
+int cybq_cache_free(cybq_ctx* ctx, cybq_cache* cache);
+/* any of the out pointers may be NULL.  Page p of layer l is page_bytes bytes at memory + l * layer_bytes + p * page_bytes (device
+ * memory).  A page's bytes mean the same wherever they stand: a caller may copy pages (a sequence that forks, pages that are swapped
+ * out), to any page and layer of any cache of the same kind and sizes; it writes nothing else there. */
+int cybq_cache_info(const cybq_cache* cache, int* kind, int64_t* layers, int64_t* kv_heads, int64_t* head_dim, int64_t* page_tokens,
+                    int64_t* pages, int64_t* page_bytes, int64_t* layer_bytes, void** memory);
+
+/* The rows of a call.  Sequence b has n = starts[b + 1] - starts[b] rows, from row starts[b] on: the last n of its lengths[b] tokens (new
+ * tokens are counted).  Row i of them is at position lengths[b] - n + i; the token at position j lies in page
+ * tables[b * table_pages + j / page_tokens].  A page id outside 0 .. pages - 1 is no page (pages that a window has left behind), nor is
+ * there one behind the table: tokens without a page are not stored, not seen, and read as zeros; so with positions below 0.
+ * starts rise from 0 to at most `rows`; rows that belong to no sequence are left as they are.  max_new is at least every n (of a longer
+ * sequence the first max_new rows are all).  A batch whose starts do not rise has no defined results, but no access leaves its buffers.
+ * starts, lengths and tables are device memory: calls neither look at them on the host nor allocate, so they can be captured
+ * and replayed with other contents.  The struct itself is read during the call. */
+typedef struct cybq_batch {
+    int64_t seqs, rows, max_new, table_pages;    /* <= 65536, <= 2^24, <= 2^24; table_pages * page_tokens <= 2^30 */
+    const int32_t* starts;                       /* [seqs + 1] */
+    const int32_t* lengths;                      /* [seqs], up to 2^30 */
+    const int32_t* tables;                       /* [seqs][table_pages] */
+} cybq_batch;
+
+/* New tokens into the cache.  k, v: rows of [kv_heads][head_dim] of dt; q: rows of [q_heads][head_dim] of dt, or NULL (then q_out is
+ * NULL too); strides in elements between rows.  q and k turn by the row's position p:
+ *     x0' = x0 c - x1 s,  x1' = x1 c + x0 s,  (c, s) = rope[p][i], i < rope_dims / 2;   rope: fp32 [rope_positions][rope_dims / 2][2]
+ * (in fp64, rounded to fp32), or not at all (rope NULL).  k and v are stored; q_out [rows][q_heads][head_dim] of qdt (F16 or BF16) is q,
+ * rounded once, zeros for a row at no position of the table.
+ * q, k, v, rope, q_out and their rows are 16-byte aligned; rope_dims is a multiple of 16, at most head_dim; rope covers the table
+ * (rope_positions >= table_pages * page_tokens); q_heads is a multiple of the cache's kv_heads.  q_out must not overlap q, k or v.  Two
+ * rows at the same place of the cache: one of them is stored, or parts of both. */
+int cybq_cache_append(cybq_ctx* ctx, cybq_cache* cache, int64_t layer, const cybq_batch* batch, const void* q, int64_t q_stride,
+                      int64_t q_heads, const void* k, int64_t k_stride, const void* v, int64_t v_stride, cybq_dtype dt,
+                      const float* rope, int64_t rope_positions, int64_t rope_dims, cybq_rope_style style, void* q_out, cybq_dtype qdt,
+                      void* stream);
+
+/* What the cache holds for the batch's rows: k, v [rows][kv_heads][head_dim] of dt (d * q rounded once), 16-byte aligned. */
+int cybq_cache_read(cybq_ctx* ctx, const cybq_cache* cache, int64_t layer, const cybq_batch* batch, void* k, void* v, cybq_dtype dt,
+                    void* stream);
+
+/* Attention of the batch's rows over their sequences' tokens, which are stored already (the rows' own among them):
+ *     y[row, h] = sum_j softmax_j(scale * q[row, h] . k[j, h / (q_heads / kv_heads)]) v[j, ..],   p - window < j <= p
+ * p: the row's position; window 0: all j <= p.  A row that sees nothing is zeros.
+ *   q: rows of [q_heads][head_dim] of qdt, q_stride elements apart, 16-byte aligned as its rows are; y [rows][q_heads][head_dim] of qdt, 8-byte
+ *   aligned, must not overlap q.  qdt: F16 on an F16 cache, BF16 on a BF16 cache, either of them on Q8 and Q4 (CYBQ_ERR_UNSUPPORTED).
+ *   scale is positive and finite; scaled scores have to stay within fp32.
+ * Scores, maxima and sums are fp32.  On Q8 and Q4 caches keys are exact, or round_f16(scale * q) where a sequence has many rows; values are
+ * round_f16(scale * q).  Calls on one context share its scratch: they (replays of its graphs too) must not overlap in time. */
+int cybq_attention(cybq_ctx* ctx, const cybq_cache* cache, int64_t layer, const cybq_batch* batch, const void* q, int64_t q_stride,
+                   cybq_dtype qdt, int64_t q_heads, float scale, int64_t window, void* y, void* stream);
+
 /* Replaces: nothing the runtime calls per token; it is the verification hook
  * ("dequantised weights match bit-exactly"): out[N,K] f32 = f32(scale) * q. */
 int cybq_dequant(cybq_ctx* ctx, const cybq_weight* w, float* out, void* stream);

@@ -17,6 +17,23 @@ pub struct cybq_weight {
     _opaque: [u8; 0],
 }
 
+#[repr(C)]
+pub struct cybq_cache {
+    _opaque: [u8; 0],
+}
+/// `starts`, `lengths` and `tables` are device pointers.
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct cybq_batch {
+    pub seqs: i64,
+    pub rows: i64,
+    pub max_new: i64,
+    pub table_pages: i64,
+    pub starts: *const i32,
+    pub lengths: *const i32,
+    pub tables: *const i32,
+}
+
 pub const CYBQ_GROUP: c_int = 32;
 pub const CYBQ_MAX_EXPERTS: c_int = 1024;
 pub const CYBQ_MAX_TOP_K: c_int = 64;
@@ -54,6 +71,14 @@ pub const CYBQ_EPI_SWIGLU: c_int = 2;
 // enum cybq_score
 pub const CYBQ_SCORE_SOFTMAX: c_int = 0;
 pub const CYBQ_SCORE_SIGMOID: c_int = 1;
+// enum cybq_cache_kind
+pub const CYBQ_CACHE_F16: c_int = 1;
+pub const CYBQ_CACHE_BF16: c_int = 2;
+pub const CYBQ_CACHE_Q4: c_int = 4;
+pub const CYBQ_CACHE_Q8: c_int = 8;
+// enum cybq_rope_style
+pub const CYBQ_ROPE_HALVES: c_int = 0;
+pub const CYBQ_ROPE_PAIRS: c_int = 1;
 
 extern "C" {
     pub fn cybq_init(device: c_int, out: *mut *mut cybq_ctx) -> c_int;
@@ -110,6 +135,22 @@ extern "C" {
                                    ids: *const i32, weights: *const c_float,
                                    residual: *const c_void, y: *mut c_void, ydt: c_int,
                                    stream: *mut c_void) -> c_int;
+    pub fn cybq_cache_create(ctx: *mut cybq_ctx, kind: c_int, layers: i64, kv_heads: i64, head_dim: i64,
+                             page_tokens: i64, pages: i64, out: *mut *mut cybq_cache) -> c_int;
+    pub fn cybq_cache_free(ctx: *mut cybq_ctx, cache: *mut cybq_cache) -> c_int;
+    pub fn cybq_cache_info(cache: *const cybq_cache, kind: *mut c_int, layers: *mut i64, kv_heads: *mut i64,
+                           head_dim: *mut i64, page_tokens: *mut i64, pages: *mut i64, page_bytes: *mut i64,
+                           layer_bytes: *mut i64, memory: *mut *mut c_void) -> c_int;
+    pub fn cybq_cache_append(ctx: *mut cybq_ctx, cache: *mut cybq_cache, layer: i64, batch: *const cybq_batch,
+                             q: *const c_void, q_stride: i64, q_heads: i64, k: *const c_void, k_stride: i64,
+                             v: *const c_void, v_stride: i64, dt: c_int, rope: *const c_float,
+                             rope_positions: i64, rope_dims: i64, style: c_int, q_out: *mut c_void, qdt: c_int,
+                             stream: *mut c_void) -> c_int;
+    pub fn cybq_cache_read(ctx: *mut cybq_ctx, cache: *const cybq_cache, layer: i64, batch: *const cybq_batch,
+                           k: *mut c_void, v: *mut c_void, dt: c_int, stream: *mut c_void) -> c_int;
+    pub fn cybq_attention(ctx: *mut cybq_ctx, cache: *const cybq_cache, layer: i64, batch: *const cybq_batch,
+                          q: *const c_void, q_stride: i64, qdt: c_int, q_heads: i64, scale: c_float, window: i64,
+                          y: *mut c_void, stream: *mut c_void) -> c_int;
     pub fn cybq_dequant(ctx: *mut cybq_ctx, w: *const cybq_weight, out: *mut c_float, stream: *mut c_void) -> c_int;
     pub fn cybq_quantize(ctx: *mut cybq_ctx, quant: c_int, src: *const c_float, N: i64, K: i64, q_out: *mut c_void,
                          scales_out: *mut c_void, stream: *mut c_void) -> c_int;

@@ -1,0 +1,236 @@
+"""Attention over the paged cache - cybq_attention - against its definition in float64.
+
+Bound of an output element, S = sum of p |v| over what its row sees, D = the largest sum of |q| |k| scale:
+  y's own rounding       half a step of its type, of y
+  values, Q8 and Q4      round_f16(scale q): 2^-11 S;   P of f16: 2^-11 S;   P of bf16 as two numbers: 2^-16 S, as one (many rows): 2^-8 S
+  scores                 products are exact, a sum of `dim` of them and its scales in fp32: (dim + 8) 2^-24 D absolute, of keys rounded to
+                         f16 (many rows on Q8, Q4) 2^-11 D more; the exponent's argument and the exponential 2^-21 more for scores up to 4;
+                         a score's error is a relative one of its P, and of the sum that divides: twice
+  sums                   fp32, at most a few hundred terms in a row before others join: 2^-15 S
+  quantised, bf16 q      a row becomes f16 behind a power of two: exact but for what is 2^-25 of its largest, below the terms above"""
+import math
+
+import numpy as np
+import pytest
+
+from cyb_amd.backend import Backend
+
+torch = pytest.importorskip("torch")
+from tests.cache_lib import HALF_STEP, TDT, Cached, normal, rope_table      # noqa: E402
+
+gpu = pytest.mark.gpu
+U = 2.0 ** -24
+
+
+def bound(kind, dt, dim, y, size, dots, many):
+    quantised = kind in ("q8", "q4")
+    p = 2.0 ** -11 if kind != "bf16" else 2.0 ** -8 if many else 2.0 ** -16
+    score = (dim + 8) * U * dots + 2.0 ** -21 + (2.0 ** -11 * dots if quantised and many else 0.0)
+    return HALF_STEP[dt] * y.abs() + size * (p + (2.0 ** -11 if quantised else 0.0) + 2 * score + 2.0 ** -15) + 2.0 ** -25
+
+
+def check(s, new, group, dt, window=0, many=False, scale=None, hidden=lambda b, j: False, rows=None, stream=0, q=None, seed=9):
+    rows = rows if rows is not None else sum(new)
+    q = q if q is not None else normal((rows, s.kv_heads * group, s.dim), seed, dt)
+    y = torch.full((rows,) + tuple(q.shape[1:]), 9.0, dtype=TDT[dt], device="cuda")
+    s.be.attention(s.cache, s.layer, s.batch(new, rows=rows), q, y, scale=scale, window=window, stream=stream)
+    torch.cuda.synchronize()
+    used = sum(new)
+    ref, size, dots = s.expected(q[:used], new, scale, window, hidden)
+    assert torch.isfinite(y).all()
+    off = (y[:used].double() - ref).abs()
+    worst = (off / bound(s.kind, dt, s.dim, ref, size, dots, many)).max().item() if used else 0.0
+    assert worst <= 1.0, worst
+    assert (y[used:] == 9.0).all()                               # rows of no sequence
+    return y
+
+
+KINDS = [("f16", "f16"), ("bf16", "bf16"), ("q8", "f16"), ("q8", "bf16"), ("q4", "f16"), ("q4", "bf16")]
+
+
+@gpu
+@pytest.mark.parametrize("kind,dt", KINDS)
+@pytest.mark.parametrize("dim", [64, 96, 128, 256])
+def test_one_token_of_every_length(backend, kind, dt, dim):
+    lengths = [1, 2, 31, 32, 33, 63, 64, 65, 255, 256, 257, 300, 511, 777]
+    s = Cached(backend, kind, lengths, kv_heads=2, dim=dim, page=64)
+    for group in (1, 4, 7):
+        check(s, [1] * len(lengths), group, dt)
+    s.close()
+
+
+@gpu
+@pytest.mark.parametrize("kind,dt", KINDS)
+@pytest.mark.parametrize("page", [32, 256, 1024])
+def test_drafts_and_windows(backend, kind, dt, page):
+    """A few new rows each: rows that see different tokens, more than a tile of them, windows that begin and end anywhere."""
+    lengths, new = [5, 40, 300, 1030, 64], [5, 3, 7, 2, 4]
+    s = Cached(backend, kind, lengths, kv_heads=2, dim=128, page=page)
+    for group in (1, 3, 5, 16):
+        for window in (0, 1, 2, 31, 32, 33, 200, 5000):
+            check(s, new, group, dt, window=window)
+    s.close()
+
+
+@gpu
+@pytest.mark.parametrize("kind,dt", KINDS)
+@pytest.mark.parametrize("dim", [64, 96, 128, 256])
+def test_prompts(backend, kind, dt, dim):
+    """Hundreds of rows: from a prompt's first token on, and behind what is cached."""
+    for lengths, new, window in (([200], [200], 0), ([333, 150, 700], [100, 150, 391], 0), ([600], [300], 100), ([513], [129], 0)):
+        s = Cached(backend, kind, lengths, kv_heads=1, dim=dim, page=64, seed=len(lengths))
+        check(s, new, 3, dt, window=window, many=True)
+        s.close()
+
+
+@gpu
+@pytest.mark.parametrize("kind,dt", KINDS)
+def test_a_long_context_is_shared_out(backend, kind, dt):
+    s = Cached(backend, kind, [20011, 130], kv_heads=2, dim=128, page=128)
+    check(s, [1, 1], 4, dt)
+    check(s, [3, 2], 5, dt, window=15000)
+    s.close()
+
+
+@gpu
+def test_more_sequences_than_lanes(backend):
+    rng = np.random.default_rng(2)
+    lengths = rng.integers(0, 200, 200).tolist()
+    lengths[100], lengths[3] = 6000, 0
+    s = Cached(backend, "q8", lengths, kv_heads=2, dim=64, page=32)
+    new = [min(L, int(n)) for L, n in zip(lengths, rng.integers(0, 4, 200))]
+    check(s, new, 3, "f16", rows=sum(new) + 5)
+    s.close()
+
+
+@gpu
+@pytest.mark.parametrize("kind,dt", [("f16", "f16"), ("q4", "bf16")])
+def test_rows_that_see_nothing(backend, kind, dt):
+    """Sequences without tokens, more rows than tokens, pages that are none, a whole window without a page: zeros, never NaN."""
+    s = Cached(backend, kind, [96, 40, 300], kv_heads=2, dim=64, page=32)
+    s.tables[0, 0] = -1
+    s.tables[2, 3:8] = 1 << 30                                    # tokens 96 .. 255 are in no page
+    group = 2
+    # rows 0 .. 31 of the first sequence see nothing
+    y = check(s, [96, 1, 60], group, dt, hidden=lambda b, j: (b == 0 and j < 32) or (b == 2 and 96 <= j < 256), many=True)
+    assert (y[:32] == 0).all()
+    y = check(s, [1, 1, 50], group, dt, window=10, hidden=lambda b, j: (b == 0 and j < 32) or (b == 2 and 96 <= j < 256))
+    assert (y[2:8] == 0).all()                                   # positions 250 .. 255 with a window of 10
+    # a length that the rows exceed, and none at all
+    q = normal((12, 4, 64), 3, dt)
+    out = torch.full_like(q, 9.0)
+    backend.attention(s.cache, 0, s.batch([7, 5, 0], lengths=[3, 0, 0]), q, out)
+    torch.cuda.synchronize()
+    assert (out[:4] == 0).all() and (out[7:] == 0).all() and torch.isfinite(out).all()
+    s.close()
+
+
+@gpu
+def test_values_at_the_ends(backend):
+    """Scores that differ by thousands, equal ones, a scale of the caller's, keys and values at the ends of the kinds, rows of NaN."""
+    for kind, dt in KINDS:
+        s = Cached(backend, kind, [100], kv_heads=1, dim=64, page=32)
+        q = normal((4, 2, 64), 1, dt) * 100
+        check(s, [4], 2, dt, q=q, scale=0.5)                     # one token has it all
+        check(s, [4], 2, dt, q=torch.zeros_like(q))              # the mean
+        check(s, [4], 2, dt, scale=1e-6)
+        q[1, 0, 5] = math.nan
+        y = torch.empty_like(q)
+        backend.attention(s.cache, 0, s.batch([4]), q, y)
+        torch.cuda.synchronize()
+        bad = torch.isnan(y).all(dim=2)
+        assert bad[1, 0] and bad.sum() == 1 and torch.isnan(y).sum() == 64
+        s.close()
+    # rows of bf16 far outside f16 on a quantised cache
+    s = Cached(backend, "q8", [50], kv_heads=1, dim=64, page=32)
+    check(s, [2], 2, "bf16", q=normal((2, 2, 64), 2, "bf16", std=1e25), scale=1e-25)
+    check(s, [2], 2, "bf16", q=normal((2, 2, 64), 2, "bf16", std=1e-25), scale=1e25)
+    s.close()
+    # infinities and NaN that were stored are finite numbers: no other row meets them
+    for kind, dt in KINDS:
+        s = Cached(backend, kind, [64], kv_heads=1, dim=64, page=32)
+        x = normal((2, 1, 64), 4, dt)
+        x[1] = math.inf
+        x[1, 0, 3] = math.nan
+        backend.cache_append(s.cache, 0, s.batch([2]), None, normal((2, 1, 64), 5, dt), x)
+        q = normal((2, 1, 64), 6, dt)
+        y, first = torch.empty_like(q), torch.empty_like(q)
+        backend.attention(s.cache, 0, s.batch([2]), q, y)
+        backend.cache_append(s.cache, 0, s.batch([2]), None, normal((2, 1, 64), 5, dt), torch.where(torch.isfinite(x), x, 0.0))
+        backend.attention(s.cache, 0, s.batch([2]), q, first)
+        torch.cuda.synchronize()
+        assert torch.equal(y[0], first[0])
+        s.close()
+
+
+@gpu
+def test_strides_streams_and_the_same_bits_twice(backend):
+    """q as a slice of the projection's rows, on a stream of its own; results do not hang on who arrives first."""
+    s = Cached(backend, "q8", [3000, 1500], kv_heads=2, dim=128, page=64)
+    wide = normal((5, 6 * 4, 128), 7, "f16")
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    a = check(s, [3, 2], 4, "f16", q=wide[:, 8:16], stream=side.cuda_stream)
+    for _ in range(3):
+        assert torch.equal(a, check(s, [3, 2], 4, "f16", q=wide[:, 8:16].contiguous()))
+    s.close()
+
+
+@gpu
+def test_a_captured_step_follows_its_lengths(backend):
+    """Append and attention recorded once, on a fresh context; replayed with other lengths, tables and rows, with eager calls in between."""
+    be = Backend(0)
+    try:
+        B, group, page, width, dim = 3, 4, 32, 100, 64
+        s = Cached(be, "q8", [700, 40, 2900], kv_heads=2, dim=dim, page=page, width=width, spare=40)
+        rope = rope_table(width * page, dim)
+        qkv = normal((B, (group + 2) * 2, dim), 11, "f16")
+        q, y = (torch.zeros((B, group * 2, dim), dtype=torch.float16, device="cuda") for _ in range(2))
+        starts = torch.arange(B + 1, dtype=torch.int32, device="cuda")
+        lengths = torch.tensor([1, 1, 1], dtype=torch.int32, device="cuda")
+        batch = be.cache_batch(starts, lengths, s.tables, B, 1)
+
+        def step(stream=0):
+            h = group * 2
+            be.cache_append(s.cache, 0, batch, qkv[:, :h], qkv[:, h:h + 2], qkv[:, h + 2:], q, rope=rope, stream=stream)
+            be.attention(s.cache, 0, batch, q, y, window=2000, stream=stream)
+
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+            step(torch.cuda.current_stream().cuda_stream)
+        for i, now in enumerate(([700, 40, 2900], [1, 39, 2], [512, 1, 2899], [700, 40, 2900])):
+            lengths.copy_(torch.tensor(now, dtype=torch.int32))
+            qkv.copy_(normal(tuple(qkv.shape), 20 + i, "f16"))
+            y.zero_()
+            q.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            got, turned_q = y.clone(), q.clone()
+            y.zero_()
+            q.zero_()
+            step()
+            torch.cuda.synchronize()
+            assert torch.equal(got, y) and torch.equal(turned_q, q) and (got != 0).any()
+        s.close()
+    finally:
+        be.close()
+
+
+@gpu
+def test_batches_that_make_no_sense_stay_inside(backend):
+    """Starts that fall or lie outside, lengths below zero and beyond the table: some rows, no access outside (checked in the kernels)."""
+    s = Cached(backend, "q8", [64, 64, 64], kv_heads=1, dim=64, page=32)
+    q = normal((8, 2, 64), 1, "f16")
+    guard = torch.full((24, 2, 64), 9.0, dtype=torch.float16, device="cuda")
+    ints = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    for starts, lengths in (([0, 8, 0, 8], [64, 64, 64]), ([-5, 3, 100, 2], [64, 64, 64]), ([0, 1 << 30, -(1 << 30), 8], [1 << 30, -7, 64]),
+                            ([0, 2, 4, 8], [-(1 << 31), (1 << 31) - 1, 70])):
+        b = backend.cache_batch(ints(starts), ints(lengths), s.tables, 8, 8)
+        y = guard[8:16]
+        backend.attention(s.cache, 0, b, q, y)
+        backend.cache_read(s.cache, 0, b, torch.empty((8, 1, 64), device="cuda"), torch.empty((8, 1, 64), device="cuda"))
+        torch.cuda.synchronize()
+        assert (guard[:8] == 9.0).all() and (guard[16:] == 9.0).all()
+    check(s, [3, 1, 2], 2, "f16")                                # and what comes after is right
+    s.close()
