@@ -263,6 +263,7 @@ class KVCache:
     def __init__(self, backend: "Backend", handle: int):
         self._backend = backend
         self._h = ctypes.c_void_p(handle)
+        self._addr = handle or 0                        # the same for the native call path; 0 once freed
         kind, memory = ctypes.c_int(), ctypes.c_void_p()
         n = [ctypes.c_int64() for _ in range(7)]
         backend._check(backend._lib.cybq_cache_info(self._h, kind, *n, memory))
@@ -280,6 +281,7 @@ class KVCache:
         if self._h and self._backend._ctx:
             self._backend._lib.cybq_cache_free(self._backend._ctx, self._h)
         self._h = ctypes.c_void_p()
+        self._addr = 0
 
     def __del__(self):
         try:
@@ -601,6 +603,11 @@ class Backend:
         [positions, pairs, 2] (fp32 cos, sin; None: not turned).  q, k and v may be slices of one projection's rows."""
         if style not in ROPE_STYLES:
             raise CybqError(-1, "invalid argument", f"unknown rope style {style!r}")
+        calls = _calls or _load_calls()
+        if calls:
+            rc = calls.append(self._addr, self.device, cache._addr, layer, batch._addr, batch._device, q, k, v, q_out, rope, ROPE_STYLES[style], stream)
+            if rc <= 0:
+                return self._check(rc)
         rows = self._check_batch(cache, batch)
         _, ks = self._check_heads(k, "k", rows, cache.kv_heads, cache.dim)
         _, vs = self._check_heads(v, "v", rows, cache.kv_heads, cache.dim)
@@ -626,6 +633,11 @@ class Backend:
 
     def cache_read(self, cache: KVCache, layer: int, batch: CacheBatch, k, v, stream: int = 0) -> None:
         """cybq_cache_read: what the cache holds for the batch's rows, to k and v [rows, kv_heads, dim]."""
+        calls = _calls or _load_calls()
+        if calls:
+            rc = calls.read(self._addr, self.device, cache._addr, layer, batch._addr, batch._device, k, v, stream)
+            if rc <= 0:
+                return self._check(rc)
         rows = self._check_batch(cache, batch)
         for t, what in ((k, "k"), (v, "v")):
             self._check_heads(t, what, rows, cache.kv_heads, cache.dim)
@@ -637,6 +649,11 @@ class Backend:
     def attention(self, cache: KVCache, layer: int, batch: CacheBatch, q, y, scale: Optional[float] = None, window: int = 0, stream: int = 0) -> None:
         """cybq_attention: y[t] = softmax(scale * q[t] . k) v over the tokens of row t's sequence up to its own, at most `window` of them (0: all).
         q, y [rows, heads, dim]; scale None: dim ** -0.5."""
+        calls = _calls or _load_calls()
+        if calls:
+            rc = calls.attention(self._addr, self.device, cache._addr, layer, batch._addr, batch._device, q, y, scale, window, stream)
+            if rc <= 0:
+                return self._check(rc)
         rows = self._check_batch(cache, batch)
         heads, qs = self._check_heads(q, "q", rows, None, cache.dim)
         self._check_heads(y, "y", rows, heads, cache.dim)

@@ -1,5 +1,5 @@
 // torch_calls.cpp - the Python binding's call path for torch tensors: Backend.matmul / matmul_ex / matmul_norm / matmul_static,
-// route / matmul_experts / matmul_experts_sum.
+// route / matmul_experts / matmul_experts_sum, cache_append / cache_read / attention.
 //
 // A small linear is bound by the host: the launch itself takes 2.9 us of host time, the kernel behind it less.  Looking
 // the tensors over in Python (shape, device, contiguity, type, address: a dozen attribute calls) and going through
@@ -11,6 +11,8 @@
 #include <Python.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/version.h>
+
+#include <cmath>
 
 #include "../../include/cybq.h"
 
@@ -268,7 +270,119 @@ PyObject* experts_sum(PyObject* const* a, Py_ssize_t n)
     return answer(rc);
 }
 
+// what the calls on a cache share: ctx, device, cache address, layer, batch address, the batch's device; stream
+struct Cached {
+    cybq_ctx* ctx;
+    cybq_cache* cache;
+    const cybq_batch* batch;
+    int device;
+    int64_t layer, kv_heads = 0, dim = 0;
+    void* stream;
+};
+
+bool cached_of(PyObject* const* a, PyObject* stream, Cached* r)
+{
+    int64_t ctx, device, cache, batch, of_batch, st;
+    if (!as_int(a[0], &ctx) || !as_int(a[1], &device) || !as_int(a[2], &cache) || !as_int(a[3], &r->layer) || !as_int(a[4], &batch) ||
+        !as_int(a[5], &of_batch) || !as_int(stream, &st) || !ctx || !cache || !batch || of_batch != device)
+        return false;
+    r->ctx = reinterpret_cast<cybq_ctx*>(static_cast<uintptr_t>(ctx));
+    r->cache = reinterpret_cast<cybq_cache*>(static_cast<uintptr_t>(cache));
+    r->batch = reinterpret_cast<const cybq_batch*>(static_cast<uintptr_t>(batch));
+    r->device = (int)device;
+    r->stream = reinterpret_cast<void*>(static_cast<uintptr_t>(st));
+    return cybq_cache_info(r->cache, nullptr, nullptr, &r->kv_heads, &r->dim, nullptr, nullptr, nullptr, nullptr, nullptr) == CYBQ_OK;
+}
+
+// rows [>= batch rows][heads][dim] -> address; rows may lie apart where the caller takes `stride`.  *heads: 0 for any, and the answer
+void* rows_of(PyObject* o, const Cached& r, int64_t* heads, int64_t* stride, int* dtype)
+{
+    if (!THPVariable_CheckExact(o)) return nullptr;
+    const at::Tensor& t = THPVariable_Unpack(o);
+    if (!t.is_cuda() || t.get_device() != r.device || t.dim() != 3 || t.size(0) < r.batch->rows || t.size(2) != r.dim || t.size(0) < 1 || t.size(1) < 1 ||
+        (*heads && t.size(1) != *heads) || t.stride(2) != 1 || (t.size(1) > 1 && t.stride(1) != r.dim))
+        return nullptr;
+    const int64_t apart = t.size(0) > 1 ? t.stride(0) : t.size(1) * r.dim;
+    if (stride) *stride = apart;
+    else if (!t.is_contiguous()) return nullptr;
+    *heads = t.size(1);
+    switch (t.scalar_type()) {
+        case at::kFloat: *dtype = CYBQ_F32; break;
+        case at::kHalf: *dtype = CYBQ_F16; break;
+        case at::kBFloat16: *dtype = CYBQ_BF16; break;
+        default: return nullptr;
+    }
+    return t.data_ptr();
+}
+
+// append(ctx, device, cache, layer, batch, batch device, q or None, k, v, q_out or None, rope or None, style, stream)
+PyObject* append(PyObject* const* a, Py_ssize_t n)
+{
+    Cached r;
+    int64_t style;
+    if (n != 13 || !cached_of(a, a[12], &r) || !as_int(a[11], &style) || (a[6] == Py_None) != (a[9] == Py_None)) return answer(kSlow);
+    int64_t kh = r.kv_heads, vh = r.kv_heads, ks, vs, qs = 0, heads = 0, positions = 0, dims = 0;
+    int dt = 0, vdt = 0, qdt = 0, out = CYBQ_F16;
+    void *k = rows_of(a[7], r, &kh, &ks, &dt), *v = rows_of(a[8], r, &vh, &vs, &vdt), *q = nullptr, *q_out = nullptr, *rope = nullptr;
+    if (!k || !v || vdt != dt) return answer(kSlow);
+    if (a[6] != Py_None && (!(q = rows_of(a[6], r, &heads, &qs, &qdt)) || qdt != dt || !(q_out = rows_of(a[9], r, &heads, nullptr, &out)))) return answer(kSlow);
+    if (a[10] != Py_None) {
+        int rdt = 0;
+        if (!(rope = address(a[10], r.device, 1, &rdt)) || rdt != CYBQ_F32) return answer(kSlow);
+        const at::Tensor& t = THPVariable_Unpack(a[10]);
+        if (t.dim() != 3 || t.size(2) != 2) return answer(kSlow);
+        positions = t.size(0);
+        dims = 2 * t.size(1);
+    }
+    int rc;
+    {
+        Unlocked u;
+        rc = cybq_cache_append(r.ctx, r.cache, r.layer, r.batch, q, qs, heads, k, ks, v, vs, (cybq_dtype)dt, static_cast<const float*>(rope), positions, dims,
+                               (cybq_rope_style)style, q_out, (cybq_dtype)out, r.stream);
+    }
+    return answer(rc);
+}
+
+// read(ctx, device, cache, layer, batch, batch device, k, v, stream)
+PyObject* read(PyObject* const* a, Py_ssize_t n)
+{
+    Cached r;
+    if (n != 9 || !cached_of(a, a[8], &r)) return answer(kSlow);
+    int64_t kh = r.kv_heads, vh = r.kv_heads;
+    int dt = 0, vdt = 0;
+    void *k = rows_of(a[6], r, &kh, nullptr, &dt), *v = rows_of(a[7], r, &vh, nullptr, &vdt);
+    if (!k || !v || vdt != dt) return answer(kSlow);
+    int rc;
+    {
+        Unlocked u;
+        rc = cybq_cache_read(r.ctx, r.cache, r.layer, r.batch, k, v, (cybq_dtype)dt, r.stream);
+    }
+    return answer(rc);
+}
+
+// attention(ctx, device, cache, layer, batch, batch device, q, y, scale or None, window, stream)
+PyObject* attention(PyObject* const* a, Py_ssize_t n)
+{
+    Cached r;
+    int64_t window;
+    if (n != 11 || !cached_of(a, a[10], &r) || !as_int(a[9], &window) || (a[8] != Py_None && !PyFloat_CheckExact(a[8]))) return answer(kSlow);
+    int64_t heads = 0, stride;
+    int dt = 0, ydt = 0;
+    void *q = rows_of(a[6], r, &heads, &stride, &dt), *y = q ? rows_of(a[7], r, &heads, nullptr, &ydt) : nullptr;
+    if (!y || ydt != dt) return answer(kSlow);
+    const float scale = (float)(a[8] == Py_None ? std::pow((double)r.dim, -0.5) : PyFloat_AS_DOUBLE(a[8]));
+    int rc;
+    {
+        Unlocked u;
+        rc = cybq_attention(r.ctx, r.cache, r.layer, r.batch, q, stride, (cybq_dtype)dt, heads, scale, window, y, r.stream);
+    }
+    return answer(rc);
+}
+
 PyMethodDef kMethods[] = {
+    {"append", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(entry<append>)), METH_FASTCALL, nullptr},
+    {"read", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(entry<read>)), METH_FASTCALL, nullptr},
+    {"attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(entry<attention>)), METH_FASTCALL, nullptr},
     {"route", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(entry<route>)), METH_FASTCALL, nullptr},
     {"experts", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(entry<experts>)), METH_FASTCALL, nullptr},
     {"experts_sum", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(entry<experts_sum>)), METH_FASTCALL, nullptr},

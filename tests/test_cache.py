@@ -83,7 +83,7 @@ def _dry():
     be = B.Backend.__new__(B.Backend)
     be._lib, be._ctx, be._addr, be.device, be.weights = B.load_library(), ctypes.c_void_p(), 0, 0, {}
     c = B.KVCache.__new__(B.KVCache)
-    c._backend, c._h, c.kind, c.kv_heads, c.dim, c.layers = be, ctypes.c_void_p(), "q8", 2, 64, 1
+    c._backend, c._h, c._addr, c.kind, c.kv_heads, c.dim, c.layers = be, ctypes.c_void_p(), 0, "q8", 2, 64, 1
     b = B.CacheBatch.__new__(B.CacheBatch)
     b.rows, b._device, b._addr = 3, 0, 0
     return be, c, b
