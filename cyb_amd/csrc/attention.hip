@@ -29,10 +29,13 @@ struct AttnArgs {
     float* slabs;
     unsigned* tickets;
     int group, qdt, window, target, least;       // least: blocks of a part
+    int few;                                     // > 0: sequences of up to so many rows per kv head are the rows kernel's, others not
     float scale;                                 // times log2 e
 };
 
 constexpr int kMaxUnits = 1 << 24;               // of a call
+constexpr int kTarget = 256, kTileTarget = 512;  // parts of all, rows and tiles kernel
+constexpr int kFewRows = 64;                     // rows of a sequence and kv head (new tokens times group) that the rows kernel takes
 
 struct Unit {
     Seq s;
@@ -48,7 +51,15 @@ __device__ __forceinline__ void seen(const AttnArgs& a, int p_first, int p_last,
     *hi = end < first ? *lo : (int)(end >> 5) + 1;
 }
 
-template <int ROWS>
+// tiles of a sequence, 0: the other kernel's
+template <int ROWS, bool MANY>
+__device__ __forceinline__ int tiles_of(const AttnArgs& a, const Seq& s)
+{
+    const int rows = s.n * a.group;
+    return a.few && (rows > a.few) != MANY ? 0 : (rows + ROWS - 1) / ROWS;
+}
+
+template <int ROWS, bool MANY>
 __device__ __forceinline__ bool find_unit(const AttnArgs& a, int u, Unit* out)
 {
     const int lane = threadIdx.x & 63;
@@ -60,7 +71,7 @@ __device__ __forceinline__ bool find_unit(const AttnArgs& a, int u, Unit* out)
             const Seq s = seq_of(a.t, base + lane);
             int lo, hi;
             seen(a, s.len - s.n, s.len - 1, capacity, &lo, &hi);
-            work += (float)((s.n * a.group + ROWS - 1) / ROWS) * (float)(hi - lo);
+            work += (float)tiles_of<ROWS, MANY>(a, s) * (float)(hi - lo);
         }
     }
 #pragma unroll
@@ -77,7 +88,7 @@ __device__ __forceinline__ bool find_unit(const AttnArgs& a, int u, Unit* out)
             s = seq_of(a.t, base + lane);
             int lo, hi;
             seen(a, s.len - s.n, s.len - 1, capacity, &lo, &hi);
-            tiles = (s.n * a.group + ROWS - 1) / ROWS;
+            tiles = tiles_of<ROWS, MANY>(a, s);
             splits = max(1, (hi - lo + part - 1) / part);
         }
         // (a batch whose starts make no sense may add up to anything: what cannot be right stays above every grid)
@@ -93,11 +104,13 @@ __device__ __forceinline__ bool find_unit(const AttnArgs& a, int u, Unit* out)
             out->b = base + l;
             out->splits = __builtin_amdgcn_readlane(splits, l);
             const int at = u - (int)units - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(mine, l));
-            out->split = at % out->splits;
-            const int rest = at / out->splits;
-            out->head = rest % heads;
-            out->tile = rest / heads;
-            out->slab = slabs + __builtin_amdgcn_readlane(slab_upto, l) - __builtin_amdgcn_readlane(mine, l) + at;
+            // heads first: workgroups of one head, which read the same blocks, go to the same XCDs where there are 2, 4 or 8 of them; the last
+            // tiles first, which see the most
+            out->head = at % heads;
+            out->split = at / heads % out->splits;
+            out->tile = __builtin_amdgcn_readlane(tiles, l) - 1 - at / heads / out->splits;
+            const int rest = out->tile * heads + out->head;
+            out->slab = slabs + __builtin_amdgcn_readlane(slab_upto, l) - __builtin_amdgcn_readlane(mine, l) + rest * out->splits + out->split;
             out->ticket = tickets + __builtin_amdgcn_readlane(ticket_upto, l) - __builtin_amdgcn_readlane(rows, l) + rest;
         }
         units += total;
@@ -129,6 +142,15 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi)
 {
     const half2_t v = {(_Float16)lo, (_Float16)hi};
     return as_u32(v);
+}
+
+// rows of bf16 as f16: the power of two that brings the row's largest to 2^14 .. 2^15; *c, the scores' factor, takes it off again
+__device__ __forceinline__ float row_power(float top, float* c)
+{
+    const int e = (int)(__builtin_bit_cast(uint32_t, top) >> 23);
+    const int up = e == 0 || e == 255 ? 0 : max(-126, min(126, 141 - e));           // 2^up, and 2^-up, are normal numbers
+    *c *= __builtin_bit_cast(float, (uint32_t)(127 - up) << 23);
+    return __builtin_bit_cast(float, (uint32_t)(127 + up) << 23);
 }
 
 // a block's keys or values and their scales, as a lane has them from memory
@@ -235,7 +257,7 @@ __global__ __launch_bounds__(64 * kWaves) void attention_rows_kernel(AttnArgs a)
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q4 = lane >> 4, r = lane & 15;
     const uint32_t magic = q4_magic_vgpr();
     Unit u;
-    if (!find_unit<kRows>(a, blockIdx.x, &u)) return;
+    if (!find_unit<kRows, false>(a, blockIdx.x, &u)) return;
     const int64_t capacity = (int64_t)a.t.table_pages << (a.c.page_shift + 5);
     const int r0 = u.tile * kRows, rows = min(kRows, u.s.n * a.group - r0);
     const int p0 = u.s.len - u.s.n, i_first = r0 / a.group, i_last = (r0 + rows - 1) / a.group;
@@ -268,10 +290,7 @@ __global__ __launch_bounds__(64 * kWaves) void attention_rows_kernel(AttnArgs a)
             }
             top = fmaxf(top, other_quarter<16>(top));
             top = fmaxf(top, other_quarter<32>(top));
-            const int e = (int)(__builtin_bit_cast(uint32_t, top) >> 23);
-            const int up = e == 0 || e == 255 ? 0 : max(-126, min(126, 141 - e));           // 2^up, and 2^-up, are normal numbers
-            const float f = __builtin_bit_cast(float, (uint32_t)(127 + up) << 23);
-            c *= __builtin_bit_cast(float, (uint32_t)(127 - up) << 23);
+            const float f = row_power(top, &c);
 #pragma unroll
             for (int g = 0; g < G; g++)
 #pragma unroll
@@ -324,7 +343,7 @@ __global__ __launch_bounds__(64 * kWaves) void attention_rows_kernel(AttnArgs a)
                 }
             }
         }
-        const int tok = blk * kBlockTokens + 4 * q4;
+        const int tok = blk * kBlockTokens + 16 * (q4 >> 1) + 4 * (q4 & 1);
         const uint8_t* next;
         const int next_blk = next_there(blk + kWaves, &next);
         if (next) k.load(next, lane);
@@ -333,7 +352,7 @@ __global__ __launch_bounds__(64 * kWaves) void attention_rows_kernel(AttnArgs a)
             for (int t = 0; t < 2; t++)
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    const int j = tok + 16 * t + e;
+                    const int j = tok + 8 * t + e;
                     if (j < row_lo || j > row_hi) s[t][e] = none;
                 }
         }
@@ -469,6 +488,406 @@ __global__ __launch_bounds__(64 * kWaves) void attention_rows_kernel(AttnArgs a)
     }
 }
 
+// ---- many rows ------------------------------------------------------------------------------------------------
+
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+
+template <int KIND>
+__device__ __forceinline__ f32x16_t mfma32(Frag16 a, Frag16 b, f32x16_t c)
+{
+    if constexpr (KIND == kCacheBF16) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.b, b.b, c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_32x32x16_f16(a.h, b.h, c, 0, 0, 0);
+}
+
+// 16 bytes per lane from base + off (the lane's own) to LDS bytes lds_off + 16 * lane, past the registers
+__device__ __forceinline__ void copy_to_lds(uint32_t lds_off, const void* base, uint32_t off)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(lds_off)), "v"(off), "s"(base));
+}
+
+template <int G>
+struct TileShape {
+    static constexpr int kBlocks = G <= 4 ? 2 : 1;            // blocks of a step
+    static constexpr int kWaves = G <= 4 ? 8 : 4;             // waves, each with 32 rows
+    static constexpr int kRows = 32 * kWaves;
+    static constexpr int kHalf = kBlocks * kBlockTokens * 32 * G * 2;         // bytes of a step's keys, or values
+    static constexpr int kLds = 4 * kHalf;                    // two steps of each
+    static constexpr int kSlab = kRows * 32 * G + 2 * kRows;  // floats of a part
+};
+
+// A step's keys or values on their way to LDS in the order of 32 x 32 x 16 operands: [block][dimensions 16 step ..][half of 8][32 tokens] 16 B,
+// [block][dimensions 32 dtile ..][16 tokens j][half][32 dimensions] 16 B.  16-bit caches: copied there, a lane's 16 B each from its place.
+// Q8, Q4: asked for in registers, and turned into f16 (scales on them, rounded once) when the step ahead is done.
+template <int KIND, int G>
+struct Stage {
+    typedef TileShape<G> T;
+    static constexpr bool kQuant = cache_quantised(KIND);
+    static constexpr int N = kQuant ? Half<KIND, G>::N : 2 * G;                          // 1 KiB pieces of a block's half
+    static constexpr int PER = (T::kBlocks * N + T::kWaves - 1) / T::kWaves;             // pieces per wave
+    struct Piece {
+        u32x4_t d, s[2];
+    };
+    Piece raw[kQuant ? PER : 1];
+
+    // `values`: that half; where: LDS byte offset
+    template <bool VALUES>
+    __device__ __forceinline__ void ask(const uint8_t* const (&block)[T::kBlocks], uint32_t where, int wv, int lane)
+    {
+#pragma unroll
+        for (int e = 0; e < PER; e++) {
+            const int p = wv + e * T::kWaves;
+            if (T::kBlocks * N % T::kWaves && p >= T::kBlocks * N) break;
+            const int bl = T::kBlocks == 1 ? 0 : p / N, i = p - bl * N;
+            const uint8_t* const from = T::kBlocks == 1 || bl == 0 ? block[0] : block[T::kBlocks - 1];
+            if constexpr (!kQuant) {
+                uint32_t off;
+                if (!VALUES) off = ((lane >> 3 & 1) * G * 64 + ((lane & 31) >> 4 << 3 | (lane & 7)) + (lane >> 5) * 16) * 16 + (i >> 1) * 1024 + (i & 1) * 512;
+                else off = cache_half_bytes(KIND, 32 * G) + (i >> 1) * 2048 + (lane >> 4 & 1) * 1024 + (lane & 15) * 16 + (lane >> 5) * 256 + (i & 1) * 512;
+                copy_to_lds(where + p * 1024, from, off);
+            } else {
+                const uint8_t* const src = from + (VALUES ? cache_half_bytes(KIND, 32 * G) : 0);
+                const uint8_t* const sc = src + cache_data_bytes(KIND, 32 * G);
+                Piece& r = raw[e];
+                if (KIND == kCacheQ4 && (G & 1) && i == N - 1) {
+                    const u32x2_t v = *reinterpret_cast<const u32x2_t*>(src + i * 1024 + lane * 8);
+                    r.d = u32x4_t{v[0], v[1], 0u, 0u};
+                } else {
+                    r.d = *reinterpret_cast<const u32x4_t*>(src + i * 1024 + lane * 16);
+                }
+                constexpr int GROUPS = KIND == kCacheQ4 ? 2 : 1;
+#pragma unroll
+                for (int gg = 0; gg < GROUPS; gg++) {
+                    const int g = min(GROUPS * i + gg, G - 1);
+                    if (VALUES) r.s[gg] = *reinterpret_cast<const u32x4_t*>(sc + (g * 4 + (lane >> 4)) * 16);
+                    else {
+                        const uint16_t* at = reinterpret_cast<const uint16_t*>(sc) + (g * 4 + ((lane & 15) >> 2)) * 8 + (lane & 3);
+                        r.s[0][2 * gg] = at[0] * 0x10001u;
+                        r.s[0][2 * gg + 1] = at[4] * 0x10001u;
+                    }
+                }
+            }
+        }
+    }
+    template <bool VALUES>
+    __device__ __forceinline__ void put(uint8_t* lds, uint32_t where, int wv, int lane, uint32_t magic)
+    {
+        if constexpr (kQuant) {
+            const int m = lane & 15, q4 = lane >> 4;
+#pragma unroll
+            for (int e = 0; e < PER; e++) {
+                const int p = wv + e * T::kWaves;
+                if (T::kBlocks * N % T::kWaves && p >= T::kBlocks * N) break;
+                const int bl = T::kBlocks == 1 ? 0 : p / N, i = p - bl * N;
+                const Piece& r = raw[e];
+                constexpr int GROUPS = KIND == kCacheQ4 ? 2 : 1;
+#pragma unroll
+                for (int gg = 0; gg < GROUPS; gg++) {
+                    const int g = GROUPS * i + gg;
+                    if (GROUPS * N != G && g >= G) break;
+#pragma unroll
+                    for (int t = 0; t < 2; t++) {             // keys: tile of 16 tokens; values: tile of 16 dimensions
+                        uint32_t o[4];
+                        if constexpr (KIND == kCacheQ8) unpack_q8_f16(r.d[2 * t], r.d[2 * t + 1], o);
+                        else if (!VALUES) nibbles_f16(r.d[2 * gg + t], magic, o);
+                        else {
+                            const half2_t sub = {(_Float16)-1032.0f, (_Float16)-1032.0f}, mul = {(_Float16)0.0625f, (_Float16)0.0625f},
+                                          add = {(_Float16)-72.0f, (_Float16)-72.0f};
+#pragma unroll
+                            for (int k = 0; k < 4; k++) {
+                                const uint32_t w = r.d[2 * gg + (k >> 1)] >> (8 * (k & 1));
+                                o[k] = t ? as_u32(as_h2((w & 0x00F000F0u) | magic) * mul + add) : as_u32(as_h2((w & 0x000F000Fu) | magic) + sub);
+                            }
+                        }
+                        u32x4_t v;
+#pragma unroll
+                        for (int k = 0; k < 4; k++) v[k] = as_u32(as_h2(o[k]) * as_h2(VALUES ? r.s[gg][k] : r.s[0][2 * gg + t]));
+                        const int at = VALUES ? ((bl * G + g) * 2 + (q4 >> 1)) * 64 + t * 16 + m + (q4 & 1) * 32
+                                              : (bl * 2 * G + 2 * g + (q4 >> 1)) * 64 + ((m >> 3) << 4 | t << 3 | (m & 7)) + (q4 & 1) * 32;
+                        *reinterpret_cast<u32x4_t*>(lds + where + at * 16) = v;
+                    }
+                }
+            }
+        }
+    }
+};
+
+// Many rows: a workgroup's waves have 32 rows each and go through the same blocks, 64 tokens (a head of 256: 32) a step.  While P of a step
+// is formed the scores of the next are multiplied: its keys are in LDS one step earlier than its values.
+template <int KIND, int G>
+__global__ __launch_bounds__(64 * TileShape<G>::kWaves) void attention_tiles_kernel(AttnArgs a)
+{
+    typedef TileShape<G> T;
+    constexpr int DIM = 32 * G, BLOCK = cache_block_bytes(KIND, DIM), ROWS = T::kRows, BL = T::kBlocks;
+    // P of f16 behind 2^12, its largest below 2^15: a maximum may lag behind by 2^3 before sums are scaled anew (bf16: by 2^8)
+    constexpr float kShift = KIND == kCacheBF16 ? 0.f : 12.f, kLag = KIND == kCacheBF16 ? 8.f : 3.f;
+    extern __shared__ float4_t lds[];                                 // keys of two steps, values of two steps
+    uint8_t* const bytes = reinterpret_cast<uint8_t*>(lds);
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, r = lane & 31;
+    const uint32_t magic = q4_magic_vgpr();
+    Unit u;
+    if (!find_unit<ROWS, true>(a, blockIdx.x, &u)) return;
+    const int64_t capacity = (int64_t)a.t.table_pages << (a.c.page_shift + 5);
+    const int all_rows = u.s.n * a.group, p0 = u.s.len - u.s.n;
+    const int w0 = u.tile * ROWS, wg_rows = min(ROWS, all_rows - w0);
+    int lo, hi;
+    seen(a, p0 + w0 / a.group, p0 + (w0 + wg_rows - 1) / a.group, capacity, &lo, &hi);
+    const int each = (hi - lo) / u.splits, more = (hi - lo) % u.splits;
+    const int first = lo + u.split * each + min(u.split, more), last = first + each + (u.split < more ? 1 : 0);
+    const int steps = (last - first + BL - 1) / BL;
+    // my row, and what all of this wave's rows see
+    const int r0 = w0 + wv * 32, rows = max(0, min(32, all_rows - r0));
+    const bool real = r < rows;
+    const int i = (real ? r0 + r : w0) / a.group, in_group = (real ? r0 + r : w0) - i * a.group;
+    const int p = p0 + i;
+    const int row_hi = real ? (int)min((int64_t)p, capacity - 1) : -1;
+    const int row_lo = a.window && p >= a.window ? p - a.window + 1 : 0;
+    int wave_hi = -1, wave_lo = 0, all_hi = -1, all_lo = 0;          // some row sees wave_lo .. wave_hi, every row all_lo .. all_hi
+    if (rows) {
+        const int pf = p0 + r0 / a.group, pl = p0 + (r0 + rows - 1) / a.group;
+        wave_hi = (int)min((int64_t)pl, capacity - 1);
+        all_hi = (int)min((int64_t)pf, capacity - 1);
+        wave_lo = a.window && pf >= a.window ? pf - a.window + 1 : 0;
+        all_lo = a.window && pl >= a.window ? pl - a.window + 1 : 0;
+    }
+    const int head = u.head * a.group + in_group;
+    Frag16 qf[2 * G];
+    float c = a.scale;
+    {
+        const uint16_t* q = static_cast<const uint16_t*>(a.q) + (int64_t)(u.s.row0 + i) * a.q_stride + head * DIM + 8 * h;
+#pragma unroll
+        for (int k = 0; k < 2 * G; k++) qf[k].u = real ? *reinterpret_cast<const u32x4_t*>(q + 16 * k) : u32x4_t{0u, 0u, 0u, 0u};
+        if (cache_quantised(KIND) && a.qdt == kBF16) {
+            float top = 0.f;
+#pragma unroll
+            for (int k = 0; k < 2 * G; k++)
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    top = fmaxf(top, fmaxf(fabsf(__builtin_bit_cast(float, qf[k].u[j] << 16)), fabsf(__builtin_bit_cast(float, qf[k].u[j] & 0xffff0000u))));
+            top = fmaxf(top, other_quarter<32>(top));
+            const float f = row_power(top, &c);
+#pragma unroll
+            for (int k = 0; k < 2 * G; k++)
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    qf[k].u[j] = pack_half2(__builtin_bit_cast(float, qf[k].u[j] << 16) * f, __builtin_bit_cast(float, qf[k].u[j] & 0xffff0000u) * f);
+        }
+    }
+    const float lag = fminf(kLag / c, 1e30f);
+    const int32_t* const table = a.t.tables + (int64_t)u.b * a.t.table_pages;
+    const int in_page = (1 << a.c.page_shift) - 1;
+    // pages of a step's blocks (of none: -1), asked for one step before they are needed
+    struct Pages {
+        int id[BL];
+    };
+    auto pages_of = [&](int step) {
+        Pages g;
+#pragma unroll
+        for (int b = 0; b < BL; b++) {
+            const int blk = first + step * BL + b;
+            g.id[b] = blk < last ? table[blk >> a.c.page_shift] : -1;
+        }
+        return g;
+    };
+    auto absent = [&](const Pages& g) {
+        unsigned m = 0;
+#pragma unroll
+        for (int b = 0; b < BL; b++) m |= (unsigned)g.id[b] >= (unsigned)a.c.pages ? 1u << b : 0u;
+        return m;
+    };
+    // (a block that is not there is read from page 0: finite numbers, which nobody sees)
+    auto blocks_of = [&](int step, const Pages& g, const uint8_t* (&at)[BL]) {
+#pragma unroll
+        for (int b = 0; b < BL; b++) {
+            const int page = (unsigned)g.id[b] >= (unsigned)a.c.pages ? 0 : g.id[b];
+            at[b] = a.c.base + page * a.c.page_bytes + (int64_t)((u.head << a.c.page_shift) + ((first + step * BL + b) & in_page)) * BLOCK;
+        }
+    };
+    f32x16_t y[G];
+#pragma unroll
+    for (int d = 0; d < G; d++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) y[d][e] = 0.f;
+    const float none = -__builtin_inff();
+    float m = none, l = 0.f;
+    f32x16_t s[BL];
+    auto scores = [&](uint32_t where) __attribute__((always_inline)) {
+#pragma unroll
+        for (int b = 0; b < BL; b++) {
+#pragma unroll
+            for (int e = 0; e < 16; e++) s[b][e] = 0.f;
+#pragma unroll
+            for (int k = 0; k < 2 * G; k++) {
+                Frag16 kf;
+                kf.u = *reinterpret_cast<const u32x4_t*>(bytes + where + (b * 2 * G + k) * 1024 + lane * 16);
+                s[b] = mfma32<KIND>(kf, qf[k], s[b]);
+            }
+        }
+    };
+    Stage<KIND, G> ks, vs;
+    const uint32_t K0 = 0, V0 = 2 * T::kHalf;
+    Pages g0 = pages_of(0), g1 = pages_of(1), g2 = pages_of(2);
+    const uint8_t* at[BL];
+    if (steps) {
+        blocks_of(0, g0, at);
+        ks.template ask<false>(at, K0, wv, lane);
+        vs.template ask<true>(at, V0, wv, lane);
+        ks.template put<false>(bytes, K0, wv, lane, magic);
+        vs.template put<true>(bytes, V0, wv, lane, magic);
+        blocks_of(1, g1, at);
+        ks.template ask<false>(at, K0 + T::kHalf, wv, lane);
+        ks.template put<false>(bytes, K0 + T::kHalf, wv, lane, magic);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        scores(K0);
+        __syncthreads();                                             // (keys of step 2 go where those of step 0 were)
+    }
+    for (int t = 0; t < steps; t++) {
+        const int odd = t & 1;
+        // keys of step t + 2 and values of step t + 1 on their way; past the end they are read from page 0 and nobody looks at them
+        const Pages g3 = pages_of(t + 3);
+        blocks_of(t + 2, g2, at);
+        ks.template ask<false>(at, K0 + odd * T::kHalf, wv, lane);
+        blocks_of(t + 1, g1, at);
+        vs.template ask<true>(at, V0 + (1 - odd) * T::kHalf, wv, lane);
+        const int tok = (first + t * BL) * kBlockTokens;
+        const unsigned gone = absent(g0);
+        const bool look = tok <= wave_hi && tok + BL * kBlockTokens > wave_lo;
+        f32x16_t now[BL];
+#pragma unroll
+        for (int b = 0; b < BL; b++) now[b] = s[b];
+        if (t + 1 < steps) scores(K0 + (1 - odd) * T::kHalf);
+        if (look) {
+            if (gone || tok < all_lo || tok + BL * kBlockTokens - 1 > all_hi) {
+#pragma unroll
+                for (int b = 0; b < BL; b++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        const int j = tok + b * kBlockTokens + 8 * (e >> 2) + 4 * h + (e & 3);
+                        if (j < row_lo || j > row_hi || (gone >> b & 1)) now[b][e] = none;
+                    }
+            }
+            float top = now[0][0];
+#pragma unroll
+            for (int b = 0; b < BL; b++)
+#pragma unroll
+                for (int e = b ? 0 : 1; e < 16; e++) top = fmaxf(top, now[b][e]);
+            top = fmaxf(top, other_quarter<32>(top));
+            if (__ballot(top > m + lag)) {
+                const float up = top > m + lag ? top : m;
+                const float f = m == none ? 0.f : exp2_fast((m - up) * c);
+                m = up;
+                l *= f;
+#pragma unroll
+                for (int d = 0; d < G; d++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) y[d][e] *= f;
+            }
+            const float off = kShift - (m == none ? 0.f : m * c);
+            Frag16 pf[2 * BL];
+            float sums[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int b = 0; b < BL; b++)
+#pragma unroll
+                for (int e = 0; e < 16; e += 2) {
+                    const float x0 = exp2_fast(__builtin_fmaf(now[b][e], c, off)), x1 = exp2_fast(__builtin_fmaf(now[b][e + 1], c, off));
+                    sums[e >> 1 & 3] += x0 + x1;
+                    pf[2 * b + (e >> 3)].u[e >> 1 & 3] = KIND == kCacheBF16 ? pack_bf16x2(x0, x1) : pack_half2(x0, x1);
+                }
+            l += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+            const uint32_t where = V0 + odd * T::kHalf;
+#pragma unroll
+            for (int k = 0; k < 2 * BL; k++)
+#pragma unroll
+                for (int d = 0; d < G; d++) {
+                    Frag16 vf;
+                    vf.u = *reinterpret_cast<const u32x4_t*>(bytes + where + (((k >> 1) * G + d) * 2 + (k & 1)) * 1024 + lane * 16);
+                    y[d] = mfma32<KIND>(vf, pf[k], y[d]);
+                }
+        }
+        ks.template put<false>(bytes, K0 + odd * T::kHalf, wv, lane, magic);
+        vs.template put<true>(bytes, V0 + (1 - odd) * T::kHalf, wv, lane, magic);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        g0 = g1;
+        g1 = g2;
+        g2 = g3;
+    }
+    l += other_quarter<32>(l);
+    m = m == none ? none : m * c;
+    const int64_t row_at = ((int64_t)(u.s.row0 + i) * a.c.kv_heads * a.group + head) * DIM + 4 * h;
+    if (u.splits == 1) {
+        const float inv = l == 0.f ? 0.f : 1.0f / l;
+        if (real) {
+#pragma unroll
+            for (int d = 0; d < G; d++)
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    store_row4(a.y, a.qdt, row_at + 32 * d + 8 * e, float4_t{y[d][4 * e] * inv, y[d][4 * e + 1] * inv, y[d][4 * e + 2] * inv, y[d][4 * e + 3] * inv});
+        }
+        return;
+    }
+    // a part: its sums, then maxima and sums of probabilities of its rows
+    constexpr int SLAB = T::kSlab;
+    float* const slab = a.slabs + (size_t)u.slab * SLAB;
+    float* const stats = slab + ROWS * DIM + wv * 32 + r;
+#pragma unroll
+    for (int d = 0; d < G; d++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            uint64_t* const to = reinterpret_cast<uint64_t*>(slab + (((wv * G + d) * 4 + e) * 64 + lane) * 4);
+            __hip_atomic_store(to, __builtin_bit_cast(uint64_t, f32x2_t{y[d][4 * e], y[d][4 * e + 1]}), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+            __hip_atomic_store(to + 1, __builtin_bit_cast(uint64_t, f32x2_t{y[d][4 * e + 2], y[d][4 * e + 3]}), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+        }
+    if (h == 0) {
+        __hip_atomic_store(stats, m, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+        __hip_atomic_store(stats + ROWS, l, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    unsigned* const flag = reinterpret_cast<unsigned*>(lds);
+    if (threadIdx.x == 0) {
+        const unsigned old = __hip_atomic_fetch_add(a.tickets + u.ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const bool end = old + 1u == (unsigned)u.splits;
+        if (end) __hip_atomic_store(a.tickets + u.ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        *flag = end ? 1u : 0u;
+    }
+    __syncthreads();
+    if (*flag == 0u) return;
+    const float* const of_tile = slab - (size_t)u.split * SLAB;
+    auto part_of = [&](int e, int k) {                               // maximum (k = 0) or sum of part e for my row
+        return __hip_atomic_load(of_tile + (size_t)e * SLAB + ROWS * DIM + k * ROWS + wv * 32 + r, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+    };
+    float top = none, sum = 0.f;
+    for (int e = 0; e < u.splits; e++) top = fmaxf(top, part_of(e, 0));
+#pragma unroll
+    for (int d = 0; d < G; d++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) y[d][e] = 0.f;
+    for (int e = 0; e < u.splits; e++) {
+        const float me = part_of(e, 0), f = me == none ? 0.f : exp2_fast(me - top);
+        sum += f * part_of(e, 1);
+        const uint64_t* const from = reinterpret_cast<const uint64_t*>(of_tile + (size_t)e * SLAB + (wv * G * 4 * 64 + lane) * 4);
+#pragma unroll
+        for (int d = 0; d < G; d++)
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const uint64_t w0 = __hip_atomic_load(from + (d * 4 + k) * 128, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+                const uint64_t w1 = __hip_atomic_load(from + (d * 4 + k) * 128 + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+                const float part[4] = {__builtin_bit_cast(float, (uint32_t)w0), __builtin_bit_cast(float, (uint32_t)(w0 >> 32)), __builtin_bit_cast(float, (uint32_t)w1),
+                                       __builtin_bit_cast(float, (uint32_t)(w1 >> 32))};
+#pragma unroll
+                for (int j = 0; j < 4; j++) y[d][4 * k + j] += f == 0.f ? 0.f : part[j] * f;
+            }
+    }
+    if (!real) return;
+    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+#pragma unroll
+    for (int d = 0; d < G; d++)
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            store_row4(a.y, a.qdt, row_at + 32 * d + 8 * e, float4_t{y[d][4 * e] * inv, y[d][4 * e + 1] * inv, y[d][4 * e + 2] * inv, y[d][4 * e + 3] * inv});
+}
+
 template <int KIND, int G>
 hipError_t rows_as(const AttnArgs& a, unsigned grid, hipStream_t st)
 {
@@ -478,17 +897,51 @@ hipError_t rows_as(const AttnArgs& a, unsigned grid, hipStream_t st)
     return hipGetLastError();
 }
 
+template <int KIND, int G>
+hipError_t tiles_as(const AttnArgs& a, unsigned grid, hipStream_t st)
+{
+    (void)LdsRequest<&attention_tiles_kernel<KIND, G>, TileShape<G>::kLds>::registered;
+    hipLaunchKernelGGL((attention_tiles_kernel<KIND, G>), dim3(grid), dim3(64 * TileShape<G>::kWaves), TileShape<G>::kLds, st, a);
+    return hipGetLastError();
+}
+
+template <int KIND, int G>
+hipError_t attention_as(AttnArgs a, hipStream_t st)
+{
+    const int64_t most = (int64_t)a.t.max_new * a.group;
+    const bool many = most > kFewRows;
+    a.few = many && a.t.seqs > 1 ? kFewRows : 0;                     // (a single sequence: the kernel that its largest call needs)
+    hipError_t e = hipSuccess;
+    const int64_t rows = (int64_t)a.t.rows * a.group;
+    if (!many || a.few) {
+        a.target = kTarget;
+        a.least = kWaves;
+        const int64_t tiles = std::min(rows / kRows + a.t.seqs, a.few ? (int64_t)a.t.seqs * ((kFewRows + kRows - 1) / kRows) : rows);
+        e = rows_as<KIND, G>(a, (unsigned)(tiles * a.c.kv_heads + 2 * kTarget), st);
+    }
+    if (many && e == hipSuccess) {
+        a.target = kTileTarget;
+        a.least = 8;
+        e = tiles_as<KIND, G>(a, (unsigned)((rows / TileShape<G>::kRows + a.t.seqs) * a.c.kv_heads + 2 * kTileTarget), st);
+    }
+    return e;
+}
+
 }  // namespace
 
 // Parts of tiles that have more than one: at most 2 * target of them (a tile of b blocks has at most b / part + 1), of at most
 // `target` tiles.
-constexpr int kTarget = 256;
+static_assert((2 * std::max(kTarget, kTileTarget) + 16) * sizeof(unsigned) <= kAttnTicketBytes, "a ticket per tile");
+static_assert(kTarget * 32 * 4 <= kWaves * 2 * 2 * 64 * 16 + kWaves * 32 * 4, "maxima and sums of a tile's parts fit LDS");
 
 int64_t attention_max_units() { return kMaxUnits; }
 
-size_t attention_scratch_bytes(int dim) { return (size_t)(2 * kTarget + 16) * ((size_t)dim / 16 * 64 * 4 + 32) * sizeof(float); }
-static_assert((2 * kTarget + 16) * sizeof(unsigned) <= kAttnTicketBytes, "a ticket per tile");
-static_assert(kTarget * 32 * 4 <= kWaves * 2 * 2 * 64 * 16 + kWaves * 32 * 4, "maxima and sums of a tile's parts fit LDS");
+size_t attention_scratch_bytes(int dim)
+{
+    const size_t rows = (size_t)(2 * kTarget + 16) * ((size_t)dim / 16 * 64 * 4 + 32) * sizeof(float);
+    const size_t wave_rows = dim <= 128 ? 256 : 128;
+    return std::max(rows, (2 * kTileTarget + 16) * wave_rows * ((size_t)dim + 2) * sizeof(float));
+}
 
 int64_t attention_units_max(const BatchView& t, int kv_heads, int group)
 {
@@ -510,16 +963,13 @@ hipError_t launch_attention(const CacheView& c, const BatchView& t, const void* 
     a.group = group;
     a.qdt = qdt;
     a.window = window;
-    a.target = kTarget;
-    a.least = kWaves;
     a.scale = scale * 1.44269504088896340736f;
-    const unsigned grid = (unsigned)attention_units_max(t, c.kv_heads, group);
-#define CYBQ_ROWS(KIND)                              \
-    switch (c.dim) {                                 \
-        case 64: return rows_as<KIND, 2>(a, grid, st);  \
-        case 96: return rows_as<KIND, 3>(a, grid, st);  \
-        case 128: return rows_as<KIND, 4>(a, grid, st); \
-        default: return rows_as<KIND, 8>(a, grid, st);  \
+#define CYBQ_ROWS(KIND)                                   \
+    switch (c.dim) {                                      \
+        case 64: return attention_as<KIND, 2>(a, st);     \
+        case 96: return attention_as<KIND, 3>(a, st);     \
+        case 128: return attention_as<KIND, 4>(a, st);    \
+        default: return attention_as<KIND, 8>(a, st);     \
     }
     switch (c.kind) {
         case kCacheF16: CYBQ_ROWS(kCacheF16)

@@ -4,14 +4,16 @@
 // A page holds `page` tokens (32 << page_shift) of every kv head of one layer, head after head, a head in blocks of 32
 // tokens.  A block is its keys, then its values, each in the order in which 16 x 16 x 32 matrix instructions take operands:
 // the attention of few rows reads whole 1 KiB runs straight into registers.
-//   keys: operand A of S^T = K Q^T.  Tile t16 (0, 1) of 16 tokens, group g of 32 dimensions; lane l = token & 15 | q4 << 4 holds
-//       dimensions 32 g + 8 q4 + 0..7.
+//   Token t = b4 b3 b2 b1 b0 of a block is row m = b4 b2 b1 b0 of tile t16 = b3 of 16 tokens, so that after S^T the lanes of
+//   quarter q4 = b4 b2 have the scores of eight tokens in slots s = b3 b1 b0; in the order of 32 x 32 x 16 instructions these are the eight
+//   that half b2 of the lanes has for 16 tokens b4: values serve both shapes as they lie, and P never moves.
+//   keys: operand A of S^T = K Q^T.  Tile t16, group g of 32 dimensions; lane l = m | q4 << 4 holds dimensions 32 g + 8 q4 + 0..7.
 //         16 bits  16 B per (t16, g, lane): ((t16 G + g) 64 + l) 16
 //         Q8       8 B, both tiles in 16 B: (g 64 + l) 16 + 8 t16, byte = q + 128
 //         Q4       one word, both tiles of two groups in 16 B (of the last, odd group in 8 B); nibble of dimension slot s at bit
 //                  16 (s & 1) + 4 (s >> 1 & 1) + 8 (s >> 2), value q + 8
-//   values: operand A of Y^T = V^T P^T.  Tile dt of 16 dimensions; lane l = dimension & 15 | q4 << 4 holds the eight tokens
-//       16 (s >> 2) + 4 q4 + (s & 3), s = 0..7: the ones whose scores the same lane has after S^T, so that P never moves.
+//   values: operand A of Y^T = V^T P^T.  Tile dt of 16 dimensions; lane l = dimension & 15 | q4 << 4 holds the eight tokens of
+//       quarter q4, slot after slot.
 //         16 bits  16 B per (dt, lane), 2 B per token
 //         Q8       8 B, tiles 2 g and 2 g + 1 in 16 B; byte = q + 128.  A byte belongs to one token.
 //         Q4       8 B per (g, lane), tile 2 g in the low nibbles and 2 g + 1 in the high ones: here too a byte belongs to one
@@ -60,13 +62,13 @@ __host__ __device__ constexpr int q4_place(int g, int l, int step)
 template <int KIND, int G>
 __host__ __device__ constexpr int key_place(int t, int g, int q4)
 {
-    const int t16 = t >> 4, l = (t & 15) | q4 << 4;
+    const int t16 = t >> 3 & 1, l = (t >> 4) << 3 | (t & 7) | q4 << 4;
     return KIND == kCacheQ8 ? (g * 64 + l) * 16 + 8 * t16 : KIND == kCacheQ4 ? q4_place<G>(g, l, 4 * t16) : ((t16 * G + g) * 64 + l) * 16;
 }
 
 // slot and lane group of token t of a block
-__host__ __device__ constexpr int token_slot(int t) { return (t & 3) | (t >> 4) << 2; }
-__host__ __device__ constexpr int token_q4(int t) { return t >> 2 & 3; }
+__host__ __device__ constexpr int token_slot(int t) { return (t & 3) | (t >> 3 & 1) << 2; }
+__host__ __device__ constexpr int token_q4(int t) { return (t >> 4) << 1 | (t >> 2 & 1); }
 
 // byte offset, within the values of a block, of dimension d of token t (Q4: of the byte of dimensions d and d + 16, d & 16 == 0)
 template <int KIND, int G>

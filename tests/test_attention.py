@@ -20,6 +20,7 @@ from tests.cache_lib import HALF_STEP, TDT, Cached, normal, rope_table      # no
 
 gpu = pytest.mark.gpu
 U = 2.0 ** -24
+FEW = 64                # rows of a sequence and kv head (new tokens times group); "many rows" above are more than these
 
 
 def bound(kind, dt, dim, y, size, dots, many):
@@ -39,6 +40,7 @@ def check(s, new, group, dt, window=0, many=False, scale=None, hidden=lambda b, 
     ref, size, dots = s.expected(q[:used], new, scale, window, hidden)
     assert torch.isfinite(y).all()
     off = (y[:used].double() - ref).abs()
+    many = many or max(new) * group > FEW
     worst = (off / bound(s.kind, dt, s.dim, ref, size, dots, many)).max().item() if used else 0.0
     assert worst <= 1.0, worst
     assert (y[used:] == 9.0).all()                               # rows of no sequence
