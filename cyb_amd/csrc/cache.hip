@@ -6,8 +6,10 @@
 // The rotation is in fp64 because integers come out of it: which of two a key becomes hangs on its last bits, and two programs that
 // rotate in fp32 with and without fused multiplications disagree in one key of a few ten thousand.
 //
-// A workgroup takes the rows of one sequence that fall into one block of 32 positions, and one kv head with the query heads that share
-// it; a thread takes eight dimensions of a row.  Bound by memory: rows in, rows and blocks out.
+// A workgroup takes the rows of one sequence that fall into one block of 32 positions, and one kv head: a wave the keys, one the values, one
+// each of the query heads that share it.  Bound by memory: rows in, rows and blocks out.  Where the rows fill their block, lanes are
+// given what lies side by side in it - a key's dimensions of two tokens, eight dimensions of the eight tokens of a value's 8 or 16 bytes -, and
+// it is written 8 and 16 bytes at a time; at the ends of a chunk, and token by token, bytes are written one by one.
 #include "cache_parts.h"
 #include "cybq_internal.h"
 
@@ -15,7 +17,7 @@ namespace cybq {
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kTurnThreads = 256;
 
 // workgroup `u` of the grid -> sequence and block of positions; false: none
 __device__ __forceinline__ bool find_block(const BatchView& t, int u, int* b, Seq* s, int* block)
@@ -50,23 +52,25 @@ __device__ __forceinline__ uint8_t* block_at(const CacheView& c, const BatchView
     return c.base + page * c.page_bytes + (int64_t)((head << c.page_shift) + (block & ((1 << c.page_shift) - 1))) * block_bytes;
 }
 
+// eight elements of a row, as they come from memory
 template <int DT>
-__device__ __forceinline__ void load8(const void* x, int64_t at, float out[8])
-{
-    if constexpr (DT == kF32) {
-        const float4_t* p = reinterpret_cast<const float4_t*>(static_cast<const float*>(x) + at);
-        const float4_t a = p[0], b = p[1];
-#pragma unroll
-        for (int i = 0; i < 4; i++) out[i] = a[i], out[4 + i] = b[i];
-    } else {
-        const u32x4_t v = *reinterpret_cast<const u32x4_t*>(static_cast<const uint16_t*>(x) + at);
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            if constexpr (DT == kF16) out[2 * i] = f16_bits_to_f32(v[i] & 0xffffu), out[2 * i + 1] = f16_bits_to_f32(v[i] >> 16);
-            else out[2 * i] = __builtin_bit_cast(float, v[i] << 16), out[2 * i + 1] = __builtin_bit_cast(float, v[i] & 0xffff0000u);
-        }
+struct Eight {
+    u32x4_t v[DT == kF32 ? 2 : 1];
+    __device__ __forceinline__ void load(const void* x, int64_t at)
+    {
+        const u32x4_t* p = reinterpret_cast<const u32x4_t*>(static_cast<const char*>(x) + at * (DT == kF32 ? 4 : 2));
+        v[0] = p[0];
+        if constexpr (DT == kF32) v[1] = p[1];
     }
-}
+    __device__ __forceinline__ float operator[](int e) const
+    {
+        if constexpr (DT == kF32) {
+            const uint32_t w = v[e >> 2][e & 3];              // (a copy: of an element named in place the compiler casts the first)
+            return __builtin_bit_cast(float, w);
+        } else if constexpr (DT == kF16) return f16_bits_to_f32(v[0][e >> 1] >> (16 * (e & 1)) & 0xffffu);
+        else return __builtin_bit_cast(float, e & 1 ? v[0][e >> 1] & 0xffff0000u : v[0][e >> 1] << 16);
+    }
+};
 
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi)
 {
@@ -93,223 +97,485 @@ __device__ __forceinline__ void store8(void* y, int dt, int64_t at, const float 
     }
 }
 
-// eight dimensions from 8 c on of the row at x[at], turned; the partner's dimensions are read next to them
-template <int DT>
-__device__ __forceinline__ void load_turned(const void* x, int64_t at, int c, const float* rope, int rot, bool halves, float out[8])
+// x0 c - x1 s and x1 c + x0 s
+__device__ __forceinline__ void turn(float x0, float x1, float c, float s, float* y0, float* y1)
 {
-    load8<DT>(x, at + 8 * c, out);
-    const int d = 8 * c, half = rot >> 1;
-    if (!rope || d >= rot) return;
+    const double a = x0, b = x1, cd = c, sd = s;
+    *y0 = (float)__builtin_fma(a, cd, -(b * sd));
+    *y1 = (float)__builtin_fma(b, cd, a * sd);
+}
+
+// eight dimensions from 8 ch on of the row at x[at], turned (turn: the position's angles, or nullptr); the partner's are read next to them
+template <int DT>
+__device__ __forceinline__ void load_turned(const void* x, int64_t at, int ch, const float* angles, int rot, bool halves, float out[8])
+{
+    Eight<DT> own;
+    own.load(x, at + 8 * ch);
+#pragma unroll
+    for (int e = 0; e < 8; e++) out[e] = own[e];
+    const int d = 8 * ch, half = rot >> 1;
+    if (!angles || d >= rot) return;
     if (halves) {
         const bool upper = d >= half;
-        float other[8];
-        load8<DT>(x, at + (upper ? d - half : d + half), other);
-        const float4_t* cs = reinterpret_cast<const float4_t*>(rope + 2 * (upper ? d - half : d));
+        Eight<DT> other;
+        other.load(x, at + (upper ? d - half : d + half));
+        const float4_t* cs = reinterpret_cast<const float4_t*>(angles + 2 * (upper ? d - half : d));
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const float4_t p = cs[i];
 #pragma unroll
             for (int j = 0; j < 2; j++) {
-                const double co = p[2 * j], si = upper ? p[2 * j + 1] : -p[2 * j + 1];
-                out[2 * i + j] = (float)__builtin_fma((double)out[2 * i + j], co, (double)other[2 * i + j] * si);
+                const int e = 2 * i + j;
+                float unused;
+                turn(own[e], other[e], p[2 * j], upper ? -p[2 * j + 1] : p[2 * j + 1], &out[e], &unused);
             }
         }
     } else {
-        const float4_t* cs = reinterpret_cast<const float4_t*>(rope + d);
+        const float4_t* cs = reinterpret_cast<const float4_t*>(angles + d);
 #pragma unroll
         for (int i = 0; i < 2; i++) {
             const float4_t p = cs[i];
 #pragma unroll
-            for (int j = 0; j < 2; j++) {
-                const double a = out[4 * i + 2 * j], b = out[4 * i + 2 * j + 1], co = p[2 * j], si = p[2 * j + 1];
-                out[4 * i + 2 * j] = (float)__builtin_fma(a, co, -(b * si));
-                out[4 * i + 2 * j + 1] = (float)__builtin_fma(b, co, a * si);
-            }
+            for (int j = 0; j < 2; j++) turn(own[4 * i + 2 * j], own[4 * i + 2 * j + 1], p[2 * j], p[2 * j + 1], &out[4 * i + 2 * j], &out[4 * i + 2 * j + 1]);
         }
     }
 }
 
-// round_half_away(x / d) for the correctly rounded quotient, |x / d| <= 128: far from a half-integer the product with the
-// reciprocal decides (it is within 3 units in the last place), near one the lane divides
+// Sixteen dimensions of a query row that turn together, or lie side by side; their angles serve all heads.
+struct Angles {
+    float4_t cs[4];
+    int c0, c1;                                               // eighths of the row
+    __device__ __forceinline__ Angles(int j, const float* angles, int rot, bool halves)
+    {
+        const int turning = rot >> 4;
+        c0 = 2 * j;
+        c1 = 2 * j + 1;
+        if (halves && j < turning) c0 = j, c1 = j + turning;
+        const float4_t* p = reinterpret_cast<const float4_t*>(angles + 16 * j);
+#pragma unroll
+        for (int i = 0; i < 4; i++) cs[i] = angles && j < turning ? p[i] : float4_t{1.f, 0.f, 1.f, 0.f};
+    }
+    template <int DT>
+    __device__ __forceinline__ void turned(const Eight<DT>& a, const Eight<DT>& b, bool halves, float x[8], float y[8]) const
+    {
+        if (halves) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) turn(a[e], b[e], cs[e >> 1][2 * (e & 1)], cs[e >> 1][2 * (e & 1) + 1], &x[e], &y[e]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                turn(a[2 * e], a[2 * e + 1], cs[e >> 1][2 * (e & 1)], cs[e >> 1][2 * (e & 1) + 1], &x[2 * e], &x[2 * e + 1]);
+                turn(b[2 * e], b[2 * e + 1], cs[2 + (e >> 1)][2 * (e & 1)], cs[2 + (e >> 1)][2 * (e & 1) + 1], &y[2 * e], &y[2 * e + 1]);
+            }
+        }
+    }
+};
+
+// round_half_away of the quotient x / d rounded to fp32, d of 11 bits, without dividing and without a branch.  A quotient of an fp32 number
+// and such a d that is below a half-integer h stays below it when it is rounded (x would have to be nearer to h d than fp32 numbers lie), so
+// the answer is the f with (f - 1/2) d <= |x| < (f + 1/2) d, and these products are exact.  The product with the reciprocal finds f to
+// within one.  (The division that once stood here for quotients near a half-integer was a branch per value: a kernel of 60 KB.)
 __device__ __forceinline__ float quotient_rounded(float x, float d, float rd)
 {
-    const float h = fabsf(x * rd) + 0.5f;
-    const float f = truncf(h);
-    const float away = fminf(h - f, f + 1.0f - h);
-    float res = f;
-    if (!(away > h * (1.0f / 1048576.0f))) res = truncf(fabsf(roundf(x / d)));
-    return copysignf(res, x);
+    const float a = fabsf(x);
+    float f = truncf(__builtin_fmaf(a, rd, 0.5f));
+    f -= __builtin_fmaf(0.5f - f, d, a) < 0.f ? 1.0f : 0.f;
+    f += __builtin_fmaf(-0.5f - f, d, a) >= 0.f ? 1.0f : 0.f;
+    return copysignf(f, x);
 }
 
 // what a cache can hold: NaN as 0, the rest within its range (so that nothing read back is ever infinite, and a masked value times a
 // probability of 0 is 0)
 __device__ __forceinline__ float limited(float x, float limit) { return x != x ? 0.f : fminf(fmaxf(x, -limit), limit); }
 
-template <int KIND, int G, int DT>
-__global__ __launch_bounds__(kThreads) void append_kernel(CacheView c, BatchView t, const void* __restrict__ q, int64_t q_stride, int group,
-                                                          const void* __restrict__ k, int64_t k_stride, const void* __restrict__ v, int64_t v_stride,
-                                                          const float* __restrict__ rope, int rot, int halves, void* __restrict__ q_out, int qdt)
+// Eight dimensions as a cache holds them: integers u = q + 8, q + 128 and their group's scale; the four lanes of a group call together.
+template <int KIND>
+__device__ __forceinline__ _Float16 quantise8(const float x[8], uint32_t u[8])
 {
-    constexpr int DIM = 32 * G, CH = DIM / 8, BLOCK = cache_block_bytes(KIND, DIM), HALF = cache_half_bytes(KIND, DIM), DATA = cache_data_bytes(KIND, DIM);
-    constexpr float LIMIT = KIND == kCacheF16 ? 65504.0f : KIND == kCacheBF16 ? 3.3895313892515355e38f : 57344.0f;
     constexpr float QMAX = KIND == kCacheQ4 ? 7.0f : 127.0f;
-    int b, block;
-    Seq s;
-    if (!find_block(t, blockIdx.x, &b, &s, &block)) return;
-    const int head = blockIdx.y, p0 = s.len - s.n;
-    const int from = max(p0, block * kBlockTokens), rows = min(s.len, (block + 1) * kBlockTokens) - from;
-    uint8_t* const to = block_at(c, t, b, block, head, BLOCK);
-    const int64_t capacity = (int64_t)t.table_pages << (c.page_shift + 5);
-    const int heads = q ? group : 0;                       // (query heads of a row that this workgroup turns)
-    const int items = rows * (heads + 2) * CH;
-    for (int it = threadIdx.x; it < items; it += kThreads) {
-        const int ch = it % CH, hr = it / CH, which = hr % (heads + 2), i = hr / (heads + 2);
-        const int p = from + i;
-        const int64_t row = s.row0 + (p - p0);
-        const bool there = p >= 0 && p < capacity;
-        const float* turn = rope && there ? rope + (int64_t)p * rot : nullptr;
-        float x[8];
-        if (which < heads) {
-            const int h = head * group + which;
-            load_turned<DT>(q, row * q_stride + h * DIM, ch, turn, rot, halves, x);
-            if (!there) {
+    float amax = 0.f;
 #pragma unroll
-                for (int e = 0; e < 8; e++) x[e] = 0.f;
-            }
-            store8(q_out, qdt, (row * c.kv_heads * group + h) * DIM + 8 * ch, x);
-            continue;
-        }
-        const bool value = which == heads + 1;             // (the four threads of a group are in it together)
-        if (!to) continue;
-        if (value) load8<DT>(v, row * v_stride + head * DIM + 8 * ch, x);
-        else load_turned<DT>(k, row * k_stride + head * DIM, ch, turn, rot, halves, x);
+    for (int e = 0; e < 8; e++) amax = fmaxf(amax, fabsf(x[e]));
+    amax = fmaxf(amax, __shfl_xor(amax, 1));
+    amax = fmaxf(amax, __shfl_xor(amax, 2));
+    const _Float16 dh = (_Float16)(amax / QMAX);
+    const float d = (float)dh, rd = __builtin_amdgcn_rcpf(d);
 #pragma unroll
-        for (int e = 0; e < 8; e++) x[e] = limited(x[e], LIMIT);
-        const int tok = p & 31, g = ch >> 2, q4 = ch & 3;
-        uint8_t* const half = to + (value ? HALF : 0);
-        if constexpr (!cache_quantised(KIND)) {
-            const u32x4_t w = pack8(KIND == kCacheF16 ? kF16 : kBF16, x);
-            if (!value) *reinterpret_cast<u32x4_t*>(half + key_place<KIND, G>(tok, g, q4)) = w;
-            else {
-#pragma unroll
-                for (int e = 0; e < 8; e++) *reinterpret_cast<uint16_t*>(half + value_place<KIND, G>(tok, 8 * ch + e)) = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
-            }
-        } else {
-            float amax = 0.f;
-#pragma unroll
-            for (int e = 0; e < 8; e++) amax = fmaxf(amax, fabsf(x[e]));
-            amax = fmaxf(amax, __shfl_xor(amax, 1));
-            amax = fmaxf(amax, __shfl_xor(amax, 2));
-            const _Float16 dh = (_Float16)(amax / QMAX);
-            const float d = (float)dh, rd = __builtin_amdgcn_rcpf(d);
-            uint32_t u[8];
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const float r = d != 0.f ? quotient_rounded(x[e], d, rd) : 0.f;
-                u[e] = (uint32_t)((int)fminf(fmaxf(r, -QMAX), QMAX) + (KIND == kCacheQ4 ? 8 : 128));
-            }
-            if (q4 == 0) *reinterpret_cast<uint16_t*>(half + DATA + scale_place(tok, g)) = __builtin_bit_cast(uint16_t, dh);
-            if constexpr (KIND == kCacheQ8) {
-                if (!value) {
-                    u32x2_t w = {u[0] | u[1] << 8 | u[2] << 16 | u[3] << 24, u[4] | u[5] << 8 | u[6] << 16 | u[7] << 24};
-                    *reinterpret_cast<u32x2_t*>(half + key_place<KIND, G>(tok, g, q4)) = w;
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 8; e++) half[value_place<KIND, G>(tok, 8 * ch + e)] = (uint8_t)u[e];
-                }
-            } else {
-                if (!value) {
-                    uint32_t w = 0;
-#pragma unroll
-                    for (int e = 0; e < 8; e++) w |= u[e] << (16 * (e & 1) + 4 * (e >> 1 & 1) + 8 * (e >> 2));
-                    *reinterpret_cast<uint32_t*>(half + key_place<KIND, G>(tok, g, q4)) = w;
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        const uint32_t upper = __shfl_xor((int)u[e], 2);       // dimension + 16: two threads on
-                        if (q4 < 2) half[value_place<KIND, G>(tok, 8 * ch + e)] = (uint8_t)(u[e] | upper << 4);
-                    }
-                }
-            }
-        }
+    for (int e = 0; e < 8; e++) {
+        const float r = d != 0.f ? quotient_rounded(x[e], d, rd) : 0.f;
+        u[e] = (uint32_t)((int)fminf(fmaxf(r, -QMAX), QMAX) + (KIND == kCacheQ4 ? 8 : 128));
     }
+    return dh;
 }
 
-// eight integers of a key (dimensions 8 ch .. of a token) or of a value
+__device__ __forceinline__ uint32_t bytes4(const uint32_t u[4]) { return u[0] | u[1] << 8 | u[2] << 16 | u[3] << 24; }
+__device__ __forceinline__ uint32_t nibbles8(const uint32_t u[8])
+{
+    uint32_t w = 0;
+#pragma unroll
+    for (int e = 0; e < 8; e++) w |= u[e] << (16 * (e & 1) + 4 * (e >> 1 & 1) + 8 * (e >> 2));
+    return w;
+}
+
+template <int KIND>
+constexpr float kLimit = KIND == kCacheF16 ? 65504.0f : KIND == kCacheBF16 ? 3.3895313892515355e38f : 57344.0f;
+
+// a token's key or value, as bytes of its own
 template <int KIND, int G>
-__device__ __forceinline__ void held8(const uint8_t* half, bool value, int tok, int ch, float x[8])
+__device__ __forceinline__ void put_one(uint8_t* half, bool value, int tok, int ch, float x[8])
 {
     const int g = ch >> 2, q4 = ch & 3;
+#pragma unroll
+    for (int e = 0; e < 8; e++) x[e] = limited(x[e], kLimit<KIND>);
     if constexpr (!cache_quantised(KIND)) {
-        uint32_t w[8];
-        if (!value) {
-            const u32x4_t p = *reinterpret_cast<const u32x4_t*>(half + key_place<KIND, G>(tok, g, q4));
+        const u32x4_t w = pack8(KIND == kCacheF16 ? kF16 : kBF16, x);
+        if (!value) *reinterpret_cast<u32x4_t*>(half + key_place<KIND, G>(tok, g, q4)) = w;
+        else {
 #pragma unroll
-            for (int e = 0; e < 8; e++) w[e] = p[e >> 1] >> (16 * (e & 1)) & 0xffffu;
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; e++) w[e] = *reinterpret_cast<const uint16_t*>(half + value_place<KIND, G>(tok, 8 * ch + e));
+            for (int e = 0; e < 8; e++) *reinterpret_cast<uint16_t*>(half + value_place<KIND, G>(tok, 8 * ch + e)) = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
         }
-#pragma unroll
-        for (int e = 0; e < 8; e++) x[e] = KIND == kCacheF16 ? f16_bits_to_f32(w[e]) : __builtin_bit_cast(float, w[e] << 16);
     } else {
-        const float d = f16_bits_to_f32(*reinterpret_cast<const uint16_t*>(half + cache_data_bytes(KIND, 32 * G) + scale_place(tok, g)));
-        int u[8];
-        if (value) {
+        uint32_t u[8];
+        const _Float16 dh = quantise8<KIND>(x, u);
+        if (q4 == 0) *reinterpret_cast<uint16_t*>(half + cache_data_bytes(KIND, 32 * G) + scale_place(tok, g)) = __builtin_bit_cast(uint16_t, dh);
+        if (!value) {
+            if constexpr (KIND == kCacheQ8) *reinterpret_cast<u32x2_t*>(half + key_place<KIND, G>(tok, g, q4)) = u32x2_t{bytes4(u), bytes4(u + 4)};
+            else *reinterpret_cast<uint32_t*>(half + key_place<KIND, G>(tok, g, q4)) = nibbles8(u);
+        } else {
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                const int dim = 8 * ch + e;
-                const int byte = half[value_place<KIND, G>(tok, KIND == kCacheQ4 ? dim & ~16 : dim)];
-                u[e] = KIND == kCacheQ4 ? (byte >> (dim & 16 ? 4 : 0)) & 15 : byte;
+                if constexpr (KIND == kCacheQ8) half[value_place<KIND, G>(tok, 8 * ch + e)] = (uint8_t)u[e];
+                else {
+                    const uint32_t upper = __shfl_xor((int)u[e], 2);       // dimension + 16: two lanes on
+                    if (q4 < 2) half[value_place<KIND, G>(tok, 8 * ch + e)] = (uint8_t)(u[e] | upper << 4);
+                }
             }
-        } else if constexpr (KIND == kCacheQ8) {
-            const u32x2_t w = *reinterpret_cast<const u32x2_t*>(half + key_place<KIND, G>(tok, g, q4));
-#pragma unroll
-            for (int e = 0; e < 8; e++) u[e] = (int)(w[e >> 2] >> (8 * (e & 3)) & 255u);
-        } else {
-            const uint32_t w = *reinterpret_cast<const uint32_t*>(half + key_place<KIND, G>(tok, g, q4));
-#pragma unroll
-            for (int e = 0; e < 8; e++) u[e] = (int)(w >> (16 * (e & 1) + 4 * (e >> 1 & 1) + 8 * (e >> 2)) & 15u);
         }
-#pragma unroll
-        for (int e = 0; e < 8; e++) x[e] = (float)(u[e] - (KIND == kCacheQ4 ? 8 : 128)) * d;
     }
 }
 
-template <int KIND, int G>
-__global__ __launch_bounds__(kThreads) void read_kernel(CacheView c, BatchView t, void* __restrict__ k, void* __restrict__ v, int dt)
+// token of a block: slot s of quarter q4
+__device__ __forceinline__ int token_of(int q4, int s) { return (q4 >> 1) << 4 | (s >> 2) << 3 | (q4 & 1) << 2 | (s & 3); }
+
+// the rows of a workgroup
+struct Rows {
+    int b, block, from, rows;             // positions from .. from + rows, of block `block`
+    int64_t row0;                         // row of `from`
+    __device__ __forceinline__ bool find(const BatchView& t, int u)
+    {
+        Seq s;
+        if (!find_block(t, u, &b, &s, &block)) return false;
+        const int p0 = s.len - s.n;
+        from = max(p0, block * kBlockTokens);
+        rows = min(s.len, (block + 1) * kBlockTokens) - from;
+        row0 = s.row0 + (from - p0);
+        return true;
+    }
+};
+
+// query heads head * group .. of the rows, sixteen dimensions of a row per lane; rows at no position become zeros
+template <int G, int DT>
+__device__ __forceinline__ void turn_queries(const Rows& r, int64_t capacity, int thread, int threads, const void* q, int64_t q_stride, int head, int group,
+                                             int kv_heads, const float* rope, int rot, bool halves, void* q_out, int qdt)
 {
-    constexpr int DIM = 32 * G, CH = DIM / 8, BLOCK = cache_block_bytes(KIND, DIM), HALF = cache_half_bytes(KIND, DIM);
+    constexpr int DIM = 32 * G, N = DIM / 16;
+    for (int it = thread; it < r.rows * N; it += threads) {
+        const int i = it / N, p = r.from + i;
+        const bool there = p >= 0 && p < capacity;
+        const Angles angles(it % N, rope && there ? rope + (int64_t)p * rot : nullptr, rot, halves);
+        const int64_t from = (r.row0 + i) * q_stride + head * group * DIM, to = ((r.row0 + i) * kv_heads + head) * group * DIM;
+        constexpr int AHEAD = 4;
+        for (int h = 0; h < group; h += AHEAD) {
+            Eight<DT> a[AHEAD], b[AHEAD];
+#pragma unroll
+            for (int e = 0; e < AHEAD; e++) {
+                const int at = min(h + e, group - 1) * DIM;
+                a[e].load(q, from + at + 8 * angles.c0);
+                b[e].load(q, from + at + 8 * angles.c1);
+            }
+#pragma unroll
+            for (int e = 0; e < AHEAD; e++) {
+                if (h + e >= group) break;
+                float x[8], y[8];
+                angles.turned(a[e], b[e], halves, x, y);
+                if (!there) {
+#pragma unroll
+                    for (int d = 0; d < 8; d++) x[d] = y[d] = 0.f;
+                }
+                store8(q_out, qdt, to + (h + e) * DIM + 8 * angles.c0, x);
+                store8(q_out, qdt, to + (h + e) * DIM + 8 * angles.c1, y);
+            }
+        }
+    }
+}
+
+template <int G, int DT>
+__global__ __launch_bounds__(kTurnThreads) void turn_kernel(CacheView c, BatchView t, const void* __restrict__ q, int64_t q_stride, int group,
+                                                            const float* __restrict__ rope, int rot, int halves, void* __restrict__ q_out, int qdt)
+{
+    Rows r;
+    if (!r.find(t, blockIdx.x)) return;
+    turn_queries<G, DT>(r, (int64_t)t.table_pages << (c.page_shift + 5), threadIdx.x, kTurnThreads, q, q_stride, blockIdx.y, group, c.kv_heads, rope, rot, halves,
+                        q_out, qdt);
+}
+
+// Keys and values one token at a time: wave `wave` of `waves`
+template <int KIND, int G, int DT>
+__device__ __forceinline__ void put_rows(const Rows& r, uint8_t* to, bool value, int wave, int waves, const void* x, int64_t stride, int head, const float* rope,
+                                         int rot, bool halves)
+{
+    constexpr int DIM = 32 * G, CH = DIM / 8;
+    for (int it = wave * 64 + (threadIdx.x & 63); it < r.rows * CH; it += 64 * waves) {        // (the four lanes of a group are in it together)
+        const int ch = it % CH, i = it / CH, p = r.from + i;
+        float w[8];
+        load_turned<DT>(x, (r.row0 + i) * stride + head * DIM, ch, rope && !value ? rope + (int64_t)p * rot : nullptr, rot, halves, w);
+        put_one<KIND, G>(to + (value ? cache_half_bytes(KIND, DIM) : 0), value, p & 31, ch, w);
+    }
+}
+
+// Fewer than 32 rows of a sequence, which fill no block: one launch, a wave for the keys, one for the values, two for the queries
+template <int KIND, int G, int DT>
+__global__ __launch_bounds__(256) void append_few_kernel(CacheView c, BatchView t, const void* __restrict__ q, int64_t q_stride, int group,
+                                                         const void* __restrict__ k, int64_t k_stride, const void* __restrict__ v, int64_t v_stride,
+                                                         const float* __restrict__ rope, int rot, int halves, void* __restrict__ q_out, int qdt)
+{
+    Rows r;
+    if (!r.find(t, blockIdx.x)) return;
+    const int head = blockIdx.y, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (wave >= 2) {
+        turn_queries<G, DT>(r, (int64_t)t.table_pages << (c.page_shift + 5), threadIdx.x - 128, 128, q, q_stride, head, group, c.kv_heads, rope, rot, halves, q_out,
+                            qdt);
+        return;
+    }
+    uint8_t* const to = block_at(c, t, r.b, r.block, head, cache_block_bytes(KIND, 32 * G));
+    if (to) put_rows<KIND, G, DT>(r, to, wave == 1, 0, 1, wave == 1 ? v : k, wave == 1 ? v_stride : k_stride, head, rope, rot, halves);
+}
+
+// Whole blocks: a wave has 64 of the keys' pairs of eight dimensions, or of the values' eights of eight
+template <int G>
+struct AppendShape {
+    static constexpr int kKeyWaves = G, kValueWaves = (G + 3) / 4, kWaves = kKeyWaves + kValueWaves;
+};
+
+template <int KIND, int G, int DT>
+__global__ __launch_bounds__(64 * AppendShape<G>::kWaves) void append_kernel(CacheView c, BatchView t, const void* __restrict__ k, int64_t k_stride,
+                                                                             const void* __restrict__ v, int64_t v_stride, const float* __restrict__ rope,
+                                                                             int rot, int halves)
+{
+    typedef AppendShape<G> T;
+    constexpr int DIM = 32 * G, CH = DIM / 8, BLOCK = cache_block_bytes(KIND, DIM), HALF = cache_half_bytes(KIND, DIM), DATA = cache_data_bytes(KIND, DIM);
+    Rows r;
+    if (!r.find(t, blockIdx.x)) return;
+    const int head = blockIdx.y, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    uint8_t* const to = block_at(c, t, r.b, r.block, head, BLOCK);
+    if (!to) return;
+    const bool value = wave >= T::kKeyWaves;
+    if (r.rows < kBlockTokens) {
+        if (value) put_rows<KIND, G, DT>(r, to, true, wave - T::kKeyWaves, T::kValueWaves, v, v_stride, head, rope, rot, halves);
+        else put_rows<KIND, G, DT>(r, to, false, wave, T::kKeyWaves, k, k_stride, head, rope, rot, halves);
+        return;
+    }
+    const int64_t row0 = r.row0;
+    const int from = r.from;
+    if (!value) {                                                     // tokens m and m + 8 of every 16: their 16 bytes, or 8
+        const int it = wave * 64 + lane;
+        const int ch = it % CH, m = it / CH, g = ch >> 2, q4 = ch & 3, tok = (m >> 3) << 4 | (m & 7);
+        float x[2][8];
+#pragma unroll
+        for (int w = 0; w < 2; w++) {
+            const int i = tok + 8 * w;
+            load_turned<DT>(k, (row0 + i) * k_stride + head * DIM, ch, rope ? rope + (int64_t)(from + i) * rot : nullptr, rot, halves, x[w]);
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[w][e] = limited(x[w][e], kLimit<KIND>);
+        }
+        if constexpr (!cache_quantised(KIND)) {
+#pragma unroll
+            for (int w = 0; w < 2; w++) *reinterpret_cast<u32x4_t*>(to + key_place<KIND, G>(tok + 8 * w, g, q4)) = pack8(KIND == kCacheF16 ? kF16 : kBF16, x[w]);
+        } else {
+            uint32_t u[2][8];
+#pragma unroll
+            for (int w = 0; w < 2; w++) {
+                const _Float16 dh = quantise8<KIND>(x[w], u[w]);
+                if (q4 == 0) *reinterpret_cast<uint16_t*>(to + DATA + scale_place(tok + 8 * w, g)) = __builtin_bit_cast(uint16_t, dh);
+            }
+            if constexpr (KIND == kCacheQ8)
+                *reinterpret_cast<u32x4_t*>(to + key_place<KIND, G>(tok, g, q4)) = u32x4_t{bytes4(u[0]), bytes4(u[0] + 4), bytes4(u[1]), bytes4(u[1] + 4)};
+            else *reinterpret_cast<u32x2_t*>(to + key_place<KIND, G>(tok, g, q4)) = u32x2_t{nibbles8(u[0]), nibbles8(u[1])};
+        }
+        return;
+    }
+    // values: eight dimensions of the eight tokens of a quarter
+    const int it = (wave - T::kKeyWaves) * 64 + lane;
+    if (it >= 4 * CH) return;
+    const int ch = it % CH, q4 = it / CH, g = ch >> 2;
+    uint8_t* const half = to + HALF;
+    Eight<DT> w[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) w[j].load(v, (row0 + token_of(q4, j)) * v_stride + head * DIM + 8 * ch);
+    if constexpr (!cache_quantised(KIND)) {
+        u32x4_t out[8];                                           // dimension e: eight tokens of 16 bits
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[e] = limited(w[j][e], kLimit<KIND>);
+            const u32x4_t p = pack8(KIND == kCacheF16 ? kF16 : kBF16, x);
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const uint32_t one = p[e >> 1] >> (16 * (e & 1)) & 0xffffu;
+                out[e][j >> 1] = j & 1 ? out[e][j >> 1] | one << 16 : one;
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e++) *reinterpret_cast<u32x4_t*>(half + value_place<KIND, G>(token_of(q4, 0), 8 * ch + e)) = out[e];
+    } else {
+        u32x2_t out[8];                                           // dimension e (Q4: and e + 16): a byte of each token
+        u32x4_t scales;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            float x[8];
+            uint32_t u[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[e] = limited(w[j][e], kLimit<KIND>);
+            const uint32_t dh = __builtin_bit_cast(uint16_t, quantise8<KIND>(x, u));
+            scales[j >> 1] = j & 1 ? scales[j >> 1] | dh << 16 : dh;
+            constexpr int order[4] = {0, 2, 1, 3};
+            const int shift = 8 * (KIND == kCacheQ4 ? order[j & 3] : j & 3);
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                uint32_t one = u[e];
+                if constexpr (KIND == kCacheQ4) one |= (uint32_t)__shfl_xor((int)one, 2) << 4;     // (of use in the lower lanes)
+                out[e][j >> 2] = (j & 3) ? out[e][j >> 2] | (one & 0xffu) << shift : (one & 0xffu) << shift;
+            }
+        }
+        if (KIND == kCacheQ8 || (ch & 3) < 2) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) *reinterpret_cast<u32x2_t*>(half + value_place<KIND, G>(token_of(q4, 0), 8 * ch + e)) = out[e];
+        }
+        if ((ch & 3) == 0) *reinterpret_cast<u32x4_t*>(half + DATA + scale_place(token_of(q4, 0), g)) = scales;
+    }
+}
+
+__device__ __forceinline__ float held_bits(int kind, uint32_t w) { return kind == kCacheF16 ? f16_bits_to_f32(w & 0xffffu) : __builtin_bit_cast(float, w << 16); }
+
+// A wave reads a block's keys, one its values: whole bytes of all tokens, rows of those that are asked for.
+template <int KIND, int G>
+__global__ __launch_bounds__(128) void read_kernel(CacheView c, BatchView t, void* __restrict__ k, void* __restrict__ v, int dt)
+{
+    constexpr int DIM = 32 * G, CH = DIM / 8, BLOCK = cache_block_bytes(KIND, DIM), HALF = cache_half_bytes(KIND, DIM), DATA = cache_data_bytes(KIND, DIM);
+    constexpr float ZERO = KIND == kCacheQ4 ? 8.0f : 128.0f;
     int b, block;
     Seq s;
     if (!find_block(t, blockIdx.x, &b, &s, &block)) return;
-    const int head = blockIdx.y, p0 = s.len - s.n;
+    const int head = blockIdx.y, p0 = s.len - s.n, lane = threadIdx.x & 63;
     const int from = max(p0, block * kBlockTokens), rows = min(s.len, (block + 1) * kBlockTokens) - from;
     const uint8_t* const src = block_at(c, t, b, block, head, BLOCK);
-    const int items = rows * 2 * CH;
-    for (int it = threadIdx.x; it < items; it += kThreads) {
-        const int ch = it % CH, hr = it / CH, i = hr >> 1;
-        const bool value = hr & 1;
-        const int p = from + i;
-        float x[8] = {};
-        if (src) held8<KIND, G>(src + (value ? HALF : 0), value, p & 31, ch, x);
-        store8(value ? v : k, dt, ((int64_t)(s.row0 + (p - p0)) * c.kv_heads + head) * DIM + 8 * ch, x);
+    const int before = from - block * kBlockTokens;                       // token i of the block is row i - before of `rows`
+    const int64_t row0 = s.row0 + (from - p0);
+    auto put = [&](void* to, int tok, int ch, const float x[8]) __attribute__((always_inline)) {
+        const int i = tok - before;
+        if (i >= 0 && i < rows) store8(to, dt, ((row0 + i) * c.kv_heads + head) * DIM + 8 * ch, x);
+    };
+    if (!src) {
+        const float zeros[8] = {};
+        for (int it = threadIdx.x; it < 64 * CH; it += 128) put(it < 32 * CH ? k : v, it / CH & 31, it % CH, zeros);
+        return;
     }
+    if (threadIdx.x < 64) {
+#pragma unroll 4
+        for (int it = lane; it < 16 * CH; it += 64) {
+            const int ch = it % CH, m = it / CH, g = ch >> 2, q4 = ch & 3, tok = (m >> 3) << 4 | (m & 7);
+            float x[2][8];
+            if constexpr (!cache_quantised(KIND)) {
+#pragma unroll
+                for (int w = 0; w < 2; w++) {
+                    const u32x4_t p = *reinterpret_cast<const u32x4_t*>(src + key_place<KIND, G>(tok + 8 * w, g, q4));
+#pragma unroll
+                    for (int e = 0; e < 8; e++) x[w][e] = held_bits(KIND, p[e >> 1] >> (16 * (e & 1)));
+                }
+            } else {
+                const uint16_t* const sc = reinterpret_cast<const uint16_t*>(src + DATA + scale_place(tok, g));
+                const float d[2] = {f16_bits_to_f32(sc[0]), f16_bits_to_f32(sc[4])};
+                if constexpr (KIND == kCacheQ8) {
+                    const u32x4_t p = *reinterpret_cast<const u32x4_t*>(src + key_place<KIND, G>(tok, g, q4));
+#pragma unroll
+                    for (int e = 0; e < 16; e++) x[e >> 3][e & 7] = ((float)(p[e >> 2] >> (8 * (e & 3)) & 255u) - ZERO) * d[e >> 3];
+                } else {
+                    const u32x2_t p = *reinterpret_cast<const u32x2_t*>(src + key_place<KIND, G>(tok, g, q4));
+#pragma unroll
+                    for (int e = 0; e < 16; e++)
+                        x[e >> 3][e & 7] = ((float)(p[e >> 3] >> (16 * (e & 1) + 4 * (e >> 1 & 1) + 8 * (e >> 2 & 1)) & 15u) - ZERO) * d[e >> 3];
+                }
+            }
+#pragma unroll
+            for (int w = 0; w < 2; w++) put(k, tok + 8 * w, ch, x[w]);
+        }
+        return;
+    }
+    for (int it = lane; it < 4 * CH; it += 64) {
+        const int ch = it % CH, q4 = it / CH;
+        const uint8_t* const half = src + HALF;
+        u32x4_t p[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const int d = 8 * ch + e;
+            const uint8_t* const at = half + value_place<KIND, G>(token_of(q4, 0), KIND == kCacheQ4 ? d & ~16 : d);
+            if constexpr (!cache_quantised(KIND)) p[e] = *reinterpret_cast<const u32x4_t*>(at);
+            else {
+                const u32x2_t w = *reinterpret_cast<const u32x2_t*>(at);
+                p[e] = u32x4_t{w[0], w[1], 0u, 0u};
+            }
+        }
+        u32x4_t scales = {0u, 0u, 0u, 0u};
+        if constexpr (cache_quantised(KIND)) scales = *reinterpret_cast<const u32x4_t*>(half + DATA + scale_place(token_of(q4, 0), ch >> 2));
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            float x[8];
+            const float d = f16_bits_to_f32(scales[j >> 1] >> (16 * (j & 1)) & 0xffffu);
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                if constexpr (!cache_quantised(KIND)) x[e] = held_bits(KIND, p[e][j >> 1] >> (16 * (j & 1)));
+                else if constexpr (KIND == kCacheQ8) x[e] = ((float)(p[e][j >> 2] >> (8 * (j & 3)) & 255u) - ZERO) * d;
+                else {
+                    constexpr int order[4] = {0, 2, 1, 3};
+                    x[e] = ((float)(p[e][j >> 2] >> (8 * order[j & 3] + (ch & 2 ? 4 : 0)) & 15u) - ZERO) * d;
+                }
+            }
+            put(v, token_of(q4, j), ch, x);
+        }
+    }
+}
+
+template <int KIND, int G, int DT>
+hipError_t append_of(const CacheView& c, const BatchView& t, dim3 grid, const void* q, int64_t q_stride, int group, const void* k, int64_t k_stride,
+                     const void* v, int64_t v_stride, const float* rope, int rot, int halves, void* q_out, int qdt, hipStream_t st)
+{
+    if (t.max_new < kBlockTokens) {
+        hipLaunchKernelGGL((append_few_kernel<KIND, G, DT>), grid, dim3(q ? 256 : 128), 0, st, c, t, q, q_stride, group, k, k_stride, v, v_stride, rope, rot, halves,
+                           q_out, qdt);
+        return hipGetLastError();
+    }
+    if (q) {
+        hipLaunchKernelGGL((turn_kernel<G, DT>), grid, dim3(kTurnThreads), 0, st, c, t, q, q_stride, group, rope, rot, halves, q_out, qdt);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    hipLaunchKernelGGL((append_kernel<KIND, G, DT>), grid, dim3(64 * AppendShape<G>::kWaves), 0, st, c, t, k, k_stride, v, v_stride, rope, rot, halves);
+    return hipGetLastError();
 }
 
 template <int KIND, int G>
 hipError_t append_as(const CacheView& c, const BatchView& t, dim3 grid, const void* q, int64_t q_stride, int group, const void* k, int64_t k_stride,
                      const void* v, int64_t v_stride, int dt, const float* rope, int rot, int halves, void* q_out, int qdt, hipStream_t st)
 {
-    auto kernel = dt == kF32 ? append_kernel<KIND, G, kF32> : dt == kF16 ? append_kernel<KIND, G, kF16> : append_kernel<KIND, G, kBF16>;
-    hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, st, c, t, q, q_stride, group, k, k_stride, v, v_stride, rope, rot, halves, q_out, qdt);
-    return hipGetLastError();
+    auto call = dt == kF32 ? append_of<KIND, G, kF32> : dt == kF16 ? append_of<KIND, G, kF16> : append_of<KIND, G, kBF16>;
+    return call(c, t, grid, q, q_stride, group, k, k_stride, v, v_stride, rope, rot, halves, q_out, qdt, st);
 }
 
 template <int KIND, int G>
 hipError_t read_as(const CacheView& c, const BatchView& t, dim3 grid, void* k, void* v, int dt, hipStream_t st)
 {
-    hipLaunchKernelGGL((read_kernel<KIND, G>), grid, dim3(kThreads), 0, st, c, t, k, v, dt);
+    hipLaunchKernelGGL((read_kernel<KIND, G>), grid, dim3(128), 0, st, c, t, k, v, dt);
     return hipGetLastError();
 }
 
