@@ -171,62 +171,71 @@ struct Angles {
     }
 };
 
-// round_half_away of the quotient x / d rounded to fp32, d of 11 bits, without dividing and without a branch.  A quotient of an fp32 number
-// and such a d that is below a half-integer h stays below it when it is rounded (x would have to be nearer to h d than fp32 numbers lie), so
-// the answer is the f with (f - 1/2) d <= |x| < (f + 1/2) d, and these products are exact.  The product with the reciprocal finds f to
-// within one.  (The division that once stood here for quotients near a half-integer was a branch per value: a kernel of 60 KB.)
-__device__ __forceinline__ float quotient_rounded(float x, float d, float rd)
-{
-    const float a = fabsf(x);
-    float f = truncf(__builtin_fmaf(a, rd, 0.5f));
-    f -= __builtin_fmaf(0.5f - f, d, a) < 0.f ? 1.0f : 0.f;
-    f += __builtin_fmaf(-0.5f - f, d, a) >= 0.f ? 1.0f : 0.f;
-    return copysignf(f, x);
-}
-
 // what a cache can hold: NaN as 0, the rest within its range (so that nothing read back is ever infinite, and a masked value times a
 // probability of 0 is 0)
 __device__ __forceinline__ float limited(float x, float limit) { return x != x ? 0.f : fminf(fmaxf(x, -limit), limit); }
 
-// Eight dimensions as a cache holds them: integers u = q + 8, q + 128 and their group's scale; the four lanes of a group call together.
 template <int KIND>
-__device__ __forceinline__ _Float16 quantise8(const float x[8], uint32_t u[8])
+constexpr float kLimit = KIND == kCacheF16 ? 65504.0f : KIND == kCacheBF16 ? 3.3895313892515355e38f : 57344.0f;
+
+template <int KIND>
+__device__ __forceinline__ void limit8(float x[8])
 {
-    constexpr float QMAX = KIND == kCacheQ4 ? 7.0f : 127.0f;
+#pragma unroll
+    for (int e = 0; e < 8; e++) x[e] = limited(x[e], kLimit<KIND>);
+}
+
+// v of the lane one or two places from this one in its four
+template <int STEP>
+__device__ __forceinline__ uint32_t other_of_quad(uint32_t v)
+{
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, STEP == 1 ? 0xB1 : 0x4E, 0xf, 0xf, true);        // quad permutations [1 0 3 2], [2 3 0 1]
+}
+template <int STEP>
+__device__ __forceinline__ float other_of_quad(float v) { return __builtin_bit_cast(float, other_of_quad<STEP>(__builtin_bit_cast(uint32_t, v))); }
+
+// Eight dimensions as a cache holds them: f[e] = q + 8 or q + 128 and their group's scale; the four lanes of a group call together.
+// round_half_away of the quotient x / d rounded to fp32, d of 11 bits, without dividing and without a branch: such a quotient that is below a
+// half-integer h stays below it when it is rounded (x would have to be nearer to h d than fp32 numbers lie), so the answer is the f with
+// (f - 1/2) d <= |x| < (f + 1/2) d, and these products are exact.  The product with the reciprocal, made a little too large (2^-21: its own error
+// is 3 units in the last place), finds f or f + 1.  12 instructions per value; with a clamp of each and corrections both ways 40, which
+// is what bounded the kernel (4096 tokens, 8 heads of 128: 16 us, 9.6 of a 16-bit cache).
+template <int KIND>
+__device__ __forceinline__ _Float16 quantise8(const float x[8], float f[8])
+{
+    constexpr float QMAX = KIND == kCacheQ4 ? 7.0f : 127.0f, ZERO = KIND == kCacheQ4 ? 8.0f : 128.0f;
     float amax = 0.f;
 #pragma unroll
     for (int e = 0; e < 8; e++) amax = fmaxf(amax, fabsf(x[e]));
-    amax = fmaxf(amax, __shfl_xor(amax, 1));
-    amax = fmaxf(amax, __shfl_xor(amax, 2));
+    amax = fmaxf(amax, other_of_quad<1>(amax));
+    amax = fmaxf(amax, other_of_quad<2>(amax));
     const _Float16 dh = (_Float16)(amax / QMAX);
-    const float d = (float)dh, rd = __builtin_amdgcn_rcpf(d);
+    const float d = (float)dh;
+    const float rd = d != 0.f ? __builtin_amdgcn_rcpf(d) * (1.0f + 1.0f / 2097152.0f) : 0.f;
 #pragma unroll
     for (int e = 0; e < 8; e++) {
-        const float r = d != 0.f ? quotient_rounded(x[e], d, rd) : 0.f;
-        u[e] = (uint32_t)((int)fminf(fmaxf(r, -QMAX), QMAX) + (KIND == kCacheQ4 ? 8 : 128));
+        const float a = fabsf(x[e]);
+        float w = truncf(__builtin_fmaf(a, rd, 0.5f));
+        w -= __builtin_fmaf(0.5f - w, d, a) < 0.f ? 1.0f : 0.f;
+        f[e] = ZERO + copysignf(fminf(w, QMAX), x[e]);
     }
     return dh;
 }
 
-__device__ __forceinline__ uint32_t bytes4(const uint32_t u[4]) { return u[0] | u[1] << 8 | u[2] << 16 | u[3] << 24; }
-__device__ __forceinline__ uint32_t nibbles8(const uint32_t u[8])
+// f as byte `at` of w
+__device__ __forceinline__ uint32_t byte_in(uint32_t w, int at, float f) { return __builtin_amdgcn_cvt_pk_u8_f32(f, at, w); }
+__device__ __forceinline__ uint32_t bytes4(const float f[4]) { return byte_in(byte_in(byte_in(byte_in(0u, 0, f[0]), 1, f[1]), 2, f[2]), 3, f[3]); }
+__device__ __forceinline__ uint32_t nibbles8(const float f[8])
 {
-    uint32_t w = 0;
-#pragma unroll
-    for (int e = 0; e < 8; e++) w |= u[e] << (16 * (e & 1) + 4 * (e >> 1 & 1) + 8 * (e >> 2));
-    return w;
+    const float lo[4] = {f[0], f[4], f[1], f[5]}, hi[4] = {f[2], f[6], f[3], f[7]};
+    return bytes4(lo) | bytes4(hi) << 4;
 }
-
-template <int KIND>
-constexpr float kLimit = KIND == kCacheF16 ? 65504.0f : KIND == kCacheBF16 ? 3.3895313892515355e38f : 57344.0f;
 
 // a token's key or value, as bytes of its own
 template <int KIND, int G>
-__device__ __forceinline__ void put_one(uint8_t* half, bool value, int tok, int ch, float x[8])
+__device__ __forceinline__ void put_one(uint8_t* half, bool value, int tok, int ch, const float x[8])
 {
     const int g = ch >> 2, q4 = ch & 3;
-#pragma unroll
-    for (int e = 0; e < 8; e++) x[e] = limited(x[e], kLimit<KIND>);
     if constexpr (!cache_quantised(KIND)) {
         const u32x4_t w = pack8(KIND == kCacheF16 ? kF16 : kBF16, x);
         if (!value) *reinterpret_cast<u32x4_t*>(half + key_place<KIND, G>(tok, g, q4)) = w;
@@ -235,21 +244,21 @@ __device__ __forceinline__ void put_one(uint8_t* half, bool value, int tok, int 
             for (int e = 0; e < 8; e++) *reinterpret_cast<uint16_t*>(half + value_place<KIND, G>(tok, 8 * ch + e)) = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
         }
     } else {
-        uint32_t u[8];
-        const _Float16 dh = quantise8<KIND>(x, u);
+        float f[8];
+        const _Float16 dh = quantise8<KIND>(x, f);
         if (q4 == 0) *reinterpret_cast<uint16_t*>(half + cache_data_bytes(KIND, 32 * G) + scale_place(tok, g)) = __builtin_bit_cast(uint16_t, dh);
         if (!value) {
-            if constexpr (KIND == kCacheQ8) *reinterpret_cast<u32x2_t*>(half + key_place<KIND, G>(tok, g, q4)) = u32x2_t{bytes4(u), bytes4(u + 4)};
-            else *reinterpret_cast<uint32_t*>(half + key_place<KIND, G>(tok, g, q4)) = nibbles8(u);
+            if constexpr (KIND == kCacheQ8) *reinterpret_cast<u32x2_t*>(half + key_place<KIND, G>(tok, g, q4)) = u32x2_t{bytes4(f), bytes4(f + 4)};
+            else *reinterpret_cast<uint32_t*>(half + key_place<KIND, G>(tok, g, q4)) = nibbles8(f);
         } else {
+            uint32_t w[2] = {bytes4(f), bytes4(f + 4)};
+            if constexpr (KIND == kCacheQ4) {                     // dimensions + 16: two lanes on
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                if constexpr (KIND == kCacheQ8) half[value_place<KIND, G>(tok, 8 * ch + e)] = (uint8_t)u[e];
-                else {
-                    const uint32_t upper = __shfl_xor((int)u[e], 2);       // dimension + 16: two lanes on
-                    if (q4 < 2) half[value_place<KIND, G>(tok, 8 * ch + e)] = (uint8_t)(u[e] | upper << 4);
-                }
+                for (int e = 0; e < 2; e++) w[e] |= other_of_quad<2>(w[e]) << 4;
+                if (q4 >= 2) return;
             }
+#pragma unroll
+            for (int e = 0; e < 8; e++) half[value_place<KIND, G>(tok, 8 * ch + e)] = (uint8_t)(w[e >> 2] >> (8 * (e & 3)));
         }
     }
 }
@@ -273,19 +282,20 @@ struct Rows {
     }
 };
 
-// query heads head * group .. of the rows, sixteen dimensions of a row per lane; rows at no position become zeros
-template <int G, int DT>
+// query heads head * group .. of the rows, sixteen dimensions of a row per lane, of all its heads (AHEAD of them on their way at once) or of
+// one; rows at no position become zeros
+template <int G, int DT, int AHEAD>
 __device__ __forceinline__ void turn_queries(const Rows& r, int64_t capacity, int thread, int threads, const void* q, int64_t q_stride, int head, int group,
                                              int kv_heads, const float* rope, int rot, bool halves, void* q_out, int qdt)
 {
     constexpr int DIM = 32 * G, N = DIM / 16;
-    for (int it = thread; it < r.rows * N; it += threads) {
-        const int i = it / N, p = r.from + i;
+    const int each = AHEAD == 1 ? 1 : group, runs = AHEAD == 1 ? group : 1;
+    for (int it = thread; it < r.rows * runs * N; it += threads) {
+        const int run = it / N % runs, i = it / N / runs, p = r.from + i;
         const bool there = p >= 0 && p < capacity;
         const Angles angles(it % N, rope && there ? rope + (int64_t)p * rot : nullptr, rot, halves);
         const int64_t from = (r.row0 + i) * q_stride + head * group * DIM, to = ((r.row0 + i) * kv_heads + head) * group * DIM;
-        constexpr int AHEAD = 4;
-        for (int h = 0; h < group; h += AHEAD) {
+        for (int h = run * each; h < run * each + each; h += AHEAD) {
             Eight<DT> a[AHEAD], b[AHEAD];
 #pragma unroll
             for (int e = 0; e < AHEAD; e++) {
@@ -315,7 +325,7 @@ __global__ __launch_bounds__(kTurnThreads) void turn_kernel(CacheView c, BatchVi
 {
     Rows r;
     if (!r.find(t, blockIdx.x)) return;
-    turn_queries<G, DT>(r, (int64_t)t.table_pages << (c.page_shift + 5), threadIdx.x, kTurnThreads, q, q_stride, blockIdx.y, group, c.kv_heads, rope, rot, halves,
+    turn_queries<G, DT, 4>(r, (int64_t)t.table_pages << (c.page_shift + 5), threadIdx.x, kTurnThreads, q, q_stride, blockIdx.y, group, c.kv_heads, rope, rot, halves,
                         q_out, qdt);
 }
 
@@ -329,6 +339,7 @@ __device__ __forceinline__ void put_rows(const Rows& r, uint8_t* to, bool value,
         const int ch = it % CH, i = it / CH, p = r.from + i;
         float w[8];
         load_turned<DT>(x, (r.row0 + i) * stride + head * DIM, ch, rope && !value ? rope + (int64_t)p * rot : nullptr, rot, halves, w);
+        limit8<KIND>(w);
         put_one<KIND, G>(to + (value ? cache_half_bytes(KIND, DIM) : 0), value, p & 31, ch, w);
     }
 }
@@ -343,8 +354,8 @@ __global__ __launch_bounds__(256) void append_few_kernel(CacheView c, BatchView 
     if (!r.find(t, blockIdx.x)) return;
     const int head = blockIdx.y, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (wave >= 2) {
-        turn_queries<G, DT>(r, (int64_t)t.table_pages << (c.page_shift + 5), threadIdx.x - 128, 128, q, q_stride, head, group, c.kv_heads, rope, rot, halves, q_out,
-                            qdt);
+        turn_queries<G, DT, 1>(r, (int64_t)t.table_pages << (c.page_shift + 5), threadIdx.x - 128, 128, q, q_stride, head, group, c.kv_heads, rope, rot, halves,
+                               q_out, qdt);
         return;
     }
     uint8_t* const to = block_at(c, t, r.b, r.block, head, cache_block_bytes(KIND, 32 * G));
@@ -358,7 +369,7 @@ struct AppendShape {
 };
 
 template <int KIND, int G, int DT>
-__global__ __launch_bounds__(64 * AppendShape<G>::kWaves) void append_kernel(CacheView c, BatchView t, const void* __restrict__ k, int64_t k_stride,
+__global__ __launch_bounds__(64 * AppendShape<G>::kWaves, 6) void append_kernel(CacheView c, BatchView t, const void* __restrict__ k, int64_t k_stride,
                                                                              const void* __restrict__ v, int64_t v_stride, const float* __restrict__ rope,
                                                                              int rot, int halves)
 {
@@ -371,8 +382,8 @@ __global__ __launch_bounds__(64 * AppendShape<G>::kWaves) void append_kernel(Cac
     if (!to) return;
     const bool value = wave >= T::kKeyWaves;
     if (r.rows < kBlockTokens) {
-        if (value) put_rows<KIND, G, DT>(r, to, true, wave - T::kKeyWaves, T::kValueWaves, v, v_stride, head, rope, rot, halves);
-        else put_rows<KIND, G, DT>(r, to, false, wave, T::kKeyWaves, k, k_stride, head, rope, rot, halves);
+        put_rows<KIND, G, DT>(r, to, false, wave, T::kWaves, k, k_stride, head, rope, rot, halves);
+        put_rows<KIND, G, DT>(r, to, true, wave, T::kWaves, v, v_stride, head, rope, rot, halves);
         return;
     }
     const int64_t row0 = r.row0;
@@ -385,14 +396,13 @@ __global__ __launch_bounds__(64 * AppendShape<G>::kWaves) void append_kernel(Cac
         for (int w = 0; w < 2; w++) {
             const int i = tok + 8 * w;
             load_turned<DT>(k, (row0 + i) * k_stride + head * DIM, ch, rope ? rope + (int64_t)(from + i) * rot : nullptr, rot, halves, x[w]);
-#pragma unroll
-            for (int e = 0; e < 8; e++) x[w][e] = limited(x[w][e], kLimit<KIND>);
+            limit8<KIND>(x[w]);
         }
         if constexpr (!cache_quantised(KIND)) {
 #pragma unroll
             for (int w = 0; w < 2; w++) *reinterpret_cast<u32x4_t*>(to + key_place<KIND, G>(tok + 8 * w, g, q4)) = pack8(KIND == kCacheF16 ? kF16 : kBF16, x[w]);
         } else {
-            uint32_t u[2][8];
+            float u[2][8];
 #pragma unroll
             for (int w = 0; w < 2; w++) {
                 const _Float16 dh = quantise8<KIND>(x[w], u[w]);
@@ -404,21 +414,28 @@ __global__ __launch_bounds__(64 * AppendShape<G>::kWaves) void append_kernel(Cac
         }
         return;
     }
-    // values: eight dimensions of the eight tokens of a quarter
-    const int it = (wave - T::kKeyWaves) * 64 + lane;
-    if (it >= 4 * CH) return;
-    const int ch = it % CH, q4 = it / CH, g = ch >> 2;
+    // Values: eight dimensions of the eight tokens of a quarter.  A lane's bytes of one dimension lie 16 apart from those of the next: they meet
+    // in LDS, whence the wave writes whole lines (straight to memory every 512 bytes were 64 lines touched).
+    constexpr int CHUNKS = CH < 16 ? CH : 16, GROUP = DATA / G;               // eights of a wave; bytes of 32 dimensions
+    __shared__ u32x4_t lds[DATA / 16];
+    uint8_t* const image = reinterpret_cast<uint8_t*>(lds);
     uint8_t* const half = to + HALF;
+    const int vw = wave - T::kKeyWaves, ch = vw * 16 + lane % CHUNKS, q4 = min(lane / CHUNKS, 3), g = ch >> 2;
+    const bool mine = lane < 4 * CHUNKS;
     Eight<DT> w[8];
 #pragma unroll
     for (int j = 0; j < 8; j++) w[j].load(v, (row0 + token_of(q4, j)) * v_stride + head * DIM + 8 * ch);
+    auto row = [&](int j, float (&x)[8]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = w[j][e];
+        limit8<KIND>(x);
+    };
     if constexpr (!cache_quantised(KIND)) {
         u32x4_t out[8];                                           // dimension e: eight tokens of 16 bits
 #pragma unroll
         for (int j = 0; j < 8; j++) {
             float x[8];
-#pragma unroll
-            for (int e = 0; e < 8; e++) x[e] = limited(w[j][e], kLimit<KIND>);
+            row(j, x);
             const u32x4_t p = pack8(KIND == kCacheF16 ? kF16 : kBF16, x);
 #pragma unroll
             for (int e = 0; e < 8; e++) {
@@ -426,34 +443,44 @@ __global__ __launch_bounds__(64 * AppendShape<G>::kWaves) void append_kernel(Cac
                 out[e][j >> 1] = j & 1 ? out[e][j >> 1] | one << 16 : one;
             }
         }
+        if (mine) {
 #pragma unroll
-        for (int e = 0; e < 8; e++) *reinterpret_cast<u32x4_t*>(half + value_place<KIND, G>(token_of(q4, 0), 8 * ch + e)) = out[e];
+            for (int e = 0; e < 8; e++) *reinterpret_cast<u32x4_t*>(image + value_place<KIND, G>(token_of(q4, 0), 8 * ch + e)) = out[e];
+        }
     } else {
         u32x2_t out[8];                                           // dimension e (Q4: and e + 16): a byte of each token
         u32x4_t scales;
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            float x[8];
-            uint32_t u[8];
-#pragma unroll
-            for (int e = 0; e < 8; e++) x[e] = limited(w[j][e], kLimit<KIND>);
+            float x[8], u[8];
+            row(j, x);
             const uint32_t dh = __builtin_bit_cast(uint16_t, quantise8<KIND>(x, u));
             scales[j >> 1] = j & 1 ? scales[j >> 1] | dh << 16 : dh;
             constexpr int order[4] = {0, 2, 1, 3};
-            const int shift = 8 * (KIND == kCacheQ4 ? order[j & 3] : j & 3);
+            const int byte = KIND == kCacheQ4 ? order[j & 3] : j & 3;
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                uint32_t one = u[e];
-                if constexpr (KIND == kCacheQ4) one |= (uint32_t)__shfl_xor((int)one, 2) << 4;     // (of use in the lower lanes)
-                out[e][j >> 2] = (j & 3) ? out[e][j >> 2] | (one & 0xffu) << shift : (one & 0xffu) << shift;
-            }
+            for (int e = 0; e < 8; e++) out[e][j >> 2] = byte_in(j & 3 ? out[e][j >> 2] : 0u, byte, u[e]);
         }
-        if (KIND == kCacheQ8 || (ch & 3) < 2) {
+        if constexpr (KIND == kCacheQ4) {                             // (of use in the lower lanes of a group)
 #pragma unroll
-            for (int e = 0; e < 8; e++) *reinterpret_cast<u32x2_t*>(half + value_place<KIND, G>(token_of(q4, 0), 8 * ch + e)) = out[e];
+            for (int e = 0; e < 8; e++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const uint32_t own = out[e][j];
+                    out[e][j] = own | other_of_quad<2>(own) << 4;
+                }
         }
-        if ((ch & 3) == 0) *reinterpret_cast<u32x4_t*>(half + DATA + scale_place(token_of(q4, 0), g)) = scales;
+        if (mine && (KIND == kCacheQ8 || (ch & 3) < 2)) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) *reinterpret_cast<u32x2_t*>(image + value_place<KIND, G>(token_of(q4, 0), 8 * ch + e)) = out[e];
+        }
+        if (mine && (ch & 3) == 0) *reinterpret_cast<u32x4_t*>(half + DATA + scale_place(token_of(q4, 0), g)) = scales;
     }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    const int first = vw * 4 * GROUP, bytes = CHUNKS / 4 * GROUP;             // the wave's part of the block
+    for (int at = 16 * lane; at < bytes; at += 1024) *reinterpret_cast<u32x4_t*>(half + first + at) = *reinterpret_cast<const u32x4_t*>(image + first + at);
 }
 
 __device__ __forceinline__ float held_bits(int kind, uint32_t w) { return kind == kCacheF16 ? f16_bits_to_f32(w & 0xffffu) : __builtin_bit_cast(float, w << 16); }
