@@ -35,6 +35,7 @@ struct AttnArgs {
 
 constexpr int kMaxUnits = 1 << 24;               // of a call
 constexpr int kTarget = 256, kTileTarget = 512;  // parts of all, rows and tiles kernel
+constexpr int kLeast = 8, kTileLeast = 8;        // blocks of a part
 constexpr int kFewRows = 64;                     // rows of a sequence and kv head (new tokens times group) that the rows kernel takes
 
 struct Unit {
@@ -59,56 +60,78 @@ __device__ __forceinline__ int tiles_of(const AttnArgs& a, const Seq& s)
     return a.few && (rows > a.few) != MANY ? 0 : (rows + ROWS - 1) / ROWS;
 }
 
+// sum over the wave, the same on every lane
+__device__ __forceinline__ float wave_total(float v)
+{
+    auto step = [&](int moved) { v += __builtin_bit_cast(float, moved); };
+    step(__builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x111, 0xf, 0xf, true));       // as in wave_prefix
+    step(__builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x112, 0xf, 0xf, true));
+    step(__builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x114, 0xf, 0xf, true));
+    step(__builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x118, 0xf, 0xf, true));
+    step(__builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x142, 0xa, 0xf, false));
+    step(__builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x143, 0xc, 0xf, false));
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+}
+
+// what a lane knows of its sequence
+struct Share {
+    Seq s;
+    int tiles, blocks;
+};
+template <int ROWS, bool MANY>
+__device__ __forceinline__ Share share_of(const AttnArgs& a, int b, int64_t capacity)
+{
+    Share x = {{0, 0, 0}, 0, 0};
+    if (b < a.t.seqs) {
+        x.s = seq_of(a.t, b);
+        int lo, hi;
+        seen(a, x.s.len - x.s.n, x.s.len - 1, capacity, &lo, &hi);
+        x.tiles = tiles_of<ROWS, MANY>(a, x.s);
+        x.blocks = hi - lo;
+    }
+    return x;
+}
+
 template <int ROWS, bool MANY>
 __device__ __forceinline__ bool find_unit(const AttnArgs& a, int u, Unit* out)
 {
     const int lane = threadIdx.x & 63;
     const int64_t capacity = (int64_t)a.t.table_pages << (a.c.page_shift + 5);
     const int heads = a.c.kv_heads;
-    float work = 0.f;
-    for (int base = 0; base < a.t.seqs; base += 64) {
-        if (base + lane < a.t.seqs) {
-            const Seq s = seq_of(a.t, base + lane);
-            int lo, hi;
-            seen(a, s.len - s.n, s.len - 1, capacity, &lo, &hi);
-            work += (float)tiles_of<ROWS, MANY>(a, s) * (float)(hi - lo);
-        }
+    Share x = share_of<ROWS, MANY>(a, lane, capacity);
+    float work = (float)x.tiles * (float)x.blocks;
+    for (int base = 64; base < a.t.seqs; base += 64) {
+        const Share more = share_of<ROWS, MANY>(a, base + lane, capacity);
+        work += (float)more.tiles * (float)more.blocks;
     }
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) work += __shfl_xor(work, m);
+    work = wave_total(work);
     // (a little more, so that what is rounded never makes more parts than the slabs hold)
     const int part = max(a.least, (int)fminf(work * (float)heads / (float)a.target * 1.0001f + 1.0f, 1.0e9f));
     int64_t units = 0;
     int slabs = 0, tickets = 0;
     bool found = false;
     for (int base = 0; base < a.t.seqs; base += 64) {
-        Seq s = {0, 0, 0};
-        int tiles = 0, splits = 0;
-        if (base + lane < a.t.seqs) {
-            s = seq_of(a.t, base + lane);
-            int lo, hi;
-            seen(a, s.len - s.n, s.len - 1, capacity, &lo, &hi);
-            tiles = tiles_of<ROWS, MANY>(a, s);
-            splits = max(1, (hi - lo + part - 1) / part);
-        }
+        if (base) x = share_of<ROWS, MANY>(a, base + lane, capacity);
+        const int splits = x.tiles ? max(1, (x.blocks + part - 1) / part) : 0;
         // (a batch whose starts make no sense may add up to anything: what cannot be right stays above every grid)
-        const int rows = min(tiles * heads, kMaxUnits + 1), mine = (int)min((int64_t)rows * splits, (int64_t)kMaxUnits + 1);
+        const int rows = min(x.tiles * heads, kMaxUnits + 1), mine = (int)min((int64_t)rows * splits, (int64_t)kMaxUnits + 1);
         const int upto = wave_prefix(mine), slab_upto = wave_prefix(splits > 1 ? mine : 0), ticket_upto = wave_prefix(splits > 1 ? rows : 0);
         const int total = __builtin_amdgcn_readlane(upto, 63);
         if (!found && u < units + total) {
             found = true;
             const int l = __builtin_ctzll(__ballot((int)units + upto > u));
-            out->s.row0 = __builtin_amdgcn_readlane(s.row0, l);
-            out->s.n = __builtin_amdgcn_readlane(s.n, l);
-            out->s.len = __builtin_amdgcn_readlane(s.len, l);
+            out->s.row0 = __builtin_amdgcn_readlane(x.s.row0, l);
+            out->s.n = __builtin_amdgcn_readlane(x.s.n, l);
+            out->s.len = __builtin_amdgcn_readlane(x.s.len, l);
             out->b = base + l;
             out->splits = __builtin_amdgcn_readlane(splits, l);
             const int at = u - (int)units - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(mine, l));
             // heads first: workgroups of one head, which read the same blocks, go to the same XCDs where there are 2, 4 or 8 of them; the last
             // tiles first, which see the most
-            out->head = at % heads;
-            out->split = at / heads % out->splits;
-            out->tile = __builtin_amdgcn_readlane(tiles, l) - 1 - at / heads / out->splits;
+            const int behind = at / heads, of_tile = behind / out->splits;
+            out->head = at - behind * heads;
+            out->split = behind - of_tile * out->splits;
+            out->tile = __builtin_amdgcn_readlane(x.tiles, l) - 1 - of_tile;
             const int rest = out->tile * heads + out->head;
             out->slab = slabs + __builtin_amdgcn_readlane(slab_upto, l) - __builtin_amdgcn_readlane(mine, l) + rest * out->splits + out->split;
             out->ticket = tickets + __builtin_amdgcn_readlane(ticket_upto, l) - __builtin_amdgcn_readlane(rows, l) + rest;
@@ -297,13 +320,30 @@ __global__ __launch_bounds__(64 * kWaves) void attention_rows_kernel(AttnArgs a)
                 for (int j = 0; j < 4; j++) qf[g].u[j] = pack_half2(x[8 * g + 2 * j] * f, x[8 * g + 2 * j + 1] * f);
         }
     }
+    // my blocks are first + wv + 8 i; a lane asks for the page of one of 64 of them, those that have one are worked on
     const int32_t* const table = a.t.tables + (int64_t)u.b * a.t.table_pages;
     const int in_page = (1 << a.c.page_shift) - 1;
-    auto block_of = [&](int blk) -> const uint8_t* {
-        if (blk >= last) return nullptr;
-        const int page = table[blk >> a.c.page_shift];
-        if ((unsigned)page >= (unsigned)a.c.pages) return nullptr;
-        return a.c.base + page * a.c.page_bytes + (int64_t)((u.head << a.c.page_shift) + (blk & in_page)) * BLOCK;
+    int base = first + wv, page = -1;
+    uint64_t there = 0;
+    auto look_up = [&]() {
+        for (; base < last; base += 64 * kWaves) {
+            const int blk = base + lane * kWaves;
+            page = blk < last ? table[blk >> a.c.page_shift] : -1;
+            there = __ballot((unsigned)page < (unsigned)a.c.pages);
+            if (there) return;
+        }
+    };
+    auto next_block = [&](int* blk) -> const uint8_t* {
+        if (!there) {
+            base += 64 * kWaves;
+            look_up();
+            if (!there) return nullptr;
+        }
+        const int l = __builtin_ctzll(there);
+        there &= there - 1;
+        *blk = base + l * kWaves;
+        const int id = __builtin_amdgcn_readlane(page, l);
+        return a.c.base + id * a.c.page_bytes + (int64_t)((u.head << a.c.page_shift) + (*blk & in_page)) * BLOCK;
     };
     float4_t y[DT];
 #pragma unroll
@@ -311,14 +351,9 @@ __global__ __launch_bounds__(64 * kWaves) void attention_rows_kernel(AttnArgs a)
     const float none = -__builtin_inff();
     float m = none, l = 0.f;                                          // m: of scores without their factor
     Half<KIND, G> k, v;
-    int blk = first + wv;
-    auto next_there = [&](int from, const uint8_t** at) {             // the next of my blocks that has a page
-        for (*at = nullptr; from < last; from += kWaves)
-            if ((*at = block_of(from)) != nullptr) break;
-        return from;
-    };
-    const uint8_t* at;
-    blk = next_there(blk, &at);
+    int blk = 0;
+    look_up();
+    const uint8_t* at = there ? next_block(&blk) : nullptr;
     if (at) {
         k.load(at, lane);
         v.load(at + HALF, lane);
@@ -344,8 +379,8 @@ __global__ __launch_bounds__(64 * kWaves) void attention_rows_kernel(AttnArgs a)
             }
         }
         const int tok = blk * kBlockTokens + 16 * (q4 >> 1) + 4 * (q4 & 1);
-        const uint8_t* next;
-        const int next_blk = next_there(blk + kWaves, &next);
+        int next_blk = 0;
+        const uint8_t* const next = next_block(&next_blk);
         if (next) k.load(next, lane);
         if (blk * kBlockTokens < all_lo || blk * kBlockTokens + 31 > all_hi) {
 #pragma unroll
@@ -912,17 +947,19 @@ hipError_t attention_as(AttnArgs a, hipStream_t st)
     const bool many = most > kFewRows;
     a.few = many && a.t.seqs > 1 ? kFewRows : 0;                     // (a single sequence: the kernel that its largest call needs)
     hipError_t e = hipSuccess;
-    const int64_t rows = (int64_t)a.t.rows * a.group;
+    const int64_t rows = (int64_t)a.t.rows * a.group, blocks = (int64_t)a.t.table_pages << a.c.page_shift;
+    // tiles of all, and the parts beyond one of each: what `target` makes of them, and no more than the table has blocks for
+    auto grid = [&](int64_t tiles) { return (unsigned)(tiles * a.c.kv_heads + std::min<int64_t>(a.target, tiles * a.c.kv_heads * (blocks / a.least))); };
     if (!many || a.few) {
         a.target = kTarget;
-        a.least = kWaves;
+        a.least = kLeast;
         const int64_t tiles = std::min(rows / kRows + a.t.seqs, a.few ? (int64_t)a.t.seqs * ((kFewRows + kRows - 1) / kRows) : rows);
-        e = rows_as<KIND, G>(a, (unsigned)(tiles * a.c.kv_heads + 2 * kTarget), st);
+        e = rows_as<KIND, G>(a, grid(tiles), st);
     }
     if (many && e == hipSuccess) {
         a.target = kTileTarget;
-        a.least = 8;
-        e = tiles_as<KIND, G>(a, (unsigned)((rows / TileShape<G>::kRows + a.t.seqs) * a.c.kv_heads + 2 * kTileTarget), st);
+        a.least = kTileLeast;
+        e = tiles_as<KIND, G>(a, grid(rows / TileShape<G>::kRows + a.t.seqs), st);
     }
     return e;
 }
