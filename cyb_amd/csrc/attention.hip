@@ -34,8 +34,8 @@ struct AttnArgs {
 };
 
 constexpr int kMaxUnits = 1 << 24;               // of a call
-constexpr int kTarget = 256, kTileTarget = 512;  // parts of all, rows and tiles kernel
-constexpr int kLeast = 8, kTileLeast = 8;        // blocks of a part
+constexpr int kTarget = 512, kTileTarget = 512;  // parts of all, rows and tiles kernel
+constexpr int kLeast = 4, kTileLeast = 8;        // blocks of a part
 constexpr int kFewRows = 64;                     // rows of a sequence and kv head (new tokens times group) that the rows kernel takes
 
 struct Unit {
@@ -99,14 +99,19 @@ __device__ __forceinline__ bool find_unit(const AttnArgs& a, int u, Unit* out)
     const int64_t capacity = (int64_t)a.t.table_pages << (a.c.page_shift + 5);
     const int heads = a.c.kv_heads;
     Share x = share_of<ROWS, MANY>(a, lane, capacity);
-    float work = (float)x.tiles * (float)x.blocks;
+    float work = (float)x.tiles * (float)x.blocks, tiles = (float)x.tiles;
     for (int base = 64; base < a.t.seqs; base += 64) {
         const Share more = share_of<ROWS, MANY>(a, base + lane, capacity);
         work += (float)more.tiles * (float)more.blocks;
+        tiles += (float)more.tiles;
     }
-    work = wave_total(work);
-    // (a little more, so that what is rounded never makes more parts than the slabs hold)
-    const int part = max(a.least, (int)fminf(work * (float)heads / (float)a.target * 1.0001f + 1.0f, 1.0e9f));
+    work = wave_total(work) * (float)heads;
+    tiles = wave_total(tiles) * (float)heads;
+    // Every tile begins a part of its own, so what is to be had in one round of workgroups are `target` less the tiles; where that is less than half
+    // of a round, rounds follow each other anyway and parts are made for their balance.  (A little more, so that what is rounded never makes
+    // more parts than the slabs hold.)
+    const float more = (float)a.target - tiles, extra = more >= 0.5f * (float)a.target ? more : (float)a.target;
+    const int part = max(a.least, (int)fminf(work / extra * 1.0001f + 1.0f, 1.0e9f));
     int64_t units = 0;
     int slabs = 0, tickets = 0;
     bool found = false;
@@ -265,16 +270,61 @@ __device__ __forceinline__ void store_row4(void* y, int dt, int64_t at, float4_t
     *reinterpret_cast<u32x2_t*>(static_cast<uint16_t*>(y) + at) = w;
 }
 
-// Few rows: tiles of 16, eight waves that take a part's blocks in turn.  Keys of the next block are on their way while P is formed, values
-// while the next scores are.  Waves meet in LDS, the parts of a tile in slabs in memory: the part that is last adds them in order.
-constexpr int kWaves = 8, kRows = 16;
+// Parts travel past the caches: stores and loads at system scope, nothing flushed, nothing invalidated.
+__device__ __forceinline__ void put_float2(float* to, float x, float y)
+{
+    __hip_atomic_store(reinterpret_cast<uint64_t*>(to), __builtin_bit_cast(uint64_t, f32x2_t{x, y}), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+}
+__device__ __forceinline__ void put_float4(float* to, float4_t v)
+{
+    put_float2(to, v[0], v[1]);
+    put_float2(to + 2, v[2], v[3]);
+}
+__device__ __forceinline__ f32x2_t get_float2(const float* from)
+{
+    return __builtin_bit_cast(f32x2_t, __hip_atomic_load(reinterpret_cast<const uint64_t*>(from), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM));
+}
+__device__ __forceinline__ float4_t get_float4(const float* from)
+{
+    const f32x2_t a = get_float2(from), b = get_float2(from + 2);
+    return float4_t{a[0], a[1], b[0], b[1]};
+}
+
+// The workgroup's part has been stored: whether it is the tile's last, and all of them are there.  The ticket is left at zero for the next call;
+// parts are added in their order whoever arrives when.
+__device__ __forceinline__ bool last_part(const AttnArgs& a, const Unit& u, unsigned* flag)
+{
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                  // mine has reached memory
+    __syncthreads();                                                  // (and everybody is done reading LDS)
+    if (threadIdx.x == 0) {
+        const unsigned old = __hip_atomic_fetch_add(a.tickets + u.ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const bool end = old + 1u == (unsigned)u.splits;
+        if (end) __hip_atomic_store(a.tickets + u.ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        *flag = end ? 1u : 0u;
+    }
+    __syncthreads();
+    const bool end = *flag != 0u;
+    __syncthreads();
+    return end;
+}
+
+// Few rows: tiles of 16, four waves that take a part's blocks in turn, each with the next of its blocks on its way while it
+// works on one.  Waves meet in LDS, the parts of a tile in slabs in memory: the part that is last adds them in order.
+constexpr int kRows = 16;
+template <int G>
+struct RowsShape {
+    static constexpr int kWaves = 4;
+    static constexpr int kLds = kWaves * 2 * G * 64 * 16 + kWaves * 32 * 4;
+    static constexpr int kSlab = kRows * 32 * G + 2 * kRows;                  // floats of a part: its rows, and their maxima and sums in pairs
+};
 
 template <int KIND, int G>
-__global__ __launch_bounds__(64 * kWaves) void attention_rows_kernel(AttnArgs a)
+__global__ __launch_bounds__(64 * RowsShape<G>::kWaves) void attention_rows_kernel(AttnArgs a)
 {
+    constexpr int kWaves = RowsShape<G>::kWaves;
     constexpr int DIM = 32 * G, BLOCK = cache_block_bytes(KIND, DIM), HALF = cache_half_bytes(KIND, DIM), DT = 2 * G;
     constexpr bool SPLIT_P = KIND == kCacheBF16;
-    constexpr float kShift = SPLIT_P ? 0.f : 14.f;
+    constexpr float kShift = SPLIT_P ? 0.f : 12.f, kLag = SPLIT_P ? 8.f : 3.f;          // (as in the tiles kernel)
     extern __shared__ float4_t lds[];                                 // [waves][DT][64], then [waves][16] maxima and sums
     float* const stats = reinterpret_cast<float*>(lds + kWaves * DT * 64);
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q4 = lane >> 4, r = lane & 15;
@@ -320,7 +370,8 @@ __global__ __launch_bounds__(64 * kWaves) void attention_rows_kernel(AttnArgs a)
                 for (int j = 0; j < 4; j++) qf[g].u[j] = pack_half2(x[8 * g + 2 * j] * f, x[8 * g + 2 * j + 1] * f);
         }
     }
-    // my blocks are first + wv + 8 i; a lane asks for the page of one of 64 of them, those that have one are worked on
+    const float lag = fminf(kLag / c, 1e30f);
+    // my blocks are first + wv + kWaves i; a lane asks for the page of one of 64 of them, those that have one are worked on
     const int32_t* const table = a.t.tables + (int64_t)u.b * a.t.table_pages;
     const int in_page = (1 << a.c.page_shift) - 1;
     int base = first + wv, page = -1;
@@ -350,15 +401,22 @@ __global__ __launch_bounds__(64 * kWaves) void attention_rows_kernel(AttnArgs a)
     for (int d = 0; d < DT; d++) y[d] = float4_t{0.f, 0.f, 0.f, 0.f};
     const float none = -__builtin_inff();
     float m = none, l = 0.f;                                          // m: of scores without their factor
-    Half<KIND, G> k, v;
+    Half<KIND, G> k0, v0, k1, v1;
     int blk = 0;
     look_up();
     const uint8_t* at = there ? next_block(&blk) : nullptr;
     if (at) {
-        k.load(at, lane);
-        v.load(at + HALF, lane);
+        k0.load(at, lane);
+        v0.load(at + HALF, lane);
     }
-    while (at) {
+    // one block; the next one's keys and values go to nk, nv
+    auto work = [&](const Half<KIND, G>& k, const Half<KIND, G>& v, Half<KIND, G>& nk, Half<KIND, G>& nv) __attribute__((always_inline)) {
+        int next_blk = 0;
+        const uint8_t* const next = next_block(&next_blk);
+        if (next) {
+            nk.load(next, lane);
+            nv.load(next + HALF, lane);
+        }
         float4_t s[2];
 #pragma unroll
         for (int t = 0; t < 2; t++) {
@@ -379,9 +437,6 @@ __global__ __launch_bounds__(64 * kWaves) void attention_rows_kernel(AttnArgs a)
             }
         }
         const int tok = blk * kBlockTokens + 16 * (q4 >> 1) + 4 * (q4 & 1);
-        int next_blk = 0;
-        const uint8_t* const next = next_block(&next_blk);
-        if (next) k.load(next, lane);
         if (blk * kBlockTokens < all_lo || blk * kBlockTokens + 31 > all_hi) {
 #pragma unroll
             for (int t = 0; t < 2; t++)
@@ -394,8 +449,8 @@ __global__ __launch_bounds__(64 * kWaves) void attention_rows_kernel(AttnArgs a)
         float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
         top = fmaxf(top, other_quarter<16>(top));
         top = fmaxf(top, other_quarter<32>(top));
-        if (__ballot(top > m)) {
-            const float now = fmaxf(m, top);
+        if (__ballot(top > m + lag)) {
+            const float now = top > m + lag ? top : m;
             const float f = m == none ? 0.f : exp2_fast((m - now) * c);
             m = now;
             l *= f;
@@ -425,9 +480,13 @@ __global__ __launch_bounds__(64 * kWaves) void attention_rows_kernel(AttnArgs a)
             y[d] = mfma16<KIND>(vf, ph, y[d]);
             if constexpr (SPLIT_P) y[d] = mfma16<KIND>(vf, pl, y[d]);
         }
-        if (next) v.load(next + HALF, lane);
         at = next;
         blk = next_blk;
+    };
+    while (at) {
+        work(k0, v0, k1, v1);
+        if (!at) break;
+        work(k1, v1, k0, v0);
     }
     l += other_quarter<16>(l);
     l += other_quarter<32>(l);
@@ -449,77 +508,73 @@ __global__ __launch_bounds__(64 * kWaves) void attention_rows_kernel(AttnArgs a)
         sum += f[w] * stats[kWaves * 16 + w * 16 + r];                // (a row of NaN has a sum of NaN and no maximum)
     }
     const int64_t row_at = ((int64_t)(u.s.row0 + i) * a.c.kv_heads * a.group + head) * DIM + 4 * q4;
-    constexpr int SLAB = DT * 64 * 4 + 32;                            // floats of a part: sums, maxima and sums of probabilities
+    constexpr int SLAB = RowsShape<G>::kSlab;
     float* const slab = a.slabs + (size_t)u.slab * SLAB;
-    for (int d = wv; d < DT; d += kWaves) {
-        float4_t o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int w = 0; w < kWaves; w++) {
-            const float4_t part = lds[(w * DT + d) * 64 + lane];
-            if (f[w] != 0.f) o += part * f[w];
-        }
-        if (u.splits == 1) {
-            const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-            if (real) store_row4(a.y, a.qdt, row_at + 16 * d, o * inv);
-        } else if (real) {
-            const u32x2_t* w = reinterpret_cast<const u32x2_t*>(&o);
-            uint64_t* to = reinterpret_cast<uint64_t*>(slab + (d * 64 + lane) * 4);
-            __hip_atomic_store(to, __builtin_bit_cast(uint64_t, w[0]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
-            __hip_atomic_store(to + 1, __builtin_bit_cast(uint64_t, w[1]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
-        }
-    }
-    if (u.splits == 1) return;
-    if (threadIdx.x < 16) {
-        __hip_atomic_store(slab + DT * 64 * 4 + threadIdx.x, top, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
-        __hip_atomic_store(slab + DT * 64 * 4 + 16 + threadIdx.x, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
-    }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                  // my part of the slab has reached memory
-    __syncthreads();                                                  // (and everybody is done reading LDS)
-    unsigned* const flag = reinterpret_cast<unsigned*>(lds);
-    if (threadIdx.x == 0) {
-        const unsigned old = __hip_atomic_fetch_add(a.tickets + u.ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        const bool end = old + 1u == (unsigned)u.splits;
-        if (end) __hip_atomic_store(a.tickets + u.ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        *flag = end ? 1u : 0u;
-    }
-    __syncthreads();
-    if (*flag == 0u) return;
-    __syncthreads();
-    // every part's maxima and sums of probabilities, then its sums
-    float* const all = reinterpret_cast<float*>(lds);
-    float* const of_tile = slab - (size_t)u.split * SLAB;
-    for (int e = threadIdx.x; e < u.splits * 32; e += 64 * kWaves)
-        all[e] = __hip_atomic_load(of_tile + (size_t)(e >> 5) * SLAB + DT * 64 * 4 + (e & 31), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
-    __syncthreads();
-    top = none;
-    for (int e = 0; e < u.splits; e++) top = fmaxf(top, all[e * 32 + r]);
-    sum = 0.f;
-    for (int e = 0; e < u.splits; e++) sum += (all[e * 32 + r] == none ? 0.f : exp2_fast(all[e * 32 + r] - top)) * all[e * 32 + 16 + r];
-    if (!real) return;
     const float inv = sum == 0.f ? 0.f : 1.0f / sum;
     for (int d = wv; d < DT; d += kWaves) {
+        float4_t o = lds[d * 64 + lane] * f[0];                       // (sums of a wave without a maximum are zeros, or its row is NaN)
+#pragma unroll
+        for (int w = 1; w < kWaves; w++) o += lds[(w * DT + d) * 64 + lane] * f[w];
+        if (!real) continue;
+        if (u.splits == 1) store_row4(a.y, a.qdt, row_at + 16 * d, o * inv);
+        else put_float4(slab + r * DIM + 16 * d + 4 * q4, o);
+    }
+    if (u.splits == 1) return;
+    if (threadIdx.x < 16) put_float2(slab + kRows * DIM + 2 * r, top, sum);
+    if (!last_part(a, u, reinterpret_cast<unsigned*>(lds))) return;
+    // The rows of all parts: threads share out the rows' float4s, and the parts where there are more threads; everything is asked for at once.
+    constexpr int THREADS = 64 * kWaves, QUADS = DIM / 4, AHEAD = 8;
+    const int items = rows * QUADS, runs = max(1, THREADS / items);
+    const float* const of_tile = slab - (size_t)u.split * SLAB;
+    for (int it0 = 0; it0 < items; it0 += THREADS) {                  // (one round for up to 8 rows of 128)
+        const int run = runs == 1 ? 0 : threadIdx.x / items, it = it0 + threadIdx.x - run * items;
+        const bool mine = it < items && run < runs;
+        const int row = mine ? it / QUADS : 0, quad = mine ? it - row * QUADS : 0;
+        float m2 = none, l2 = 0.f;
         float4_t o = {0.f, 0.f, 0.f, 0.f};
-        constexpr int AHEAD = 8;
-        for (int e0 = 0; e0 < u.splits; e0 += AHEAD) {
-            uint64_t w[AHEAD][2];
+        for (int e0 = run; e0 < u.splits && mine; e0 += AHEAD * runs) {
+            float4_t part[AHEAD];
+            f32x2_t of[AHEAD];
 #pragma unroll
             for (int e = 0; e < AHEAD; e++) {
-                const uint64_t* from = reinterpret_cast<const uint64_t*>(of_tile + (size_t)min(e0 + e, u.splits - 1) * SLAB + (d * 64 + lane) * 4);
-                w[e][0] = __hip_atomic_load(from, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
-                w[e][1] = __hip_atomic_load(from + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+                const float* const from = of_tile + (size_t)min(e0 + e * runs, u.splits - 1) * SLAB;
+                part[e] = get_float4(from + row * DIM + 4 * quad);
+                of[e] = get_float2(from + kRows * DIM + 2 * row);
             }
+            float now = m2;
+#pragma unroll
+            for (int e = 0; e < AHEAD; e++) now = fmaxf(now, of[e][0]);
+            const float old = m2 == none ? 0.f : exp2_fast(m2 - now);
+            o *= old;
+            l2 *= old;
+            m2 = now;
 #pragma unroll
             for (int e = 0; e < AHEAD; e++) {
-                if (e0 + e >= u.splits) break;
-                const float me = all[(e0 + e) * 32 + r];
-                const float fe = me == none ? 0.f : exp2_fast(me - top);
-                if (fe == 0.f) continue;
-                const float4_t part = {__builtin_bit_cast(float, (uint32_t)w[e][0]), __builtin_bit_cast(float, (uint32_t)(w[e][0] >> 32)),
-                                       __builtin_bit_cast(float, (uint32_t)w[e][1]), __builtin_bit_cast(float, (uint32_t)(w[e][1] >> 32))};
-                o += part * fe;
+                const float fe = of[e][0] == none || e0 + e * runs >= u.splits ? 0.f : exp2_fast(of[e][0] - now);
+                o += part[e] * fe;
+                l2 += e0 + e * runs >= u.splits ? 0.f : of[e][1] * fe;
             }
         }
-        store_row4(a.y, a.qdt, row_at + 16 * d, o * inv);
+        if (runs > 1) {                                              // (all in one round)
+            float* const pairs = reinterpret_cast<float*>(lds + THREADS);
+            lds[threadIdx.x] = o;
+            pairs[2 * threadIdx.x] = m2;
+            pairs[2 * threadIdx.x + 1] = l2;
+            __syncthreads();
+            if (run) return;
+            for (int e = 1; e < runs; e++) {
+                const int at = threadIdx.x + e * items;
+                const float me = pairs[2 * at], now = fmaxf(m2, me);
+                const float fo = m2 == none ? 0.f : exp2_fast(m2 - now), fe = me == none ? 0.f : exp2_fast(me - now);
+                o = o * fo + lds[at] * fe;
+                l2 = l2 * fo + pairs[2 * at + 1] * fe;
+                m2 = now;
+            }
+        }
+        if (!mine) continue;
+        const int at = r0 + row, of_token = at / a.group;
+        const float by = l2 == 0.f ? 0.f : 1.0f / l2;
+        store_row4(a.y, a.qdt, (((int64_t)u.s.row0 + of_token) * a.c.kv_heads * a.group + u.head * a.group + at - of_token * a.group) * DIM + 4 * quad, o * by);
     }
 }
 
@@ -864,54 +919,34 @@ __global__ __launch_bounds__(64 * TileShape<G>::kWaves) void attention_tiles_ker
     // a part: its sums, then maxima and sums of probabilities of its rows
     constexpr int SLAB = T::kSlab;
     float* const slab = a.slabs + (size_t)u.slab * SLAB;
-    float* const stats = slab + ROWS * DIM + wv * 32 + r;
+    float* const stats = slab + ROWS * DIM + 2 * (wv * 32 + r);
 #pragma unroll
     for (int d = 0; d < G; d++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            uint64_t* const to = reinterpret_cast<uint64_t*>(slab + (((wv * G + d) * 4 + e) * 64 + lane) * 4);
-            __hip_atomic_store(to, __builtin_bit_cast(uint64_t, f32x2_t{y[d][4 * e], y[d][4 * e + 1]}), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
-            __hip_atomic_store(to + 1, __builtin_bit_cast(uint64_t, f32x2_t{y[d][4 * e + 2], y[d][4 * e + 3]}), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
-        }
-    if (h == 0) {
-        __hip_atomic_store(stats, m, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
-        __hip_atomic_store(stats + ROWS, l, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
-    }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    unsigned* const flag = reinterpret_cast<unsigned*>(lds);
-    if (threadIdx.x == 0) {
-        const unsigned old = __hip_atomic_fetch_add(a.tickets + u.ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        const bool end = old + 1u == (unsigned)u.splits;
-        if (end) __hip_atomic_store(a.tickets + u.ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        *flag = end ? 1u : 0u;
-    }
-    __syncthreads();
-    if (*flag == 0u) return;
+        for (int e = 0; e < 4; e++)
+            put_float4(slab + (((wv * G + d) * 4 + e) * 64 + lane) * 4, float4_t{y[d][4 * e], y[d][4 * e + 1], y[d][4 * e + 2], y[d][4 * e + 3]});
+    if (h == 0) put_float2(stats, m, l);
+    if (!last_part(a, u, reinterpret_cast<unsigned*>(lds))) return;
     const float* const of_tile = slab - (size_t)u.split * SLAB;
-    auto part_of = [&](int e, int k) {                               // maximum (k = 0) or sum of part e for my row
-        return __hip_atomic_load(of_tile + (size_t)e * SLAB + ROWS * DIM + k * ROWS + wv * 32 + r, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
-    };
+    auto part_of = [&](int e) { return get_float2(of_tile + (size_t)e * SLAB + ROWS * DIM + 2 * (wv * 32 + r)); };        // maximum and sum of my row
     float top = none, sum = 0.f;
-    for (int e = 0; e < u.splits; e++) top = fmaxf(top, part_of(e, 0));
+    for (int e = 0; e < u.splits; e++) top = fmaxf(top, part_of(e)[0]);
 #pragma unroll
     for (int d = 0; d < G; d++)
 #pragma unroll
         for (int e = 0; e < 16; e++) y[d][e] = 0.f;
     for (int e = 0; e < u.splits; e++) {
-        const float me = part_of(e, 0), f = me == none ? 0.f : exp2_fast(me - top);
-        sum += f * part_of(e, 1);
-        const uint64_t* const from = reinterpret_cast<const uint64_t*>(of_tile + (size_t)e * SLAB + (wv * G * 4 * 64 + lane) * 4);
+        const f32x2_t me = part_of(e);
+        const float f = me[0] == none ? 0.f : exp2_fast(me[0] - top);
+        sum += f * me[1];
+        const float* const from = of_tile + (size_t)e * SLAB + (wv * G * 4 * 64 + lane) * 4;
 #pragma unroll
         for (int d = 0; d < G; d++)
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-                const uint64_t w0 = __hip_atomic_load(from + (d * 4 + k) * 128, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
-                const uint64_t w1 = __hip_atomic_load(from + (d * 4 + k) * 128 + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
-                const float part[4] = {__builtin_bit_cast(float, (uint32_t)w0), __builtin_bit_cast(float, (uint32_t)(w0 >> 32)), __builtin_bit_cast(float, (uint32_t)w1),
-                                       __builtin_bit_cast(float, (uint32_t)(w1 >> 32))};
+                const float4_t part = get_float4(from + (d * 4 + k) * 256);
 #pragma unroll
-                for (int j = 0; j < 4; j++) y[d][4 * k + j] += f == 0.f ? 0.f : part[j] * f;
+                for (int j = 0; j < 4; j++) y[d][4 * k + j] += part[j] * f;
             }
     }
     if (!real) return;
@@ -926,9 +961,8 @@ __global__ __launch_bounds__(64 * TileShape<G>::kWaves) void attention_tiles_ker
 template <int KIND, int G>
 hipError_t rows_as(const AttnArgs& a, unsigned grid, hipStream_t st)
 {
-    constexpr int bytes = kWaves * 2 * G * 64 * 16 + kWaves * 32 * 4;
-    (void)LdsRequest<&attention_rows_kernel<KIND, G>, bytes>::registered;
-    hipLaunchKernelGGL((attention_rows_kernel<KIND, G>), dim3(grid), dim3(64 * kWaves), bytes, st, a);
+    (void)LdsRequest<&attention_rows_kernel<KIND, G>, RowsShape<G>::kLds>::registered;
+    hipLaunchKernelGGL((attention_rows_kernel<KIND, G>), dim3(grid), dim3(64 * RowsShape<G>::kWaves), RowsShape<G>::kLds, st, a);
     return hipGetLastError();
 }
 
@@ -969,13 +1003,12 @@ hipError_t attention_as(AttnArgs a, hipStream_t st)
 // Parts of tiles that have more than one: at most 2 * target of them (a tile of b blocks has at most b / part + 1), of at most
 // `target` tiles.
 static_assert((2 * std::max(kTarget, kTileTarget) + 16) * sizeof(unsigned) <= kAttnTicketBytes, "a ticket per tile");
-static_assert(kTarget * 32 * 4 <= kWaves * 2 * 2 * 64 * 16 + kWaves * 32 * 4, "maxima and sums of a tile's parts fit LDS");
 
 int64_t attention_max_units() { return kMaxUnits; }
 
 size_t attention_scratch_bytes(int dim)
 {
-    const size_t rows = (size_t)(2 * kTarget + 16) * ((size_t)dim / 16 * 64 * 4 + 32) * sizeof(float);
+    const size_t rows = (size_t)(2 * kTarget + 16) * kRows * ((size_t)dim + 2) * sizeof(float);
     const size_t wave_rows = dim <= 128 ? 256 : 128;
     return std::max(rows, (2 * kTileTarget + 16) * wave_rows * ((size_t)dim + 2) * sizeof(float));
 }
