@@ -319,7 +319,7 @@ struct RowsShape {
 };
 
 template <int KIND, int G>
-__global__ __launch_bounds__(64 * RowsShape<G>::kWaves) void attention_rows_kernel(AttnArgs a)
+__global__ __launch_bounds__(64 * RowsShape<G>::kWaves, G <= 4 ? 2 : 1) void attention_rows_kernel(AttnArgs a)
 {
     constexpr int kWaves = RowsShape<G>::kWaves;
     constexpr int DIM = 32 * G, BLOCK = cache_block_bytes(KIND, DIM), HALF = cache_half_bytes(KIND, DIM), DT = 2 * G;
