@@ -34,7 +34,8 @@ struct AttnArgs {
 };
 
 constexpr int kMaxUnits = 1 << 24;               // of a call
-constexpr int kTarget = 512, kTileTarget = 512;  // parts of all, rows and tiles kernel
+constexpr int kTarget = 512, kTileTarget = 256;  // parts of all, rows and tiles kernel
+constexpr int kRounds = 2;
 constexpr int kLeast = 4, kTileLeast = 8;        // blocks of a part
 constexpr int kFewRows = 64;                     // rows of a sequence and kv head (new tokens times group) that the rows kernel takes
 
@@ -108,9 +109,10 @@ __device__ __forceinline__ bool find_unit(const AttnArgs& a, int u, Unit* out)
     work = wave_total(work) * (float)heads;
     tiles = wave_total(tiles) * (float)heads;
     // Every tile begins a part of its own, so what is to be had in one round of workgroups are `target` less the tiles; where that is less than half
-    // of a round, rounds follow each other anyway and parts are made for their balance.  (A little more, so that what is rounded never makes
+    // of a round, rounds follow each other anyway and parts are made for their balance (48 conversations of up to 8192 tokens: kRounds 1, 2, 4, 8
+    // 111, 103, 108, 120 us).  (A little more, so that what is rounded never makes
     // more parts than the slabs hold.)
-    const float more = (float)a.target - tiles, extra = more >= 0.5f * (float)a.target ? more : (float)a.target;
+    const float more = (float)a.target - tiles, extra = more >= 0.5f * (float)a.target ? more : kRounds * (float)a.target;
     const int part = max(a.least, (int)fminf(work / extra * 1.0001f + 1.0f, 1.0e9f));
     int64_t units = 0;
     int slabs = 0, tickets = 0;
@@ -983,7 +985,7 @@ hipError_t attention_as(AttnArgs a, hipStream_t st)
     hipError_t e = hipSuccess;
     const int64_t rows = (int64_t)a.t.rows * a.group, blocks = (int64_t)a.t.table_pages << a.c.page_shift;
     // tiles of all, and the parts beyond one of each: what `target` makes of them, and no more than the table has blocks for
-    auto grid = [&](int64_t tiles) { return (unsigned)(tiles * a.c.kv_heads + std::min<int64_t>(a.target, tiles * a.c.kv_heads * (blocks / a.least))); };
+    auto grid = [&](int64_t tiles) { return (unsigned)(tiles * a.c.kv_heads + std::min<int64_t>(kRounds * a.target, tiles * a.c.kv_heads * (blocks / a.least))); };
     if (!many || a.few) {
         a.target = kTarget;
         a.least = kLeast;
@@ -1000,23 +1002,23 @@ hipError_t attention_as(AttnArgs a, hipStream_t st)
 
 }  // namespace
 
-// Parts of tiles that have more than one: at most 2 * target of them (a tile of b blocks has at most b / part + 1), of at most
-// `target` tiles.
-static_assert((2 * std::max(kTarget, kTileTarget) + 16) * sizeof(unsigned) <= kAttnTicketBytes, "a ticket per tile");
+// Parts of tiles that have more than one: at most twice those beyond one of each tile, of which there are kRounds * target
+constexpr int kMostParts = 2 * kRounds * std::max(kTarget, kTileTarget) + 16;
+static_assert(kMostParts * sizeof(unsigned) <= kAttnTicketBytes, "a ticket per tile");
 
 int64_t attention_max_units() { return kMaxUnits; }
 
 size_t attention_scratch_bytes(int dim)
 {
-    const size_t rows = (size_t)(2 * kTarget + 16) * kRows * ((size_t)dim + 2) * sizeof(float);
+    const size_t rows = (size_t)(2 * kRounds * kTarget + 16) * kRows * ((size_t)dim + 2) * sizeof(float);
     const size_t wave_rows = dim <= 128 ? 256 : 128;
-    return std::max(rows, (2 * kTileTarget + 16) * wave_rows * ((size_t)dim + 2) * sizeof(float));
+    return std::max(rows, (2 * kRounds * kTileTarget + 16) * wave_rows * ((size_t)dim + 2) * sizeof(float));
 }
 
 int64_t attention_units_max(const BatchView& t, int kv_heads, int group)
 {
     // tiles: (n * group + 15) / 16 of a sequence; parts: at most target more than tiles
-    return ((int64_t)t.rows * group / kRows + t.seqs) * kv_heads + 2 * kTarget;
+    return ((int64_t)t.rows * group / kRows + t.seqs) * kv_heads + kRounds * std::max(kTarget, kTileTarget);
 }
 
 hipError_t launch_attention(const CacheView& c, const BatchView& t, const void* q, int64_t q_stride, int qdt, int group, float scale, int window, void* y,
