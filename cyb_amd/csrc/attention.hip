@@ -28,14 +28,17 @@ struct AttnArgs {
     int64_t q_stride;
     float* slabs;
     unsigned* tickets;
-    int group, qdt, window, target, least;       // least: blocks of a part
+    int group, qdt, window, target, least;       // workgroups of a round; blocks of a part, at least
+    float rounds;                                // of workgroups, where there are more tiles than one has
     int few;                                     // > 0: sequences of up to so many rows per kv head are the rows kernel's, others not
     float scale;                                 // times log2 e
 };
 
 constexpr int kMaxUnits = 1 << 24;               // of a call
-constexpr int kTarget = 512, kTileTarget = 256;  // parts of all, rows and tiles kernel
-constexpr int kRounds = 2;
+// Workgroups of a round (two of four waves to a CU, one of eight, one of heads of 256), and how many parts there may be beyond one of each tile:
+// rounds * target, twice that in the tiles kernel, whose tiles may see half as much on average as the one that sees the most
+constexpr int kTarget = 512, kMostExtra = 1024;
+constexpr float kRounds = 2.f, kTileRounds = 1.f;
 constexpr int kLeast = 4, kTileLeast = 8;        // blocks of a part
 constexpr int kFewRows = 64;                     // rows of a sequence and kv head (new tokens times group) that the rows kernel takes
 
@@ -74,21 +77,25 @@ __device__ __forceinline__ float wave_total(float v)
     return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
 
-// what a lane knows of its sequence
+// what a lane knows of its sequence: its tiles, the blocks of the one that sees the most, and of one on average (at least half of that)
 struct Share {
     Seq s;
     int tiles, blocks;
+    float mean;
 };
 template <int ROWS, bool MANY>
 __device__ __forceinline__ Share share_of(const AttnArgs& a, int b, int64_t capacity)
 {
-    Share x = {{0, 0, 0}, 0, 0};
+    Share x = {{0, 0, 0}, 0, 0, 0.f};
     if (b < a.t.seqs) {
         x.s = seq_of(a.t, b);
         int lo, hi;
         seen(a, x.s.len - x.s.n, x.s.len - 1, capacity, &lo, &hi);
         x.tiles = tiles_of<ROWS, MANY>(a, x.s);
         x.blocks = hi - lo;
+        if (MANY && a.window) x.blocks = min(x.blocks, (int)(((int64_t)a.window + ROWS / a.group + 2) >> 5) + 2);
+        x.mean = (float)x.blocks;
+        if (MANY && !a.window) x.mean -= fminf((float)(x.s.n >> 6), 0.5f * x.mean);
     }
     return x;
 }
@@ -100,19 +107,19 @@ __device__ __forceinline__ bool find_unit(const AttnArgs& a, int u, Unit* out)
     const int64_t capacity = (int64_t)a.t.table_pages << (a.c.page_shift + 5);
     const int heads = a.c.kv_heads;
     Share x = share_of<ROWS, MANY>(a, lane, capacity);
-    float work = (float)x.tiles * (float)x.blocks, tiles = (float)x.tiles;
+    float work = (float)x.tiles * x.mean, tiles = (float)x.tiles;
     for (int base = 64; base < a.t.seqs; base += 64) {
         const Share more = share_of<ROWS, MANY>(a, base + lane, capacity);
-        work += (float)more.tiles * (float)more.blocks;
+        work += (float)more.tiles * more.mean;
         tiles += (float)more.tiles;
     }
     work = wave_total(work) * (float)heads;
     tiles = wave_total(tiles) * (float)heads;
     // Every tile begins a part of its own, so what is to be had in one round of workgroups are `target` less the tiles; where that is less than half
-    // of a round, rounds follow each other anyway and parts are made for their balance (48 conversations of up to 8192 tokens: kRounds 1, 2, 4, 8
-    // 111, 103, 108, 120 us).  (A little more, so that what is rounded never makes
+    // of a round, rounds follow each other anyway and parts are made for their balance (48 conversations of up to 8192 tokens, rows kernel: 1, 2, 4, 8
+    // rounds 111, 103, 108, 120 us).  (A little more, so that what is rounded never makes
     // more parts than the slabs hold.)
-    const float more = (float)a.target - tiles, extra = more >= 0.5f * (float)a.target ? more : kRounds * (float)a.target;
+    const float more = (float)a.target - tiles, extra = more >= 0.5f * (float)a.target ? more : a.rounds * (float)a.target;
     const int part = max(a.least, (int)fminf(work / extra * 1.0001f + 1.0f, 1.0e9f));
     int64_t units = 0;
     int slabs = 0, tickets = 0;
@@ -597,11 +604,13 @@ __device__ __forceinline__ void copy_to_lds(uint32_t lds_off, const void* base, 
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(lds_off)), "v"(off), "s"(base));
 }
 
-template <int G>
+template <int KIND, int G>
 struct TileShape {
     static constexpr int kBlocks = G <= 4 ? 2 : 1;            // blocks of a step
-    static constexpr int kWaves = G <= 4 ? 8 : 4;             // waves, each with 32 rows
+    // waves, each with 32 rows: two workgroups of four to a CU, or eight that share the work of unpacking
+    static constexpr int kWaves = G <= 4 && cache_quantised(KIND) ? 8 : 4;
     static constexpr int kRows = 32 * kWaves;
+    static constexpr int kTarget = G <= 4 && kWaves == 4 ? 512 : 256;
     static constexpr int kHalf = kBlocks * kBlockTokens * 32 * G * 2;         // bytes of a step's keys, or values
     static constexpr int kLds = 4 * kHalf;                    // two steps of each
     static constexpr int kSlab = kRows * 32 * G + 2 * kRows;  // floats of a part
@@ -612,7 +621,7 @@ struct TileShape {
 // Q8, Q4: asked for in registers, and turned into f16 (scales on them, rounded once) when the step ahead is done.
 template <int KIND, int G>
 struct Stage {
-    typedef TileShape<G> T;
+    typedef TileShape<KIND, G> T;
     static constexpr bool kQuant = cache_quantised(KIND);
     static constexpr int N = kQuant ? Half<KIND, G>::N : 2 * G;                          // 1 KiB pieces of a block's half
     static constexpr int PER = (T::kBlocks * N + T::kWaves - 1) / T::kWaves;             // pieces per wave
@@ -632,10 +641,11 @@ struct Stage {
             const int bl = T::kBlocks == 1 ? 0 : p / N, i = p - bl * N;
             const uint8_t* const from = T::kBlocks == 1 || bl == 0 ? block[0] : block[T::kBlocks - 1];
             if constexpr (!kQuant) {
-                uint32_t off;
-                if (!VALUES) off = ((lane >> 3 & 1) * G * 64 + ((lane & 31) >> 4 << 3 | (lane & 7)) + (lane >> 5) * 16) * 16 + (i >> 1) * 1024 + (i & 1) * 512;
-                else off = cache_half_bytes(KIND, 32 * G) + (i >> 1) * 2048 + (lane >> 4 & 1) * 1024 + (lane & 15) * 16 + (lane >> 5) * 256 + (i & 1) * 512;
-                copy_to_lds(where + p * 1024, from, off);
+                // (a lane's place in a piece is the same in all of them: one register for the keys' offsets, one for the values')
+                const uint32_t off = VALUES ? (lane >> 4 & 1) * 1024 + (lane & 15) * 16 + (lane >> 5) * 256
+                                            : ((lane >> 3 & 1) * G * 64 + ((lane & 31) >> 4 << 3 | (lane & 7)) + (lane >> 5) * 16) * 16;
+                const uint8_t* const piece = from + (VALUES ? cache_half_bytes(KIND, 32 * G) + (i >> 1) * 2048 : (i >> 1) * 1024) + (i & 1) * 512;
+                copy_to_lds(where + p * 1024, piece, off);
             } else {
                 const uint8_t* const src = from + (VALUES ? cache_half_bytes(KIND, 32 * G) : 0);
                 const uint8_t* const sc = src + cache_data_bytes(KIND, 32 * G);
@@ -706,9 +716,9 @@ struct Stage {
 // Many rows: a workgroup's waves have 32 rows each and go through the same blocks, 64 tokens (a head of 256: 32) a step.  While P of a step
 // is formed the scores of the next are multiplied: its keys are in LDS one step earlier than its values.
 template <int KIND, int G>
-__global__ __launch_bounds__(64 * TileShape<G>::kWaves) void attention_tiles_kernel(AttnArgs a)
+__global__ __launch_bounds__((64 * TileShape<KIND, G>::kWaves), (G <= 4 ? 2 : 1)) void attention_tiles_kernel(AttnArgs a)
 {
-    typedef TileShape<G> T;
+    typedef TileShape<KIND, G> T;
     constexpr int DIM = 32 * G, BLOCK = cache_block_bytes(KIND, DIM), ROWS = T::kRows, BL = T::kBlocks;
     // P of f16 behind 2^12, its largest below 2^15: a maximum may lag behind by 2^3 before sums are scaled anew (bf16: by 2^8)
     constexpr float kShift = KIND == kCacheBF16 ? 0.f : 12.f, kLag = KIND == kCacheBF16 ? 8.f : 3.f;
@@ -733,12 +743,10 @@ __global__ __launch_bounds__(64 * TileShape<G>::kWaves) void attention_tiles_ker
     const int p = p0 + i;
     const int row_hi = real ? (int)min((int64_t)p, capacity - 1) : -1;
     const int row_lo = a.window && p >= a.window ? p - a.window + 1 : 0;
-    int wave_hi = -1, wave_lo = 0, all_hi = -1, all_lo = 0;          // some row sees wave_lo .. wave_hi, every row all_lo .. all_hi
+    int all_hi = -1, all_lo = 0;                                     // every row sees all_lo .. all_hi
     if (rows) {
         const int pf = p0 + r0 / a.group, pl = p0 + (r0 + rows - 1) / a.group;
-        wave_hi = (int)min((int64_t)pl, capacity - 1);
         all_hi = (int)min((int64_t)pf, capacity - 1);
-        wave_lo = a.window && pf >= a.window ? pf - a.window + 1 : 0;
         all_lo = a.window && pl >= a.window ? pl - a.window + 1 : 0;
     }
     const int head = u.head * a.group + in_group;
@@ -801,108 +809,155 @@ __global__ __launch_bounds__(64 * TileShape<G>::kWaves) void attention_tiles_ker
         for (int e = 0; e < 16; e++) y[d][e] = 0.f;
     const float none = -__builtin_inff();
     float m = none, l = 0.f;
-    f32x16_t s[BL];
-    auto scores = [&](uint32_t where) __attribute__((always_inline)) {
-#pragma unroll
-        for (int b = 0; b < BL; b++) {
-#pragma unroll
-            for (int e = 0; e < 16; e++) s[b][e] = 0.f;
-#pragma unroll
-            for (int k = 0; k < 2 * G; k++) {
-                Frag16 kf;
-                kf.u = *reinterpret_cast<const u32x4_t*>(bytes + where + (b * 2 * G + k) * 1024 + lane * 16);
-                s[b] = mfma32<KIND>(kf, qf[k], s[b]);
-            }
-        }
+    auto key_at = [&](uint32_t where, int k, int b) __attribute__((always_inline)) {
+        Frag16 f;
+        f.u = *reinterpret_cast<const u32x4_t*>(bytes + where + (b * 2 * G + k) * 1024 + lane * 16);
+        return f;
     };
+    auto value_at = [&](uint32_t where, int k, int d) __attribute__((always_inline)) {
+        Frag16 f;
+        f.u = *reinterpret_cast<const u32x4_t*>(bytes + where + (((k >> 1) * G + d) * 2 + (k & 1)) * 1024 + lane * 16);
+        return f;
+    };
+    const f32x16_t zeros = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     Stage<KIND, G> ks, vs;
-    const uint32_t K0 = 0, V0 = 2 * T::kHalf;
-    Pages g0 = pages_of(0), g1 = pages_of(1), g2 = pages_of(2);
+    constexpr uint32_t K0 = 0, V0 = 2 * T::kHalf;
+    constexpr int N = 2 * G * BL;                                    // matrix instructions of a step's scores, and of its values
+    Pages g0 = pages_of(0), g1 = pages_of(1), g2 = pages_of(2);      // of steps t, t + 1, t + 2
     const uint8_t* at[BL];
+    f32x16_t s[BL];                                                  // scores of step t
+    Frag16 pf[2 * BL];                                               // P of step t - 1, not yet on the sums
+#pragma unroll
+    for (int k = 0; k < 2 * BL; k++) pf[k].u = u32x4_t{0u, 0u, 0u, 0u};
     if (steps) {
         blocks_of(0, g0, at);
         ks.template ask<false>(at, K0, wv, lane);
-        vs.template ask<true>(at, V0, wv, lane);
+        vs.template ask<true>(at, V0 + T::kHalf, wv, lane);          // (values of "step -1", for a P of zeros: any finite ones)
         ks.template put<false>(bytes, K0, wv, lane, magic);
-        vs.template put<true>(bytes, V0, wv, lane, magic);
+        vs.template put<true>(bytes, V0 + T::kHalf, wv, lane, magic);
         blocks_of(1, g1, at);
         ks.template ask<false>(at, K0 + T::kHalf, wv, lane);
         ks.template put<false>(bytes, K0 + T::kHalf, wv, lane, magic);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
-        scores(K0);
+#pragma unroll
+        for (int b = 0; b < BL; b++)
+#pragma unroll
+            for (int k = 0; k < 2 * G; k++) s[b] = mfma32<KIND>(key_at(K0, k, b), qf[k], k ? s[b] : zeros);
         __syncthreads();                                             // (keys of step 2 go where those of step 0 were)
     }
-    for (int t = 0; t < steps; t++) {
-        const int odd = t & 1;
-        // keys of step t + 2 and values of step t + 1 on their way; past the end they are read from page 0 and nobody looks at them
-        const Pages g3 = pages_of(t + 3);
-        blocks_of(t + 2, g2, at);
-        ks.template ask<false>(at, K0 + odd * T::kHalf, wv, lane);
-        blocks_of(t + 1, g1, at);
-        vs.template ask<true>(at, V0 + (1 - odd) * T::kHalf, wv, lane);
+    float top = none;
+    // whether some row does not see all of step t's tokens (g0: its pages)
+    auto hides = [&](int t) {
         const int tok = (first + t * BL) * kBlockTokens;
-        const unsigned gone = absent(g0);
-        const bool look = tok <= wave_hi && tok + BL * kBlockTokens > wave_lo;
-        f32x16_t now[BL];
-#pragma unroll
-        for (int b = 0; b < BL; b++) now[b] = s[b];
-        if (t + 1 < steps) scores(K0 + (1 - odd) * T::kHalf);
-        if (look) {
-            if (gone || tok < all_lo || tok + BL * kBlockTokens - 1 > all_hi) {
-#pragma unroll
-                for (int b = 0; b < BL; b++)
-#pragma unroll
-                    for (int e = 0; e < 16; e++) {
-                        const int j = tok + b * kBlockTokens + 8 * (e >> 2) + 4 * h + (e & 3);
-                        if (j < row_lo || j > row_hi || (gone >> b & 1)) now[b][e] = none;
-                    }
-            }
-            float top = now[0][0];
+        return absent(g0) != 0 || tok < all_lo || tok + BL * kBlockTokens - 1 > all_hi;
+    };
+    // Steps whose rows see everything and whose maxima have grown by less than the lag follow each other in the inner loop; at any other its scores
+    // are masked, P that waits is added and the sums are scaled outside of it.  (In a branch of the loop the sums had two homes, 64
+    // registers and as many moves.)
+    for (int t = 0; t < steps;) {
+        if (hides(t)) {
+            const unsigned gone = absent(g0);
+            const int tok = (first + t * BL) * kBlockTokens;
 #pragma unroll
             for (int b = 0; b < BL; b++)
 #pragma unroll
-                for (int e = b ? 0 : 1; e < 16; e++) top = fmaxf(top, now[b][e]);
-            top = fmaxf(top, other_quarter<32>(top));
-            if (__ballot(top > m + lag)) {
-                const float up = top > m + lag ? top : m;
-                const float f = m == none ? 0.f : exp2_fast((m - up) * c);
-                m = up;
-                l *= f;
-#pragma unroll
-                for (int d = 0; d < G; d++)
-#pragma unroll
-                    for (int e = 0; e < 16; e++) y[d][e] *= f;
-            }
-            const float off = kShift - (m == none ? 0.f : m * c);
-            Frag16 pf[2 * BL];
-            float sums[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int b = 0; b < BL; b++)
-#pragma unroll
-                for (int e = 0; e < 16; e += 2) {
-                    const float x0 = exp2_fast(__builtin_fmaf(now[b][e], c, off)), x1 = exp2_fast(__builtin_fmaf(now[b][e + 1], c, off));
-                    sums[e >> 1 & 3] += x0 + x1;
-                    pf[2 * b + (e >> 3)].u[e >> 1 & 3] = KIND == kCacheBF16 ? pack_bf16x2(x0, x1) : pack_half2(x0, x1);
-                }
-            l += (sums[0] + sums[1]) + (sums[2] + sums[3]);
-            const uint32_t where = V0 + odd * T::kHalf;
-#pragma unroll
-            for (int k = 0; k < 2 * BL; k++)
-#pragma unroll
-                for (int d = 0; d < G; d++) {
-                    Frag16 vf;
-                    vf.u = *reinterpret_cast<const u32x4_t*>(bytes + where + (((k >> 1) * G + d) * 2 + (k & 1)) * 1024 + lane * 16);
-                    y[d] = mfma32<KIND>(vf, pf[k], y[d]);
+                for (int e = 0; e < 16; e++) {
+                    const int j = tok + b * kBlockTokens + 8 * (e >> 2) + 4 * h + (e & 3);
+                    if (j < row_lo || j > row_hi || (gone >> b & 1)) s[b][e] = none;
                 }
         }
-        ks.template put<false>(bytes, K0 + odd * T::kHalf, wv, lane, magic);
-        vs.template put<true>(bytes, V0 + (1 - odd) * T::kHalf, wv, lane, magic);
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
-        g0 = g1;
-        g1 = g2;
-        g2 = g3;
+        top = s[0][0];
+#pragma unroll
+        for (int b = 0; b < BL; b++)
+#pragma unroll
+            for (int e = b ? 0 : 1; e < 16; e++) top = fmaxf(top, s[b][e]);
+        top = fmaxf(top, other_quarter<32>(top));
+        const uint32_t before = V0 + (t & 1 ? 0 : T::kHalf);
+#pragma unroll
+        for (int i = 0; i < N; i++) y[i % G] = mfma32<KIND>(value_at(before, i / G, i % G), pf[i / G], y[i % G]);
+#pragma unroll
+        for (int k = 0; k < 2 * BL; k++) pf[k].u = u32x4_t{0u, 0u, 0u, 0u};
+        const float up = top > m + lag ? top : m;
+        const float f = m == none ? 0.f : exp2_fast((m - up) * c);
+        m = up;
+        l *= f;
+#pragma unroll
+        for (int d = 0; d < G; d++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) y[d][e] *= f;
+        do {
+            // P of step t while the values of step t - 1 are multiplied, and behind that the first scores of step t + 1 (of none: of what is in LDS,
+            // and nobody looks at them).  A wave issues in order, and a 32 x 32 instruction takes as long as eight others: the order below puts
+            // about a pair's exponentials behind each.
+            const uint32_t odd = t & 1 ? T::kHalf : 0, even = T::kHalf - odd;
+            const Pages g3 = pages_of(t + 3);
+            blocks_of(t + 2, g2, at);
+            ks.template ask<false>(at, K0 + odd, wv, lane);
+            blocks_of(t, g0, at);
+            vs.template ask<true>(at, V0 + odd, wv, lane);
+            constexpr int PAIRS = 8 * BL, EARLY = BL == 2 ? 11 : PAIRS, LOOK = 3;
+            const float off = kShift - (m == none ? 0.f : m * c);
+            Frag16 frag[N], pn[2 * BL];
+            float sums[4] = {0.f, 0.f, 0.f, 0.f};
+            auto pairs = [&](int from, int to) __attribute__((always_inline)) {
+#pragma unroll
+                for (int i = from; i < to; i++) {
+                    const int b = i >> 3, e = 2 * (i & 7);
+                    const float x0 = exp2_fast(__builtin_fmaf(s[b][e], c, off)), x1 = exp2_fast(__builtin_fmaf(s[b][e + 1], c, off));
+                    sums[i & 3] += x0 + x1;
+                    pn[i >> 2].u[i & 3] = KIND == kCacheBF16 ? pack_bf16x2(x0, x1) : pack_half2(x0, x1);
+                }
+            };
+#pragma unroll
+            for (int i = 0; i < LOOK; i++) frag[i] = value_at(V0 + even, i / G, i % G);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                if (i + LOOK < N) frag[i + LOOK] = value_at(V0 + even, (i + LOOK) / G, (i + LOOK) % G);
+                y[i % G] = mfma32<KIND>(frag[i], pf[i / G], y[i % G]);
+                pairs(i * EARLY / N, (i + 1) * EARLY / N);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            // scores: all of the first block, then of the second
+#pragma unroll
+            for (int i = 0; i < LOOK; i++) frag[i] = key_at(K0 + even, i % (2 * G), i / (2 * G));
+            f32x16_t sn[BL];
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                const int k = i % (2 * G), b = i / (2 * G);
+                if (i + LOOK < N) frag[i + LOOK] = key_at(K0 + even, (i + LOOK) % (2 * G), (i + LOOK) / (2 * G));
+                sn[b] = mfma32<KIND>(frag[i], qf[k], k ? sn[b] : zeros);
+                if (b == 0) pairs(EARLY + k * (PAIRS - EARLY) / (2 * G), EARLY + (k + 1) * (PAIRS - EARLY) / (2 * G));
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            l += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+            top = sn[0][0];
+#pragma unroll
+            for (int b = 0; b < BL; b++)
+#pragma unroll
+                for (int e = b ? 0 : 1; e < 16; e++) top = fmaxf(top, sn[b][e]);
+            top = fmaxf(top, other_quarter<32>(top));
+#pragma unroll
+            for (int b = 0; b < BL; b++) s[b] = sn[b];
+#pragma unroll
+            for (int k = 0; k < 2 * BL; k++) pf[k] = pn[k];
+            ks.template put<false>(bytes, K0 + odd, wv, lane, magic);
+            vs.template put<true>(bytes, V0 + odd, wv, lane, magic);
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            g0 = g1;
+            g1 = g2;
+            g2 = g3;
+            t++;
+        } while (t < steps && !hides(t) && !__ballot(top > m + lag));
+    }
+    {
+        const uint32_t before = V0 + (steps & 1 ? 0 : T::kHalf);
+        if (steps) {
+#pragma unroll
+            for (int i = 0; i < N; i++) y[i % G] = mfma32<KIND>(value_at(before, i / G, i % G), pf[i / G], y[i % G]);
+        }
     }
     l += other_quarter<32>(l);
     m = m == none ? none : m * c;
@@ -931,7 +986,8 @@ __global__ __launch_bounds__(64 * TileShape<G>::kWaves) void attention_tiles_ker
     if (!last_part(a, u, reinterpret_cast<unsigned*>(lds))) return;
     const float* const of_tile = slab - (size_t)u.split * SLAB;
     auto part_of = [&](int e) { return get_float2(of_tile + (size_t)e * SLAB + ROWS * DIM + 2 * (wv * 32 + r)); };        // maximum and sum of my row
-    float top = none, sum = 0.f;
+    top = none;
+    float sum = 0.f;
     for (int e = 0; e < u.splits; e++) top = fmaxf(top, part_of(e)[0]);
 #pragma unroll
     for (int d = 0; d < G; d++)
@@ -971,8 +1027,9 @@ hipError_t rows_as(const AttnArgs& a, unsigned grid, hipStream_t st)
 template <int KIND, int G>
 hipError_t tiles_as(const AttnArgs& a, unsigned grid, hipStream_t st)
 {
-    (void)LdsRequest<&attention_tiles_kernel<KIND, G>, TileShape<G>::kLds>::registered;
-    hipLaunchKernelGGL((attention_tiles_kernel<KIND, G>), dim3(grid), dim3(64 * TileShape<G>::kWaves), TileShape<G>::kLds, st, a);
+    typedef TileShape<KIND, G> T;
+    (void)LdsRequest<&attention_tiles_kernel<KIND, G>, T::kLds>::registered;
+    hipLaunchKernelGGL((attention_tiles_kernel<KIND, G>), dim3(grid), dim3(64 * T::kWaves), T::kLds, st, a);
     return hipGetLastError();
 }
 
@@ -985,40 +1042,41 @@ hipError_t attention_as(AttnArgs a, hipStream_t st)
     hipError_t e = hipSuccess;
     const int64_t rows = (int64_t)a.t.rows * a.group, blocks = (int64_t)a.t.table_pages << a.c.page_shift;
     // tiles of all, and the parts beyond one of each: what `target` makes of them, and no more than the table has blocks for
-    auto grid = [&](int64_t tiles) { return (unsigned)(tiles * a.c.kv_heads + std::min<int64_t>(kRounds * a.target, tiles * a.c.kv_heads * (blocks / a.least))); };
+    auto grid = [&](int64_t tiles) { return (unsigned)(tiles * a.c.kv_heads + std::min<int64_t>(kMostExtra, tiles * a.c.kv_heads * (blocks / a.least))); };
     if (!many || a.few) {
         a.target = kTarget;
         a.least = kLeast;
+        a.rounds = kRounds;
         const int64_t tiles = std::min(rows / kRows + a.t.seqs, a.few ? (int64_t)a.t.seqs * ((kFewRows + kRows - 1) / kRows) : rows);
         e = rows_as<KIND, G>(a, grid(tiles), st);
     }
     if (many && e == hipSuccess) {
-        a.target = kTileTarget;
+        a.target = TileShape<KIND, G>::kTarget;
         a.least = kTileLeast;
-        e = tiles_as<KIND, G>(a, grid(rows / TileShape<G>::kRows + a.t.seqs), st);
+        a.rounds = kTileRounds;
+        e = tiles_as<KIND, G>(a, grid(rows / TileShape<KIND, G>::kRows + a.t.seqs), st);
     }
     return e;
 }
 
 }  // namespace
 
-// Parts of tiles that have more than one: at most twice those beyond one of each tile, of which there are kRounds * target
-constexpr int kMostParts = 2 * kRounds * std::max(kTarget, kTileTarget) + 16;
-static_assert(kMostParts * sizeof(unsigned) <= kAttnTicketBytes, "a ticket per tile");
+// Parts of tiles that have more than one: at most twice those beyond one of each tile
+static_assert(2 * kMostExtra * sizeof(unsigned) <= kAttnTicketBytes, "a ticket per tile");
 
 int64_t attention_max_units() { return kMaxUnits; }
 
 size_t attention_scratch_bytes(int dim)
 {
-    const size_t rows = (size_t)(2 * kRounds * kTarget + 16) * kRows * ((size_t)dim + 2) * sizeof(float);
-    const size_t wave_rows = dim <= 128 ? 256 : 128;
-    return std::max(rows, (2 * kRounds * kTileTarget + 16) * wave_rows * ((size_t)dim + 2) * sizeof(float));
+    // (the tiles kernel's: 2 * 1024 parts of 128 rows, or 2 * 512 of 256 or of rows of 256)
+    const size_t rows = (size_t)2 * kMostExtra * kRows, tile_rows = (size_t)2 * kMostExtra * (dim <= 128 ? 128 : 64);
+    return std::max(rows, tile_rows) * ((size_t)dim + 2) * sizeof(float);
 }
 
 int64_t attention_units_max(const BatchView& t, int kv_heads, int group)
 {
     // tiles: (n * group + 15) / 16 of a sequence; parts: at most target more than tiles
-    return ((int64_t)t.rows * group / kRows + t.seqs) * kv_heads + kRounds * std::max(kTarget, kTileTarget);
+    return ((int64_t)t.rows * group / kRows + t.seqs) * kv_heads + kMostExtra;
 }
 
 hipError_t launch_attention(const CacheView& c, const BatchView& t, const void* q, int64_t q_stride, int qdt, int group, float scale, int window, void* y,
