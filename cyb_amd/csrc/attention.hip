@@ -35,9 +35,14 @@ struct AttnArgs {
 };
 
 constexpr int kMaxUnits = 1 << 24;               // of a call
-// Workgroups of a round (two of four waves to a CU, one of eight, one of heads of 256), and how many parts there may be beyond one of each tile:
-// rounds * target, twice that in the tiles kernel, whose tiles may see half as much on average as the one that sees the most
-constexpr int kTarget = 512, kMostExtra = 1024;
+// A maximum may lag behind the scores by 2^kLag before sums are scaled anew: every scaling is a detour of a wave that all others of its
+// workgroup wait for (with a lag of 2^3 one step in seven, the tiles kernel of attn_mixed 216 us; 2^11: PLACEHOLDER).  P of f16 stands behind 2^kShift:
+// its largest stays below 2^15, and probabilities count down to 2^-28 of the largest.
+constexpr float kShiftF16 = 4.f, kLagF16 = 11.f, kLagBF16 = 16.f;
+
+// Workgroups of a round of the rows kernel (two to a CU), and how many parts there may be beyond one of each tile: rounds * target, twice that in
+// the tiles kernel, whose tiles may see half as much on average as the one that sees the most
+constexpr int kTarget = 512, kMostExtra = 2 * kTarget;
 constexpr float kRounds = 2.f, kTileRounds = 1.f;
 constexpr int kLeast = 4, kTileLeast = 8;        // blocks of a part
 constexpr int kFewRows = 64;                     // rows of a sequence and kv head (new tokens times group) that the rows kernel takes
@@ -333,7 +338,7 @@ __global__ __launch_bounds__(64 * RowsShape<G>::kWaves, G <= 4 ? 2 : 1) void att
     constexpr int kWaves = RowsShape<G>::kWaves;
     constexpr int DIM = 32 * G, BLOCK = cache_block_bytes(KIND, DIM), HALF = cache_half_bytes(KIND, DIM), DT = 2 * G;
     constexpr bool SPLIT_P = KIND == kCacheBF16;
-    constexpr float kShift = SPLIT_P ? 0.f : 12.f, kLag = SPLIT_P ? 8.f : 3.f;          // (as in the tiles kernel)
+    constexpr float kShift = SPLIT_P ? 0.f : kShiftF16, kLag = SPLIT_P ? kLagBF16 : kLagF16;
     extern __shared__ float4_t lds[];                                 // [waves][DT][64], then [waves][16] maxima and sums
     float* const stats = reinterpret_cast<float*>(lds + kWaves * DT * 64);
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q4 = lane >> 4, r = lane & 15;
@@ -610,9 +615,13 @@ struct TileShape {
     // waves, each with 32 rows: two workgroups of four to a CU, or eight that share the work of unpacking
     static constexpr int kWaves = G <= 4 && cache_quantised(KIND) ? 8 : 4;
     static constexpr int kRows = 32 * kWaves;
-    static constexpr int kTarget = G <= 4 && kWaves == 4 ? 512 : 256;
+    // Steps of keys, and of values, that LDS holds: three where two workgroups (of short heads: three) still fit a CU, so that copies have two steps to
+    // arrive in; a step of heads of 128 is long enough for one
+    static constexpr int kRing = !cache_quantised(KIND) && G != 4 ? 3 : 2;
+    static constexpr int kPerCu = G > 4 || kWaves == 8 ? 1 : G == 2 ? 3 : 2;              // workgroups
+    static constexpr int kTarget = 256 * kPerCu, kMostExtra = 2 * kTarget;
     static constexpr int kHalf = kBlocks * kBlockTokens * 32 * G * 2;         // bytes of a step's keys, or values
-    static constexpr int kLds = 4 * kHalf;                    // two steps of each
+    static constexpr int kLds = 2 * kRing * kHalf;
     static constexpr int kSlab = kRows * 32 * G + 2 * kRows;  // floats of a part
 };
 
@@ -716,13 +725,12 @@ struct Stage {
 // Many rows: a workgroup's waves have 32 rows each and go through the same blocks, 64 tokens (a head of 256: 32) a step.  While P of a step
 // is formed the scores of the next are multiplied: its keys are in LDS one step earlier than its values.
 template <int KIND, int G>
-__global__ __launch_bounds__((64 * TileShape<KIND, G>::kWaves), (G <= 4 ? 2 : 1)) void attention_tiles_kernel(AttnArgs a)
+__global__ __launch_bounds__((64 * TileShape<KIND, G>::kWaves), (TileShape<KIND, G>::kWaves * TileShape<KIND, G>::kPerCu / 4)) void attention_tiles_kernel(AttnArgs a)
 {
     typedef TileShape<KIND, G> T;
     constexpr int DIM = 32 * G, BLOCK = cache_block_bytes(KIND, DIM), ROWS = T::kRows, BL = T::kBlocks;
-    // P of f16 behind 2^12, its largest below 2^15: a maximum may lag behind by 2^3 before sums are scaled anew (bf16: by 2^8)
-    constexpr float kShift = KIND == kCacheBF16 ? 0.f : 12.f, kLag = KIND == kCacheBF16 ? 8.f : 3.f;
-    extern __shared__ float4_t lds[];                                 // keys of two steps, values of two steps
+    constexpr float kShift = KIND == kCacheBF16 ? 0.f : kShiftF16, kLag = KIND == kCacheBF16 ? kLagBF16 : kLagF16;
+    extern __shared__ float4_t lds[];                                 // keys of kRing steps, values of as many
     uint8_t* const bytes = reinterpret_cast<uint8_t*>(lds);
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, r = lane & 31;
     const uint32_t magic = q4_magic_vgpr();
@@ -775,30 +783,28 @@ __global__ __launch_bounds__((64 * TileShape<KIND, G>::kWaves), (G <= 4 ? 2 : 1)
     const float lag = fminf(kLag / c, 1e30f);
     const int32_t* const table = a.t.tables + (int64_t)u.b * a.t.table_pages;
     const int in_page = (1 << a.c.page_shift) - 1;
-    // pages of a step's blocks (of none: -1), asked for one step before they are needed
-    struct Pages {
-        int id[BL];
+    // Pages of the part's blocks, 64 to a register (-1: none): of blocks from_block .. + 128, counted from the part's first
+    auto pages_from = [&](int i) {
+        const int blk = first + i + lane;
+        return blk < last ? table[blk >> a.c.page_shift] : -1;
     };
-    auto pages_of = [&](int step) {
-        Pages g;
-#pragma unroll
-        for (int b = 0; b < BL; b++) {
-            const int blk = first + step * BL + b;
-            g.id[b] = blk < last ? table[blk >> a.c.page_shift] : -1;
-        }
-        return g;
+    int from_block = 0, near_ids = pages_from(0), far_ids = pages_from(64);
+    auto page_of = [&](int i) {
+        const int at = i - from_block;
+        return __builtin_amdgcn_readlane(at < 64 ? near_ids : far_ids, at & 63);
     };
-    auto absent = [&](const Pages& g) {
+    // which of a step's blocks are in no page
+    auto absent = [&](int step) {
         unsigned m = 0;
 #pragma unroll
-        for (int b = 0; b < BL; b++) m |= (unsigned)g.id[b] >= (unsigned)a.c.pages ? 1u << b : 0u;
+        for (int b = 0; b < BL; b++) m |= (unsigned)page_of(step * BL + b) >= (unsigned)a.c.pages ? 1u << b : 0u;
         return m;
     };
     // (a block that is not there is read from page 0: finite numbers, which nobody sees)
-    auto blocks_of = [&](int step, const Pages& g, const uint8_t* (&at)[BL]) {
+    auto blocks_of = [&](int step, const uint8_t* (&at)[BL]) {
 #pragma unroll
         for (int b = 0; b < BL; b++) {
-            const int page = (unsigned)g.id[b] >= (unsigned)a.c.pages ? 0 : g.id[b];
+            const int id = page_of(step * BL + b), page = (unsigned)id >= (unsigned)a.c.pages ? 0 : id;
             at[b] = a.c.base + page * a.c.page_bytes + (int64_t)((u.head << a.c.page_shift) + ((first + step * BL + b) & in_page)) * BLOCK;
         }
     };
@@ -820,44 +826,57 @@ __global__ __launch_bounds__((64 * TileShape<KIND, G>::kWaves), (G <= 4 ? 2 : 1)
         return f;
     };
     const f32x16_t zeros = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    Stage<KIND, G> ks, vs;
-    constexpr uint32_t K0 = 0, V0 = 2 * T::kHalf;
+    constexpr bool QUANT = cache_quantised(KIND);
+    constexpr int R = T::kRing;
+    constexpr uint32_t K0 = 0, V0 = R * T::kHalf;
     constexpr int N = 2 * G * BL;                                    // matrix instructions of a step's scores, and of its values
-    Pages g0 = pages_of(0), g1 = pages_of(1), g2 = pages_of(2);      // of steps t, t + 1, t + 2
+    Stage<KIND, G> ks, vs;
     const uint8_t* at[BL];
     f32x16_t s[BL];                                                  // scores of step t
     Frag16 pf[2 * BL];                                               // P of step t - 1, not yet on the sums
 #pragma unroll
     for (int k = 0; k < 2 * BL; k++) pf[k].u = u32x4_t{0u, 0u, 0u, 0u};
+    // Keys of step t + 1 and values of step t - 1 are in LDS when step t begins: step j in place j of R, counted round.
+    auto fill = [&](bool values, int step, int place) __attribute__((always_inline)) {
+        blocks_of(step, at);
+        const uint32_t where = (values ? V0 : K0) + place * T::kHalf;
+        if (values) vs.template ask<true>(at, where, wv, lane), vs.template put<true>(bytes, where, wv, lane, magic);
+        else ks.template ask<false>(at, where, wv, lane), ks.template put<false>(bytes, where, wv, lane, magic);
+    };
     if (steps) {
-        blocks_of(0, g0, at);
-        ks.template ask<false>(at, K0, wv, lane);
-        vs.template ask<true>(at, V0 + T::kHalf, wv, lane);          // (values of "step -1", for a P of zeros: any finite ones)
-        ks.template put<false>(bytes, K0, wv, lane, magic);
-        vs.template put<true>(bytes, V0 + T::kHalf, wv, lane, magic);
-        blocks_of(1, g1, at);
-        ks.template ask<false>(at, K0 + T::kHalf, wv, lane);
-        ks.template put<false>(bytes, K0 + T::kHalf, wv, lane, magic);
+#pragma unroll
+        for (int j = 0; j < R; j++) fill(false, j, j);
+        fill(true, 0, R - 1);                                        // (values of "step -1", for a P of zeros: any finite ones)
+        if constexpr (R == 3) fill(true, 0, 0);
+        if constexpr (QUANT) {                                       // (turned and put into LDS in step 0)
+            blocks_of(2, at);
+            ks.template ask<false>(at, 0, wv, lane);
+            blocks_of(0, at);
+            vs.template ask<true>(at, 0, wv, lane);
+        }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
 #pragma unroll
         for (int b = 0; b < BL; b++)
 #pragma unroll
             for (int k = 0; k < 2 * G; k++) s[b] = mfma32<KIND>(key_at(K0, k, b), qf[k], k ? s[b] : zeros);
-        __syncthreads();                                             // (keys of step 2 go where those of step 0 were)
+        __syncthreads();                                             // (keys of step R go where those of step 0 were)
     }
+    uint32_t ring[R];                                                // places of steps t, t + 1, .. (and t - 1, the last)
+#pragma unroll
+    for (int j = 0; j < R; j++) ring[j] = j * T::kHalf;
     float top = none;
-    // whether some row does not see all of step t's tokens (g0: its pages)
+    // whether some row does not see all of step t's tokens
     auto hides = [&](int t) {
         const int tok = (first + t * BL) * kBlockTokens;
-        return absent(g0) != 0 || tok < all_lo || tok + BL * kBlockTokens - 1 > all_hi;
+        return absent(t) != 0 || tok < all_lo || tok + BL * kBlockTokens - 1 > all_hi;
     };
     // Steps whose rows see everything and whose maxima have grown by less than the lag follow each other in the inner loop; at any other its scores
     // are masked, P that waits is added and the sums are scaled outside of it.  (In a branch of the loop the sums had two homes, 64
     // registers and as many moves.)
     for (int t = 0; t < steps;) {
         if (hides(t)) {
-            const unsigned gone = absent(g0);
+            const unsigned gone = absent(t);
             const int tok = (first + t * BL) * kBlockTokens;
 #pragma unroll
             for (int b = 0; b < BL; b++)
@@ -873,7 +892,7 @@ __global__ __launch_bounds__((64 * TileShape<KIND, G>::kWaves), (G <= 4 ? 2 : 1)
 #pragma unroll
             for (int e = b ? 0 : 1; e < 16; e++) top = fmaxf(top, s[b][e]);
         top = fmaxf(top, other_quarter<32>(top));
-        const uint32_t before = V0 + (t & 1 ? 0 : T::kHalf);
+        const uint32_t before = V0 + ring[R - 1];
 #pragma unroll
         for (int i = 0; i < N; i++) y[i % G] = mfma32<KIND>(value_at(before, i / G, i % G), pf[i / G], y[i % G]);
 #pragma unroll
@@ -890,15 +909,21 @@ __global__ __launch_bounds__((64 * TileShape<KIND, G>::kWaves), (G <= 4 ? 2 : 1)
             // P of step t while the values of step t - 1 are multiplied, and behind that the first scores of step t + 1 (of none: of what is in LDS,
             // and nobody looks at them).  A wave issues in order, and a 32 x 32 instruction takes as long as eight others: the order below puts
             // about a pair's exponentials behind each.
-            const uint32_t odd = t & 1 ? T::kHalf : 0, even = T::kHalf - odd;
-            const Pages g3 = pages_of(t + 3);
-            blocks_of(t + 2, g2, at);
-            ks.template ask<false>(at, K0 + odd, wv, lane);
-            blocks_of(t, g0, at);
-            vs.template ask<true>(at, V0 + odd, wv, lane);
-            constexpr int PAIRS = 8 * BL, EARLY = BL == 2 ? 11 : PAIRS, LOOK = 3;
+            if constexpr (!QUANT) {                                  // past the end they are read from page 0 and nobody looks at them
+                blocks_of(t + R, at);
+                ks.template ask<false>(at, K0 + ring[0], wv, lane);
+                blocks_of(t + R - 2, at);
+                vs.template ask<true>(at, V0 + ring[R - 2], wv, lane);
+            }
+            const uint32_t values_at = V0 + ring[R - 1], keys_at = K0 + ring[1];
+            constexpr int PAIRS = 8 * BL, EARLY = BL == 2 ? 11 : PAIRS, LOOK = 6;
             const float off = kShift - (m == none ? 0.f : m * c);
-            Frag16 frag[N], pn[2 * BL];
+            Frag16 frag[2 * N], pn[2 * BL];
+            // operands in the order of their use: values, then keys of the first block and of the second
+            auto fetch = [&](int i) __attribute__((always_inline)) {
+                if (i < N) frag[i] = value_at(values_at, i / G, i % G);
+                else if (i < 2 * N) frag[i] = key_at(keys_at, (i - N) % (2 * G), (i - N) / (2 * G));
+            };
             float sums[4] = {0.f, 0.f, 0.f, 0.f};
             auto pairs = [&](int from, int to) __attribute__((always_inline)) {
 #pragma unroll
@@ -910,24 +935,32 @@ __global__ __launch_bounds__((64 * TileShape<KIND, G>::kWaves), (G <= 4 ? 2 : 1)
                 }
             };
 #pragma unroll
-            for (int i = 0; i < LOOK; i++) frag[i] = value_at(V0 + even, i / G, i % G);
+            for (int i = 0; i < LOOK; i++) fetch(i);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int i = 0; i < N; i++) {
-                if (i + LOOK < N) frag[i + LOOK] = value_at(V0 + even, (i + LOOK) / G, (i + LOOK) % G);
+                fetch(i + LOOK);
                 y[i % G] = mfma32<KIND>(frag[i], pf[i / G], y[i % G]);
                 pairs(i * EARLY / N, (i + 1) * EARLY / N);
+                if constexpr (QUANT) {                               // what was asked for a step ago, and the next of it
+                    if (i == N / 4) ks.template put<false>(bytes, K0 + ring[0], wv, lane, magic);
+                    if (i == 3 * N / 4) vs.template put<true>(bytes, V0 + ring[0], wv, lane, magic);
+                    if (i == N - 1) {
+                        blocks_of(t + 3, at);
+                        ks.template ask<false>(at, 0, wv, lane);
+                        blocks_of(t + 1, at);
+                        vs.template ask<true>(at, 0, wv, lane);
+                    }
+                }
                 __builtin_amdgcn_sched_barrier(0);
             }
             // scores: all of the first block, then of the second
-#pragma unroll
-            for (int i = 0; i < LOOK; i++) frag[i] = key_at(K0 + even, i % (2 * G), i / (2 * G));
             f32x16_t sn[BL];
 #pragma unroll
             for (int i = 0; i < N; i++) {
                 const int k = i % (2 * G), b = i / (2 * G);
-                if (i + LOOK < N) frag[i + LOOK] = key_at(K0 + even, (i + LOOK) % (2 * G), (i + LOOK) / (2 * G));
-                sn[b] = mfma32<KIND>(frag[i], qf[k], k ? sn[b] : zeros);
+                fetch(N + i + LOOK);
+                sn[b] = mfma32<KIND>(frag[N + i], qf[k], k ? sn[b] : zeros);
                 if (b == 0) pairs(EARLY + k * (PAIRS - EARLY) / (2 * G), EARLY + (k + 1) * (PAIRS - EARLY) / (2 * G));
                 __builtin_amdgcn_sched_barrier(0);
             }
@@ -942,22 +975,25 @@ __global__ __launch_bounds__((64 * TileShape<KIND, G>::kWaves), (G <= 4 ? 2 : 1)
             for (int b = 0; b < BL; b++) s[b] = sn[b];
 #pragma unroll
             for (int k = 0; k < 2 * BL; k++) pf[k] = pn[k];
-            ks.template put<false>(bytes, K0 + odd, wv, lane, magic);
-            vs.template put<true>(bytes, V0 + odd, wv, lane, magic);
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            // what was asked for before this step is there (Q8, Q4: compiler's loads, and it waits for them)
+            if constexpr (!QUANT) asm volatile("s_waitcnt vmcnt(%0)" ::"i"((R - 2) * 2 * Stage<KIND, G>::PER) : "memory");
             __syncthreads();
-            g0 = g1;
-            g1 = g2;
-            g2 = g3;
+            const uint32_t first_place = ring[0];
+#pragma unroll
+            for (int j = 0; j + 1 < R; j++) ring[j] = ring[j + 1];
+            ring[R - 1] = first_place;
             t++;
+            if (t * BL - from_block >= 64) {
+                from_block += 64;
+                near_ids = far_ids;
+                far_ids = pages_from(from_block + 64);
+            }
         } while (t < steps && !hides(t) && !__ballot(top > m + lag));
     }
-    {
-        const uint32_t before = V0 + (steps & 1 ? 0 : T::kHalf);
-        if (steps) {
+    if (steps) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");             // (copies that nobody waited for do not outlive the workgroup's use of LDS)
 #pragma unroll
-            for (int i = 0; i < N; i++) y[i % G] = mfma32<KIND>(value_at(before, i / G, i % G), pf[i / G], y[i % G]);
-        }
+        for (int i = 0; i < N; i++) y[i % G] = mfma32<KIND>(value_at(V0 + ring[R - 1], i / G, i % G), pf[i / G], y[i % G]);
     }
     l += other_quarter<32>(l);
     m = m == none ? none : m * c;
@@ -1042,19 +1078,19 @@ hipError_t attention_as(AttnArgs a, hipStream_t st)
     hipError_t e = hipSuccess;
     const int64_t rows = (int64_t)a.t.rows * a.group, blocks = (int64_t)a.t.table_pages << a.c.page_shift;
     // tiles of all, and the parts beyond one of each: what `target` makes of them, and no more than the table has blocks for
-    auto grid = [&](int64_t tiles) { return (unsigned)(tiles * a.c.kv_heads + std::min<int64_t>(kMostExtra, tiles * a.c.kv_heads * (blocks / a.least))); };
+    auto grid = [&](int64_t tiles, int extra) { return (unsigned)(tiles * a.c.kv_heads + std::min<int64_t>(extra, tiles * a.c.kv_heads * (blocks / a.least))); };
     if (!many || a.few) {
         a.target = kTarget;
         a.least = kLeast;
         a.rounds = kRounds;
         const int64_t tiles = std::min(rows / kRows + a.t.seqs, a.few ? (int64_t)a.t.seqs * ((kFewRows + kRows - 1) / kRows) : rows);
-        e = rows_as<KIND, G>(a, grid(tiles), st);
+        e = rows_as<KIND, G>(a, grid(tiles, kMostExtra), st);
     }
     if (many && e == hipSuccess) {
         a.target = TileShape<KIND, G>::kTarget;
         a.least = kTileLeast;
         a.rounds = kTileRounds;
-        e = tiles_as<KIND, G>(a, grid(rows / TileShape<KIND, G>::kRows + a.t.seqs), st);
+        e = tiles_as<KIND, G>(a, grid(rows / TileShape<KIND, G>::kRows + a.t.seqs, TileShape<KIND, G>::kMostExtra), st);
     }
     return e;
 }
@@ -1062,21 +1098,30 @@ hipError_t attention_as(AttnArgs a, hipStream_t st)
 }  // namespace
 
 // Parts of tiles that have more than one: at most twice those beyond one of each tile
-static_assert(2 * kMostExtra * sizeof(unsigned) <= kAttnTicketBytes, "a ticket per tile");
-
 int64_t attention_max_units() { return kMaxUnits; }
 
 size_t attention_scratch_bytes(int dim)
 {
-    // (the tiles kernel's: 2 * 1024 parts of 128 rows, or 2 * 512 of 256 or of rows of 256)
-    const size_t rows = (size_t)2 * kMostExtra * kRows, tile_rows = (size_t)2 * kMostExtra * (dim <= 128 ? 128 : 64);
-    return std::max(rows, tile_rows) * ((size_t)dim + 2) * sizeof(float);
+    const size_t rows = (size_t)2 * kMostExtra * kRows * (dim + 2);
+    auto tiles = [](int extra, int slab) { return (size_t)2 * extra * slab; };
+    size_t many;
+    switch (dim) {                                                   // (the quantised kinds have half as many parts of twice the rows, or fewer)
+        case 64: many = tiles(TileShape<kCacheF16, 2>::kMostExtra, TileShape<kCacheF16, 2>::kSlab); break;
+        case 96: many = tiles(TileShape<kCacheF16, 3>::kMostExtra, TileShape<kCacheF16, 3>::kSlab); break;
+        case 128: many = tiles(TileShape<kCacheF16, 4>::kMostExtra, TileShape<kCacheF16, 4>::kSlab); break;
+        default: many = tiles(TileShape<kCacheF16, 8>::kMostExtra, TileShape<kCacheF16, 8>::kSlab); break;
+    }
+    return std::max(rows, many) * sizeof(float);
 }
+template <int G>
+constexpr bool kPartsFit = TileShape<kCacheQ8, G>::kMostExtra * TileShape<kCacheQ8, G>::kSlab <= TileShape<kCacheF16, G>::kMostExtra * TileShape<kCacheF16, G>::kSlab;
+static_assert(kPartsFit<2> && kPartsFit<3> && kPartsFit<4> && kPartsFit<8>, "parts of all kinds fit the scratch");
+static_assert(2 * std::max(kMostExtra, TileShape<kCacheF16, 2>::kMostExtra) * sizeof(unsigned) <= kAttnTicketBytes, "a ticket per tile");
 
 int64_t attention_units_max(const BatchView& t, int kv_heads, int group)
 {
     // tiles: (n * group + 15) / 16 of a sequence; parts: at most target more than tiles
-    return ((int64_t)t.rows * group / kRows + t.seqs) * kv_heads + kMostExtra;
+    return ((int64_t)t.rows * group / kRows + t.seqs) * kv_heads + std::max(kMostExtra, TileShape<kCacheF16, 2>::kMostExtra);
 }
 
 hipError_t launch_attention(const CacheView& c, const BatchView& t, const void* q, int64_t q_stride, int qdt, int group, float scale, int window, void* y,
