@@ -615,292 +615,6 @@ struct TileShape {
     // Waves, each with 32 rows: eight where they share the work of unpacking (Q8, Q4: 216 us instead of 308 for 512 rows after 16384 tokens) or where
     // three steps of copies fit a CU once only (heads of 128: 2040 us instead of 2150 for 4096 rows after 28672 tokens); else four, in more workgroups
     // (heads of 64: 62 us instead of 69 for 2000 rows)
-    static constexpr int kWaves = 4;
-    static constexpr int kLds = kWaves * 2 * G * 64 * 16 + kWaves * 32 * 4;
-    static constexpr int kSlab = kRows * 32 * G + 2 * kRows;                  // floats of a part: its rows, and their maxima and sums in pairs
-};
-
-template <int KIND, int G>
-__global__ __launch_bounds__(64 * RowsShape<G>::kWaves, G <= 4 ? 2 : 1) void attention_rows_kernel(AttnArgs a)
-{
-    constexpr int kWaves = RowsShape<G>::kWaves;
-    constexpr int DIM = 32 * G, BLOCK = cache_block_bytes(KIND, DIM), HALF = cache_half_bytes(KIND, DIM), DT = 2 * G;
-    constexpr bool SPLIT_P = KIND == kCacheBF16;
-    constexpr float kShift = SPLIT_P ? 0.f : kShiftF16, kLag = SPLIT_P ? kLagBF16 : kLagF16;
-    extern __shared__ float4_t lds[];                                 // [waves][DT][64], then [waves][16] maxima and sums
-    float* const stats = reinterpret_cast<float*>(lds + kWaves * DT * 64);
-    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q4 = lane >> 4, r = lane & 15;
-    const uint32_t magic = q4_magic_vgpr();
-    Unit u;
-    if (!find_unit<kRows, false>(a, blockIdx.x, &u)) return;
-    const int64_t capacity = (int64_t)a.t.table_pages << (a.c.page_shift + 5);
-    const int r0 = u.tile * kRows, rows = min(kRows, u.s.n * a.group - r0);
-    const int p0 = u.s.len - u.s.n, i_first = r0 / a.group, i_last = (r0 + rows - 1) / a.group;
-    int lo, hi;
-    seen(a, p0 + i_first, p0 + i_last, capacity, &lo, &hi);
-    const int each = (hi - lo) / u.splits, more = (hi - lo) % u.splits;
-    const int first = lo + u.split * each + min(u.split, more), last = first + each + (u.split < more ? 1 : 0);
-    // my row
-    const bool real = r < rows;
-    const int i = (r0 + (real ? r : 0)) / a.group, in_group = (r0 + (real ? r : 0)) - i * a.group;
-    const int p = p0 + i;
-    const int row_hi = real ? (int)min((int64_t)p, capacity - 1) : -1;
-    const int row_lo = a.window && p >= a.window ? p - a.window + 1 : 0;
-    const int all_hi = (int)min((int64_t)(p0 + i_first), capacity - 1);                       // every real row sees all of all_lo .. all_hi
-    const int all_lo = a.window && p0 + i_last >= a.window ? p0 + i_last - a.window + 1 : 0;
-    const int head = u.head * a.group + in_group;
-    Frag16 qf[G];
-    float c = a.scale;
-    {
-        const uint16_t* q = static_cast<const uint16_t*>(a.q) + (int64_t)(u.s.row0 + i) * a.q_stride + head * DIM + 8 * q4;
-#pragma unroll
-        for (int g = 0; g < G; g++) qf[g].u = real ? *reinterpret_cast<const u32x4_t*>(q + 32 * g) : u32x4_t{0u, 0u, 0u, 0u};
-        if (cache_quantised(KIND) && a.qdt == kBF16) {                // to f16: the row's largest at 2^14 .. 2^15
-            float x[8 * G], top = 0.f;
-#pragma unroll
-            for (int e = 0; e < 8 * G; e++) {
-                const uint32_t w = qf[e >> 3].u[(e & 7) >> 1];
-                x[e] = __builtin_bit_cast(float, e & 1 ? w & 0xffff0000u : w << 16);
-                top = fmaxf(top, fabsf(x[e]));
-            }
-            top = fmaxf(top, other_quarter<16>(top));
-            top = fmaxf(top, other_quarter<32>(top));
-            const float f = row_power(top, &c);
-#pragma unroll
-            for (int g = 0; g < G; g++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) qf[g].u[j] = pack_half2(x[8 * g + 2 * j] * f, x[8 * g + 2 * j + 1] * f);
-        }
-    }
-    const float lag = fminf(kLag / c, 1e30f);
-    // my blocks are first + wv + kWaves i; a lane asks for the page of one of 64 of them, those that have one are worked on
-    const int32_t* const table = a.t.tables + (int64_t)u.b * a.t.table_pages;
-    const int in_page = (1 << a.c.page_shift) - 1;
-    int base = first + wv, page = -1;
-    uint64_t there = 0;
-    auto look_up = [&]() {
-        for (; base < last; base += 64 * kWaves) {
-            const int blk = base + lane * kWaves;
-            page = blk < last ? table[blk >> a.c.page_shift] : -1;
-            there = __ballot((unsigned)page < (unsigned)a.c.pages);
-            if (there) return;
-        }
-    };
-    auto next_block = [&](int* blk) -> const uint8_t* {
-        if (!there) {
-            base += 64 * kWaves;
-            look_up();
-            if (!there) return nullptr;
-        }
-        const int l = __builtin_ctzll(there);
-        there &= there - 1;
-        *blk = base + l * kWaves;
-        const int id = __builtin_amdgcn_readlane(page, l);
-        return a.c.base + id * a.c.page_bytes + (int64_t)((u.head << a.c.page_shift) + (*blk & in_page)) * BLOCK;
-    };
-    float4_t y[DT];
-#pragma unroll
-    for (int d = 0; d < DT; d++) y[d] = float4_t{0.f, 0.f, 0.f, 0.f};
-    const float none = -__builtin_inff();
-    float m = none, l = 0.f;                                          // m: of scores without their factor
-    Half<KIND, G> k0, v0, k1, v1;
-    int blk = 0;
-    look_up();
-    const uint8_t* at = there ? next_block(&blk) : nullptr;
-    if (at) {
-        k0.load(at, lane);
-        v0.load(at + HALF, lane);
-    }
-    // one block; the next one's keys and values go to nk, nv
-    auto work = [&](const Half<KIND, G>& k, const Half<KIND, G>& v, Half<KIND, G>& nk, Half<KIND, G>& nv) __attribute__((always_inline)) {
-        int next_blk = 0;
-        const uint8_t* const next = next_block(&next_blk);
-        if (next) {
-            nk.load(next, lane);
-            nv.load(next + HALF, lane);
-        }
-        float4_t s[2];
-#pragma unroll
-        for (int t = 0; t < 2; t++) {
-            s[t] = float4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int g = 0; g < G; g++) {
-                const Frag16 kf = key_operand<KIND, G>(k, t, g, magic);
-                if constexpr (cache_quantised(KIND)) {
-                    const float4_t part = mfma16<KIND>(kf, qf[g], float4_t{0.f, 0.f, 0.f, 0.f});
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const half2_t sc = as_h2(k.s[g][2 * t + (e >> 1)]);
-                        s[t][e] = __builtin_fmaf((float)sc[e & 1], part[e], s[t][e]);
-                    }
-                } else {
-                    s[t] = mfma16<KIND>(kf, qf[g], s[t]);
-                }
-            }
-        }
-        const int tok = blk * kBlockTokens + 16 * (q4 >> 1) + 4 * (q4 & 1);
-        if (blk * kBlockTokens < all_lo || blk * kBlockTokens + 31 > all_hi) {
-#pragma unroll
-            for (int t = 0; t < 2; t++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const int j = tok + 8 * t + e;
-                    if (j < row_lo || j > row_hi) s[t][e] = none;
-                }
-        }
-        float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
-        top = fmaxf(top, other_quarter<16>(top));
-        top = fmaxf(top, other_quarter<32>(top));
-        if (__ballot(top > m + lag)) {
-            const float now = top > m + lag ? top : m;
-            const float f = m == none ? 0.f : exp2_fast((m - now) * c);
-            m = now;
-            l *= f;
-#pragma unroll
-            for (int d = 0; d < DT; d++) y[d] *= f;
-        }
-        const float off = kShift - (m == none ? 0.f : m * c);
-        Frag16 ph, pl;
-        float pr[8];
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            pr[e] = exp2_fast(__builtin_fmaf(s[e >> 2][e & 3], c, off));
-            l += pr[e];
-        }
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            if constexpr (SPLIT_P) {
-                ph.u[j] = pack_bf16x2(pr[2 * j], pr[2 * j + 1]);
-                pl.u[j] = pack_bf16x2(pr[2 * j] - __builtin_bit_cast(float, ph.u[j] << 16), pr[2 * j + 1] - __builtin_bit_cast(float, ph.u[j] & 0xffff0000u));
-            } else {
-                ph.u[j] = pack_half2(pr[2 * j], pr[2 * j + 1]);
-            }
-        }
-#pragma unroll
-        for (int d = 0; d < DT; d++) {
-            const Frag16 vf = value_operand<KIND, G>(v, d, magic);
-            y[d] = mfma16<KIND>(vf, ph, y[d]);
-            if constexpr (SPLIT_P) y[d] = mfma16<KIND>(vf, pl, y[d]);
-        }
-        at = next;
-        blk = next_blk;
-    };
-    while (at) {
-        work(k0, v0, k1, v1);
-        if (!at) break;
-        work(k1, v1, k0, v0);
-    }
-    l += other_quarter<16>(l);
-    l += other_quarter<32>(l);
-    // waves meet
-    if (lane < 16) {
-        stats[wv * 16 + lane] = m * c;
-        stats[kWaves * 16 + wv * 16 + lane] = l;
-    }
-#pragma unroll
-    for (int d = 0; d < DT; d++) lds[(wv * DT + d) * 64 + lane] = y[d];
-    __syncthreads();
-    float top = none, sum = 0.f, f[kWaves];
-#pragma unroll
-    for (int w = 0; w < kWaves; w++) top = fmaxf(top, stats[w * 16 + r]);
-#pragma unroll
-    for (int w = 0; w < kWaves; w++) {
-        const float mw = stats[w * 16 + r];
-        f[w] = mw == none ? 0.f : exp2_fast(mw - top);
-        sum += f[w] * stats[kWaves * 16 + w * 16 + r];                // (a row of NaN has a sum of NaN and no maximum)
-    }
-    const int64_t row_at = ((int64_t)(u.s.row0 + i) * a.c.kv_heads * a.group + head) * DIM + 4 * q4;
-    constexpr int SLAB = RowsShape<G>::kSlab;
-    float* const slab = a.slabs + (size_t)u.slab * SLAB;
-    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-    for (int d = wv; d < DT; d += kWaves) {
-        float4_t o = lds[d * 64 + lane] * f[0];                       // (sums of a wave without a maximum are zeros, or its row is NaN)
-#pragma unroll
-        for (int w = 1; w < kWaves; w++) o += lds[(w * DT + d) * 64 + lane] * f[w];
-        if (!real) continue;
-        if (u.splits == 1) store_row4(a.y, a.qdt, row_at + 16 * d, o * inv);
-        else put_float4(slab + r * DIM + 16 * d + 4 * q4, o);
-    }
-    if (u.splits == 1) return;
-    if (threadIdx.x < 16) put_float2(slab + kRows * DIM + 2 * r, top, sum);
-    if (!last_part(a, u, reinterpret_cast<unsigned*>(lds))) return;
-    // The rows of all parts: threads share out the rows' float4s, and the parts where there are more threads; everything is asked for at once.
-    constexpr int THREADS = 64 * kWaves, QUADS = DIM / 4, AHEAD = 8;
-    const int items = rows * QUADS, runs = max(1, THREADS / items);
-    const float* const of_tile = slab - (size_t)u.split * SLAB;
-    for (int it0 = 0; it0 < items; it0 += THREADS) {                  // (one round for up to 8 rows of 128)
-        const int run = runs == 1 ? 0 : threadIdx.x / items, it = it0 + threadIdx.x - run * items;
-        const bool mine = it < items && run < runs;
-        const int row = mine ? it / QUADS : 0, quad = mine ? it - row * QUADS : 0;
-        float m2 = none, l2 = 0.f;
-        float4_t o = {0.f, 0.f, 0.f, 0.f};
-        for (int e0 = run; e0 < u.splits && mine; e0 += AHEAD * runs) {
-            float4_t part[AHEAD];
-            f32x2_t of[AHEAD];
-#pragma unroll
-            for (int e = 0; e < AHEAD; e++) {
-                const float* const from = of_tile + (size_t)min(e0 + e * runs, u.splits - 1) * SLAB;
-                part[e] = get_float4(from + row * DIM + 4 * quad);
-                of[e] = get_float2(from + kRows * DIM + 2 * row);
-            }
-            float now = m2;
-#pragma unroll
-            for (int e = 0; e < AHEAD; e++) now = fmaxf(now, of[e][0]);
-            const float old = m2 == none ? 0.f : exp2_fast(m2 - now);
-            o *= old;
-            l2 *= old;
-            m2 = now;
-#pragma unroll
-            for (int e = 0; e < AHEAD; e++) {
-                const float fe = of[e][0] == none || e0 + e * runs >= u.splits ? 0.f : exp2_fast(of[e][0] - now);
-                o += part[e] * fe;
-                l2 += e0 + e * runs >= u.splits ? 0.f : of[e][1] * fe;
-            }
-        }
-        if (runs > 1) {                                              // (all in one round)
-            float* const pairs = reinterpret_cast<float*>(lds + THREADS);
-            lds[threadIdx.x] = o;
-            pairs[2 * threadIdx.x] = m2;
-            pairs[2 * threadIdx.x + 1] = l2;
-            __syncthreads();
-            if (run) return;
-            for (int e = 1; e < runs; e++) {
-                const int at = threadIdx.x + e * items;
-                const float me = pairs[2 * at], now = fmaxf(m2, me);
-                const float fo = m2 == none ? 0.f : exp2_fast(m2 - now), fe = me == none ? 0.f : exp2_fast(me - now);
-                o = o * fo + lds[at] * fe;
-                l2 = l2 * fo + pairs[2 * at + 1] * fe;
-                m2 = now;
-            }
-        }
-        if (!mine) continue;
-        const int at = r0 + row, of_token = at / a.group;
-        const float by = l2 == 0.f ? 0.f : 1.0f / l2;
-        store_row4(a.y, a.qdt, (((int64_t)u.s.row0 + of_token) * a.c.kv_heads * a.group + u.head * a.group + at - of_token * a.group) * DIM + 4 * quad, o * by);
-    }
-}
-
-// ---- many rows ------------------------------------------------------------------------------------------------
-
-typedef float f32x16_t __attribute__((ext_vector_type(16)));
-
-template <int KIND>
-__device__ __forceinline__ f32x16_t mfma32(Frag16 a, Frag16 b, f32x16_t c)
-{
-    if constexpr (KIND == kCacheBF16) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.b, b.b, c, 0, 0, 0);
-    else return __builtin_amdgcn_mfma_f32_32x32x16_f16(a.h, b.h, c, 0, 0, 0);
-}
-
-// 16 bytes per lane from base + off (the lane's own) to LDS bytes lds_off + 16 * lane, past the registers
-__device__ __forceinline__ void copy_to_lds(uint32_t lds_off, const void* base, uint32_t off)
-{
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(lds_off)), "v"(off), "s"(base));
-}
-
-template <int KIND, int G>
-struct TileShape {
-    static constexpr int kBlocks = G <= 4 ? 2 : 1;            // blocks of a step
-    // waves, each with 32 rows: two workgroups of four to a CU, or eight that share the work of unpacking
     static constexpr int kWaves = G <= 4 && (cache_quantised(KIND) || G >= 3) ? 8 : 4;
     static constexpr int kRows = 32 * kWaves;
     // Steps of keys, and of values, that LDS holds: three, so that copies have two steps to arrive in; quantised bytes wait in registers instead
