@@ -7,15 +7,16 @@ piece, then `Answer { tokens, tok_per_s, tok_in_s, tok_out_s, .. }`
 (/root/reference/shell/src/worlds/soma_bridge.rs:252-277); the UI keeps running
 means of `tok_in_s` / `tok_out_s` (/root/reference/shell/src/worlds/models/mod.rs:44-52)
 and compares them with `SPEED_ANCHORS` (same file, :116).  This module walks the
-same two phases over the quantised linears only (and, with --experts, over the router and the experts of every layer):
+same two phases over the quantised linears only (with --experts, over the router and the experts of every layer too; with
+--cache, over whole layers: norms, RoPE, the paged cache and its attention among them):
 
   prefill  the prompt in chunks of `chunk` tokens, every chunk one pass of
            `cybq_matmul_many` over the stack with bf16 activations (M = chunk),
   decode   one pass per new token with f16 activations (M = batch).
 
-Attention, norms, RoPE, sampling and the tokenizer are not part of the path, so the
-rates are those of the weight-bound part of a step; they are upper bounds for a
-whole model.  Nothing is computed on the host.
+With a cache each of the `batch` conversations reads the prompt and keeps it.  Without one, attention, norms
+and RoPE are not part of the path, so the rates are those of the weight-bound part of a step; they are upper
+bounds for a whole model.  Sampling and the tokenizer never are.  Nothing is computed on the host.
 """
 from __future__ import annotations
 
@@ -37,13 +38,19 @@ class Answer:
 
 def ask(backend: Backend, st, prompt_tokens: int, new_tokens: int, chunk: int = 512,
         batch: int = 1, shapes: Optional[Dict[str, tuple]] = None, stream: int = 0) -> Iterator[dict]:
-    """Walks a LinearStack or an ExpertStack.  Yields {"Prefill": {"done", "total"}} per chunk, {"Delta": i} per decode step and finally
+    """Walks a LinearStack, an ExpertStack or a CachedStack.  Yields {"Prefill": {"done", "total"}} per chunk, {"Delta": i} per decode step and finally
     {"Answer": Answer}.  Device work is timed with events on the launch stream."""
     import torch
     if prompt_tokens < 0 or new_tokens < 0 or chunk < 1 or batch < 1 or batch > 16:
         raise ValueError("prompt_tokens, new_tokens >= 0; chunk >= 1; 1 <= batch <= 16")
+    cached = isinstance(st, stk.CachedStack)
+    if cached:
+        if batch > st.conversations or prompt_tokens + new_tokens + 1 > st.context:
+            raise ValueError("the cache has fewer conversations, or pages for fewer tokens")
+        st.set_lengths(0)
+    read = prompt_tokens * batch if cached else prompt_tokens
     t_wall = time.time()
-    yield {"Prefill": {"done": 0, "total": prompt_tokens}}
+    yield {"Prefill": {"done": 0, "total": read}}
     ms_in = 0.0
     steps = {}
 
@@ -53,23 +60,25 @@ def ask(backend: Backend, st, prompt_tokens: int, new_tokens: int, chunk: int = 
         return steps[M]
 
     done = 0
-    while done < prompt_tokens:
-        M = min(chunk, prompt_tokens - done)
+    while done < read:
+        M = min(chunk, prompt_tokens - done % prompt_tokens)
         step = step_for(M, torch.bfloat16 if M > 16 else torch.float16)
         a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
         a.record()
-        step(stream)
+        step(stream, done // prompt_tokens) if cached else step(stream)
         b.record()
         b.synchronize()
         ms_in += a.elapsed_time(b)
         done += M
-        yield {"Prefill": {"done": done, "total": prompt_tokens}}
+        yield {"Prefill": {"done": done, "total": read}}
 
     ms_out = 0.0
     if new_tokens:
-        step = step_for(batch, torch.float16)
+        step = st.stepper(batch, torch.float16, count=batch) if cached else step_for(batch, torch.float16)
         step(stream)                                           # first touch of this plan's buffers, untimed
         torch.cuda.synchronize()
+        if cached:
+            st.set_lengths(prompt_tokens, batch)
         a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
         a.record()
         for i in range(new_tokens):
@@ -81,8 +90,8 @@ def ask(backend: Backend, st, prompt_tokens: int, new_tokens: int, chunk: int = 
             yield {"Delta": i}
     wall = max(time.time() - t_wall, 1e-9)
     yield {"Answer": Answer(tokens=new_tokens * batch,
-                            tok_per_s=(prompt_tokens + new_tokens * batch) / wall,
-                            tok_in_s=prompt_tokens / (ms_in * 1e-3) if ms_in else 0.0,
+                            tok_per_s=(read + new_tokens * batch) / wall,
+                            tok_in_s=read / (ms_in * 1e-3) if ms_in else 0.0,
                             tok_out_s=new_tokens * batch / (ms_out * 1e-3) if ms_out else 0.0)}
 
 
@@ -98,13 +107,20 @@ def main(argv=None) -> int:
     ap.add_argument("--epilogues", action="store_true", help="SwiGLU and residual adds fused into the linears")
     ap.add_argument("--experts", type=int, default=0, help="FFNs of this many experts (hidden 2048, width 768) instead of the Llama-3-8B shapes")
     ap.add_argument("--top-k", type=int, default=8, help="experts per token")
+    ap.add_argument("--cache", choices=["f16", "bf16", "q8", "q4"], help="whole layers, with a cache of this kind")
+    ap.add_argument("--window", type=int, default=0, help="tokens that attention looks back at (with --cache; 0: all)")
     args = ap.parse_args(argv)
+    if args.cache and (args.experts or args.separate):
+        ap.error("--cache walks whole layers of the Llama-3-8B shapes")
     import torch
     torch.cuda.init()          # torch brings its own HIP runtime: let it find the device before libcybq does
     be = Backend(0)
     shapes = None if args.separate else stk.fused_shapes()
     if args.experts:
         st = stk.build_experts(be, layers=args.layers, experts=args.experts, top_k=args.top_k)
+    elif args.cache:
+        st = stk.build_cached(be, layers=args.layers, kind=args.cache, conversations=args.batch, context=args.prompt + args.new + 1,
+                              window=args.window)
     else:
         st = stk.build(be, layers=args.layers, shapes=shapes, order=list(shapes) if shapes else None,
                        epilogues=args.epilogues and shapes is not None)

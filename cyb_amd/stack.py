@@ -6,8 +6,9 @@ proj -> residual -> norm -> FFN -> residual" x layers -
 /root/reference/decide/pipeline.md:51).  This module builds that list of graph
 nodes for a random-init Llama-3-8B-shaped model and runs it through
 `cybq_matmul_many`.  The glue between the linears (norm, RoPE, attention,
-SwiGLU) is not part of the path: every linear reads a fresh seeded N(0,1) f16
-input of its width, so each output can be checked on its own.
+SwiGLU) is not part of LinearStack's path: every linear reads a fresh seeded N(0,1) f16
+input of its width, so each output can be checked on its own.  CachedStack runs whole
+layers, the cache and its attention among them.
 
 Weights are generated and quantised on the device (torch.randn ->
 cybq_quantize -> cybq_weight_from_device): 7 B weights never exist on the host.
@@ -15,10 +16,10 @@ cybq_quantize -> cybq_weight_from_device): 7 B weights never exist on the host.
 from __future__ import annotations
 
 from dataclasses import dataclass, field
-from typing import Dict, List
+from typing import Dict, List, Optional
 
 from . import formats, synth
-from .backend import Backend, CybqError, QMatMul, QWeight
+from .backend import Backend, CybqError, KVCache, QMatMul, QWeight
 
 LINEAR_ORDER = ["q_proj", "k_proj", "v_proj", "o_proj", "gate_proj", "up_proj", "down_proj"]
 _PREFIX = {"q_proj": "self_attn", "k_proj": "self_attn", "v_proj": "self_attn", "o_proj": "self_attn",
@@ -152,7 +153,7 @@ def plan(stack: LinearStack, edges):
 
 def stepper(stack, M: int, shapes: Dict[str, tuple] = None, xdtype=None):
     """One step of M rows as a call: step(stream).  The plan and its buffers live as long as the call does."""
-    if isinstance(stack, ExpertStack):
+    if isinstance(stack, (ExpertStack, CachedStack)):
         return stack.stepper(M, xdtype)
     edges = edges_for(stack, M, shapes=shapes, xdtype=xdtype)
     p = plan(stack, edges)
@@ -253,4 +254,134 @@ def build_experts(backend: Backend, layers: int = 4, bits: int = formats.Q4, exp
         gate.free()
         up.free()
         st.down.append(tensor(bits, experts * hidden, width, f"model.layers.{i}.mlp.experts.down_proj.weight"))
+    return st
+
+
+@dataclass
+class CachedStack:
+    """Whole decoder layers of `conversations` conversations: the fused linears with their norms and epilogues, RoPE, the paged cache and its
+    attention; hidden rows in, hidden rows out.  Conversation c's pages are its own, shuffled over the cache; its length is on the device."""
+    backend: Backend
+    layers: int
+    bits: int
+    hidden: int
+    heads: int
+    kv_heads: int
+    head_dim: int
+    context: int                # tokens a conversation has pages for
+    window: int
+    cache: KVCache
+    tables: object              # int32 [conversations, pages of one]
+    lengths: object             # int32 [conversations]
+    rope: object                # fp32 [context, head_dim / 2, 2]
+    eps: float = 1e-5
+    qkv: List[QWeight] = field(default_factory=list)
+    o: List[QWeight] = field(default_factory=list)
+    gate_up: List[QWeight] = field(default_factory=list)      # fuse_pairs
+    down: List[QWeight] = field(default_factory=list)
+    norms: List[tuple] = field(default_factory=list)          # gammas in front of qkv and of gate_up
+
+    @property
+    def weights(self) -> List[QWeight]:
+        return self.qkv + self.o + self.gate_up + self.down
+
+    @property
+    def weight_bytes(self) -> int:
+        return sum(w.algorithmic_bytes for w in self.weights)
+
+    @property
+    def nodes(self) -> List[str]:
+        """The calls of one step."""
+        return ["qkv", "append", "attention", "o", "gate_up", "down"] * self.layers
+
+    @property
+    def conversations(self) -> int:
+        return self.tables.shape[0]
+
+    def set_lengths(self, tokens: int, count: Optional[int] = None) -> None:
+        """The first `count` conversations (None: all) hold their first `tokens` tokens (0: they begin again)."""
+        self.lengths[:count].fill_(tokens)
+
+    def stepper(self, M: int, xdtype=None, count: int = 1, seed: int = 5):
+        """step(stream, first): M new tokens, M / count for each of the conversations first .. first + count.  Tokens behind a conversation's
+        pages are not stored: counting them is the caller's affair."""
+        import torch
+        if count < 1 or M % count:
+            raise CybqError(-2, "bad shape", "the rows are shared by the conversations evenly")
+        xdtype = xdtype or torch.float16
+        be, dev, n = self.backend, f"cuda:{self.backend.device}", M // count
+        qdtype = {"f16": torch.float16, "bf16": torch.bfloat16}.get(self.cache.kind, xdtype)
+        heads, kvh, dim = self.heads, self.kv_heads, self.head_dim
+
+        def rows(cols, dtype=xdtype):
+            return torch.empty((M, cols), dtype=dtype, device=dev)
+        b = {"x": torch.from_numpy(synth.activations(seed, M, self.hidden)).to(dev).to(xdtype), "qkv": rows((heads + 2 * kvh) * dim),
+             "q": rows(heads * dim, qdtype).view(M, heads, dim), "attn": rows(heads * dim, qdtype), "mid": rows(self.hidden),
+             "h": rows(self.down[0].K), "y": rows(self.hidden)}
+        q, k, v = b["qkv"].view(M, heads + 2 * kvh, dim).split([heads, kvh, kvh], dim=1)
+        starts = torch.arange(0, M + 1, n, dtype=torch.int32, device=dev)
+        batches = {}
+
+        def step(stream: int = 0, first: int = 0) -> None:
+            if first not in batches:
+                if not 0 <= first <= self.conversations - count:
+                    raise CybqError(-1, "invalid argument", "no such conversations")
+                batches[first] = be.cache_batch(starts, self.lengths[first:first + count], self.tables[first:first + count], M, n)
+            batch, x = batches[first], b["x"]
+            with torch.cuda.stream(torch.cuda.ExternalStream(stream) if stream else torch.cuda.default_stream(be.device)):
+                batch.keep[1].add_(n)
+            for i in range(self.layers):
+                be.matmul_norm(self.qkv[i], x, self.norms[i][0], self.eps, b["qkv"], stream=stream)
+                be.cache_append(self.cache, i, batch, q, k, v, b["q"], self.rope, stream=stream)
+                be.attention(self.cache, i, batch, b["q"], b["attn"].view(M, heads, dim), window=self.window, stream=stream)
+                be.matmul_ex(self.o[i], b["attn"], b["mid"], "add", x, stream=stream)
+                be.matmul_norm(self.gate_up[i], b["mid"], self.norms[i][1], self.eps, b["h"], "swiglu", stream=stream)
+                be.matmul_ex(self.down[i], b["h"], b["y"], "add", b["mid"], stream=stream)
+                x = b["y"]
+        step.edges = b
+        return step
+
+    def free(self) -> None:
+        for w in self.weights:
+            w.free()
+        self.cache.free()
+
+
+def build_cached(backend: Backend, layers: int = 32, bits: int = formats.Q4, kind: str = "q8", conversations: int = 1, context: int = 4096,
+                 heads: int = 32, kv_heads: int = 8, head_dim: int = 128, width: int = 14336, page: int = 64, window: int = 0,
+                 base: float = 500000.0, seed: int = 5) -> CachedStack:
+    """Random-init stack of whole layers (Llama-3-8B shapes unless told otherwise; hidden = heads * head_dim) with N(0, 0.02) weights
+    quantised on the device, gammas 1 +- 0.1, and an empty cache of `kind` for `conversations` conversations of `context` tokens."""
+    import torch
+    hidden = heads * head_dim
+    if context < 1 or conversations < 1 or width % 32 or kv_heads < 1 or heads % kv_heads:
+        raise CybqError(-2, "bad shape", "width must be a multiple of 32, heads one of kv_heads, context and conversations at least 1")
+    dev, per = f"cuda:{backend.device}", -(-context // page)
+    gen = torch.Generator(device=dev)
+    gen.manual_seed((synth.BASE_SEED ^ seed) & 0x7FFFFFFF)
+    shuffled = torch.randperm(conversations * per, generator=gen, device=dev).to(torch.int32).view(conversations, per)
+    angle = torch.arange(per * page, dtype=torch.float64, device=dev).unsqueeze(1) * base ** (
+        -torch.arange(0, head_dim, 2, dtype=torch.float64, device=dev) / head_dim)
+    st = CachedStack(backend, layers, bits, hidden, heads, kv_heads, head_dim, context, window,
+                     backend.kv_cache(kind, layers, kv_heads, head_dim, page, conversations * per), shuffled,
+                     torch.zeros(conversations, dtype=torch.int32, device=dev), torch.stack([angle.cos(), angle.sin()], dim=2).float())
+
+    def tensor(N: int, K: int, name: str = None) -> QWeight:
+        w = torch.empty((N, K), dtype=torch.float32, device=dev).normal_(0.0, 0.02, generator=gen)
+        q = torch.empty(N * K * bits // 8, dtype=torch.uint8, device=dev)
+        s = torch.empty(N * (K // 32), dtype=torch.int16, device=dev)
+        backend.quantize(bits, w, N, K, q, s)
+        out = backend.weight_from_device(bits, N, K, q, s, name=name)
+        torch.cuda.synchronize()                                      # w, q and s are released
+        return out
+
+    for i in range(layers):
+        st.qkv.append(tensor((heads + 2 * kv_heads) * head_dim, hidden, tensor_name(i, "qkv_proj")))
+        st.o.append(tensor(hidden, hidden, tensor_name(i, "o_proj")))
+        gate, up = tensor(width, hidden), tensor(width, hidden)
+        st.gate_up.append(backend.fuse_pairs(gate, up, name=tensor_name(i, "gate_up_proj")))
+        gate.free()
+        up.free()
+        st.down.append(tensor(hidden, width, tensor_name(i, "down_proj")))
+        st.norms.append(tuple((1.0 + 0.1 * torch.empty(hidden, device=dev).normal_(generator=gen)).half() for _ in range(2)))
     return st

@@ -81,6 +81,29 @@ private:
     cybq_weight* h_ = nullptr;
 };
 
+// The paged keys and values of a model's layers.  Its Backend outlives it.
+class Cache {
+public:
+    Cache() = default;
+    Cache(const Cache&) = delete;
+    Cache& operator=(const Cache&) = delete;
+    Cache(Cache&& o) noexcept { *this = std::move(o); }
+    Cache& operator=(Cache&& o) noexcept
+    {
+        if (this != &o) { reset(); ctx_ = o.ctx_; h_ = o.h_; o.h_ = nullptr; }
+        return *this;
+    }
+    ~Cache() { reset(); }
+    cybq_cache* get() const { return h_; }
+    explicit operator bool() const { return h_ != nullptr; }
+    void reset() { if (h_) { cybq_cache_free(ctx_, h_); h_ = nullptr; } }
+
+private:
+    friend class Backend;
+    cybq_ctx* ctx_ = nullptr;
+    cybq_cache* h_ = nullptr;
+};
+
 class Backend {
 public:
     // never throws: check ok() / status()
@@ -160,6 +183,31 @@ public:
                               const float* weights, const void* residual, void* y, cybq_dtype ydt, void* stream = nullptr)
     {
         return wrap(cybq_matmul_experts_sum(ctx_, w.get(), E, x, xdt, T, top_k, ids, weights, residual, y, ydt, stream));
+    }
+    // paged key-value cache: created once per model, then per layer and step append and attention (the batch's arrays on the device)
+    Status make_cache(cybq_cache_kind kind, int64_t layers, int64_t kv_heads, int64_t head_dim, int64_t page_tokens, int64_t pages, Cache& out)
+    {
+        Cache c;
+        c.ctx_ = ctx_;
+        Status s = wrap(cybq_cache_create(ctx_, kind, layers, kv_heads, head_dim, page_tokens, pages, &c.h_));
+        if (s) out = std::move(c);
+        return s;
+    }
+    Status cache_append(const Cache& c, int64_t layer, const cybq_batch& batch, const void* q, int64_t q_stride, int64_t q_heads, const void* k,
+                        int64_t k_stride, const void* v, int64_t v_stride, cybq_dtype dt, const float* rope, int64_t rope_positions,
+                        int64_t rope_dims, cybq_rope_style style, void* q_out, cybq_dtype qdt, void* stream = nullptr)
+    {
+        return wrap(cybq_cache_append(ctx_, c.get(), layer, &batch, q, q_stride, q_heads, k, k_stride, v, v_stride, dt, rope, rope_positions,
+                                      rope_dims, style, q_out, qdt, stream));
+    }
+    Status cache_read(const Cache& c, int64_t layer, const cybq_batch& batch, void* k, void* v, cybq_dtype dt, void* stream = nullptr)
+    {
+        return wrap(cybq_cache_read(ctx_, c.get(), layer, &batch, k, v, dt, stream));
+    }
+    Status attention(const Cache& c, int64_t layer, const cybq_batch& batch, const void* q, int64_t q_stride, cybq_dtype qdt, int64_t q_heads,
+                     float scale, int64_t window, void* y, void* stream = nullptr)
+    {
+        return wrap(cybq_attention(ctx_, c.get(), layer, &batch, q, q_stride, qdt, q_heads, scale, window, y, stream));
     }
     Status dequant(const Weight& w, float* out, void* stream = nullptr)
     {
