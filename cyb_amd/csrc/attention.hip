@@ -7,8 +7,9 @@
 // twice, and the scores are, as they lie, the operand of Y^T = V^T P^T.
 //
 // Operands.  16-bit caches: their own type, P of bf16 as two numbers (its 8 bits alone would be the result's error).  Q8, Q4: f16.  Keys are
-// the exact integers, their scales come in fp32 on each group's products; values are round_f16(scale q), 2^-12; P is f16 behind 2^14
-// (probabilities down to 2^-38 of the largest count, whatever their number); rows of bf16 become f16 behind a power of two.
+// the exact integers, their scales come in fp32 on each group's products; values are round_f16(scale q), 2^-12, and P is two numbers, so that this
+// rounding stands alone (48 conversations: 3.5e-4 off with one number, 2.9e-4 with two, 2.1e-4 of them y's own; no slower, memory is what such
+// calls wait for); rows of bf16 become f16 behind a power of two.
 #include <algorithm>
 
 #include "cache_parts.h"
@@ -337,8 +338,8 @@ __global__ __launch_bounds__(64 * RowsShape<G>::kWaves, G <= 4 ? 2 : 1) void att
 {
     constexpr int kWaves = RowsShape<G>::kWaves;
     constexpr int DIM = 32 * G, BLOCK = cache_block_bytes(KIND, DIM), HALF = cache_half_bytes(KIND, DIM), DT = 2 * G;
-    constexpr bool SPLIT_P = KIND == kCacheBF16;
-    constexpr float kShift = SPLIT_P ? 0.f : kShiftF16, kLag = SPLIT_P ? kLagBF16 : kLagF16;
+    constexpr bool BF = KIND == kCacheBF16, SPLIT_P = KIND != kCacheF16;
+    constexpr float kShift = BF ? 0.f : kShiftF16, kLag = BF ? kLagBF16 : kLagF16;
     extern __shared__ float4_t lds[];                                 // [waves][DT][64], then [waves][16] maxima and sums
     float* const stats = reinterpret_cast<float*>(lds + kWaves * DT * 64);
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q4 = lane >> 4, r = lane & 15;
@@ -481,11 +482,12 @@ __global__ __launch_bounds__(64 * RowsShape<G>::kWaves, G <= 4 ? 2 : 1) void att
         }
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            if constexpr (SPLIT_P) {
+            if constexpr (BF) {
                 ph.u[j] = pack_bf16x2(pr[2 * j], pr[2 * j + 1]);
                 pl.u[j] = pack_bf16x2(pr[2 * j] - __builtin_bit_cast(float, ph.u[j] << 16), pr[2 * j + 1] - __builtin_bit_cast(float, ph.u[j] & 0xffff0000u));
             } else {
                 ph.u[j] = pack_half2(pr[2 * j], pr[2 * j + 1]);
+                if constexpr (SPLIT_P) pl.u[j] = pack_half2(pr[2 * j] - (float)as_h2(ph.u[j])[0], pr[2 * j + 1] - (float)as_h2(ph.u[j])[1]);
             }
         }
 #pragma unroll
