@@ -1082,10 +1082,10 @@ hipError_t tiles_as(const AttnArgs& a, unsigned grid, hipStream_t st)
 }
 
 template <int KIND, int G>
-hipError_t attention_as(AttnArgs a, hipStream_t st)
+hipError_t attention_as(AttnArgs a, bool exact, hipStream_t st)
 {
     const int64_t most = (int64_t)a.t.max_new * a.group;
-    const bool many = most > kFewRows;
+    const bool many = !exact && most > kFewRows;
     a.few = many && a.t.seqs > 1 ? kFewRows : 0;                     // (a single sequence: the kernel that its largest call needs)
     hipError_t e = hipSuccess;
     const int64_t rows = (int64_t)a.t.rows * a.group, blocks = (int64_t)a.t.table_pages << a.c.page_shift;
@@ -1117,7 +1117,7 @@ size_t attention_scratch_bytes(int dim)
     const size_t rows = (size_t)2 * kMostExtra * kRows * (dim + 2);
     auto tiles = [](int extra, int slab) { return (size_t)2 * extra * slab; };
     size_t many;
-    switch (dim) {                                                   // (the quantised kinds have half as many parts of twice the rows, or fewer)
+    switch (dim) {                                                   // (the quantised kinds have as many, or half as many of twice the rows)
         case 64: many = tiles(TileShape<kCacheF16, 2>::kMostExtra, TileShape<kCacheF16, 2>::kSlab); break;
         case 96: many = tiles(TileShape<kCacheF16, 3>::kMostExtra, TileShape<kCacheF16, 3>::kSlab); break;
         case 128: many = tiles(TileShape<kCacheF16, 4>::kMostExtra, TileShape<kCacheF16, 4>::kSlab); break;
@@ -1136,7 +1136,7 @@ int64_t attention_units_max(const BatchView& t, int kv_heads, int group)
     return ((int64_t)t.rows * group / kRows + t.seqs) * kv_heads + std::max(kMostExtra, TileShape<kCacheF16, 2>::kMostExtra);
 }
 
-hipError_t launch_attention(const CacheView& c, const BatchView& t, const void* q, int64_t q_stride, int qdt, int group, float scale, int window, void* y,
+hipError_t launch_attention(const CacheView& c, const BatchView& t, const void* q, int64_t q_stride, int qdt, int group, float scale, int window, bool exact, void* y,
                             void* scratch, void* tickets, hipStream_t st)
 {
     AttnArgs a;
@@ -1153,10 +1153,10 @@ hipError_t launch_attention(const CacheView& c, const BatchView& t, const void* 
     a.scale = scale * 1.44269504088896340736f;
 #define CYBQ_ROWS(KIND)                                   \
     switch (c.dim) {                                      \
-        case 64: return attention_as<KIND, 2>(a, st);     \
-        case 96: return attention_as<KIND, 3>(a, st);     \
-        case 128: return attention_as<KIND, 4>(a, st);    \
-        default: return attention_as<KIND, 8>(a, st);     \
+        case 64: return attention_as<KIND, 2>(a, exact, st); \
+        case 96: return attention_as<KIND, 3>(a, exact, st); \
+        case 128: return attention_as<KIND, 4>(a, exact, st);    \
+        default: return attention_as<KIND, 8>(a, exact, st); \
     }
     switch (c.kind) {
         case kCacheF16: CYBQ_ROWS(kCacheF16)

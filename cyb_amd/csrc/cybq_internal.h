@@ -133,7 +133,7 @@ constexpr size_t kAttnTicketBytes = (size_t)1 << 16;
 size_t attention_scratch_bytes(int dim);
 int64_t attention_units_max(const BatchView& t, int kv_heads, int group);       // the call is for launch_attention up to ..
 int64_t attention_max_units();                                                  // .. this many
-hipError_t launch_attention(const CacheView& c, const BatchView& t, const void* q, int64_t q_stride, int qdt, int group, float scale, int window, void* y,
+hipError_t launch_attention(const CacheView& c, const BatchView& t, const void* q, int64_t q_stride, int qdt, int group, float scale, int window, bool exact, void* y,
                             void* scratch, void* tickets, hipStream_t st);
 
 // Kernels that need more dynamic LDS than the default 64 KB say so when the library is loaded:

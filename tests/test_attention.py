@@ -87,6 +87,26 @@ def test_prompts(backend, kind, dt, dim):
 
 @gpu
 @pytest.mark.parametrize("kind,dt", KINDS)
+def test_prompts_exactly(backend, kind, dt):
+    """Many rows with the prefill mode EXACT: the bound of few."""
+    backend.set_prefill_mode("exact")
+    try:
+        for lengths, new, window, dim in (([333, 150, 700], [100, 150, 391], 0, 128), ([600], [300], 100, 64), ([513], [129], 0, 256)):
+            s = Cached(backend, kind, lengths, kv_heads=2, dim=dim, page=64, seed=len(lengths))
+            q = normal((sum(new), 6, dim), 9, dt)
+            y = torch.empty_like(q)
+            backend.attention(s.cache, 0, s.batch(new), q, y, window=window)
+            torch.cuda.synchronize()
+            ref, size, dots = s.expected(q, new, None, window)
+            worst = ((y.double() - ref).abs() / bound(kind, dt, dim, ref, size, dots, False)).max().item()
+            assert worst <= 1.0, worst
+            s.close()
+    finally:
+        backend.set_prefill_mode("fast")
+
+
+@gpu
+@pytest.mark.parametrize("kind,dt", KINDS)
 def test_a_long_context_is_shared_out(backend, kind, dt):
     s = Cached(backend, kind, [20011, 130], kv_heads=2, dim=128, page=128)
     check(s, [1, 1], 4, dt)
