@@ -44,9 +44,21 @@ constexpr float kShiftF16 = 4.f, kLagF16 = 11.f, kLagBF16 = 16.f;
 // Workgroups of a round of the rows kernel (two to a CU), and how many parts there may be beyond one of each tile: rounds * target, twice that in
 // the tiles kernel, whose tiles may see half as much on average as the one that sees the most
 constexpr int kTarget = 512, kMostExtra = 2 * kTarget;
-constexpr float kRounds = 2.f, kTileRounds = 1.f;
+// Rounds where there are tiles for more than half of one already.  Rows kernel, 48 conversations of up to 8192 tokens: 1, 2, 4, 8 rounds 111, 103,
+// 108, 120 us.  Tiles kernel, prompts: the parts of half a round are those of the few tiles that see much more than others (2000 rows of heads of 64
+// 35 us, 0.75 and 1 round 47; of 128 60 and 83; sequences of 700 to 5000 tokens none 124, 0.25 65, 0.5 58, 1 90).
+constexpr float kRounds = 2.f, kTileRounds = 0.5f;
 constexpr int kLeast = 4, kTileLeast = 8;        // blocks of a part
-constexpr int kFewRows = 64;                     // rows of a sequence and kv head (new tokens times group) that the rows kernel takes
+// A tile of the tiles kernel has up to sqrt(kJoin * its blocks) parts: each adds 1.5 us to the time that the last of them takes to join (300 tokens alone,
+// 0.1 and 0.2: 18 us, 0.4 and more: 26; 96 rows of 4000 tokens 51, 45, 45, with no limit 64; 1000 rows 34, 37, 37)
+constexpr float kJoin = 0.2f;
+
+// Rows of a sequence and kv head (new tokens times group) that the rows kernel takes.  Where there are few in all, many too: the other kernel's
+// tiles, each of 256 rows, would be fewer than there are CUs, their parts many and long to join (heads of 128, 4 query heads to each of 8 kv heads;
+// us, rows kernel and tiles kernel.  F16: 128 rows of 1000 tokens 11 and 34, 16 x 24 of 3000 73 and 81, 8 x 64 60 and 59, 32 x 32 166 and 115;
+// Q4: 2 x 128 55 and 52, 8 x 64 80 and 62, 32 x 16 of 4000 106 and 127).
+constexpr int kFewRows = 64, kFewAlone = 512;
+constexpr int few_in_all(int kind) { return cache_quantised(kind) ? 1 << 13 : 1 << 14; }
 
 struct Unit {
     Seq s;
@@ -132,7 +144,8 @@ __device__ __forceinline__ bool find_unit(const AttnArgs& a, int u, Unit* out)
     bool found = false;
     for (int base = 0; base < a.t.seqs; base += 64) {
         if (base) x = share_of<ROWS, MANY>(a, base + lane, capacity);
-        const int splits = x.tiles ? max(1, (x.blocks + part - 1) / part) : 0;
+        int splits = x.tiles ? max(1, (x.blocks + part - 1) / part) : 0;
+        if (MANY) splits = min(splits, max(1, (int)__builtin_sqrtf(kJoin * (float)x.blocks)));
         // (a batch whose starts make no sense may add up to anything: what cannot be right stays above every grid)
         const int rows = min(x.tiles * heads, kMaxUnits + 1), mine = (int)min((int64_t)rows * splits, (int64_t)kMaxUnits + 1);
         const int upto = wave_prefix(mine), slab_upto = wave_prefix(splits > 1 ? mine : 0), ticket_upto = wave_prefix(splits > 1 ? rows : 0);
@@ -621,7 +634,7 @@ struct TileShape {
     static constexpr int kRows = 32 * kWaves;
     // Steps of keys, and of values, that LDS holds: three, so that copies have two steps to arrive in; quantised bytes wait in registers instead
     static constexpr int kRing = cache_quantised(KIND) ? 2 : 3;
-    static constexpr int kPerCu = G > 4 || kWaves == 8 ? 1 : G == 2 ? 3 : 2;              // workgroups
+    static constexpr int kPerCu = G > 4 || kWaves == 8 ? 1 : 2;              // workgroups
     static constexpr int kTarget = 256 * kPerCu, kMostExtra = 2 * kTarget;
     static constexpr int kHalf = kBlocks * kBlockTokens * 32 * G * 2;         // bytes of a step's keys, or values
     static constexpr int kLds = 2 * kRing * kHalf;
@@ -754,7 +767,7 @@ __global__ __launch_bounds__((64 * TileShape<KIND, G>::kWaves), (TileShape<KIND,
     const int p = p0 + i;
     const int row_hi = real ? (int)min((int64_t)p, capacity - 1) : -1;
     const int row_lo = a.window && p >= a.window ? p - a.window + 1 : 0;
-    int all_hi = -1, all_lo = 0;                                     // every row sees all_lo .. all_hi
+    int all_hi = 0x7fffffff, all_lo = 0;                             // every row sees all_lo .. all_hi (a wave without rows: nobody looks at what it sees)
     if (rows) {
         const int pf = p0 + r0 / a.group, pl = p0 + (r0 + rows - 1) / a.group;
         all_hi = (int)min((int64_t)pf, capacity - 1);
@@ -786,29 +799,31 @@ __global__ __launch_bounds__((64 * TileShape<KIND, G>::kWaves), (TileShape<KIND,
     const float lag = fminf(kLag / c, 1e30f);
     const int32_t* const table = a.t.tables + (int64_t)u.b * a.t.table_pages;
     const int in_page = (1 << a.c.page_shift) - 1;
-    // Pages of the part's blocks, 64 to a register (-1: none): of blocks from_block .. + 128, counted from the part's first
+    // Where the part's blocks lie, a lane for each of 64 from `from_block` on, counted from the part's first (a block that is not there is
+    // read from page 0: finite numbers, which nobody sees), and the pages of the 64 behind them.  Scalar arithmetic of 64 bits for every step and
+    // wave, in its place, took a fifth of a step of heads of 64.
     auto pages_from = [&](int i) {
         const int blk = first + i + lane;
         return blk < last ? table[blk >> a.c.page_shift] : -1;
     };
-    int from_block = 0, near_ids = pages_from(0), far_ids = pages_from(64);
-    auto page_of = [&](int i) {
-        const int at = i - from_block;
-        return __builtin_amdgcn_readlane(at < 64 ? near_ids : far_ids, at & 63);
+    int from_block = 0, far_ids = pages_from(64);
+    uint32_t at_lo, at_hi;
+    uint64_t there;
+    auto look_up = [&](int id) {
+        const bool real_page = (unsigned)id < (unsigned)a.c.pages;
+        there = __ballot(real_page);
+        const uint64_t at = reinterpret_cast<uint64_t>(a.c.base) + (uint64_t)(real_page ? id : 0) * (uint64_t)a.c.page_bytes +
+                            (uint64_t)((u.head << a.c.page_shift) + ((first + from_block + lane) & in_page)) * (uint64_t)BLOCK;
+        at_lo = (uint32_t)at;
+        at_hi = (uint32_t)(at >> 32);
     };
-    // which of a step's blocks are in no page
-    auto absent = [&](int step) {
-        unsigned m = 0;
-#pragma unroll
-        for (int b = 0; b < BL; b++) m |= (unsigned)page_of(step * BL + b) >= (unsigned)a.c.pages ? 1u << b : 0u;
-        return m;
-    };
-    // (a block that is not there is read from page 0: finite numbers, which nobody sees)
+    look_up(pages_from(0));
+    // of a step within those 64
     auto blocks_of = [&](int step, const uint8_t* (&at)[BL]) {
 #pragma unroll
         for (int b = 0; b < BL; b++) {
-            const int id = page_of(step * BL + b), page = (unsigned)id >= (unsigned)a.c.pages ? 0 : id;
-            at[b] = a.c.base + page * a.c.page_bytes + (int64_t)((u.head << a.c.page_shift) + ((first + step * BL + b) & in_page)) * BLOCK;
+            const int i = step * BL + b - from_block;
+            at[b] = reinterpret_cast<const uint8_t*>((uint64_t)(uint32_t)__builtin_amdgcn_readlane(at_hi, i) << 32 | (uint32_t)__builtin_amdgcn_readlane(at_lo, i));
         }
     };
     f32x16_t y[G];
@@ -834,7 +849,10 @@ __global__ __launch_bounds__((64 * TileShape<KIND, G>::kWaves), (TileShape<KIND,
     constexpr uint32_t K0 = 0, V0 = R * T::kHalf;
     constexpr int N = 2 * G * BL;                                    // matrix instructions of a step's scores, and of its values
     Stage<KIND, G> ks, vs;
+    constexpr int AHEAD = QUANT ? 3 : R;                             // keys of step t + AHEAD are asked for in step t, values of t + AHEAD - 2
     const uint8_t* at[BL];
+    const uint8_t* queue[3][BL];                                     // blocks of steps t + AHEAD - 2 ..
+    uint32_t present;                                                // BL bits for each step from t on: whether its blocks are in a page
     f32x16_t s[BL];                                                  // scores of step t
     Frag16 pf[2 * BL];                                               // P of step t - 1, not yet on the sums
 #pragma unroll
@@ -865,28 +883,31 @@ __global__ __launch_bounds__((64 * TileShape<KIND, G>::kWaves), (TileShape<KIND,
             for (int k = 0; k < 2 * G; k++) s[b] = mfma32<KIND>(key_at(K0, k, b), qf[k], k ? s[b] : zeros);
         __syncthreads();                                             // (keys of step R go where those of step 0 were)
     }
+    blocks_of(AHEAD - 2, queue[0]);
+    blocks_of(AHEAD - 1, queue[1]);
+    present = (uint32_t)there & ((1u << AHEAD * BL) - 1u);
     uint32_t ring[R];                                                // places of steps t, t + 1, .. (and t - 1, the last)
 #pragma unroll
     for (int j = 0; j < R; j++) ring[j] = j * T::kHalf;
     float top = none;
+    constexpr uint32_t ALL = (1u << BL) - 1u;
     // whether some row does not see all of step t's tokens
     auto hides = [&](int t) {
         const int tok = (first + t * BL) * kBlockTokens;
-        return absent(t) != 0 || tok < all_lo || tok + BL * kBlockTokens - 1 > all_hi;
+        return (present & ALL) != ALL || tok < all_lo || tok + BL * kBlockTokens - 1 > all_hi;
     };
     // Steps whose rows see everything and whose maxima have grown by less than the lag follow each other in the inner loop; at any other its scores
     // are masked, P that waits is added and the sums are scaled outside of it.  (In a branch of the loop the sums had two homes, 64
     // registers and as many moves.)
     for (int t = 0; t < steps;) {
         if (hides(t)) {
-            const unsigned gone = absent(t);
             const int tok = (first + t * BL) * kBlockTokens;
 #pragma unroll
             for (int b = 0; b < BL; b++)
 #pragma unroll
                 for (int e = 0; e < 16; e++) {
                     const int j = tok + b * kBlockTokens + 8 * (e >> 2) + 4 * h + (e & 3);
-                    if (j < row_lo || j > row_hi || (gone >> b & 1)) s[b][e] = none;
+                    if (j < row_lo || j > row_hi || !(present >> b & 1)) s[b][e] = none;
                 }
         }
         top = s[0][0];
@@ -914,25 +935,23 @@ __global__ __launch_bounds__((64 * TileShape<KIND, G>::kWaves), (TileShape<KIND,
             // about a pair's exponentials behind each.
             // Copies for steps to come (past the end they are read from page 0 and nobody looks at them), spread over the step: a CU takes 64 bytes a cycle
             // from its L1, and asked for in a row they held the waves up for 1000 of a step's 2500 cycles.
-            const uint8_t* key_blocks[BL];
-            const uint8_t* value_blocks[BL];
-            blocks_of(QUANT ? t + 3 : t + R, key_blocks);
-            blocks_of(QUANT ? t + 1 : t + R - 2, value_blocks);
+            blocks_of(t + AHEAD, queue[2]);
+            present |= (uint32_t)(there >> ((t + AHEAD) * BL - from_block) & ALL) << AHEAD * BL;
             constexpr int SLOTS = R == 2 ? N : 2 * N, PER = Stage<KIND, G>::PER;       // (of two steps that LDS holds the next needs them all)
             auto copies = [&](int i) __attribute__((always_inline)) {
                 if constexpr (QUANT) {                               // what was asked for a step ago, and the next of it
                     if (i == N / 4) {
                         ks.template put<false>(bytes, K0 + ring[0], wv, lane, magic);
-                        ks.template ask<false>(key_blocks, 0, wv, lane);
+                        ks.template ask<false>(queue[2], 0, wv, lane);
                     }
                     if (i == 3 * N / 4) {
                         vs.template put<true>(bytes, V0 + ring[0], wv, lane, magic);
-                        vs.template ask<true>(value_blocks, 0, wv, lane);
+                        vs.template ask<true>(queue[0], 0, wv, lane);
                     }
                 } else if (i < SLOTS) {
                     const int from = i * 2 * PER / SLOTS, to = (i + 1) * 2 * PER / SLOTS;
-                    if (from < PER) ks.template ask<false>(key_blocks, K0 + ring[0], wv, lane, from, to < PER ? to : PER);
-                    if (to > PER) vs.template ask<true>(value_blocks, V0 + ring[R - 2], wv, lane, from > PER ? from - PER : 0, to - PER);
+                    if (from < PER) ks.template ask<false>(queue[2], K0 + ring[0], wv, lane, from, to < PER ? to : PER);
+                    if (to > PER) vs.template ask<true>(queue[0], V0 + ring[R - 2], wv, lane, from > PER ? from - PER : 0, to - PER);
                 }
             };
             const uint32_t values_at = V0 + ring[R - 1], keys_at = K0 + ring[1];
@@ -951,7 +970,9 @@ __global__ __launch_bounds__((64 * TileShape<KIND, G>::kWaves), (TileShape<KIND,
                     const int b = i >> 3, e = 2 * (i & 7);
                     const float x0 = exp2_fast(__builtin_fmaf(s[b][e], c, off)), x1 = exp2_fast(__builtin_fmaf(s[b][e + 1], c, off));
                     sums[i & 3] += x0 + x1;
-                    pn[i >> 2].u[i & 3] = KIND == kCacheBF16 ? pack_bf16x2(x0, x1) : pack_half2(x0, x1);
+                    uint32_t w = KIND == kCacheBF16 ? pack_bf16x2(x0, x1) : pack_half2(x0, x1);
+                    asm volatile("" : "+v"(w));                      // (here, and not where the next step needs it)
+                    pn[i >> 2].u[i & 3] = w;
                 }
             };
 #pragma unroll
@@ -995,9 +1016,15 @@ __global__ __launch_bounds__((64 * TileShape<KIND, G>::kWaves), (TileShape<KIND,
             for (int j = 0; j + 1 < R; j++) ring[j] = ring[j + 1];
             ring[R - 1] = first_place;
             t++;
-            if (t * BL - from_block >= 64) {
+            present >>= BL;
+#pragma unroll
+            for (int b = 0; b < BL; b++) {
+                queue[0][b] = queue[1][b];
+                queue[1][b] = queue[2][b];
+            }
+            if ((t + AHEAD) * BL - from_block >= 64) {
                 from_block += 64;
-                near_ids = far_ids;
+                look_up(far_ids);
                 far_ids = pages_from(from_block + 64);
             }
         } while (t < steps && !hides(t) && !__ballot(top > m + lag));
@@ -1036,24 +1063,29 @@ __global__ __launch_bounds__((64 * TileShape<KIND, G>::kWaves), (TileShape<KIND,
     auto part_of = [&](int e) { return get_float2(of_tile + (size_t)e * SLAB + ROWS * DIM + 2 * (wv * 32 + r)); };        // maximum and sum of my row
     top = none;
     float sum = 0.f;
-    for (int e = 0; e < u.splits; e++) top = fmaxf(top, part_of(e)[0]);
+    for (int e = 0; e < u.splits; e += 4) {
+        f32x2_t of[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) of[k] = part_of(min(e + k, u.splits - 1));
+#pragma unroll
+        for (int k = 0; k < 4; k++) top = fmaxf(top, of[k][0]);
+    }
 #pragma unroll
     for (int d = 0; d < G; d++)
 #pragma unroll
         for (int e = 0; e < 16; e++) y[d][e] = 0.f;
     for (int e = 0; e < u.splits; e++) {
         const f32x2_t me = part_of(e);
+        const float* const from = of_tile + (size_t)e * SLAB + (wv * G * 4 * 64 + lane) * 4;
+        float4_t part[4 * G];                                        // asked for at once: past the caches a load takes a microsecond or two
+#pragma unroll
+        for (int k = 0; k < 4 * G; k++) part[k] = get_float4(from + k * 256);
         const float f = me[0] == none ? 0.f : exp2_fast(me[0] - top);
         sum += f * me[1];
-        const float* const from = of_tile + (size_t)e * SLAB + (wv * G * 4 * 64 + lane) * 4;
 #pragma unroll
-        for (int d = 0; d < G; d++)
+        for (int k = 0; k < 4 * G; k++)
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const float4_t part = get_float4(from + (d * 4 + k) * 256);
-#pragma unroll
-                for (int j = 0; j < 4; j++) y[d][4 * k + j] += part[j] * f;
-            }
+            for (int j = 0; j < 4; j++) y[k / 4][4 * (k % 4) + j] += part[k][j] * f;
     }
     if (!real) return;
     const float inv = sum == 0.f ? 0.f : 1.0f / sum;
@@ -1085,8 +1117,9 @@ template <int KIND, int G>
 hipError_t attention_as(AttnArgs a, bool exact, hipStream_t st)
 {
     const int64_t most = (int64_t)a.t.max_new * a.group;
-    const bool many = !exact && most > kFewRows;
-    a.few = many && a.t.seqs > 1 ? kFewRows : 0;                     // (a single sequence: the kernel that its largest call needs)
+    const int few = (int64_t)a.t.rows * a.group * a.c.kv_heads <= few_in_all(KIND) ? kFewAlone : kFewRows;
+    const bool many = !exact && most > few;
+    a.few = many && a.t.seqs > 1 ? few : 0;                     // (a single sequence: the kernel that its largest call needs)
     hipError_t e = hipSuccess;
     const int64_t rows = (int64_t)a.t.rows * a.group, blocks = (int64_t)a.t.table_pages << a.c.page_shift;
     // tiles of all, and the parts beyond one of each: what `target` makes of them, and no more than the table has blocks for
@@ -1095,7 +1128,7 @@ hipError_t attention_as(AttnArgs a, bool exact, hipStream_t st)
         a.target = kTarget;
         a.least = kLeast;
         a.rounds = kRounds;
-        const int64_t tiles = std::min(rows / kRows + a.t.seqs, a.few ? (int64_t)a.t.seqs * ((kFewRows + kRows - 1) / kRows) : rows);
+        const int64_t tiles = std::min(rows / kRows + a.t.seqs, a.few ? (int64_t)a.t.seqs * ((few + kRows - 1) / kRows) : rows);
         e = rows_as<KIND, G>(a, grid(tiles, kMostExtra), st);
     }
     if (many && e == hipSuccess) {

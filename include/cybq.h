@@ -409,8 +409,8 @@ int cybq_cache_read(cybq_ctx* ctx, const cybq_cache* cache, int64_t layer, const
  *   aligned, must not overlap q.  qdt: F16 on an F16 cache, BF16 on a BF16 cache, either of them on Q8 and Q4 (CYBQ_ERR_UNSUPPORTED).
  *   scale is positive and finite; scaled scores have to stay within fp32.
  * Scores, maxima and sums are fp32.  Values of Q8 and Q4 caches are round_f16(scale * q).  Up to 64 rows of a sequence and kv head (new
- * tokens times q_heads / kv_heads), any number with CYBQ_PREFILL_EXACT: keys are exact, and so are probabilities but on F16 caches (2^-11).  More
- * rows with CYBQ_PREFILL_FAST: keys of Q8 and Q4 are round_f16(scale * q) too, probabilities one number of f16 (a BF16 cache: bf16).  Calls on
+ * tokens times q_heads / kv_heads), any number with CYBQ_PREFILL_EXACT: keys are exact, and so are probabilities but on F16 caches (2^-11).  Of
+ * more rows with CYBQ_PREFILL_FAST keys of Q8 and Q4 may be round_f16(scale * q) too, probabilities one number of f16 (a BF16 cache: bf16).  Calls on
  * one context share its scratch: they (replays of its graphs too) must not overlap in time. */
 int cybq_attention(cybq_ctx* ctx, const cybq_cache* cache, int64_t layer, const cybq_batch* batch, const void* q, int64_t q_stride,
                    cybq_dtype qdt, int64_t q_heads, float scale, int64_t window, void* y, void* stream);
