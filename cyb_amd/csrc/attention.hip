@@ -337,7 +337,11 @@ __device__ __forceinline__ bool last_part(const AttnArgs& a, const Unit& u, unsi
 }
 
 // Few rows: tiles of 16, four waves that take a part's blocks in turn, each with the next of its blocks on its way while it
-// works on one.  Waves meet in LDS, the parts of a tile in slabs in memory: the part that is last adds them in order.
+// works on one.  Waves meet in LDS, the parts of a tile in slabs in memory: the part that is last adds them in order.  Bound by HBM where the
+// context is long: 100001 tokens of a Q8 cache, 8 heads of 128, 218 MB: 45 - 51 us = 4.3 - 4.9 TB/s (three waves to a SIMD with one block each: 75);
+// 48 conversations of up to 8192 tokens, 452 MB: 98 us = 4.6 TB/s.  Short contexts wait for one thing after another (1000 tokens: 7.8 us): lengths 1.5,
+// table and block 2, its products 1.3, the way of the parts through memory 3.  Two tiles of rows to a workgroup, so that what a block needs is done
+// once for 32 rows, have registers for one block at a time only: 8 drafts of 5 tokens with 7 heads each 24 us instead of 19.
 constexpr int kRows = 16;
 template <int G>
 struct RowsShape {
@@ -739,7 +743,11 @@ struct Stage {
 };
 
 // Many rows: a workgroup's waves have 32 rows each and go through the same blocks, 64 tokens (a head of 256: 32) a step.  While P of a step
-// is formed the scores of the next are multiplied: its keys are in LDS one step earlier than its values.
+// is formed the scores of the next are multiplied: its keys are in LDS one step earlier than its values.  Bound by issue: matrix instructions
+// are 57 % of a SIMD's cycles, vector instructions 50, and the card clocks down to 1.64 GHz under them (4096 rows, 32 heads of 128, after 28672 tokens of F16:
+// 1850 - 1930 us = 1.07 - 1.11 PFLOP/s; the library's product of 8192 x 8192 x 8192 1.27).  Q8: each value is also unpacked, once for 256 rows (512 rows
+// after 15872 tokens 175 us = 0.78 PFLOP/s).  Short prompts are as long as the tile that sees the most (2000 rows, heads of 64: 34 us, 25 of them
+// that tile's 32 steps).
 template <int KIND, int G>
 __global__ __launch_bounds__((64 * TileShape<KIND, G>::kWaves), (TileShape<KIND, G>::kWaves * TileShape<KIND, G>::kPerCu / 4)) void attention_tiles_kernel(AttnArgs a)
 {
