@@ -37,8 +37,8 @@ struct AttnArgs {
 
 constexpr int kMaxUnits = 1 << 24;               // of a call
 // A maximum may lag behind the scores by 2^kLag before sums are scaled anew: every scaling is a detour of a wave that all others of its
-// workgroup wait for (with a lag of 2^3 one step in seven, 512 rows of a Q8 cache after 16384 tokens took 216 us; with 2^11: 198).  P of f16 stands behind 2^kShift:
-// its largest stays below 2^15, and probabilities count down to 2^-28 of the largest.
+// workgroup wait for (with a lag of 2^3 one step in seven, 512 rows of a Q8 cache after 15872 tokens took 216 us; with 2^11: 198).  P of f16
+// stands behind 2^kShift: its largest stays below 2^15, and probabilities count down to 2^-28 of the largest.
 constexpr float kShiftF16 = 4.f, kLagF16 = 11.f, kLagBF16 = 16.f;
 
 // Workgroups of a round of the rows kernel (two to a CU), and how many parts there may be beyond one of each tile: rounds * target, twice that in
@@ -339,9 +339,10 @@ __device__ __forceinline__ bool last_part(const AttnArgs& a, const Unit& u, unsi
 // Few rows: tiles of 16, four waves that take a part's blocks in turn, each with the next of its blocks on its way while it
 // works on one.  Waves meet in LDS, the parts of a tile in slabs in memory: the part that is last adds them in order.  Bound by HBM where the
 // context is long: 100001 tokens of a Q8 cache, 8 heads of 128, 218 MB: 45 - 51 us = 4.3 - 4.9 TB/s (three waves to a SIMD with one block each: 75);
-// 48 conversations of up to 8192 tokens, 452 MB: 98 us = 4.6 TB/s.  Short contexts wait for one thing after another (1000 tokens: 7.8 us): lengths 1.5,
-// table and block 2, its products 1.3, the way of the parts through memory 3.  Two tiles of rows to a workgroup, so that what a block needs is done
-// once for 32 rows, have registers for one block at a time only: 8 drafts of 5 tokens with 7 heads each 24 us instead of 19.
+// 48 conversations of up to 8192 tokens, 452 MB: 98 us = 4.6 TB/s.  Short contexts wait for one thing after another (1000 tokens: 7.8 us):
+// lengths 1.5, products 1.3, the rest the table, the block and the way of the parts through memory.  Two tiles of rows to a workgroup, so that
+// what a block needs is done once for 32 rows, have registers for one block at a time only: 8 drafts of 5 tokens with 7 heads each 24 us instead
+// of 19.
 constexpr int kRows = 16;
 template <int G>
 struct RowsShape {
@@ -631,10 +632,10 @@ __device__ __forceinline__ void copy_to_lds(uint32_t lds_off, const void* base, 
 template <int KIND, int G>
 struct TileShape {
     static constexpr int kBlocks = G <= 4 ? 2 : 1;            // blocks of a step
-    // Waves, each with 32 rows: eight where they share the work of unpacking (Q8, Q4: 216 us instead of 308 for 512 rows after 16384 tokens) or where
+    // Waves, each with 32 rows: eight where they share the work of unpacking (Q8, Q4: 216 us instead of 308 for 512 rows after 15872 tokens) or where
     // three steps of copies fit a CU once only (heads of 128: 2040 us instead of 2150 for 4096 rows after 28672 tokens); else four, in more workgroups
     // (heads of 64: 62 us instead of 69 for 2000 rows)
-    static constexpr int kWaves = G <= 4 && (cache_quantised(KIND) || G >= 3) ? 8 : 4;
+    static constexpr int kWaves = cache_quantised(KIND) ? (G <= 4 ? 8 : 4) : (G == 4 ? 8 : 4);
     static constexpr int kRows = 32 * kWaves;
     // Steps of keys, and of values, that LDS holds: three, so that copies have two steps to arrive in; quantised bytes wait in registers instead
     static constexpr int kRing = cache_quantised(KIND) ? 2 : 3;
@@ -654,6 +655,7 @@ struct Stage {
     static constexpr bool kQuant = cache_quantised(KIND);
     static constexpr int N = kQuant ? Half<KIND, G>::N : 2 * G;                          // 1 KiB pieces of a block's half
     static constexpr int PER = (T::kBlocks * N + T::kWaves - 1) / T::kWaves;             // pieces per wave
+    static_assert(kQuant || T::kBlocks * N % T::kWaves == 0, "every wave has as many copies in flight as its waits count");
     struct Piece {
         u32x4_t d, s[2];
     };
@@ -945,7 +947,7 @@ __global__ __launch_bounds__((64 * TileShape<KIND, G>::kWaves), (TileShape<KIND,
             // from its L1, and asked for in a row they held the waves up for 1000 of a step's 2500 cycles.
             blocks_of(t + AHEAD, queue[2]);
             present |= (uint32_t)(there >> ((t + AHEAD) * BL - from_block) & ALL) << AHEAD * BL;
-            constexpr int SLOTS = R == 2 ? N : 2 * N, PER = Stage<KIND, G>::PER;       // (of two steps that LDS holds the next needs them all)
+            constexpr int SLOTS = 2 * N, PER = Stage<KIND, G>::PER;
             auto copies = [&](int i) __attribute__((always_inline)) {
                 if constexpr (QUANT) {                               // what was asked for a step ago, and the next of it
                     if (i == N / 4) {
@@ -956,7 +958,7 @@ __global__ __launch_bounds__((64 * TileShape<KIND, G>::kWaves), (TileShape<KIND,
                         vs.template put<true>(bytes, V0 + ring[0], wv, lane, magic);
                         vs.template ask<true>(queue[0], 0, wv, lane);
                     }
-                } else if (i < SLOTS) {
+                } else {
                     const int from = i * 2 * PER / SLOTS, to = (i + 1) * 2 * PER / SLOTS;
                     if (from < PER) ks.template ask<false>(queue[2], K0 + ring[0], wv, lane, from, to < PER ? to : PER);
                     if (to > PER) vs.template ask<true>(queue[0], V0 + ring[R - 2], wv, lane, from > PER ? from - PER : 0, to - PER);

@@ -8,11 +8,11 @@
 //
 // A workgroup takes the rows of one sequence that fall into one block of 32 positions, and one kv head.  Bound by memory: rows in, rows and
 // blocks out.  Fewer than 32 new rows of a sequence: one launch for keys, values and queries, bytes written one by one (one token, or 48 of one
-// each: 3.6 us, most of it the way from the lengths to the table to the page).  More: queries in a launch of their own (4096 tokens, 32 heads of 128, 67 MB:
-// 16 us = 4.1 TB/s; next to the keys in one launch their registers halved the waves that both had, 45 us for what takes 33 now), and a
-// block's keys and values by waves that have what lies side by side in it - a key's dimensions of two tokens, eight dimensions of the eight tokens
-// of a value's 8 or 16 bytes -, written 8 and 16 bytes at a time (4096 tokens, 8 heads of 128, bf16 to Q8: 12.4 us; byte by byte 31).  Reading back:
-// a block's bytes come once and rows go out 16 bytes to a lane (80000 tokens, 8 heads of 128, Q8 to bf16, 359 MB: 68 - 79 us = 4.5 - 5.3 TB/s).
+// each: 3.6 us, most of it the way from the lengths to the table to the page).  More: queries in a launch of their own (4096 tokens, 32 heads of
+// 128, 67 MB: 16 - 20 us = 3.4 - 4.1 TB/s), whose registers then cost the other kernel no waves, and a block's keys and values by waves that have
+// what lies side by side in it - a key's dimensions of two tokens, eight dimensions of the eight tokens of a value's 8 or 16 bytes -, written
+// 8 and 16 bytes at a time (4096 tokens, 8 heads of 128, bf16 to Q8: 12.4 - 14 us).  Reading back: a block's bytes come once and rows go out 16
+// bytes to a lane (80000 tokens, 8 heads of 128, Q8 to bf16, 359 MB: 68 - 79 us = 4.5 - 5.3 TB/s).
 #include "cache_parts.h"
 #include "cybq_internal.h"
 
