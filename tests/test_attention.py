@@ -256,3 +256,190 @@ def test_batches_that_make_no_sense_stay_inside(backend):
         assert (guard[:8] == 9.0).all() and (guard[16:] == 9.0).all()
     check(s, [3, 1, 2], 2, "f16")                                # and what comes after is right
     s.close()
+
+
+@gpu
+@pytest.mark.parametrize("kind,dt", [("f16", "f16"), ("bf16", "bf16"), ("q8", "bf16"), ("q4", "f16")])
+@pytest.mark.parametrize("dim", [64, 96, 128, 256])
+def test_many_rows_of_a_long_context(backend, kind, dt, dim):
+    """Parts of more blocks than a register of pages has, pages that are missing among them, next to single tokens and a short prompt."""
+    lengths, new, group, page = [5000, 300, 40, 2100], [515, 1, 1, 100], 4, 32
+    s = Cached(backend, kind, lengths, kv_heads=4, dim=dim, page=page, seed=dim)
+    s.tables[0, 70], s.tables[0, 129], s.tables[3, 5] = -1, s.cache.pages, -7
+    hidden = lambda b, j: (b == 0 and j // page in (70, 129)) or (b == 3 and j // page == 5)
+    y = check(s, new, group, dt, hidden=hidden)
+    assert torch.equal(y, check(s, new, group, dt, hidden=hidden))
+    check(s, new, group, dt, window=2300, hidden=hidden)
+    s.close()
+
+
+@gpu
+@pytest.mark.parametrize("kind,dt,dim", [("f16", "f16", 128), ("bf16", "bf16", 64), ("q8", "f16", 128), ("q4", "bf16", 96), ("f16", "f16", 256)])
+def test_tiles_that_are_not_cut(backend, kind, dt, dim):
+    """As many tiles as there are workgroups, each with all of its blocks (150 of the last); odd rows in the last."""
+    s = Cached(backend, kind, [4800], kv_heads=8, dim=dim, page=256)
+    check(s, [1027 if dim > 64 else 2051], 4, dt)
+    s.close()
+
+
+@gpu
+def test_pages_past_4_gib(backend):
+    """A page whose bytes lie more than 2^32 behind the cache's first, few rows and many; and the caller's copy of it elsewhere."""
+    page, pages = 1024, 1100
+    cache = backend.kv_cache("f16", 1, 8, 128, page, pages)
+    assert cache.page_bytes * pages > 1 << 32
+    ints = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    n = 1500
+    k, v = normal((n, 8, 128), 1, "f16"), normal((n, 8, 128), 2, "f16")
+    q = normal((n, 16, 128), 3, "f16")
+    outs = []
+    for table in ([pages - 1, 1050], [0, 1]):
+        b = backend.cache_batch(ints([0, n]), ints([n]), ints([table]), n)
+        backend.cache_append(cache, 0, b, None, k, v)
+        k2, v2 = torch.empty_like(k), torch.empty_like(v)
+        backend.cache_read(cache, 0, b, k2, v2)
+        few = backend.cache_batch(ints([0, 3]), ints([n]), ints([table]), 3)
+        y, y3 = torch.empty_like(q), torch.empty_like(q[:3])
+        backend.attention(cache, 0, b, q, y)
+        backend.attention(cache, 0, few, q[n - 3:], y3)
+        torch.cuda.synchronize()
+        assert torch.equal(k2, k) and torch.equal(v2, v)
+        outs.append((y, y3))
+    assert all(torch.equal(a, b) for a, b in zip(*outs)) and (outs[0][0] != 0).any()
+    cache.free()
+
+
+@gpu
+def test_a_captured_prompt(backend):
+    """Many rows next to few in a graph, replayed with other lengths with eager calls of other shapes in between; a context of its own."""
+    be = Backend(0)
+    try:
+        s = Cached(be, "q8", [900, 2000, 60], kv_heads=2, dim=128, page=64, width=40)
+        ints = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")
+        starts, lengths = ints([0, 600, 601, 604]), ints([900, 2000, 60])
+        batch = be.cache_batch(starts, lengths, s.tables, 604, 2000)
+        q = normal((604, 20, 128), 5, "f16")
+        y = torch.zeros_like(q)
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+            be.attention(s.cache, 0, batch, q, y, stream=torch.cuda.current_stream().cuda_stream)
+        for st, ln in (([0, 600, 601, 604], [900, 2000, 60]), ([0, 1, 602, 604], [900, 1999, 60]), ([0, 3, 6, 9], [5, 1200, 60]), ([0, 600, 601, 604], [600, 64, 3])):
+            starts.copy_(ints(st))
+            lengths.copy_(ints(ln))
+            y.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            got = y.clone()
+            check(s, [2, 1, 3], 4, "f16", rows=7)
+            y.zero_()
+            be.attention(s.cache, 0, batch, q, y)
+            torch.cuda.synchronize()
+            assert torch.equal(got, y) and (got[:st[-1]] != 0).any() and (got[st[-1]:] == 0).all()
+        s.close()
+    finally:
+        be.close()
+
+
+@gpu
+def test_two_contexts_on_one_cache(backend):
+    """Another context appends to and reads pages of its own, on a stream of its own, while the first attends to others."""
+    other = Backend(0)
+    try:
+        s = Cached(backend, "q8", [3000, 800], kv_heads=2, dim=128, page=64, spare=20)
+        free = sorted(set(range(s.cache.pages)) - set(s.tables.flatten().tolist()))
+        ints = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")
+        k, v = normal((500, 2, 128), 1, "f16"), normal((500, 2, 128), 2, "f16")
+        q = normal((500, 8, 128), 3, "f16")
+        b = other.cache_batch(ints([0, 500]), ints([500]), ints([free[:8]]), 500)
+        want = torch.empty_like(q)
+        backend.cache_append(s.cache, 0, b, None, k, v)
+        backend.attention(s.cache, 0, b, q, want)
+        side = torch.cuda.Stream()
+        first = check(s, [4, 3], 4, "f16")
+        mine = normal((7, 8, 128), 9, "f16")
+        got, y = torch.empty_like(q), torch.empty_like(mine)
+        batch = s.batch([4, 3])
+        torch.cuda.synchronize()
+        for _ in range(20):
+            other.cache_append(s.cache, 0, b, None, k, v, stream=side.cuda_stream)
+            other.attention(s.cache, 0, b, q, got, stream=side.cuda_stream)
+            backend.attention(s.cache, 0, batch, mine, y)
+        torch.cuda.synchronize()
+        assert torch.equal(got, want) and torch.equal(y, first)
+        s.close()
+    finally:
+        other.close()
+
+
+@gpu
+def test_many_rows_of_batches_that_make_no_sense(backend):
+    """As above for calls of many rows; rows outside of the call's stay as they were."""
+    s = Cached(backend, "bf16", [2000, 64, 64], kv_heads=8, dim=64, page=32)
+    q = normal((1000, 32, 64), 1, "bf16")
+    guard = torch.full((1400, 32, 64), 9.0, dtype=torch.bfloat16, device="cuda")
+    ints = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    for starts, lengths in (([0, 1000, 0, 1000], [2000, 64, 64]), ([-5, 3, 4000, 2], [2000, 64, 64]), ([0, 1 << 30, -(1 << 30), 1000], [1 << 30, -7, 64]),
+                            ([0, 200, 600, 1000], [-(1 << 31), (1 << 31) - 1, 70])):
+        b = backend.cache_batch(ints(starts), ints(lengths), s.tables, 1000, 1000)
+        backend.attention(s.cache, 0, b, q, guard[200:1200])
+        torch.cuda.synchronize()
+        assert (guard[:200] == 9.0).all() and (guard[1200:] == 9.0).all()
+    check(s, [900, 1, 2], 4, "bf16")
+    s.close()
+
+
+@gpu
+@pytest.mark.parametrize("rows", [3, 300])
+def test_the_plain_binding_gives_the_same(backend, monkeypatch, rows):
+    """Without the native call path: the same bits, the same refusals; a cache that was freed is refused by both."""
+    from cyb_amd import backend as module
+    from cyb_amd.backend import CybqError
+    s = Cached(backend, "q8", [rows + 50], kv_heads=2, dim=64, page=32)
+    wide, rope = normal((rows, 8, 64), 3, "f16"), rope_table(s.tables.shape[1] * 32, 64)
+    outs = []
+
+    def status(call):
+        with pytest.raises(CybqError) as e:
+            call()
+        return e.value.status
+
+    for native in (True, False):
+        if not native:
+            monkeypatch.setattr(module, "_calls", False)
+        batch, q = s.batch([rows]), torch.empty((rows, 4, 64), dtype=torch.float16, device="cuda")
+        y, k, v = torch.empty_like(q), torch.empty((rows, 2, 64), device="cuda"), torch.empty((rows, 2, 64), device="cuda")
+        backend.cache_append(s.cache, 0, batch, wide[:, :4], wide[:, 4:6], wide[:, 6:], q, rope=rope, style="pairs")
+        backend.cache_read(s.cache, 0, batch, k, v)
+        backend.attention(s.cache, 0, batch, q, y, scale=0.2, window=40)
+        torch.cuda.synchronize()
+        refused = [status(lambda: backend.attention(s.cache, 1, batch, q, y)), status(lambda: backend.attention(s.cache, 0, batch, q[:, :3], y[:, :3])),
+                   status(lambda: backend.attention(s.cache, 0, batch, q, y.float())), status(lambda: backend.attention(s.cache, 0, batch, q, y, scale=-1.0)),
+                   status(lambda: backend.attention(s.cache, 0, batch, q, y, window=-1)), status(lambda: backend.attention(s.cache, 0, batch, q[:rows - 1], y)),
+                   status(lambda: backend.attention(s.cache, 0, batch, q, y.cpu())), status(lambda: backend.cache_read(s.cache, 0, batch, k, v[:, :1])),
+                   status(lambda: backend.cache_append(s.cache, 0, batch, None, k, v.half())), status(lambda: backend.cache_append(s.cache, 0, batch, wide[:, :4], k, v)),
+                   status(lambda: backend.cache_append(s.cache, 0, batch, None, k, v, rope=rope[:32]))]
+        gone = backend.kv_cache("q8", 1, 2, 64, 32, 4)
+        gone.free()
+        refused.append(status(lambda: backend.cache_read(gone, 0, batch, k, v)))
+        outs.append((q, y, k, v, refused))
+    assert all(torch.equal(a, b) for a, b in zip(outs[0][:4], outs[1][:4])) and outs[0][4] == outs[1][4] and 0 not in outs[0][4]
+    s.close()
+
+
+@gpu
+def test_nothing_to_do(backend):
+    """No sequences, no rows, sequences without new rows: nothing is written, and nothing refused."""
+    s = Cached(backend, "f16", [64, 64], kv_heads=1, dim=64, page=32)
+    ints = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    y = torch.full((4, 2, 64), 9.0, dtype=torch.float16, device="cuda")
+    k = torch.full((4, 1, 64), 9.0, dtype=torch.float16, device="cuda")
+    for b in (backend.cache_batch(ints([0]), ints([]), s.tables[:0], 4), backend.cache_batch(ints([0, 0, 0]), ints([64, 64]), s.tables, 0),
+              backend.cache_batch(ints([0, 0, 0]), ints([64, 64]), s.tables, 4), backend.cache_batch(ints([0, 0, 0]), ints([64, 64]), s.tables, 4, 1000)):
+        backend.cache_append(s.cache, 0, b, torch.zeros_like(y), torch.zeros_like(k), torch.zeros_like(k), y)
+        backend.cache_read(s.cache, 0, b, k, k.clone())
+        backend.attention(s.cache, 0, b, torch.zeros_like(y), y)
+        torch.cuda.synchronize()
+        assert (y == 9.0).all() and (k == 9.0).all()
+    check(s, [2, 1], 2, "f16")
+    s.close()
