@@ -30,7 +30,6 @@ struct AttnArgs {
     float* slabs;
     unsigned* tickets;
     int group, qdt, window, target, least;       // workgroups of a round; blocks of a part, at least
-    float rounds;                                // of workgroups, where there are more tiles than one has
     int few;                                     // > 0: sequences of up to so many rows per kv head are the rows kernel's, others not
     float scale;                                 // times log2 e
 };
@@ -41,16 +40,16 @@ constexpr int kMaxUnits = 1 << 24;               // of a call
 // stands behind 2^kShift: its largest stays below 2^15, and probabilities count down to 2^-28 of the largest.
 constexpr float kShiftF16 = 4.f, kLagF16 = 11.f, kLagBF16 = 16.f;
 
-// Workgroups of a round of the rows kernel (two to a CU), and how many parts there may be beyond one of each tile: rounds * target, twice that in
-// the tiles kernel, whose tiles may see half as much on average as the one that sees the most
+// Workgroups of a round of the rows kernel (two to a CU), and how many parts there may be beyond one of each tile: twice as many (in the tiles
+// kernel because tiles may see half as much on average as the one that sees the most)
 constexpr int kTarget = 512, kMostExtra = 2 * kTarget;
-// Rounds where there are tiles for more than half of one already.  Rows kernel, 48 conversations of up to 8192 tokens: 1, 2, 4, 8 rounds 111, 103,
-// 108, 120 us.  Tiles kernel, prompts: the parts of half a round are those of the few tiles that see much more than others (2000 rows of heads of 64
-// 35 us, 0.75 and 1 round 47; of 128 60 and 83; sequences of 700 to 5000 tokens none 124, 0.25 65, 0.5 58, 1 90).
-constexpr float kRounds = 2.f, kTileRounds = 0.5f;
+constexpr float kRounds = 2.f;                   // (rows kernel)
 constexpr int kLeast = 4, kTileLeast = 8;        // blocks of a part
-// A tile of the tiles kernel has up to sqrt(kJoin * its blocks) parts: each adds 1.5 us to the time that the last of them takes to join (300 tokens alone,
-// 0.1 and 0.2: 18 us, 0.4 and more: 26; 96 rows of 4000 tokens 51, 45, 45, with no limit 64; 1000 rows 34, 37, 37)
+// Tiles kernel.  A tile is cut where that makes it kJoinBlocks shorter: storing the parts, waiting for the last and adding them takes about that long
+// (prompts of one sequence, 28, 40 blocks: 1800 tokens of heads of 128 76, 54 us, 2000 85, 60, 2000 of heads of 64 48, 33; 16: 1000 tokens 40, 34), into
+// up to sqrt(kJoin * its blocks) parts: each adds 1.5 us to what the last of them has to do (96 rows of 4000 tokens 0.1, 0.2, 0.4: 51, 45, 45 us, with
+// no limit 64).
+constexpr int kJoinBlocks = 40;
 constexpr float kJoin = 0.2f;
 
 // Rows of a sequence and kv head (new tokens times group) that the rows kernel takes.  Where there are few in all, many too: the other kernel's
@@ -133,23 +132,47 @@ __device__ __forceinline__ bool find_unit(const AttnArgs& a, int u, Unit* out)
     }
     work = wave_total(work) * (float)heads;
     tiles = wave_total(tiles) * (float)heads;
-    // Every tile begins a part of its own, so what is to be had in one round of workgroups are `target` less the tiles; where that is less than half
-    // of a round, rounds follow each other anyway and parts are made for their balance (48 conversations of up to 8192 tokens, rows kernel: 1, 2, 4, 8
-    // rounds 111, 103, 108, 120 us).  (A little more, so that what is rounded never makes
-    // more parts than the slabs hold.)
-    const float more = (float)a.target - tiles, extra = more >= 0.5f * (float)a.target ? more : a.rounds * (float)a.target;
-    const int part = max(a.least, (int)fminf(work / extra * 1.0001f + 1.0f, 1.0e9f));
+    int part;
+    if constexpr (!MANY) {
+        // Every tile begins a part of its own, so what is to be had in one round of workgroups are `target` less the tiles; where that is less than half
+        // of a round, rounds follow each other anyway and parts are made for their balance (48 conversations of up to 8192 tokens: 1, 2, 4, 8 rounds 111,
+        // 103, 108, 120 us).  (A little more, so that what is rounded never makes more parts than the slabs hold.)
+        const float more = (float)a.target - tiles, extra = more >= 0.5f * (float)a.target ? more : kRounds * (float)a.target;
+        part = max(a.least, (int)fminf(work / extra * 1.0001f + 1.0f, 1.0e9f));
+    } else {
+        // Only what is longer than a workgroup's share by kJoinBlocks is cut; where the tiles are one round, into the shortest parts that still are.
+        const float share = work / (float)a.target;
+        part = max(a.least, (int)fminf(share * 1.0001f + (float)(kJoinBlocks + 1), 1.0e9f));
+        if (a.t.seqs <= 64 && tiles <= (float)a.target && __ballot((float)x.blocks - share >= (float)kJoinBlocks)) {
+            for (int k = 0; k < 5; k++) {
+                const int shorter = max(a.least, (int)(share * (1.0f + 0.1f * (float)k)) + 1);
+                const float all = wave_total((float)(x.tiles * heads) * __builtin_ceilf((float)x.blocks * __builtin_amdgcn_rcpf((float)shorter)));
+                if (all <= (float)a.target) {
+                    part = min(part, shorter);
+                    break;
+                }
+            }
+        }
+    }
     int64_t units = 0;
     int slabs = 0, tickets = 0;
     bool found = false;
     for (int base = 0; base < a.t.seqs; base += 64) {
         if (base) x = share_of<ROWS, MANY>(a, base + lane, capacity);
         int splits = x.tiles ? max(1, (x.blocks + part - 1) / part) : 0;
-        if (MANY) splits = min(splits, max(1, (int)__builtin_sqrtf(kJoin * (float)x.blocks)));
+        if (MANY) {
+            splits = min(splits, max(1, (int)__builtin_sqrtf(kJoin * (float)x.blocks)));
+            if (splits > 1 && x.blocks - x.blocks / splits < kJoinBlocks) splits = 1;
+        }
         // (a batch whose starts make no sense may add up to anything: what cannot be right stays above every grid)
         const int rows = min(x.tiles * heads, kMaxUnits + 1), mine = (int)min((int64_t)rows * splits, (int64_t)kMaxUnits + 1);
         const int upto = wave_prefix(mine), slab_upto = wave_prefix(splits > 1 ? mine : 0), ticket_upto = wave_prefix(splits > 1 ? rows : 0);
         const int total = __builtin_amdgcn_readlane(upto, 63);
+        // All in one round, two workgroups to a CU: next to the one that sees the most goes the one that sees the least
+        if (MANY && a.t.seqs <= 64 && total <= a.target && u < total) {
+            const int half = a.target / 2 / heads * heads;
+            if (u >= half) u = total - heads - (u - half) / heads * heads + (u - half) % heads;
+        }
         if (!found && u < units + total) {
             found = true;
             const int l = __builtin_ctzll(__ballot((int)units + upto > u));
@@ -1137,14 +1160,12 @@ hipError_t attention_as(AttnArgs a, bool exact, hipStream_t st)
     if (!many || a.few) {
         a.target = kTarget;
         a.least = kLeast;
-        a.rounds = kRounds;
         const int64_t tiles = std::min(rows / kRows + a.t.seqs, a.few ? (int64_t)a.t.seqs * ((few + kRows - 1) / kRows) : rows);
         e = rows_as<KIND, G>(a, grid(tiles, kMostExtra), st);
     }
     if (many && e == hipSuccess) {
         a.target = TileShape<KIND, G>::kTarget;
         a.least = kTileLeast;
-        a.rounds = kTileRounds;
         e = tiles_as<KIND, G>(a, grid(rows / TileShape<KIND, G>::kRows + a.t.seqs, TileShape<KIND, G>::kMostExtra), st);
     }
     return e;
