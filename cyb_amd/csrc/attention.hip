@@ -228,7 +228,7 @@ __device__ __forceinline__ float row_power(float top, float* c)
 {
     const int e = (int)(__builtin_bit_cast(uint32_t, top) >> 23);
     const int up = e == 0 || e == 255 ? 0 : max(-126, min(126, 141 - e));           // 2^up, and 2^-up, are normal numbers
-    *c *= __builtin_bit_cast(float, (uint32_t)(127 - up) << 23);
+    *c = fmaxf(*c * __builtin_bit_cast(float, (uint32_t)(127 - up) << 23), 0x1p-126f);     // (never 0: a hidden score times it stays -inf)
     return __builtin_bit_cast(float, (uint32_t)(127 + up) << 23);
 }
 
@@ -1214,7 +1214,7 @@ hipError_t launch_attention(const CacheView& c, const BatchView& t, const void* 
     a.group = group;
     a.qdt = qdt;
     a.window = window;
-    a.scale = scale * 1.44269504088896340736f;
+    a.scale = std::max(scale * 1.44269504088896340736f, 0x1p-126f);
 #define CYBQ_ROWS(KIND)                                   \
     switch (c.dim) {                                      \
         case 64: return attention_as<KIND, 2>(a, exact, st); \

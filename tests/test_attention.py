@@ -443,3 +443,25 @@ def test_nothing_to_do(backend):
         assert (y == 9.0).all() and (k == 9.0).all()
     check(s, [2, 1], 2, "f16")
     s.close()
+
+
+@gpu
+@pytest.mark.parametrize("kind,dt", KINDS)
+def test_one_kv_head_for_hundreds(backend, kind, dt):
+    """Groups wider than a tile of either kernel, so that a token's heads are several tiles."""
+    s = Cached(backend, kind, [700, 90], kv_heads=1, dim=64, page=32)
+    for group in (71, 600):
+        check(s, [1, 2], group, dt)
+    s.close()
+
+
+@gpu
+@pytest.mark.parametrize("new", [3, 200])
+def test_factors_that_vanish(backend, new):
+    """Rows and scales so small that a score's factor is below fp32: every token weighs the same, and hidden ones nothing."""
+    for kind in ("q8", "q4", "bf16"):
+        s = Cached(backend, kind, [300], kv_heads=1, dim=64, page=32)
+        q = normal((new, 4, 64), 2, "bf16", std=1e-30)
+        check(s, [new], 4, "bf16", q=q, scale=1e-25, window=100)
+        check(s, [new], 4, "bf16", q=normal((new, 4, 64), 2, "bf16"), scale=1e-44, window=100)
+        s.close()
