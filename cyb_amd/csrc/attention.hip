@@ -770,7 +770,7 @@ struct Stage {
 // Many rows: a workgroup's waves have 32 rows each and go through the same blocks, 64 tokens (a head of 256: 32) a step.  While P of a step
 // is formed the scores of the next are multiplied: its keys are in LDS one step earlier than its values.  Bound by issue: matrix instructions
 // are 57 % of a SIMD's cycles, vector instructions 50, and the card clocks down to 1.64 GHz under them (4096 rows, 32 heads of 128, after 28672 tokens of F16:
-// 1850 - 1930 us = 1.07 - 1.11 PFLOP/s; the library's product of 8192 x 8192 x 8192 1.27).  Q8: each value is also unpacked, once for 256 rows (512 rows
+// 1850 - 1975 us = 1.04 - 1.11 PFLOP/s; the library's product of 8192 x 8192 x 8192 1.27).  Q8: each value is also unpacked, once for 256 rows (512 rows
 // after 15872 tokens 175 us = 0.78 PFLOP/s).  Short prompts are as long as the tile that sees the most (2000 rows, heads of 64: 34 us, 25 of them
 // that tile's 32 steps).
 template <int KIND, int G>
