@@ -11,6 +11,7 @@
 // rounding stands alone (48 conversations: 3.5e-4 off with one number, 2.9e-4 with two, 2.1e-4 of them y's own; no slower, memory is what such
 // calls wait for); rows of bf16 become f16 behind a power of two.
 #include <algorithm>
+#include <type_traits>
 
 #include "cache_parts.h"
 #include "cybq_internal.h"
@@ -579,60 +580,86 @@ __global__ __launch_bounds__(64 * RowsShape<G>::kWaves, G <= 4 ? 2 : 1) void att
     if (u.splits == 1) return;
     if (threadIdx.x < 16) put_float2(slab + kRows * DIM + 2 * r, top, sum);
     if (!last_part(a, u, reinterpret_cast<unsigned*>(lds))) return;
-    // The rows of all parts: threads share out the rows' float4s, and the parts where there are more threads; everything is asked for at once.
-    constexpr int THREADS = 64 * kWaves, QUADS = DIM / 4, AHEAD = 8;
+    // The rows of all parts: threads share out the rows' float4s, and the parts where there are more threads; everything is asked for at once (of
+    // more than 8 rows of 128 two float4s to a thread and six parts: a second round would wait for memory again, 1.3 us).
+    constexpr int THREADS = 64 * kWaves, QUADS = DIM / 4;
     const int items = rows * QUADS, runs = max(1, THREADS / items);
     const float* const of_tile = slab - (size_t)u.split * SLAB;
-    for (int it0 = 0; it0 < items; it0 += THREADS) {                  // (one round for up to 8 rows of 128)
-        const int run = runs == 1 ? 0 : threadIdx.x / items, it = it0 + threadIdx.x - run * items;
-        const bool mine = it < items && run < runs;
-        const int row = mine ? it / QUADS : 0, quad = mine ? it - row * QUADS : 0;
-        float m2 = none, l2 = 0.f;
-        float4_t o = {0.f, 0.f, 0.f, 0.f};
-        for (int e0 = run; e0 < u.splits && mine; e0 += AHEAD * runs) {
-            float4_t part[AHEAD];
-            f32x2_t of[AHEAD];
+    auto join = [&](auto at_once, auto parts_ahead) __attribute__((always_inline)) {
+        constexpr int N = decltype(at_once)::value, AHEAD = decltype(parts_ahead)::value;
+        for (int it0 = 0; it0 < items; it0 += N * THREADS) {
+            const int run = N > 1 || runs == 1 ? 0 : threadIdx.x / items;
+            bool mine[N];
+            int row[N], quad[N];
+            float m2[N], l2[N];
+            float4_t o[N];
 #pragma unroll
-            for (int e = 0; e < AHEAD; e++) {
-                const float* const from = of_tile + (size_t)min(e0 + e * runs, u.splits - 1) * SLAB;
-                part[e] = get_float4(from + row * DIM + 4 * quad);
-                of[e] = get_float2(from + kRows * DIM + 2 * row);
+            for (int n = 0; n < N; n++) {
+                const int it = it0 + n * THREADS + threadIdx.x - run * items;
+                mine[n] = it < items && run < runs;
+                row[n] = mine[n] ? it / QUADS : 0;
+                quad[n] = mine[n] ? it - row[n] * QUADS : 0;
+                m2[n] = none;
+                l2[n] = 0.f;
+                o[n] = float4_t{0.f, 0.f, 0.f, 0.f};
             }
-            float now = m2;
+            for (int e0 = run; e0 < u.splits && mine[0]; e0 += AHEAD * runs) {
+                float4_t part[N][AHEAD];
+                f32x2_t of[N][AHEAD];
 #pragma unroll
-            for (int e = 0; e < AHEAD; e++) now = fmaxf(now, of[e][0]);
-            const float old = m2 == none ? 0.f : exp2_fast(m2 - now);
-            o *= old;
-            l2 *= old;
-            m2 = now;
+                for (int e = 0; e < AHEAD; e++) {
+                    const float* const from = of_tile + (size_t)min(e0 + e * runs, u.splits - 1) * SLAB;
 #pragma unroll
-            for (int e = 0; e < AHEAD; e++) {
-                const float fe = of[e][0] == none || e0 + e * runs >= u.splits ? 0.f : exp2_fast(of[e][0] - now);
-                o += part[e] * fe;
-                l2 += e0 + e * runs >= u.splits ? 0.f : of[e][1] * fe;
+                    for (int n = 0; n < N; n++) {
+                        part[n][e] = get_float4(from + row[n] * DIM + 4 * quad[n]);
+                        of[n][e] = get_float2(from + kRows * DIM + 2 * row[n]);
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < N; n++) {
+                    float now = m2[n];
+#pragma unroll
+                    for (int e = 0; e < AHEAD; e++) now = fmaxf(now, of[n][e][0]);
+                    const float old = m2[n] == none ? 0.f : exp2_fast(m2[n] - now);
+                    o[n] *= old;
+                    l2[n] *= old;
+                    m2[n] = now;
+#pragma unroll
+                    for (int e = 0; e < AHEAD; e++) {
+                        const float fe = of[n][e][0] == none || e0 + e * runs >= u.splits ? 0.f : exp2_fast(of[n][e][0] - now);
+                        o[n] += part[n][e] * fe;
+                        l2[n] += e0 + e * runs >= u.splits ? 0.f : of[n][e][1] * fe;
+                    }
+                }
+            }
+            if (N == 1 && runs > 1) {                                // (all in one round)
+                float* const pairs = reinterpret_cast<float*>(lds + THREADS);
+                lds[threadIdx.x] = o[0];
+                pairs[2 * threadIdx.x] = m2[0];
+                pairs[2 * threadIdx.x + 1] = l2[0];
+                __syncthreads();
+                if (run) return;
+                for (int e = 1; e < runs; e++) {
+                    const int at = threadIdx.x + e * items;
+                    const float me = pairs[2 * at], now = fmaxf(m2[0], me);
+                    const float fo = m2[0] == none ? 0.f : exp2_fast(m2[0] - now), fe = me == none ? 0.f : exp2_fast(me - now);
+                    o[0] = o[0] * fo + lds[at] * fe;
+                    l2[0] = l2[0] * fo + pairs[2 * at + 1] * fe;
+                    m2[0] = now;
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < N; n++) {
+                if (!mine[n]) continue;
+                const int at = r0 + row[n], of_token = at / a.group;
+                const float by = l2[n] == 0.f ? 0.f : 1.0f / l2[n];
+                store_row4(a.y, a.qdt, (((int64_t)u.s.row0 + of_token) * a.c.kv_heads * a.group + u.head * a.group + at - of_token * a.group) * DIM + 4 * quad[n],
+                           o[n] * by);
             }
         }
-        if (runs > 1) {                                              // (all in one round)
-            float* const pairs = reinterpret_cast<float*>(lds + THREADS);
-            lds[threadIdx.x] = o;
-            pairs[2 * threadIdx.x] = m2;
-            pairs[2 * threadIdx.x + 1] = l2;
-            __syncthreads();
-            if (run) return;
-            for (int e = 1; e < runs; e++) {
-                const int at = threadIdx.x + e * items;
-                const float me = pairs[2 * at], now = fmaxf(m2, me);
-                const float fo = m2 == none ? 0.f : exp2_fast(m2 - now), fe = me == none ? 0.f : exp2_fast(me - now);
-                o = o * fo + lds[at] * fe;
-                l2 = l2 * fo + pairs[2 * at + 1] * fe;
-                m2 = now;
-            }
-        }
-        if (!mine) continue;
-        const int at = r0 + row, of_token = at / a.group;
-        const float by = l2 == 0.f ? 0.f : 1.0f / l2;
-        store_row4(a.y, a.qdt, (((int64_t)u.s.row0 + of_token) * a.c.kv_heads * a.group + u.head * a.group + at - of_token * a.group) * DIM + 4 * quad, o * by);
-    }
+    };
+    if (items > THREADS) join(std::integral_constant<int, 2>{}, std::integral_constant<int, 6>{});
+    else join(std::integral_constant<int, 1>{}, std::integral_constant<int, 8>{});
 }
 
 // ---- many rows ------------------------------------------------------------------------------------------------
