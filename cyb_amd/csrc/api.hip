@@ -1037,8 +1037,8 @@ int cybq_attention(cybq_ctx* ctx, const cybq_cache* cache, int64_t layer, const 
     if (cybq::attention_scratch_bytes(c.dim) > ctx->workspace_bytes - cybq::kDecodeScratchBytes) return fail(ctx, CYBQ_ERR_UNSUPPORTED, "scratch too small");
     DeviceGuard guard(ctx->device);
     if (guard.err != hipSuccess) return fail_hip(ctx, guard.err, "hipSetDevice");
-    const hipError_t e = cybq::launch_attention(c, t, q, q_stride, qdt, group, scale, (int)std::min<int64_t>(window, (int64_t)1 << 30), ctx->prefill_exact, y, ctx->workspace,
-                                                static_cast<char*>(ctx->workspace) + ctx->workspace_bytes, static_cast<hipStream_t>(stream));
+    const hipError_t e = cybq::launch_attention(c, t, q, q_stride, qdt, group, scale, (int)std::min<int64_t>(window, (int64_t)1 << 30), ctx->prefill_exact, y,
+                                                ctx->workspace, static_cast<char*>(ctx->workspace) + ctx->workspace_bytes, static_cast<hipStream_t>(stream));
     if (e != hipSuccess) return fail_hip(ctx, e, "attention launch");
     return CYBQ_OK;
 }

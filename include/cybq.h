@@ -203,7 +203,7 @@ int cybq_matmul_static(cybq_ctx* ctx, const cybq_weight* w, const void* x, cybq_
 
 /* Replaces: a backend configuration knob (the reference picks a backend per run:
  * `--backend honeycrisp|wgpu|cpu`, shell/src/worlds/models/mod.rs:113-115); here
- * it selects the numeric mode of the prefill kernel for this context. */
+ * it selects the numeric mode of the prefill kernel, and of cybq_attention, for this context. */
 int cybq_set_prefill_mode(cybq_ctx* ctx, cybq_prefill_mode mode);
 
 /* Same knob for the decode kernel (see cybq_decode_mode). */
