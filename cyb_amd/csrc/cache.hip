@@ -148,20 +148,25 @@ __device__ __forceinline__ void load_turned(const void* x, int64_t at, int ch, c
 struct Angles {
     float4_t cs[4];
     int c0, c1;                                               // eighths of the row
+    bool turns;
     __device__ __forceinline__ Angles(int j, const float* angles, int rot, bool halves)
     {
         const int turning = rot >> 4;
         c0 = 2 * j;
         c1 = 2 * j + 1;
         if (halves && j < turning) c0 = j, c1 = j + turning;
+        turns = angles && j < turning;
         const float4_t* p = reinterpret_cast<const float4_t*>(angles + 16 * j);
 #pragma unroll
-        for (int i = 0; i < 4; i++) cs[i] = angles && j < turning ? p[i] : float4_t{1.f, 0.f, 1.f, 0.f};
+        for (int i = 0; i < 4; i++) cs[i] = turns ? p[i] : float4_t{1.f, 0.f, 1.f, 0.f};
     }
     template <int DT>
     __device__ __forceinline__ void turned(const Eight<DT>& a, const Eight<DT>& b, bool halves, float x[8], float y[8]) const
     {
-        if (halves) {
+        if (!turns) {                                         // (not by an angle of 0: infinity times its sine is NaN, and -0 + 0 is 0)
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[e] = a[e], y[e] = b[e];
+        } else if (halves) {
 #pragma unroll
             for (int e = 0; e < 8; e++) turn(a[e], b[e], cs[e >> 1][2 * (e & 1)], cs[e >> 1][2 * (e & 1) + 1], &x[e], &y[e]);
         } else {

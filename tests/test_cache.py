@@ -359,3 +359,31 @@ def test_many_sequences_layers_and_copied_pages(backend):
     torch.cuda.synchronize()
     assert torch.equal(k.double(), s.k[tokens]) and torch.equal(v.double(), s.v[tokens])
     s.close()
+
+
+@gpu
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("new", [3, 40])
+def test_queries_that_do_not_turn_are_as_they_were(backend, dt, new):
+    """Infinities, NaN and signed zeros in dimensions that do not turn - all of them without angles, those behind rope_dims with - reach q_out as
+    they are, and none of them another dimension."""
+    kv, group, dim, page = 2, 3, 64, 32
+    s = Cached(backend, "q8", [50], kv_heads=kv, dim=dim, page=page)
+    for style, dims in (("none", 0), ("halves", 32), ("pairs", 16)):
+        x = normal((new, kv * group, dim), 7, dt)
+        for row in range(new):                                   # (every pair of neighbours and of halves meets each of them somewhere)
+            for head in range(kv * group):
+                at = dims + (5 * row + 11 * head) % (dim - dims)
+                x[row, head, at] = (math.inf, -math.inf, math.nan)[(row + head) % 3]
+                x[row, head, dims + (at - dims + 3) % (dim - dims)] = -0.0
+        rope = rope_table(s.tables.shape[1] * page, dims) if dims else None
+        k = normal((new, kv, dim), 8, dt)
+        want = turned(x, list(range(50 - new, 50)), rope, style)
+        for qdt in (torch.float16, torch.bfloat16):
+            q_out = torch.full((new, kv * group, dim), 9.0, dtype=qdt, device="cuda")
+            backend.cache_append(s.cache, 0, s.batch([new]), x, k, k, q_out, rope=rope, style="halves" if style == "none" else style)
+            torch.cuda.synchronize()
+            bad = torch.isnan(x)
+            assert torch.equal(torch.isnan(q_out), bad)
+            assert torch.equal(q_out.view(torch.int16)[~bad], want.to(qdt).view(torch.int16)[~bad])
+    s.close()
