@@ -30,7 +30,7 @@ struct AttnArgs {
     int64_t q_stride;
     float* slabs;
     unsigned* tickets;
-    int group, qdt, window, target, least;       // workgroups of a round; blocks of a part, at least
+    int group, qdt, window, target;              // target: workgroups of a round of the tiles kernel
     int few;                                     // > 0: sequences of up to so many rows per kv head are the rows kernel's, others not
     float scale;                                 // times log2 e
 };
@@ -138,15 +138,15 @@ __device__ __forceinline__ bool find_unit(const AttnArgs& a, int u, Unit* out)
         // Every tile begins a part of its own, so what is to be had in one round of workgroups are `target` less the tiles; where that is less than half
         // of a round, rounds follow each other anyway and parts are made for their balance (48 conversations of up to 8192 tokens: 1, 2, 4, 8 rounds 111,
         // 103, 108, 120 us).  (A little more, so that what is rounded never makes more parts than the slabs hold.)
-        const float more = (float)a.target - tiles, extra = more >= 0.5f * (float)a.target ? more : kRounds * (float)a.target;
-        part = max(a.least, (int)fminf(work / extra * 1.0001f + 1.0f, 1.0e9f));
+        const float more = (float)kTarget - tiles, extra = more >= 0.5f * (float)kTarget ? more : kRounds * (float)kTarget;
+        part = max(kLeast, (int)fminf(work / extra * 1.0001f + 1.0f, 1.0e9f));
     } else {
         // Only what is longer than a workgroup's share by kJoinBlocks is cut; where the tiles are one round, into the shortest parts that still are.
         const float share = work / (float)a.target;
-        part = max(a.least, (int)fminf(share * 1.0001f + (float)(kJoinBlocks + 1), 1.0e9f));
+        part = max(kTileLeast, (int)fminf(share * 1.0001f + (float)(kJoinBlocks + 1), 1.0e9f));
         if (a.t.seqs <= 64 && tiles <= (float)a.target && __ballot((float)x.blocks - share >= (float)kJoinBlocks)) {
             for (int k = 0; k < 5; k++) {
-                const int shorter = max(a.least, (int)(share * (1.0f + 0.1f * (float)k)) + 1);
+                const int shorter = max(kTileLeast, (int)(share * (1.0f + 0.1f * (float)k)) + 1);
                 const float all = wave_total((float)(x.tiles * heads) * __builtin_ceilf((float)x.blocks * __builtin_amdgcn_rcpf((float)shorter)));
                 if (all <= (float)a.target) {
                     part = min(part, shorter);
@@ -376,13 +376,12 @@ struct RowsShape {
 };
 
 template <int KIND, int G>
-__global__ __launch_bounds__(64 * RowsShape<G>::kWaves, G <= 4 ? 2 : 1) void attention_rows_kernel(AttnArgs a)
+__device__ __forceinline__ void rows_part(const AttnArgs& a, float4_t* lds)       // lds: [waves][DT][64], then [waves][16] maxima and sums
 {
     constexpr int kWaves = RowsShape<G>::kWaves;
     constexpr int DIM = 32 * G, BLOCK = cache_block_bytes(KIND, DIM), HALF = cache_half_bytes(KIND, DIM), DT = 2 * G;
     constexpr bool BF = KIND == kCacheBF16, SPLIT_P = KIND != kCacheF16;
     constexpr float kShift = BF ? 0.f : kShiftF16, kLag = BF ? kLagBF16 : kLagF16;
-    extern __shared__ float4_t lds[];                                 // [waves][DT][64], then [waves][16] maxima and sums
     float* const stats = reinterpret_cast<float*>(lds + kWaves * DT * 64);
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q4 = lane >> 4, r = lane & 15;
     const uint32_t magic = q4_magic_vgpr();
@@ -662,6 +661,13 @@ __global__ __launch_bounds__(64 * RowsShape<G>::kWaves, G <= 4 ? 2 : 1) void att
     else join(std::integral_constant<int, 1>{}, std::integral_constant<int, 8>{});
 }
 
+template <int KIND, int G>
+__global__ __launch_bounds__(64 * RowsShape<G>::kWaves, G <= 4 ? 2 : 1) void attention_rows_kernel(AttnArgs a)
+{
+    extern __shared__ float4_t lds[];
+    rows_part<KIND, G>(a, lds);
+}
+
 // ---- many rows ------------------------------------------------------------------------------------------------
 
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
@@ -692,7 +698,7 @@ struct TileShape {
     static constexpr int kPerCu = G > 4 || kWaves == 8 ? 1 : 2;              // workgroups
     static constexpr int kTarget = 256 * kPerCu, kMostExtra = 2 * kTarget;
     static constexpr int kHalf = kBlocks * kBlockTokens * 32 * G * 2;         // bytes of a step's keys, or values
-    static constexpr int kLds = 2 * kRing * kHalf;
+    static constexpr int kLds = std::max(2 * kRing * kHalf, RowsShape<G>::kLds);         // (a single sequence of few rows)
     static constexpr int kSlab = kRows * 32 * G + 2 * kRows;  // floats of a part
 };
 
@@ -811,7 +817,12 @@ __global__ __launch_bounds__((64 * TileShape<KIND, G>::kWaves), (TileShape<KIND,
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, r = lane & 31;
     const uint32_t magic = q4_magic_vgpr();
     Unit u;
-    if (!find_unit<ROWS, true>(a, blockIdx.x, &u)) return;
+    if (!find_unit<ROWS, true>(a, blockIdx.x, &u)) {
+        // A single sequence is launched once: that it has few rows only the device knows (a launch of the rows kernel beside this one: 2000 rows of
+        // heads of 64 33.8 -> 36.8 us)
+        if (a.t.seqs == 1 && wv < RowsShape<G>::kWaves && seq_of(a.t, 0).n * a.group <= a.few) rows_part<KIND, G>(a, lds);
+        return;
+    }
     const int64_t capacity = (int64_t)a.t.table_pages << (a.c.page_shift + 5);
     const int all_rows = u.s.n * a.group, p0 = u.s.len - u.s.n;
     const int w0 = u.tile * ROWS, wg_rows = min(ROWS, all_rows - w0);
@@ -1176,26 +1187,24 @@ hipError_t tiles_as(const AttnArgs& a, unsigned grid, hipStream_t st)
 template <int KIND, int G>
 hipError_t attention_as(AttnArgs a, bool exact, hipStream_t st)
 {
-    const int64_t most = (int64_t)a.t.max_new * a.group;
+    // (max_new and rows bound a sequence's rows, no more: one token of a padded call, or of one that was captured for prompts, is the rows kernel's)
+    const int64_t most = (int64_t)std::min(a.t.max_new, a.t.rows) * a.group;
     const int few = (int64_t)a.t.rows * a.group * a.c.kv_heads <= few_in_all(KIND) ? kFewAlone : kFewRows;
     const bool many = !exact && most > few;
-    a.few = many && a.t.seqs > 1 ? few : 0;                     // (a single sequence: the kernel that its largest call needs)
-    hipError_t e = hipSuccess;
+    a.few = many ? few : 0;
     const int64_t rows = (int64_t)a.t.rows * a.group, blocks = (int64_t)a.t.table_pages << a.c.page_shift;
     // tiles of all, and the parts beyond one of each: what `target` makes of them, and no more than the table has blocks for
-    auto grid = [&](int64_t tiles, int extra) { return (unsigned)(tiles * a.c.kv_heads + std::min<int64_t>(extra, tiles * a.c.kv_heads * (blocks / a.least))); };
-    if (!many || a.few) {
-        a.target = kTarget;
-        a.least = kLeast;
-        const int64_t tiles = std::min(rows / kRows + a.t.seqs, a.few ? (int64_t)a.t.seqs * ((few + kRows - 1) / kRows) : rows);
-        e = rows_as<KIND, G>(a, grid(tiles, kMostExtra), st);
-    }
-    if (many && e == hipSuccess) {
-        a.target = TileShape<KIND, G>::kTarget;
-        a.least = kTileLeast;
-        e = tiles_as<KIND, G>(a, grid(rows / TileShape<KIND, G>::kRows + a.t.seqs, TileShape<KIND, G>::kMostExtra), st);
-    }
-    return e;
+    auto grid = [&](int64_t tiles, int extra, int least) {
+        return (unsigned)(tiles * a.c.kv_heads + std::min<int64_t>(extra, tiles * a.c.kv_heads * (blocks / least)));
+    };
+    const int64_t few_tiles = std::min(rows / kRows + a.t.seqs, many ? (int64_t)a.t.seqs * ((few + kRows - 1) / kRows) : rows);
+    const unsigned few_grid = grid(few_tiles, kMostExtra, kLeast);
+    if (!many) return rows_as<KIND, G>(a, few_grid, st);
+    a.target = TileShape<KIND, G>::kTarget;
+    const unsigned many_grid = grid(rows / TileShape<KIND, G>::kRows + a.t.seqs, TileShape<KIND, G>::kMostExtra, kTileLeast);
+    if (a.t.seqs == 1) return tiles_as<KIND, G>(a, std::max(few_grid, many_grid), st);
+    const hipError_t e = rows_as<KIND, G>(a, few_grid, st);
+    return e == hipSuccess ? tiles_as<KIND, G>(a, many_grid, st) : e;
 }
 
 }  // namespace
