@@ -224,12 +224,16 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi)
     return as_u32(v);
 }
 
+// A score's factor is a normal number: of 0 a hidden score would be NaN, of infinity one of 0.  (Scores that are not 0 are multiples of 2^-48 on
+// quantised caches: where the largest factor takes the place of a larger one, one token has it all either way.)
+constexpr float kLeastFactor = 0x1p-126f, kMostFactor = 0x1.fffffep127f;
+
 // rows of bf16 as f16: the power of two that brings the row's largest to 2^14 .. 2^15; *c, the scores' factor, takes it off again
 __device__ __forceinline__ float row_power(float top, float* c)
 {
     const int e = (int)(__builtin_bit_cast(uint32_t, top) >> 23);
     const int up = e == 0 || e == 255 ? 0 : max(-126, min(126, 141 - e));           // 2^up, and 2^-up, are normal numbers
-    *c = fmaxf(*c * __builtin_bit_cast(float, (uint32_t)(127 - up) << 23), 0x1p-126f);     // (never 0: a hidden score times it stays -inf)
+    *c = fminf(fmaxf(*c * __builtin_bit_cast(float, (uint32_t)(127 - up) << 23), kLeastFactor), kMostFactor);
     return __builtin_bit_cast(float, (uint32_t)(127 + up) << 23);
 }
 
@@ -1250,7 +1254,7 @@ hipError_t launch_attention(const CacheView& c, const BatchView& t, const void* 
     a.group = group;
     a.qdt = qdt;
     a.window = window;
-    a.scale = std::max(scale * 1.44269504088896340736f, 0x1p-126f);
+    a.scale = std::min(std::max(scale * 1.44269504088896340736f, kLeastFactor), kMostFactor);
 #define CYBQ_ROWS(KIND)                                   \
     switch (c.dim) {                                      \
         case 64: return attention_as<KIND, 2>(a, exact, st); \

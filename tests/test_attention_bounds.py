@@ -1,10 +1,10 @@
-"""Attention over the paged cache in calls whose sizes say little about their rows.  Against float64; the bound of an element is that of
+"""Attention over the paged cache in calls whose sizes say little about their rows, with scales of any size.  Against float64; the bound of an element is that of
 test_attention.py."""
 import pytest
 
 torch = pytest.importorskip("torch")
-from tests.cache_lib import TDT, Cached, normal            # noqa: E402
-from tests.test_attention import FEW, KINDS, bound         # noqa: E402
+from tests.cache_lib import TDT, Cached, held, normal      # noqa: E402
+from tests.test_attention import FEW, KINDS, bound, check  # noqa: E402
 
 gpu = pytest.mark.gpu
 
@@ -48,4 +48,26 @@ def test_one_sequence_is_what_its_rows_make_it(backend, kind, dt):
 def test_each_sequence_of_a_mixed_call_has_its_own_bound(backend, kind, dt):
     s = Cached(backend, kind, [900, 300, 40, 700], kv_heads=8, dim=64, page=64)
     check_each(s, [400, 1, 5, 16], 4, dt, rows=430)
+    s.close()
+
+
+def set_tokens(s, k, v):
+    """The tokens of the only sequence of s: fp32 k, v [tokens, kv heads, dim]."""
+    s.be.cache_append(s.cache, s.layer, s.batch(s.lengths), None, k, v)
+    torch.cuda.synchronize()
+    s.k, s.v = held(s.kind, k), held(s.kind, v)
+
+
+@gpu
+@pytest.mark.parametrize("new", [3, 200])
+@pytest.mark.parametrize("kind,dt", KINDS)
+def test_scales_at_the_end_of_fp32(backend, kind, dt, new):
+    """Rows of zeros, or rows on keys of zeros, times the largest scales: every token weighs the same, hidden ones nothing."""
+    s = Cached(backend, kind, [300], kv_heads=1, dim=64, page=32)
+    zeros = torch.zeros((new, 4, 64), dtype=TDT[dt], device="cuda")
+    check(s, [new], 4, dt, q=zeros, scale=3e38, window=100)
+    set_tokens(s, torch.zeros((300, 1, 64), device="cuda"), normal((300, 1, 64), 3))
+    check(s, [new], 4, dt, q=normal((new, 4, 64), 4, dt), scale=3e38, window=100)
+    if dt == "bf16":
+        check(s, [new], 4, dt, q=normal((new, 4, 64), 4, dt).sign() * 1e38, scale=1e10, window=100)
     s.close()
