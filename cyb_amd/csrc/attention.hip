@@ -40,6 +40,7 @@ constexpr int kMaxUnits = 1 << 24;               // of a call
 // workgroup wait for (with a lag of 2^3 one step in seven, 512 rows of a Q8 cache after 15872 tokens took 216 us; with 2^11: 198).  P of f16
 // stands behind 2^kShift: its largest stays below 2^15, and probabilities count down to 2^-28 of the largest.
 constexpr float kShiftF16 = 4.f, kLagF16 = 11.f, kLagBF16 = 16.f;
+constexpr float kFar = 4096.f;                   // up to here a product of a score and its factor is off by at most 2^-13
 
 // Workgroups of a round of the rows kernel (two to a CU), and how many parts there may be beyond one of each tile: twice as many (in the tiles
 // kernel because tiles may see half as much on average as the one that sees the most)
@@ -517,12 +518,12 @@ __device__ __forceinline__ void rows_part(const AttnArgs& a, float4_t* lds)     
 #pragma unroll
             for (int d = 0; d < DT; d++) y[d] *= f;
         }
-        const float off = kShift - (m == none ? 0.f : m * c);
+        const float least = m == none ? 0.f : m;                      // (taken off before the factor comes in: m c may be known to no more than its 24 bits)
         Frag16 ph, pl;
         float pr[8];
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-            pr[e] = exp2_fast(__builtin_fmaf(s[e >> 2][e & 3], c, off));
+            pr[e] = exp2_fast(__builtin_fmaf(s[e >> 2][e & 3] - least, c, kShift));
             l += pr[e];
         }
 #pragma unroll
@@ -966,6 +967,10 @@ __global__ __launch_bounds__((64 * TileShape<KIND, G>::kWaves), (TileShape<KIND,
     for (int j = 0; j < R; j++) ring[j] = j * T::kHalf;
     float top = none;
     constexpr uint32_t ALL = (1u << BL) - 1u;
+    // The exponent is s c - m c in one instruction.  Where m c is so large that its rounding counts (far), m is taken off the scores first, and every
+    // step begins outside of the inner loop.
+    float off = kShift;
+    bool far = false;
     // whether some row does not see all of step t's tokens
     auto hides = [&](int t) {
         const int tok = (first + t * BL) * kBlockTokens;
@@ -1004,6 +1009,15 @@ __global__ __launch_bounds__((64 * TileShape<KIND, G>::kWaves), (TileShape<KIND,
         for (int d = 0; d < G; d++)
 #pragma unroll
             for (int e = 0; e < 16; e++) y[d][e] *= f;
+        const float largest = m == none ? 0.f : m;
+        far = __ballot(fabsf(largest * c) > kFar);
+        off = kShift - (far ? 0.f : largest * c);
+        if (far) {
+#pragma unroll
+            for (int b = 0; b < BL; b++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) s[b][e] -= largest;
+        }
         do {
             // P of step t while the values of step t - 1 are multiplied, and behind that the first scores of step t + 1 (of none: of what is in LDS,
             // and nobody looks at them).  A wave issues in order, and a 32 x 32 instruction takes as long as eight others: the order below puts
@@ -1031,7 +1045,6 @@ __global__ __launch_bounds__((64 * TileShape<KIND, G>::kWaves), (TileShape<KIND,
             };
             const uint32_t values_at = V0 + ring[R - 1], keys_at = K0 + ring[1];
             constexpr int PAIRS = 8 * BL, EARLY = BL == 2 ? 11 : PAIRS, LOOK = 6;
-            const float off = kShift - (m == none ? 0.f : m * c);
             Frag16 frag[2 * N], pn[2 * BL];
             // operands in the order of their use: values, then keys of the first block and of the second
             auto fetch = [&](int i) __attribute__((always_inline)) {
@@ -1102,7 +1115,7 @@ __global__ __launch_bounds__((64 * TileShape<KIND, G>::kWaves), (TileShape<KIND,
                 look_up(far_ids);
                 far_ids = pages_from(from_block + 64);
             }
-        } while (t < steps && !hides(t) && !__ballot(top > m + lag));
+        } while (t < steps && !far && !hides(t) && !__ballot(top > m + lag));
     }
     if (steps) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");             // (copies that nobody waited for do not outlive the workgroup's use of LDS)

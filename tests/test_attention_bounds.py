@@ -1,5 +1,5 @@
-"""Attention over the paged cache in calls whose sizes say little about their rows, with scales of any size.  Against float64; the bound of an element is that of
-test_attention.py."""
+"""Attention over the paged cache in calls whose sizes say little about their rows, and with scores of any
+size.  Against float64; the bound of an element is that of test_attention.py."""
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -9,9 +9,10 @@ from tests.test_attention import FEW, KINDS, bound, check  # noqa: E402
 gpu = pytest.mark.gpu
 
 
-def check_each(s, new, group, dt, window=0, scale=None, rows=None, max_new=None, q=None, seed=9, exact=False, unit=1.0):
+def check_each(s, new, group, dt, window=0, scale=None, rows=None, max_new=None, q=None, seed=9, exact=False, unit=1.0, exact_scores=False):
     """As `check`, each sequence against the bound of its own number of rows (exact: of few), values counted in `unit`.  Scores of any size: what
-    the exponent's argument and the factors that scale sums anew lose, at most 4 U of the largest score, is counted as four dimensions more."""
+    the exponent's argument and the factors that scale sums anew lose, at most 4 U of the largest score, is counted as four dimensions more; exact_scores:
+    they are equal or far apart, and nothing is lost."""
     rows = sum(new) if rows is None else rows
     q = normal((rows, s.kv_heads * group, s.dim), seed, dt) if q is None else q
     y = torch.full(q.shape, 9.0, dtype=TDT[dt], device="cuda")
@@ -19,6 +20,7 @@ def check_each(s, new, group, dt, window=0, scale=None, rows=None, max_new=None,
     torch.cuda.synchronize()
     used = sum(new)
     ref, size, dots = s.expected(q[:used], new, scale, window)
+    dots = dots * (0.0 if exact_scores else 1.0)
     many = torch.tensor([n * group > FEW and not exact for n in new for _ in range(n)], device="cuda").reshape(-1, 1, 1)
     most = torch.where(many, *(bound(s.kind, dt, s.dim + 4, ref / unit, size / unit, dots, m) * unit for m in (True, False)))
     assert torch.isfinite(y[:used]).all()
@@ -70,4 +72,46 @@ def test_scales_at_the_end_of_fp32(backend, kind, dt, new):
     check(s, [new], 4, dt, q=normal((new, 4, 64), 4, dt), scale=3e38, window=100)
     if dt == "bf16":
         check(s, [new], 4, dt, q=normal((new, 4, 64), 4, dt).sign() * 1e38, scale=1e10, window=100)
+    s.close()
+
+
+@gpu
+@pytest.mark.parametrize("new", [4, 200])
+@pytest.mark.parametrize("kind,dt", KINDS)
+@pytest.mark.parametrize("scale", [40.0, 4.1e3, 2.3e6, 1.7e9, 3e20, 1e36])
+def test_scores_at_the_end_of_fp32(backend, kind, dt, new, scale):
+    """Scores of up to 84 scales in fifteen stairs, 12 scales apart: those on a row's highest stair share it."""
+    L, dim = 3000, 64
+    s = Cached(backend, kind, [L], kv_heads=2, dim=dim, page=64)
+    k, v = normal((L, 2, dim), 3) * 0.25, normal((L, 2, dim), 4)
+    k[:, :, 1] = 15.875 if kind == "q8" else 7.0                 # (absmax of its group of 32: d = 1/8, or 1)
+    k[:, :, 0] = (torch.arange(L, device="cuda") * 15 // L - 7.0).reshape(-1, 1)
+    set_tokens(s, k, v)
+    q = torch.zeros((new, 6, dim), dtype=TDT[dt], device="cuda")
+    q[:, 0::2, 0], q[:, 1::2, 0], q[:, 4, 0] = 12.0, -12.0, 0.0
+    for window in (0, 1700):
+        check_each(s, [new], 3, dt, q=q, scale=scale, window=window, exact=kind != "bf16", exact_scores=True)
+    s.close()
+
+
+@gpu
+@pytest.mark.parametrize("new", [4, 200])
+@pytest.mark.parametrize("kind,dt", KINDS)
+@pytest.mark.parametrize("dim", [64, 96, 128, 256])
+def test_peaks_late_in_a_long_context(backend, kind, dt, dim, new):
+    """Scores that climb in fifteen stairs of 12 (2^17 each), or fall, or stand: sums are scaled anew at every stair, in parts and waves of their own.  Of a
+    row only one dimension is not 0, and the keys there are multiples of a power of two, so that no kind rounds them, nor do many rows: the bound of
+    few holds but for P of bf16."""
+    L = 3000
+    s = Cached(backend, kind, [L], kv_heads=2, dim=dim, page=64)
+    k, v = normal((L, 2, dim), 3) * 0.25, normal((L, 2, dim), 4)
+    k[:, :, 1] = 15.875 if kind == "q8" else 7.0                 # (absmax of its group of 32: d = 1/8, or 1)
+    k[:, :, 0] = (torch.arange(L, device="cuda") * 15 // L - 7.0).reshape(-1, 1)
+    set_tokens(s, k, v)
+    q = torch.zeros((new, 6, dim), dtype=TDT[dt], device="cuda")
+    q[:, 0::2, 0], q[:, 1::2, 0], q[:, 4, 0] = 12.0, -12.0, 0.0
+    q[1, :, 0] = 6.0
+    check_each(s, [new], 3, dt, q=q, scale=1.0, exact=kind != "bf16")
+    check_each(s, [new], 3, dt, q=q, scale=1.0, exact=kind != "bf16", window=1700)
+    check_each(s, [new], 3, dt, q=normal((new, 6, dim), 5, dt), scale=2.0)
     s.close()
