@@ -410,9 +410,10 @@ int cybq_cache_read(cybq_ctx* ctx, const cybq_cache* cache, int64_t layer, const
  *   q_heads is at most 65536, rows * q_heads / 16 + seqs * kv_heads at most 2^24 less 1024 (CYBQ_ERR_UNSUPPORTED); scale is positive and finite;
  *   scaled scores have to stay within fp32.
  * Scores, maxima and sums are fp32.  Values of Q8 and Q4 caches are round_f16(scale * q).  Up to 64 rows of a sequence and kv head (new
- * tokens times q_heads / kv_heads), any number with CYBQ_PREFILL_EXACT: keys are exact, and so are probabilities but on F16 caches (2^-11).  Of
- * more rows with CYBQ_PREFILL_FAST keys of Q8 and Q4 may be round_f16(scale * q) too, probabilities one number of f16 (a BF16 cache: bf16).  Calls on
- * one context share its scratch: they (replays of its graphs too) must not overlap in time. */
+ * tokens times q_heads / kv_heads), any number with CYBQ_PREFILL_EXACT: keys are exact, probabilities rounded by 2^-11 of themselves on an F16 cache,
+ * 2^-16 on BF16, 2^-22 on Q8 and Q4, and by 2^-37 of the row's largest (not on BF16).  Of more rows with CYBQ_PREFILL_FAST keys of Q8 and Q4 may be
+ * round_f16(scale * q) too, probabilities one number of f16: 2^-11, and 2^-29 of the largest (a BF16 cache: of bf16, 2^-8).
+ * Calls on one context share its scratch: they (replays of its graphs too) must not overlap in time. */
 int cybq_attention(cybq_ctx* ctx, const cybq_cache* cache, int64_t layer, const cybq_batch* batch, const void* q, int64_t q_stride,
                    cybq_dtype qdt, int64_t q_heads, float scale, int64_t window, void* y, void* stream);
 

@@ -1,5 +1,7 @@
-"""Attention over the paged cache in calls whose sizes say little about their rows, and with scores of any
-size.  Against float64; the bound of an element is that of test_attention.py."""
+"""Attention over the paged cache in calls whose sizes say little about their rows, with scores of any
+size, probabilities far apart.  Against float64; the bound of an element is that of test_attention.py."""
+import math
+
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -114,4 +116,31 @@ def test_peaks_late_in_a_long_context(backend, kind, dt, dim, new):
     check_each(s, [new], 3, dt, q=q, scale=1.0, exact=kind != "bf16")
     check_each(s, [new], 3, dt, q=q, scale=1.0, exact=kind != "bf16", window=1700)
     check_each(s, [new], 3, dt, q=normal((new, 6, dim), 5, dt), scale=2.0)
+    s.close()
+
+
+@gpu
+@pytest.mark.parametrize("kind,dt", KINDS)
+@pytest.mark.parametrize("below", [10.3, 17.3, 20.3, 23.3, 26.3])
+def test_many_small_probabilities_next_to_large_ones(backend, kind, dt, below):
+    """A token in every block whose probability is 2^below of the others', and whose value is nothing: y is what the others have, each as exact as its
+    own probability is.  Few rows, and many with the prefill mode EXACT."""
+    L, dim = 3000, 128
+    s = Cached(backend, kind, [L], kv_heads=1, dim=dim, page=64)
+    k, v = normal((L, 1, dim), 3), 64.0 + 8.0 * normal((L, 1, dim), 4)
+    k[:, :, 0] = 0.0
+    k[7::32], v[7::32] = 0.0, 0.0
+    k[7::32, :, 0] = 1.0
+    set_tokens(s, k, v)
+    top = s.k[7, 0, 0].item()
+    # y is about 31 tokens of 64 to each large one: 2^(11 - below), in f16 a subnormal number from 2^-14 down, whose half step is 2^-25
+    unit = 1.0 if dt == "f16" else 2.0 ** -below
+    for new in (2, 100):
+        q = torch.zeros((new, 2, dim), dtype=TDT[dt], device="cuda")
+        q[:, :, 0] = 4.0
+        backend.set_prefill_mode("exact")
+        try:
+            check_each(s, [new], 2, dt, q=q, scale=below * math.log(2.0) / 4.0 / top, exact=True, unit=unit)
+        finally:
+            backend.set_prefill_mode("fast")
     s.close()
