@@ -40,8 +40,10 @@ constexpr int kMaxUnits = 1 << 24;               // of a call
 // workgroup wait for (with a lag of 2^3 one step in seven, 512 rows of a Q8 cache after 15872 tokens took 216 us; with 2^11: 198).  P of f16
 // stands behind 2^kShift: its largest stays at 2^15, and a probability is exact to its bits down to 2^(-14 - kShift) of the largest, to 2^(-25 - kShift)
 // of the largest below.  The rows kernel's waves wait for nobody: there nearly all of f16's range is below the largest.
-constexpr float kShiftF16 = 4.f, kLagF16 = 11.f, kLagBF16 = 16.f;
+constexpr float kShiftF16 = 4.f, kLagF16 = 11.f;
 constexpr float kRowsShift = 12.f, kRowsLag = 3.f;            // (f16; a lag of 2^1 costs 8 drafts of 5 tokens 16.7 -> 16.8 us)
+// P of bf16 stays at 1 or below: sums of p |v| are never more than those of |v|, which may be anything that fp32 holds.
+constexpr float kShiftBF16 = -16.f, kLagBF16 = 16.f;
 constexpr float kFar = 4096.f;                   // up to here a product of a score and its factor is off by at most 2^-13
 
 // Workgroups of a round of the rows kernel (two to a CU), and how many parts there may be beyond one of each tile: twice as many (in the tiles
@@ -388,7 +390,7 @@ __device__ __forceinline__ void rows_part(const AttnArgs& a, float4_t* lds)     
     constexpr int kWaves = RowsShape<G>::kWaves;
     constexpr int DIM = 32 * G, BLOCK = cache_block_bytes(KIND, DIM), HALF = cache_half_bytes(KIND, DIM), DT = 2 * G;
     constexpr bool BF = KIND == kCacheBF16, SPLIT_P = KIND != kCacheF16;
-    constexpr float kShift = BF ? 0.f : kRowsShift, kLag = BF ? kLagBF16 : kRowsLag;
+    constexpr float kShift = BF ? kShiftBF16 : kRowsShift, kLag = BF ? kLagBF16 : kRowsLag;
     float* const stats = reinterpret_cast<float*>(lds + kWaves * DT * 64);
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q4 = lane >> 4, r = lane & 15;
     const uint32_t magic = q4_magic_vgpr();
@@ -818,7 +820,7 @@ __global__ __launch_bounds__((64 * TileShape<KIND, G>::kWaves), (TileShape<KIND,
 {
     typedef TileShape<KIND, G> T;
     constexpr int DIM = 32 * G, BLOCK = cache_block_bytes(KIND, DIM), ROWS = T::kRows, BL = T::kBlocks;
-    constexpr float kShift = KIND == kCacheBF16 ? 0.f : kShiftF16, kLag = KIND == kCacheBF16 ? kLagBF16 : kLagF16;
+    constexpr float kShift = KIND == kCacheBF16 ? kShiftBF16 : kShiftF16, kLag = KIND == kCacheBF16 ? kLagBF16 : kLagF16;
     extern __shared__ float4_t lds[];                                 // keys of kRing steps, values of as many
     uint8_t* const bytes = reinterpret_cast<uint8_t*>(lds);
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, r = lane & 31;

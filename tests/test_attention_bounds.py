@@ -1,5 +1,5 @@
 """Attention over the paged cache in calls whose sizes say little about their rows, with scores of any
-size, probabilities far apart.  Against float64; the bound of an element is that of test_attention.py."""
+size, probabilities and values far apart.  Against float64; the bound of an element is that of test_attention.py."""
 import math
 
 import pytest
@@ -143,4 +143,21 @@ def test_many_small_probabilities_next_to_large_ones(backend, kind, dt, below):
             check_each(s, [new], 2, dt, q=q, scale=below * math.log(2.0) / 4.0 / top, exact=True, unit=unit)
         finally:
             backend.set_prefill_mode("fast")
+    s.close()
+
+
+@gpu
+@pytest.mark.parametrize("new", [3, 300])
+@pytest.mark.parametrize("power", [110, 60, -60, -90])
+def test_values_of_bf16_far_from_one(backend, new, power):
+    """Values of 2^power, whose sum over the tokens is within fp32, under scores of 0 in some blocks and 10 in others: less apart than what a maximum may
+    lag by, so that probabilities stand far above the first block's."""
+    L, dim, kv = 40000, 64, 8
+    s = Cached(backend, "bf16", [L], kv_heads=kv, dim=dim, page=32)
+    k, v = torch.zeros((L, kv, dim), device="cuda"), (1.0 + 0.5 * normal((L, kv, dim), 4).clamp(-0.9, 0.9)) * 2.0 ** power
+    k[:, :, 0] = torch.where(normal((L // 32, kv), 6) < 0.0, 0.0, 10.0).repeat_interleave(32, dim=0)
+    set_tokens(s, k, v)
+    q = torch.zeros((new, 2 * kv, dim), dtype=torch.bfloat16, device="cuda")
+    q[:, :, 0] = 1.0
+    check_each(s, [new], 2, "bf16", q=q, scale=1.0, unit=2.0 ** power)
     s.close()
