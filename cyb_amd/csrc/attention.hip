@@ -1218,11 +1218,14 @@ hipError_t attention_as(AttnArgs a, bool exact, hipStream_t st)
     auto grid = [&](int64_t tiles, int extra, int least) {
         return (unsigned)(tiles * a.c.kv_heads + std::min<int64_t>(extra, tiles * a.c.kv_heads * (blocks / least)));
     };
-    const int64_t few_tiles = std::min(rows / kRows + a.t.seqs, many ? (int64_t)a.t.seqs * ((few + kRows - 1) / kRows) : rows);
+    // (a tile has a row, and a sequence of many rows more than `few`: a batch is mostly sequences without any, and each of a grid's workgroups looks
+    // at all of them)
+    const int64_t few_tiles = std::min({rows / kRows + a.t.seqs, many ? (int64_t)a.t.seqs * ((few + kRows - 1) / kRows) : rows, rows});
     const unsigned few_grid = grid(few_tiles, kMostExtra, kLeast);
     if (!many) return rows_as<KIND, G>(a, few_grid, st);
     a.target = TileShape<KIND, G>::kTarget;
-    const unsigned many_grid = grid(rows / TileShape<KIND, G>::kRows + a.t.seqs, TileShape<KIND, G>::kMostExtra, kTileLeast);
+    const int64_t many_tiles = rows / TileShape<KIND, G>::kRows + std::min<int64_t>(a.t.seqs, rows / (few + 1));
+    const unsigned many_grid = grid(many_tiles, TileShape<KIND, G>::kMostExtra, kTileLeast);
     if (a.t.seqs == 1) return tiles_as<KIND, G>(a, std::max(few_grid, many_grid), st);
     const hipError_t e = rows_as<KIND, G>(a, few_grid, st);
     return e == hipSuccess ? tiles_as<KIND, G>(a, many_grid, st) : e;
@@ -1230,8 +1233,16 @@ hipError_t attention_as(AttnArgs a, bool exact, hipStream_t st)
 
 }  // namespace
 
+// A launch has fewer than 2^32 threads.  Rows kernel: 256 to a unit.  Tiles kernel, per kv head: rows / kRows tiles and one more for each sequence of more
+// than kFewRows; rows of all heads are at most kRows kMaxUnits.
+int64_t attention_max_units() { return kMaxUnits - 1; }
+template <int KIND, int G>
+constexpr bool kLaunches = ((int64_t)kRows * kMaxUnits / TileShape<KIND, G>::kRows + (int64_t)kRows * kMaxUnits / (kFewRows + 1) + TileShape<KIND, G>::kMostExtra) *
+                               (64 * TileShape<KIND, G>::kWaves) < (int64_t)1 << 32;
+static_assert(kLaunches<kCacheF16, 2> && kLaunches<kCacheF16, 4> && kLaunches<kCacheF16, 8> && kLaunches<kCacheQ8, 2> && kLaunches<kCacheQ8, 8>, "a grid's threads");
+static_assert((int64_t)(kMaxUnits - 1) * 64 * RowsShape<2>::kWaves < (int64_t)1 << 32, "a grid's threads");
+
 // Parts of tiles that have more than one: at most twice those beyond one of each tile
-int64_t attention_max_units() { return kMaxUnits; }
 
 size_t attention_scratch_bytes(int dim)
 {

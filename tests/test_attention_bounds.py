@@ -161,3 +161,35 @@ def test_values_of_bf16_far_from_one(backend, new, power):
     q[:, :, 0] = 1.0
     check_each(s, [new], 2, "bf16", q=q, scale=1.0, unit=2.0 ** power)
     s.close()
+
+
+@gpu
+def test_batches_that_are_mostly_empty(backend):
+    """A prompt and single tokens among as many sequences as a call may have, next to many kv heads: a tile for every sequence and head would be
+    a launch of 2^32 threads."""
+    B, heads = 65536, 128
+    lengths = [0] * B
+    lengths[41] = 520
+    for i in range(20):
+        lengths[3000 * i + 77] = 10 * i + 1
+    lengths[B - 1] = 30
+    new = [500 if b == 41 else min(n, 1) for b, n in enumerate(lengths)]
+    s = Cached(backend, "q4", lengths, kv_heads=heads, dim=64, page=64)
+    check_each(s, new, 1, "f16", rows=600)
+    s.close()
+
+
+@gpu
+def test_the_largest_call(backend):
+    """rows * q_heads / 16 + seqs * kv_heads of 2^24 - 1024 are refused: one unit more than a launch has threads for."""
+    import ctypes
+    seqs, rows, heads = 7168, 4094, 65536
+    assert rows * heads // 16 + seqs == (1 << 24) - 1024
+    s = Cached(backend, "q4", [5], kv_heads=1, dim=64, page=32)
+    zeros = torch.zeros(seqs + 1, dtype=torch.int32, device="cuda")          # sequences without rows
+    b = backend.cache_batch(zeros, zeros[1:], zeros[1:].reshape(-1, 1), rows)
+    q, y = (torch.full((8, 64), 7.0, dtype=torch.float16, device="cuda") for _ in range(2))
+    status = backend._lib.cybq_attention(backend._ctx, s.cache.handle, 0, b._addr, q.data_ptr(), heads * 64, 1, heads, ctypes.c_float(1.0), 0, y.data_ptr(), None)
+    torch.cuda.synchronize()
+    assert status == -7 and (y == 7.0).all()
+    s.close()
