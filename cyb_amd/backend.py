@@ -25,6 +25,7 @@ import importlib.util
 import os
 import sys
 import warnings
+import weakref
 from dataclasses import dataclass, field
 from typing import Dict, Optional
 
@@ -269,6 +270,7 @@ class KVCache:
         backend._check(backend._lib.cybq_cache_info(self._h, kind, *n, memory))
         self.kind = next(k for k, v in CACHE_KINDS.items() if v == kind.value)
         self.layers, self.kv_heads, self.dim, self.page, self.pages, self.page_bytes, self.layer_bytes = (v.value for v in n)
+        backend._caches.add(self)
         self.memory = memory.value                      # page p of layer l: page_bytes at memory + l * layer_bytes + p * page_bytes
 
     @property
@@ -327,6 +329,7 @@ class Backend:
         self._addr = self._ctx.value
         self.device = device
         self.weights: Dict[str, QWeight] = {}
+        self._caches: "weakref.WeakSet[KVCache]" = weakref.WeakSet()     # those that close() frees
 
     # ---- plumbing
     def _check(self, rc: int) -> None:
@@ -338,6 +341,8 @@ class Backend:
         for w in list(self.weights.values()):
             w.free()
         self.weights.clear()
+        for c in list(self._caches):
+            c.free()
         if self._ctx:
             self._lib.cybq_destroy(self._ctx)
             self._ctx = ctypes.c_void_p()

@@ -387,3 +387,55 @@ def test_queries_that_do_not_turn_are_as_they_were(backend, dt, new):
             assert torch.equal(torch.isnan(q_out), bad)
             assert torch.equal(q_out.view(torch.int16)[~bad], want.to(qdt).view(torch.int16)[~bad])
     s.close()
+
+
+def test_a_backend_that_closes_frees_its_caches():
+    """cybq_cache_free for every cache that is still there, before cybq_destroy; not again afterwards, nor for one that was freed."""
+    import ctypes
+    import weakref
+    from cyb_amd import backend as B
+
+    class Library:
+        def __init__(self):
+            self.calls, self.made = [], 0
+
+        def cybq_cache_create(self, ctx, kind, layers, heads, dim, page, pages, out):
+            self.made += 1
+            ctypes.cast(out, ctypes.POINTER(ctypes.c_void_p))[0] = 4096 * self.made
+            return 0
+
+        def cybq_cache_info(self, h, kind, *rest):
+            kind.value = 8
+            return 0
+
+        def cybq_cache_free(self, ctx, h):
+            assert ctx.value == 64
+            self.calls.append(h.value)
+            return 0
+
+        def cybq_destroy(self, ctx):
+            self.calls.append("destroy")
+
+    be = B.Backend.__new__(B.Backend)
+    be._lib, be._ctx, be._addr, be.device, be.weights, be._caches = Library(), ctypes.c_void_p(64), 64, 0, {}, weakref.WeakSet()
+    first, second, third = (be.kv_cache("q8", 1, 2, 64, 64, 1) for _ in range(3))
+    second.free()
+    be.close()
+    assert be._lib.calls[0] == 8192 and sorted(be._lib.calls[1:3]) == [4096, 12288] and be._lib.calls[3:] == ["destroy"]
+    for c in (first, second, third):
+        c.free()
+        with pytest.raises(CybqError, match="already freed"):
+            c.handle
+    assert len(be._lib.calls) == 4
+
+
+@gpu
+def test_a_closed_backend_holds_no_cache():
+    be = Backend(0)
+    torch.cuda.synchronize()
+    before = torch.cuda.mem_get_info()[0]
+    cache = be.kv_cache("f16", 2, 8, 128, 64, 4096)              # 2 GiB
+    assert torch.cuda.mem_get_info()[0] < before - (1 << 30)
+    be.close()
+    assert torch.cuda.mem_get_info()[0] >= before
+    cache.free()
