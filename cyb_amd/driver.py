@@ -44,10 +44,17 @@ def ask(backend: Backend, st, prompt_tokens: int, new_tokens: int, chunk: int = 
     if prompt_tokens < 0 or new_tokens < 0 or chunk < 1 or batch < 1 or batch > 16:
         raise ValueError("prompt_tokens, new_tokens >= 0; chunk >= 1; 1 <= batch <= 16")
     cached = isinstance(st, stk.CachedStack)
+    if cached and (batch > st.conversations or prompt_tokens + new_tokens + 1 > st.context):
+        raise ValueError("the cache has fewer conversations, or pages for fewer tokens")
+    launch = torch.cuda.ExternalStream(stream, device=backend.device) if stream else torch.cuda.default_stream(backend.device)
+
+    def on_launch(f, *args, **kw):                             # torch's own work among the steps': buffers, lengths
+        with torch.cuda.stream(launch):
+            return f(*args, **kw)
+
+    torch.cuda.synchronize(backend.device)                     # the stack was made on whatever stream was current
     if cached:
-        if batch > st.conversations or prompt_tokens + new_tokens + 1 > st.context:
-            raise ValueError("the cache has fewer conversations, or pages for fewer tokens")
-        st.set_lengths(0)
+        on_launch(st.set_lengths, 0)
     read = prompt_tokens * batch if cached else prompt_tokens
     t_wall = time.time()
     yield {"Prefill": {"done": 0, "total": read}}
@@ -56,7 +63,7 @@ def ask(backend: Backend, st, prompt_tokens: int, new_tokens: int, chunk: int = 
 
     def step_for(M: int, xdtype):
         if M not in steps:
-            steps[M] = stk.stepper(st, M, shapes=shapes, xdtype=xdtype)
+            steps[M] = on_launch(stk.stepper, st, M, shapes=shapes, xdtype=xdtype)
         return steps[M]
 
     done = 0
@@ -64,9 +71,9 @@ def ask(backend: Backend, st, prompt_tokens: int, new_tokens: int, chunk: int = 
         M = min(chunk, prompt_tokens - done % prompt_tokens)
         step = step_for(M, torch.bfloat16 if M > 16 else torch.float16)
         a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
-        a.record()
+        a.record(launch)
         step(stream, done // prompt_tokens) if cached else step(stream)
-        b.record()
+        b.record(launch)
         b.synchronize()
         ms_in += a.elapsed_time(b)
         done += M
@@ -74,16 +81,16 @@ def ask(backend: Backend, st, prompt_tokens: int, new_tokens: int, chunk: int = 
 
     ms_out = 0.0
     if new_tokens:
-        step = st.stepper(batch, torch.float16, count=batch) if cached else step_for(batch, torch.float16)
+        step = on_launch(st.stepper, batch, torch.float16, count=batch) if cached else step_for(batch, torch.float16)
         step(stream)                                           # first touch of this plan's buffers, untimed
         torch.cuda.synchronize()
         if cached:
-            st.set_lengths(prompt_tokens, batch)
+            on_launch(st.set_lengths, prompt_tokens, batch)
         a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
-        a.record()
+        a.record(launch)
         for i in range(new_tokens):
             step(stream)
-        b.record()
+        b.record(launch)
         b.synchronize()
         ms_out = a.elapsed_time(b)
         for i in range(new_tokens):

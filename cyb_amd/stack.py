@@ -304,7 +304,8 @@ class CachedStack:
 
     def stepper(self, M: int, xdtype=None, count: int = 1, seed: int = 5):
         """step(stream, first): M new tokens, M / count for each of the conversations first .. first + count.  Tokens behind a conversation's
-        pages are not stored: counting them is the caller's affair."""
+        pages are not stored: counting them is the caller's affair.  Its buffers are made on torch's current stream, which steps on another one
+        have to wait for."""
         import torch
         if count < 1 or M % count:
             raise CybqError(-2, "bad shape", "the rows are shared by the conversations evenly")

@@ -206,3 +206,29 @@ def test_cpp_cache():
         pytest.fail("tests/cpp/_build/cache_test missing: run __graft_entry__.build()")
     out = subprocess.run([CACHE_TEST, "--run"], capture_output=True, text=True, timeout=100)
     assert out.returncode == 0 and out.stdout.startswith("stored same"), out.stdout + out.stderr
+
+
+@gpu
+def test_the_driver_on_a_stream_of_its_own(backend):
+    """Lengths that are set late - work is in front of them on the stream that they are set on - are there for the steps that count on them."""
+    from cyb_amd import driver, stack
+    st = stack.build_cached(backend, layers=1, kind="q8", conversations=2, context=80, heads=4, kv_heads=2, head_dim=64, width=256)
+    starts, lengths = (torch.tensor(v, dtype=torch.int32, device="cuda") for v in ([0, 53, 106], [53, 53]))
+    batch, kept = backend.cache_batch(starts, lengths, st.tables, 106), []
+    side, set_now = torch.cuda.Stream(), st.set_lengths
+
+    def set_late(*args):
+        torch.cuda._sleep(20_000_000)
+        set_now(*args)
+    st.set_lengths = set_late
+    for stream in (0, side.cuda_stream):
+        evs = list(driver.ask(backend, st, prompt_tokens=50, new_tokens=3, chunk=32, batch=2, stream=stream))
+        torch.cuda.synchronize()
+        assert st.lengths.tolist() == [53, 53] and evs[-1]["Answer"].tokens == 6
+        kv = [torch.empty((106, 2, 64), device="cuda") for _ in range(2)]
+        backend.cache_read(st.cache, 0, batch, *kv)
+        torch.cuda.synchronize()
+        kept.append(kv)
+        st.set_lengths(80)
+    assert torch.equal(kept[0][0], kept[1][0]) and torch.equal(kept[0][1], kept[1][1])
+    st.free()
