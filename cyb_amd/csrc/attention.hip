@@ -323,9 +323,16 @@ __device__ __forceinline__ Frag16 value_operand(const Half<KIND, G>& v, int dt, 
     return f;
 }
 
+// An f16 row is a mean of f16 values: what the rounding of its probabilities lifts past the largest of them is that number (NaN stays).
+__device__ __forceinline__ float within_f16(float x) { return x > 65504.f ? 65504.f : x < -65504.f ? -65504.f : x; }
+
 __device__ __forceinline__ void store_row4(void* y, int dt, int64_t at, float4_t v)
 {
     u32x2_t w;
+    if (dt == kF16) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] = within_f16(v[e]);
+    }
     if (dt == kF16) w = u32x2_t{pack_half2(v[0], v[1]), pack_half2(v[2], v[3])};
     else w = u32x2_t{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
     *reinterpret_cast<u32x2_t*>(static_cast<uint16_t*>(y) + at) = w;

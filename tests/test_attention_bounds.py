@@ -193,3 +193,22 @@ def test_the_largest_call(backend):
     torch.cuda.synchronize()
     assert status == -7 and (y == 7.0).all()
     s.close()
+
+
+@gpu
+@pytest.mark.parametrize("new", [3, 300])
+def test_values_at_the_end_of_f16_stay_finite(backend, new):
+    """A token in every block with twice the others' probability, less so little that P of f16 is rounded up by all that a rounding can be: on values of
+    the largest number y is that number, and not the infinity behind it."""
+    L = 700
+    s = Cached(backend, "f16", [L], kv_heads=2, dim=64, page=32)
+    k, v = torch.zeros((L, 2, 64), device="cuda"), torch.full((L, 2, 64), math.inf, device="cuda")
+    k[5::32, :, 0] = 1.0
+    v[:, 1] *= -1.0
+    set_tokens(s, k, v)
+    assert (s.v.abs() == 65504.0).all()
+    q = torch.zeros((new, 4, 64), dtype=torch.float16, device="cuda")
+    q[:, :, 0] = 1.0
+    y = check_each(s, [new], 2, "f16", q=q, scale=math.log(2.0) - math.log(1.0 + 1.05 * 2.0 ** -11))
+    assert (y.abs() >= 65504.0 * (1.0 - 2.0 ** -10)).all()
+    s.close()
