@@ -323,17 +323,19 @@ __device__ __forceinline__ Frag16 value_operand(const Half<KIND, G>& v, int dt, 
     return f;
 }
 
-// An f16 row is a mean of f16 values: what the rounding of its probabilities lifts past the largest of them is that number (NaN stays).
+// Rows on an F16 cache are means of f16 values: what the rounding of their probabilities lifts past the largest of them is that number (NaN
+// stays).  (Q8 and Q4 hold nothing near it, and fp32 sums of bf16 values none.)
 __device__ __forceinline__ float within_f16(float x) { return x > 65504.f ? 65504.f : x < -65504.f ? -65504.f : x; }
 
+template <int KIND>
 __device__ __forceinline__ void store_row4(void* y, int dt, int64_t at, float4_t v)
 {
     u32x2_t w;
-    if (dt == kF16) {
+    if constexpr (KIND == kCacheF16) {
 #pragma unroll
         for (int e = 0; e < 4; e++) v[e] = within_f16(v[e]);
     }
-    if (dt == kF16) w = u32x2_t{pack_half2(v[0], v[1]), pack_half2(v[2], v[3])};
+    if (KIND == kCacheF16 || dt == kF16) w = u32x2_t{pack_half2(v[0], v[1]), pack_half2(v[2], v[3])};
     else w = u32x2_t{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
     *reinterpret_cast<u32x2_t*>(static_cast<uint16_t*>(y) + at) = w;
 }
@@ -589,7 +591,7 @@ __device__ __forceinline__ void rows_part(const AttnArgs& a, float4_t* lds)     
 #pragma unroll
         for (int w = 1; w < kWaves; w++) o += lds[(w * DT + d) * 64 + lane] * f[w];
         if (!real) continue;
-        if (u.splits == 1) store_row4(a.y, a.qdt, row_at + 16 * d, o * inv);
+        if (u.splits == 1) store_row4<KIND>(a.y, a.qdt, row_at + 16 * d, o * inv);
         else put_float4(slab + r * DIM + 16 * d + 4 * q4, o);
     }
     if (u.splits == 1) return;
@@ -668,7 +670,7 @@ __device__ __forceinline__ void rows_part(const AttnArgs& a, float4_t* lds)     
                 if (!mine[n]) continue;
                 const int at = r0 + row[n], of_token = at / a.group;
                 const float by = l2[n] == 0.f ? 0.f : 1.0f / l2[n];
-                store_row4(a.y, a.qdt, (((int64_t)u.s.row0 + of_token) * a.c.kv_heads * a.group + u.head * a.group + at - of_token * a.group) * DIM + 4 * quad[n],
+                store_row4<KIND>(a.y, a.qdt, (((int64_t)u.s.row0 + of_token) * a.c.kv_heads * a.group + u.head * a.group + at - of_token * a.group) * DIM + 4 * quad[n],
                            o[n] * by);
             }
         }
@@ -1143,7 +1145,7 @@ __global__ __launch_bounds__((64 * TileShape<KIND, G>::kWaves), (TileShape<KIND,
             for (int d = 0; d < G; d++)
 #pragma unroll
                 for (int e = 0; e < 4; e++)
-                    store_row4(a.y, a.qdt, row_at + 32 * d + 8 * e, float4_t{y[d][4 * e] * inv, y[d][4 * e + 1] * inv, y[d][4 * e + 2] * inv, y[d][4 * e + 3] * inv});
+                    store_row4<KIND>(a.y, a.qdt, row_at + 32 * d + 8 * e, float4_t{y[d][4 * e] * inv, y[d][4 * e + 1] * inv, y[d][4 * e + 2] * inv, y[d][4 * e + 3] * inv});
         }
         return;
     }
@@ -1192,7 +1194,7 @@ __global__ __launch_bounds__((64 * TileShape<KIND, G>::kWaves), (TileShape<KIND,
     for (int d = 0; d < G; d++)
 #pragma unroll
         for (int e = 0; e < 4; e++)
-            store_row4(a.y, a.qdt, row_at + 32 * d + 8 * e, float4_t{y[d][4 * e] * inv, y[d][4 * e + 1] * inv, y[d][4 * e + 2] * inv, y[d][4 * e + 3] * inv});
+            store_row4<KIND>(a.y, a.qdt, row_at + 32 * d + 8 * e, float4_t{y[d][4 * e] * inv, y[d][4 * e + 1] * inv, y[d][4 * e + 2] * inv, y[d][4 * e + 3] * inv});
 }
 
 template <int KIND, int G>
