@@ -36,14 +36,14 @@ struct AttnArgs {
 };
 
 constexpr int kMaxUnits = 1 << 24;               // of a call
-// A maximum may lag behind the scores by 2^kLag before sums are scaled anew: every scaling is a detour of a wave that all others of its
-// workgroup wait for (with a lag of 2^3 one step in seven, 512 rows of a Q8 cache after 15872 tokens took 216 us; with 2^11: 198).  P of f16
-// stands behind 2^kShift: its largest stays at 2^15, and a probability is exact to its bits down to 2^(-14 - kShift) of the largest, to 2^(-25 - kShift)
-// of the largest below.  The rows kernel's waves wait for nobody: there nearly all of f16's range is below the largest.
-constexpr float kShiftF16 = 4.f, kLagF16 = 11.f;
-constexpr float kRowsShift = 12.f, kRowsLag = 3.f;            // (f16; a lag of 2^1 costs 8 drafts of 5 tokens 16.7 -> 16.8 us)
-// P of bf16 stays at 1 or below: sums of p |v| are never more than those of |v|, which may be anything that fp32 holds.
-constexpr float kShiftBF16 = -16.f, kLagBF16 = 16.f;
+// Probabilities are 2^((s - m) c + kShift): a row's m is its largest score, or near it, and may lag behind the scores by kLagF16 (in exponents) before sums
+// are scaled anew: every scaling is a detour of a wave that all others of its workgroup wait for (with a lag of 3 one step in seven, 512 rows of a Q8
+// cache after 15872 tokens took 216 us; with 11: 198).
+// P of f16 stays at 2^15 or below; it is exact to its bits from 2^-14 on and to 2^-25 below, of a row's largest 2^-18 and 2^-29 for many rows.  The rows
+// kernel's waves wait for nobody: m is put kRowsBelow below the largest, so that 2^-26 and 2^-37 of it are left (8 drafts of 5 tokens 16.5 -> 16.6 us).
+// P of bf16 has fp32's range: m is put kAhead above the largest, and sums of p |v| are never more than those of |v|, which may be anything that fp32 holds.
+constexpr float kShiftF16 = 4.f, kLagF16 = 11.f, kRowsBelow = 8.f;
+constexpr float kAhead = 16.f;
 constexpr float kFar = 4096.f;                   // up to here a product of a score and its factor is off by at most 2^-13
 
 // Workgroups of a round of the rows kernel (two to a CU), and how many parts there may be beyond one of each tile: twice as many (in the tiles
@@ -399,7 +399,7 @@ __device__ __forceinline__ void rows_part(const AttnArgs& a, float4_t* lds)     
     constexpr int kWaves = RowsShape<G>::kWaves;
     constexpr int DIM = 32 * G, BLOCK = cache_block_bytes(KIND, DIM), HALF = cache_half_bytes(KIND, DIM), DT = 2 * G;
     constexpr bool BF = KIND == kCacheBF16, SPLIT_P = KIND != kCacheF16;
-    constexpr float kShift = BF ? kShiftBF16 : kRowsShift, kLag = BF ? kLagBF16 : kRowsLag;
+    constexpr float kShift = BF ? 0.f : kShiftF16;
     float* const stats = reinterpret_cast<float*>(lds + kWaves * DT * 64);
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q4 = lane >> 4, r = lane & 15;
     const uint32_t magic = q4_magic_vgpr();
@@ -444,7 +444,7 @@ __device__ __forceinline__ void rows_part(const AttnArgs& a, float4_t* lds)     
                 for (int j = 0; j < 4; j++) qf[g].u[j] = pack_half2(x[8 * g + 2 * j] * f, x[8 * g + 2 * j + 1] * f);
         }
     }
-    const float lag = fminf(kLag / c, 1e30f);
+    const float lag = fminf((BF ? kAhead : kLagF16) / c, 1e30f);
     // my blocks are first + wv + kWaves i; a lane asks for the page of one of 64 of them, those that have one are worked on
     const int32_t* const table = a.t.tables + (int64_t)u.b * a.t.table_pages;
     const int in_page = (1 << a.c.page_shift) - 1;
@@ -523,8 +523,10 @@ __device__ __forceinline__ void rows_part(const AttnArgs& a, float4_t* lds)     
         float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
         top = fmaxf(top, other_quarter<16>(top));
         top = fmaxf(top, other_quarter<32>(top));
-        if (__ballot(top > m + lag)) {
-            const float now = top > m + lag ? top : m;
+        if (__ballot(top > (BF ? m : m + lag))) {
+            float to = BF ? top + lag : __builtin_fmaf(lag, -kRowsBelow / kLagF16, top);
+            if (!BF && top - to > lag) to = top;                      // (where fp32 scores are that far from each other)
+            const float now = top > (BF ? m : m + lag) ? to : m;
             const float f = m == none ? 0.f : exp2_fast((m - now) * c);
             m = now;
             l *= f;
@@ -829,7 +831,8 @@ __global__ __launch_bounds__((64 * TileShape<KIND, G>::kWaves), (TileShape<KIND,
 {
     typedef TileShape<KIND, G> T;
     constexpr int DIM = 32 * G, BLOCK = cache_block_bytes(KIND, DIM), ROWS = T::kRows, BL = T::kBlocks;
-    constexpr float kShift = KIND == kCacheBF16 ? kShiftBF16 : kShiftF16, kLag = KIND == kCacheBF16 ? kLagBF16 : kLagF16;
+    constexpr bool BF = KIND == kCacheBF16;
+    constexpr float kShift = BF ? 0.f : kShiftF16;
     extern __shared__ float4_t lds[];                                 // keys of kRing steps, values of as many
     uint8_t* const bytes = reinterpret_cast<uint8_t*>(lds);
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, r = lane & 31;
@@ -885,7 +888,7 @@ __global__ __launch_bounds__((64 * TileShape<KIND, G>::kWaves), (TileShape<KIND,
                     qf[k].u[j] = pack_half2(__builtin_bit_cast(float, qf[k].u[j] << 16) * f, __builtin_bit_cast(float, qf[k].u[j] & 0xffff0000u) * f);
         }
     }
-    const float lag = fminf(kLag / c, 1e30f);
+    const float lag = fminf((BF ? kAhead : kLagF16) / c, 1e30f);
     const int32_t* const table = a.t.tables + (int64_t)u.b * a.t.table_pages;
     const int in_page = (1 << a.c.page_shift) - 1;
     // Where the part's blocks lie, a lane for each of 64 from `from_block` on, counted from the part's first (a block that is not there is
@@ -1014,7 +1017,7 @@ __global__ __launch_bounds__((64 * TileShape<KIND, G>::kWaves), (TileShape<KIND,
         for (int i = 0; i < N; i++) y[i % G] = mfma32<KIND>(value_at(before, i / G, i % G), pf[i / G], y[i % G]);
 #pragma unroll
         for (int k = 0; k < 2 * BL; k++) pf[k].u = u32x4_t{0u, 0u, 0u, 0u};
-        const float up = top > m + lag ? top : m;
+        const float up = top > (BF ? m : m + lag) ? (BF ? top + lag : top) : m;
         const float f = m == none ? 0.f : exp2_fast((m - up) * c);
         m = up;
         l *= f;
@@ -1128,7 +1131,7 @@ __global__ __launch_bounds__((64 * TileShape<KIND, G>::kWaves), (TileShape<KIND,
                 look_up(far_ids);
                 far_ids = pages_from(from_block + 64);
             }
-        } while (t < steps && !far && !hides(t) && !__ballot(top > m + lag));
+        } while (t < steps && !far && !hides(t) && !__ballot(top > (BF ? m : m + lag)));
     }
     if (steps) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");             // (copies that nobody waited for do not outlive the workgroup's use of LDS)
