@@ -46,22 +46,25 @@ constexpr float kShiftF16 = 4.f, kLagF16 = 11.f, kRowsBelow = 8.f;
 constexpr float kAhead = 16.f;
 constexpr float kFar = 4096.f;                   // up to here a product of a score and its factor is off by at most 2^-13
 
-// Workgroups of a round of the rows kernel (two to a CU), and how many parts there may be beyond one of each tile: twice as many (in the tiles
-// kernel because tiles may see half as much on average as the one that sees the most)
+// Workgroups of a round of the rows kernel (two to a CU), and how many parts there may be beyond one of each tile: twice as many.  Grids, slabs and
+// tickets are made for these.  Rows kernel: a part is work / extra blocks or more, extra at most kRounds target, so that the tiles' blocks make that many
+// parts at most.  Tiles kernel: a part is work / target blocks or more, and work counts at least half of the blocks of each tile.  Parts that need a slab are
+// those of tiles with two or more: at most twice the parts beyond one of each.
 constexpr int kTarget = 512, kMostExtra = 2 * kTarget;
 constexpr float kRounds = 2.f;                   // (rows kernel)
 constexpr int kLeast = 4, kTileLeast = 8;        // blocks of a part
 // Tiles kernel.  A tile is cut where that makes it kJoinBlocks shorter: storing the parts, waiting for the last and adding them takes about that long
 // (prompts of one sequence, 28, 40 blocks: 1800 tokens of heads of 128 76, 54 us, 2000 85, 60, 2000 of heads of 64 48, 33; 16: 1000 tokens 40, 34), into
 // up to sqrt(kJoin * its blocks) parts: each adds 1.5 us to what the last of them has to do (96 rows of 4000 tokens 0.1, 0.2, 0.4: 51, 45, 45 us, with
-// no limit 64).
+// no limit 64).  Measured on F16 of 128 and BF16 of 64; a block of larger heads or of Q8 and Q4 takes longer, and there the same numbers cut less than
+// might pay.
 constexpr int kJoinBlocks = 40;
 constexpr float kJoin = 0.2f;
 
 // Rows of a sequence and kv head (new tokens times group) that the rows kernel takes.  Where there are few in all, many too: the other kernel's
 // tiles, each of 256 rows, would be fewer than there are CUs, their parts many and long to join (heads of 128, 4 query heads to each of 8 kv heads;
 // us, rows kernel and tiles kernel.  F16: 128 rows of 1000 tokens 11 and 34, 16 x 24 of 3000 73 and 81, 8 x 64 60 and 59, 32 x 32 166 and 115;
-// Q4: 2 x 128 55 and 52, 8 x 64 80 and 62, 32 x 16 of 4000 106 and 127).
+// Q4: 2 x 128 55 and 52, 8 x 64 80 and 62, 32 x 16 of 4000 106 and 127; other heads go by the same numbers, which were not measured on them).
 constexpr int kFewRows = 64, kFewAlone = 512;
 constexpr int few_in_all(int kind) { return cache_quantised(kind) ? 1 << 13 : 1 << 14; }
 
@@ -380,11 +383,12 @@ __device__ __forceinline__ bool last_part(const AttnArgs& a, const Unit& u, unsi
 
 // Few rows: tiles of 16, four waves that take a part's blocks in turn, each with the next of its blocks on its way while it
 // works on one.  Waves meet in LDS, the parts of a tile in slabs in memory: the part that is last adds them in order.  Bound by HBM where the
-// context is long: 100001 tokens of a Q8 cache, 8 heads of 128, 218 MB: 45 - 51 us = 4.3 - 4.9 TB/s (three waves to a SIMD with one block each: 75);
-// 48 conversations of up to 8192 tokens, 452 MB: 98 us = 4.6 TB/s.  Short contexts wait for one thing after another (1000 tokens: 7.8 us):
-// lengths 1.5, products 1.3, the rest the table, the block and the way of the parts through memory.  Two tiles of rows to a workgroup, so that
-// what a block needs is done once for 32 rows, have registers for one block at a time only: 8 drafts of 5 tokens with 7 heads each 24 us instead
-// of 19.
+// context is long: 100001 tokens of a Q8 cache, 8 heads of 128, 218 MB: 45 - 51 us = 4.3 - 4.9 TB/s (three waves to a SIMD with one block each: 75), of
+// F16 84, BF16 86, Q4 36; 48 conversations of up to 8192 tokens, Q8, 452 MB: 98 us = 4.6 TB/s, F16 158 = 5.4, BF16 165 = 5.2, Q4 74 = 3.2 (unpacking
+// counts there); 4 heads of 256 F16 and BF16 159, Q8 123, Q4 97 (one wave to a SIMD, sums that move between the two halves of its registers).  Short
+// contexts wait for one thing after another (1000 tokens: 8.1 - 8.9 us): lengths 1.5, products 1.3, the rest the table, the block and the way of the
+// parts through memory.  Two tiles of rows to a workgroup, so that what a block needs is done once for 32 rows, have registers for one block at a
+// time only: 8 drafts of 5 tokens with 7 heads each 24 us instead of 19.  (16.7 as it is: 35 rows are three tiles, and each unpacks every block.)
 constexpr int kRows = 16;
 template <int G>
 struct RowsShape {
@@ -823,8 +827,10 @@ struct Stage {
 // Many rows: a workgroup's waves have 32 rows each and go through the same blocks, 64 tokens (a head of 256: 32) a step.  While P of a step
 // is formed the scores of the next are multiplied: its keys are in LDS one step earlier than its values.  Bound by issue: matrix instructions
 // are 57 % of a SIMD's cycles, vector instructions 50, and the card clocks down to 1.64 GHz under them (4096 rows, 32 heads of 128, after 28672 tokens of F16:
-// 1850 - 1975 us = 1.04 - 1.11 PFLOP/s; the library's product of 8192 x 8192 x 8192 1.27).  Q8: each value is also unpacked, once for 256 rows (512 rows
-// after 15872 tokens 175 us = 0.78 PFLOP/s).  Short prompts are as long as the tile that sees the most (2000 rows, heads of 64: 34 us, 25 of them
+// 1850 - 1975 us = 1.04 - 1.11 PFLOP/s; the library's product of 8192 x 8192 x 8192 1.27).  512 rows of 16384 tokens: F16 154 us, BF16 146, Q8 164 = 0.83
+// PFLOP/s, Q4 161 (heads of 64: 99, 95, 104, 106; 96: 128, 123, 139, 141; 4 of 256: 167, 160, 204, 200).  Q8 and Q4: each value is also unpacked, once for 128 or
+// 256 rows, and their loads are flat ones - a block's address comes from two lane reads, and the compiler cannot tell that it is global memory -: they
+// count with the LDS reads, so that the operands fetched ahead are waited for to the last one five to ten times a step.  Short prompts are as long as the tile that sees the most (2000 rows, heads of 64: 34 us, 25 of them
 // that tile's 32 steps).
 template <int KIND, int G>
 __global__ __launch_bounds__((64 * TileShape<KIND, G>::kWaves), (TileShape<KIND, G>::kWaves * TileShape<KIND, G>::kPerCu / 4)) void attention_tiles_kernel(AttnArgs a)
@@ -1254,8 +1260,7 @@ constexpr bool kLaunches = ((int64_t)kRows * kMaxUnits / TileShape<KIND, G>::kRo
 static_assert(kLaunches<kCacheF16, 2> && kLaunches<kCacheF16, 4> && kLaunches<kCacheF16, 8> && kLaunches<kCacheQ8, 2> && kLaunches<kCacheQ8, 8>, "a grid's threads");
 static_assert((int64_t)(kMaxUnits - 1) * 64 * RowsShape<2>::kWaves < (int64_t)1 << 32, "a grid's threads");
 
-// Parts of tiles that have more than one: at most twice those beyond one of each tile
-
+// Slabs: of parts of tiles that have more than one, at most twice those beyond one of each tile
 size_t attention_scratch_bytes(int dim)
 {
     const size_t rows = (size_t)2 * kMostExtra * kRows * (dim + 2);
@@ -1276,7 +1281,7 @@ static_assert(2 * std::max(kMostExtra, TileShape<kCacheF16, 2>::kMostExtra) * si
 
 int64_t attention_units_max(const BatchView& t, int kv_heads, int group)
 {
-    // tiles: (n * group + 15) / 16 of a sequence; parts: at most target more than tiles
+    // tiles: (n * group + 15) / 16 of a sequence; parts: at most kMostExtra more than tiles
     return ((int64_t)t.rows * group / kRows + t.seqs) * kv_heads + std::max(kMostExtra, TileShape<kCacheF16, 2>::kMostExtra);
 }
 

@@ -11,7 +11,8 @@
 // each: 3.6 us, most of it the way from the lengths to the table to the page).  More: queries in a launch of their own (4096 tokens, 32 heads of
 // 128, 67 MB: 16 - 20 us = 3.4 - 4.1 TB/s), whose registers then cost the other kernel no waves, and a block's keys and values by waves that have
 // what lies side by side in it - a key's dimensions of two tokens, eight dimensions of the eight tokens of a value's 8 or 16 bytes -, written
-// 8 and 16 bytes at a time (4096 tokens, 8 heads of 128, bf16 to Q8: 12.4 - 14 us).  Reading back: a block's bytes come once and rows go out 16
+// 8 and 16 bytes at a time (4096 tokens, 8 heads of 128, bf16 to Q8, 26 MB: 12.4 - 14 us = 1.8 - 2.1 TB/s: of its five waves the one that has the values
+// has 64 of them to a lane, the others 16, so that a workgroup has that one's time).  Reading back: a block's bytes come once and rows go out 16
 // bytes to a lane (80000 tokens, 8 heads of 128, Q8 to bf16, 359 MB: 68 - 79 us = 4.5 - 5.3 TB/s).
 #include "cache_parts.h"
 #include "cybq_internal.h"

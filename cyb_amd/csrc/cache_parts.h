@@ -83,7 +83,7 @@ __host__ __device__ constexpr int value_place(int t, int d)
 // byte offset of a scale behind the data
 __host__ __device__ constexpr int scale_place(int t, int g) { return ((g * 4 + token_q4(t)) * 8 + token_slot(t)) * 2; }
 
-// One sequence's rows: row0 .. row0 + n are its last n tokens, of len; positions at and behind `cap` have no page.
+// One sequence's rows: row0 .. row0 + n are its last n tokens, of len; positions at and behind the table's end have no page.
 // Starts that fall, or leave 0 .. rows, make a sequence without rows, or one that ends with the rows.
 struct Seq {
     int row0, n, len;

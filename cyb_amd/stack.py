@@ -273,7 +273,7 @@ class CachedStack:
     cache: KVCache
     tables: object              # int32 [conversations, pages of one]
     lengths: object             # int32 [conversations]
-    rope: object                # fp32 [context, head_dim / 2, 2]
+    rope: object                # fp32 [tokens of a conversation's pages, head_dim / 2, 2]: the table's length, not less
     eps: float = 1e-5
     qkv: List[QWeight] = field(default_factory=list)
     o: List[QWeight] = field(default_factory=list)
