@@ -212,3 +212,34 @@ def test_values_at_the_end_of_f16_stay_finite(backend, new):
     y = check_each(s, [new], 2, "f16", q=q, scale=math.log(2.0) - math.log(1.0 + 1.05 * 2.0 ** -11))
     assert (y.abs() >= 65504.0 * (1.0 - 2.0 ** -10)).all()
     s.close()
+
+
+@gpu
+@pytest.mark.parametrize("kind,dt", [("f16", "f16"), ("bf16", "bf16"), ("q8", "f16"), ("q4", "bf16")])
+@pytest.mark.parametrize("dim", [64, 96, 128, 256])
+def test_a_captured_sequence_of_any_number_of_rows(backend, kind, dt, dim):
+    """A call of one sequence, recorded for a prompt and replayed with fewer rows, down to one and none, between eager calls: each the bits of a call
+    that is made for its rows alone; and the bound of a few rows where they are few, over parts of a long context."""
+    L, rows = 5000, 700
+    s = Cached(backend, kind, [L], kv_heads=2, dim=dim, page=64)
+    ints = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    starts, lengths = ints([0, rows]), ints([L])
+    batch = backend.cache_batch(starts, lengths, s.tables, rows)
+    q = normal((rows, 8, dim), 5, dt)
+    y = torch.zeros_like(q)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+        backend.attention(s.cache, 0, batch, q, y, stream=torch.cuda.current_stream().cuda_stream)
+    for n in (rows, 1, 0, 5, 16, 300, 1, rows):
+        starts.copy_(ints([0, n]))
+        y.fill_(9.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = y.clone()
+        assert (got[n:] == 9.0).all()
+        if n:
+            alone = check_each(s, [n], 4, dt, q=q[:n].contiguous())
+            if n * 4 <= FEW or n == rows:                        # (of rows between, a call made for them may be the other kernel's)
+                assert torch.equal(got[:n], alone)
+    s.close()
