@@ -407,7 +407,8 @@ int cybq_cache_read(cybq_ctx* ctx, const cybq_cache* cache, int64_t layer, const
  * p: the row's position; window 0: all j <= p.  A row that sees nothing is zeros.
  *   q: rows of [q_heads][head_dim] of qdt, q_stride elements apart, 16-byte aligned as its rows are; y [rows][q_heads][head_dim] of qdt, 8-byte
  *   aligned, must not overlap q.  qdt: F16 on an F16 cache, BF16 on a BF16 cache, either of them on Q8 and Q4 (CYBQ_ERR_UNSUPPORTED).
- *   q_heads is at most 65536, rows * q_heads / 16 + seqs * kv_heads less than 2^24 - 1024 (CYBQ_ERR_UNSUPPORTED); scale is positive and finite;
+ *   q_heads is at most 65536, rows * q_heads / 16 + seqs * kv_heads less than 2^24 - 1024 (CYBQ_ERR_UNSUPPORTED); scale is positive and finite (below
+ *   2^-126 and above 2^127 it counts as about that);
  *   q . k, scaled scores (below 2^127) and, over the tokens that a row sees, sums of |v| have to stay within fp32.
  * Scores, maxima and sums are fp32.  Values of Q8 and Q4 caches are round_f16(scale * q).  Up to 64 rows of a sequence and kv head (new
  * tokens times q_heads / kv_heads), any number with CYBQ_PREFILL_EXACT: keys are exact, probabilities rounded by 2^-11 of themselves on an F16 cache,
