@@ -329,7 +329,7 @@ class CachedStack:
                     raise CybqError(-1, "invalid argument", "no such conversations")
                 batches[first] = be.cache_batch(starts, self.lengths[first:first + count], self.tables[first:first + count], M, n)
             batch, x = batches[first], b["x"]
-            with torch.cuda.stream(torch.cuda.ExternalStream(stream) if stream else torch.cuda.default_stream(be.device)):
+            with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=be.device) if stream else torch.cuda.default_stream(be.device)):
                 batch.keep[1].add_(n)
             for i in range(self.layers):
                 be.matmul_norm(self.qkv[i], x, self.norms[i][0], self.eps, b["qkv"], stream=stream)
@@ -373,7 +373,7 @@ def build_cached(backend: Backend, layers: int = 32, bits: int = formats.Q4, kin
         s = torch.empty(N * (K // 32), dtype=torch.int16, device=dev)
         backend.quantize(bits, w, N, K, q, s)
         out = backend.weight_from_device(bits, N, K, q, s, name=name)
-        torch.cuda.synchronize()                                      # w, q and s are released
+        torch.cuda.synchronize(dev)                                      # w, q and s are released
         return out
 
     for i in range(layers):

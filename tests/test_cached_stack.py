@@ -232,3 +232,18 @@ def test_the_driver_on_a_stream_of_its_own(backend):
         st.set_lengths(80)
     assert torch.equal(kept[0][0], kept[1][0]) and torch.equal(kept[0][1], kept[1][1])
     st.free()
+
+
+@gpu
+def test_lengths_are_counted_on_the_stacks_device(backend, monkeypatch):
+    """A step's own torch work goes to its stream on the backend's device, whichever device is the current one."""
+    from cyb_amd import stack
+    st = stack.build_cached(backend, layers=1, kind="q8", conversations=1, context=40, heads=2, kv_heads=1, head_dim=64, width=64, page=32)
+    step, side, made = st.stepper(1), torch.cuda.Stream(), []
+    torch.cuda.synchronize()
+    stream_of = torch.cuda.ExternalStream
+    monkeypatch.setattr(torch.cuda, "ExternalStream", lambda *a, **kw: made.append((a, kw)) or stream_of(*a, **kw))
+    step(side.cuda_stream)
+    torch.cuda.synchronize()
+    assert made == [((side.cuda_stream,), {"device": backend.device})] and st.lengths.tolist() == [1]
+    st.free()
